@@ -1,0 +1,26 @@
+// qw_chunk_attn.h -- host interface of the ragged chunk attention (qw_chunk_attn.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace qw {
+
+constexpr int kChunkMaxBatch = 1024;  // sequences of one call (their schedule lies in shared memory)
+
+struct ChunkArgs {
+    const void *q, *k, *v;  // q (rows, ld_q): heads side by side; k, v: one layer's pages
+    const int *page_table, *slots, *row_start, *kv_len;
+    void *out;
+    float *lse;
+    int *err;
+    void *workspace;
+    long long ld_q, ld_out;
+    int batch, rows, H, Hkv, G, d, ps, log2_ps, num_pages, max_pages, window;
+    float sl2;  // scale * log2(e)
+};
+
+cudaError_t chunk_attn_launch(const ChunkArgs &a, int dtype, cudaStream_t st);
+size_t chunk_attn_workspace(int heads, int kv_heads, int head_dim);
+
+}  // namespace qw

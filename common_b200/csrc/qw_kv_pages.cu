@@ -1,0 +1,187 @@
+// qw_kv_pages.cu -- moving rows of the paged KV cache of every layer in one launch: page copies (the partly filled
+// page of a forked sequence, whole pages of a duplicated one) and compaction (the kept positions of a sequence
+// gathered into new pages, their keys turned to the positions they take).
+//
+// Cache layout: [layer][page][kv_head][page_size][head_dim]; one (layer, page, head) holds page_size contiguous
+// rows.  Both operators are bound by HBM: every row is read once and written once.
+#include <cuda_runtime.h>
+#include <string>
+
+#include "../../include/qwen3_b200.h"
+#include "qw_internal.cuh"
+#include "qw_ops.h"
+
+namespace qw {
+namespace {
+
+constexpr int kCopyThreads = 256;
+constexpr int kCompactThreads = 256;
+
+// One CTA per (page pair, layer, K or V, head): rows [0, n) of the head are contiguous in both pages.
+__global__ void __launch_bounds__(kCopyThreads)
+    qw_kv_copy_kernel(uint4 *kp, uint4 *vp, int layers, int num_pages, int heads, int ps, int row_vec, const int *src,
+                      const int *dst, const int *rows) {
+    const int pair = blockIdx.x;
+    const int s = src[pair], d = dst[pair];
+    if ((unsigned)s >= (unsigned)num_pages || (unsigned)d >= (unsigned)num_pages || s == d) return;
+    const int n = rows ? min(max(rows[pair], 0), ps) * row_vec : ps * row_vec;
+    const int u = blockIdx.y;  // (layer, K or V, head)
+    const int head = u % heads, kv = (u / heads) & 1, layer = u / heads / 2;
+    uint4 *base = kv ? vp : kp;
+    const size_t unit = (size_t)ps * row_vec;
+    const uint4 *from = base + (((size_t)layer * num_pages + s) * heads + head) * unit;
+    uint4 *to = base + (((size_t)layer * num_pages + d) * heads + head) * unit;
+    for (int i = threadIdx.x; i < n; i += kCopyThreads) to[i] = from[i];
+}
+
+// turn 8 pairs (x, y) back by the table's angle: (x cos + y sin, y cos - x sin), in fp32, rounded once
+__device__ __forceinline__ void turn_back(float (&x)[8], float (&y)[8], const float2 *cs) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float2 c = cs[e];
+        const float a = x[e] * c.x + y[e] * c.y;
+        y[e] = y[e] * c.x - x[e] * c.y;
+        x[e] = a;
+    }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
+    const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    v[0] = bf16lo(u.x); v[1] = bf16hi(u.x); v[2] = bf16lo(u.y); v[3] = bf16hi(u.y);
+    v[4] = bf16lo(u.z); v[5] = bf16hi(u.z); v[6] = bf16lo(u.w); v[7] = bf16hi(u.w);
+}
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    return (uint32_t)f2bf_bits(lo) | (uint32_t)f2bf_bits(hi) << 16;
+}
+__device__ __forceinline__ void put8(__nv_bfloat16 *p, const float (&v)[8]) {
+    *reinterpret_cast<uint4 *>(p) =
+        make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+__device__ __forceinline__ void put8(float *p, const float (&v)[8]) {
+    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+struct CompactArgs {
+    void *k, *v;
+    int layers, num_pages, heads, ps, log2_ps, d;
+    const int *src_table, *dst_table;
+    int max_pages;
+    const int *keep, *keep_start, *dst_base;
+    int batch, rows;
+    const float2 *rope;
+    int rope_len;
+};
+
+// One warp per (kept row, layer): the row of every head, keys turned back, values as they are.
+template <typename T>
+__global__ void __launch_bounds__(kCompactThreads) qw_kv_compact_kernel(const CompactArgs a) {
+    const int r = blockIdx.x * (kCompactThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= a.rows) return;
+    // the sequence that row r belongs to: the last b with keep_start[b] <= r
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.keep_start[mid] <= r) lo = mid;
+        else hi = mid - 1;
+    }
+    const int i = r - a.keep_start[lo];
+    if (i < 0 || r >= a.keep_start[lo + 1]) return;
+    const int come = a.keep[r], to = (a.dst_base ? a.dst_base[lo] : 0) + i;
+    const int cp = come >> a.log2_ps, tp = to >> a.log2_ps;
+    if (come < 0 || to < 0 || cp >= a.max_pages || tp >= a.max_pages) return;
+    const int sp = a.src_table[(size_t)lo * a.max_pages + cp], dp = a.dst_table[(size_t)lo * a.max_pages + tp];
+    if ((unsigned)sp >= (unsigned)a.num_pages || (unsigned)dp >= (unsigned)a.num_pages) return;
+    const int layer = blockIdx.y, d = a.d, half = d / 2, hv = half / 8;
+    const size_t head_elems = (size_t)a.ps * d;
+    const size_t from = ((size_t)layer * a.num_pages + sp) * a.heads * head_elems + (size_t)(come & (a.ps - 1)) * d;
+    const size_t dest = ((size_t)layer * a.num_pages + dp) * a.heads * head_elems + (size_t)(to & (a.ps - 1)) * d;
+    T *k = reinterpret_cast<T *>(a.k), *v = reinterpret_cast<T *>(a.v);
+    const int delta = come - to;
+    const bool turn = a.rope && delta > 0 && delta < a.rope_len;
+    for (int u = lane; u < a.heads * hv; u += 32) {
+        const int h = u / hv, c = (u % hv) * 8;
+        const T *p = k + from + h * head_elems + c;
+        T *o = k + dest + h * head_elems + c;
+        float x[8], y[8];
+        load8(p, x);
+        load8(p + half, y);
+        if (turn) turn_back(x, y, a.rope + (size_t)delta * half + c);
+        put8(o, x);
+        put8(o + half, y);
+        const T *pv = v + from + h * head_elems + c;
+        T *ov = v + dest + h * head_elems + c;
+        load8(pv, x);
+        load8(pv + half, y);
+        put8(ov, x);
+        put8(ov + half, y);
+    }
+}
+
+int log2_exact(int x) {
+    int l = 0;
+    while ((1 << l) < x) l++;
+    return l;
+}
+
+qw_status check_pool(const qw_kv_pool *p) {
+    if (!p || !p->k || !p->v) return op_fail(QW_ERR_ARG, "null cache pool");
+    if (((uintptr_t)p->k | (uintptr_t)p->v) & 15) return op_fail(QW_ERR_ARG, "cache pools must be 16-byte aligned");
+    if (p->dtype != QW_DTYPE_F32 && p->dtype != QW_DTYPE_BF16) return op_fail(QW_ERR_UNSUPPORTED, "cache dtype");
+    if (p->layers < 1 || p->num_pages < 1 || p->kv_heads < 1 || p->head_dim < 16 || p->head_dim % 16)
+        return op_fail(QW_ERR_SHAPE, "layers, pages, heads >= 1 and head_dim a positive multiple of 16");
+    if (p->page_size < 1 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
+        return op_fail(QW_ERR_SHAPE, "page_size must be a power of two up to 256");
+    if ((long long)p->layers * 2 * p->kv_heads > 65535) return op_fail(QW_ERR_SHAPE, "layers x KV heads beyond 32767");
+    return QW_OK;
+}
+
+}  // namespace
+}  // namespace qw
+
+using namespace qw;
+
+extern "C" qw_status qw_op_kv_copy_pages(const qw_kv_pool *pool, const int32_t *src, const int32_t *dst,
+                                         const int32_t *rows, int32_t n, void *stream) {
+    qw_status s = check_pool(pool);
+    if (s) return s;
+    if (n < 0) return op_fail(QW_ERR_SHAPE, "n must not be negative");
+    if (n == 0) return QW_OK;
+    if (!src || !dst) return op_fail(QW_ERR_ARG, "null device pointer");
+    const int row_vec = pool->head_dim * (pool->dtype == QW_DTYPE_F32 ? 4 : 2) / 16;
+    qw_kv_copy_kernel<<<dim3(n, pool->layers * 2 * pool->kv_heads), kCopyThreads, 0, (cudaStream_t)stream>>>(
+        (uint4 *)pool->k, (uint4 *)pool->v, pool->layers, pool->num_pages, pool->kv_heads, pool->page_size, row_vec, src,
+        dst, rows);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return op_fail(QW_ERR_CUDA, std::string("page copy launch: ") + cudaGetErrorString(e));
+    return QW_OK;
+}
+
+extern "C" qw_status qw_op_kv_compact(const qw_kv_pool *pool, const int32_t *src_table, const int32_t *dst_table,
+                                      int32_t max_pages, const int32_t *keep, const int32_t *keep_start,
+                                      const int32_t *dst_base, int32_t batch, int32_t rows, const float *rope,
+                                      int32_t rope_len, void *stream) {
+    qw_status s = check_pool(pool);
+    if (s) return s;
+    if (batch < 1 || max_pages < 1 || rows < 0) return op_fail(QW_ERR_SHAPE, "batch, max_pages >= 1 and rows >= 0");
+    if (rope && rope_len < 1) return op_fail(QW_ERR_SHAPE, "rope_len must be positive");
+    if (rows == 0) return QW_OK;
+    if (!src_table || !dst_table || !keep || !keep_start) return op_fail(QW_ERR_ARG, "null device pointer");
+    if ((uintptr_t)rope & 15) return op_fail(QW_ERR_ARG, "rope must be 16-byte aligned");
+    CompactArgs a{};
+    a.k = pool->k; a.v = pool->v; a.layers = pool->layers; a.num_pages = pool->num_pages; a.heads = pool->kv_heads;
+    a.ps = pool->page_size; a.log2_ps = log2_exact(pool->page_size); a.d = pool->head_dim;
+    a.src_table = src_table; a.dst_table = dst_table; a.max_pages = max_pages;
+    a.keep = keep; a.keep_start = keep_start; a.dst_base = dst_base; a.batch = batch; a.rows = rows;
+    a.rope = (const float2 *)rope; a.rope_len = rope_len;
+    const int per = kCompactThreads / 32;
+    const dim3 grid((rows + per - 1) / per, pool->layers);
+    if (pool->dtype == QW_DTYPE_F32) qw_kv_compact_kernel<float><<<grid, kCompactThreads, 0, (cudaStream_t)stream>>>(a);
+    else qw_kv_compact_kernel<__nv_bfloat16><<<grid, kCompactThreads, 0, (cudaStream_t)stream>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return op_fail(QW_ERR_CUDA, std::string("compaction launch: ") + cudaGetErrorString(e));
+    return QW_OK;
+}

@@ -26,7 +26,8 @@ EXPORTS = ("qw_abi_version", "qw_build_info", "qw_get_unique_id", "qw_create", "
            "qw_finalize_weights", "qw_reset", "qw_reserve", "qw_decode_step", "qw_forward_hidden", "qw_prefill",
            "qw_generate", "qw_decode_step_device", "qw_capture_decode", "qw_replay_decode", "qw_synchronize",
            "qw_stream", "qw_last_launch_count", "qw_last_error", "qw_destroy", "qw_profile_decode",
-           "qw_set_device_inputs", "qw_profile_prefill", "qw_op_lm_head_argmax", "qw_op_lm_head_argmax_static", "qw_op_linear", "qw_set_sampling", "qw_decode_sample", "qw_op_sample")
+           "qw_set_device_inputs", "qw_profile_prefill", "qw_op_lm_head_argmax", "qw_op_lm_head_argmax_static", "qw_op_linear", "qw_set_sampling", "qw_decode_sample", "qw_op_sample",
+           "qw_op_chunk_attn", "qw_op_chunk_attn_workspace", "qw_op_kv_copy_pages", "qw_op_kv_compact")
 KERNEL_NAMES = {0: "other", 1: "qkv", 2: "attn", 3: "o_proj", 4: "gate_up", 5: "down", 6: "lm_head", 7: "step"}
 
 
@@ -36,6 +37,21 @@ class QwConfig(C.Structure):
         "qk_norm", "has_qkv_bias", "weight_dtype", "kv_dtype", "max_batch", "max_tokens", "page_size", "num_pages",
         "decode_kernels", "wait_limit_us", "test_stall_cta")] + \
         [("reserved", C.c_int32 * 2), ("rope_theta", C.c_double), ("eps", C.c_double)]
+
+
+class ChunkAttnArgs(C.Structure):
+    """qw_chunk_attn_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k_cache", "v_cache", "page_table", "slots", "row_start", "kv_len",
+                                          "out", "lse", "workspace", "err")] + \
+        [("ld_q", C.c_int64), ("ld_out", C.c_int64), ("workspace_bytes", C.c_uint64)] + \
+        [(n, C.c_int32) for n in ("dtype", "batch", "rows", "heads", "kv_heads", "head_dim", "page_size", "num_pages",
+                                  "max_pages", "window")] + [("scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class KvPool(C.Structure):
+    """qw_kv_pool: KvPool(k_ptr, v_ptr, layers, num_pages, kv_heads, page_size, head_dim, dtype)"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + \
+        [(n, C.c_int32) for n in ("layers", "num_pages", "kv_heads", "page_size", "head_dim", "dtype")]
 
 
 class QwenError(RuntimeError):
@@ -90,6 +106,10 @@ def load() -> C.CDLL:
         "qw_decode_sample": (I32, [P, PI, PI, PI, I32, PI]),
         "qw_op_sample": (I32, [P, I32, I32, I32, C.c_double, C.c_double, I32, P, P, P, P]),
         "qw_op_linear": (I32, [P, I32, I32, P, I32, I32, P, P, P, P]),
+        "qw_op_chunk_attn": (I32, [C.POINTER(ChunkAttnArgs), P]),
+        "qw_op_chunk_attn_workspace": (C.c_uint64, [I32, I32, I32]),
+        "qw_op_kv_copy_pages": (I32, [C.POINTER(KvPool), P, P, P, I32, P]),
+        "qw_op_kv_compact": (I32, [C.POINTER(KvPool), P, P, I32, P, P, P, I32, I32, P, I32, P]),
         "qw_op_lm_head_argmax_static": (I32, [P, I32, I32, I32, P, P, C.c_double, I32, P, P, P]),
     }
     for name, (res, args) in sig.items():
@@ -163,6 +183,56 @@ def op_lm_head_argmax_static(w_ptr: int, w_dtype: int, vocab: int, dim: int, x_p
     """qw_op_lm_head_argmax_static over raw device pointers (scratch in the library's static array)."""
     st = load().qw_op_lm_head_argmax_static(w_ptr, w_dtype, vocab, dim, x_ptr, norm_ptr, eps, batch,
                                             logits_ptr or None, argmax_ptr, stream or None)
+    if st:
+        raise QwenError(st, op_error())
+
+
+def chunk_attn_workspace(heads: int, kv_heads: int, head_dim: int) -> int:
+    """Workspace bytes of ChunkAttention (qw_op_chunk_attn_workspace)."""
+    n = load().qw_op_chunk_attn_workspace(heads, kv_heads, head_dim)
+    if not n:
+        raise QwenError(8, f"chunk attention: {heads} heads, {kv_heads} KV heads, head_dim {head_dim}")
+    return n
+
+
+class ChunkAttention:
+    """qw_op_chunk_attn over raw device pointers: the geometry and the workspace once, then one call per layer and
+    step.  The workspace (chunk_attn_workspace bytes, zeroed by the caller before the first call) serves one call at a
+    time: calls that overlap on the GPU need a ChunkAttention with a workspace of its own."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, max_pages: int,
+                 workspace_ptr: int, workspace_bytes: int, window: int = 0, scale: float = 0.0,
+                 dtype: int = DTYPE_BF16):
+        self._fn = load().qw_op_chunk_attn
+        a = self.args = ChunkAttnArgs()
+        a.heads, a.kv_heads, a.head_dim, a.dtype = heads, kv_heads, head_dim, dtype
+        a.page_size, a.num_pages, a.max_pages = page_size, num_pages, max_pages
+        a.workspace, a.workspace_bytes, a.window, a.scale = workspace_ptr, workspace_bytes, window, scale
+        self._ref = C.byref(a)
+
+    def __call__(self, q: int, k_cache: int, v_cache: int, page_table: int, row_start: int, kv_len: int, batch: int,
+                 rows: int, out: int, lse: int = 0, slots: int = 0, ld_q: int = 0, ld_out: int = 0, err: int = 0,
+                 stream: int = 0) -> None:
+        a = self.args
+        a.q, a.k_cache, a.v_cache, a.page_table, a.row_start, a.kv_len = q, k_cache, v_cache, page_table, row_start, kv_len
+        a.batch, a.rows, a.out, a.lse, a.slots, a.ld_q, a.ld_out, a.err = batch, rows, out, lse, slots, ld_q, ld_out, err
+        st = self._fn(self._ref, stream)
+        if st:
+            raise QwenError(st, op_error())
+
+
+def op_kv_copy_pages(pool: KvPool, src_ptr: int, dst_ptr: int, rows_ptr: int, n: int, stream: int = 0) -> None:
+    """qw_op_kv_copy_pages over raw device pointers (rows_ptr 0: whole pages)."""
+    st = load().qw_op_kv_copy_pages(C.byref(pool), src_ptr, dst_ptr, rows_ptr or None, n, stream or None)
+    if st:
+        raise QwenError(st, op_error())
+
+
+def op_kv_compact(pool: KvPool, src_table: int, dst_table: int, max_pages: int, keep: int, keep_start: int, batch: int,
+                  rows: int, rope: int = 0, rope_len: int = 0, dst_base: int = 0, stream: int = 0) -> None:
+    """qw_op_kv_compact over raw device pointers."""
+    st = load().qw_op_kv_compact(C.byref(pool), src_table, dst_table, max_pages, keep, keep_start, dst_base or None,
+                                 batch, rows, rope or None, rope_len, stream or None)
     if st:
         raise QwenError(st, op_error())
 

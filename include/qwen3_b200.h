@@ -298,6 +298,72 @@ qw_status qw_op_lm_head_argmax_static(const void *w, int32_t w_dtype, int32_t vo
                                       const float *norm_w, double eps, int32_t batch, float *logits_out,
                                       int32_t *argmax_out, void *stream);
 
+/* ---- a shared paged KV cache ----------------------------------------------------------------
+ * One layer of the cache is [page][kv_head][page_size][head_dim]; page_table[slot][i] (max_pages entries per
+ * slot) names the page of positions [i * page_size, (i + 1) * page_size), any other value than a page's number
+ * meaning that there is none.  The reference keeps one contiguous cache per sequence
+ * (engine/ml/src/main/java/org/almostrealism/ml/AttentionFeatures.java:823-877) and has none of these. */
+
+/* Arguments of qw_op_chunk_attn; all pointers are device pointers.  Zero-initialise the struct. */
+typedef struct qw_chunk_attn_args {
+    const void *q;             /* (rows, ld_q) in dtype: heads x head_dim values of every row, RoPE applied */
+    const void *k_cache;       /* this layer's keys and values in dtype, the new rows' already written */
+    const void *v_cache;
+    const int32_t *page_table; /* [slot][max_pages] */
+    const int32_t *slots;      /* (batch) table row of each sequence; NULL = 0..batch-1 */
+    const int32_t *row_start;  /* (batch + 1) sequence b's new rows are row_start[b] .. row_start[b + 1] - 1 */
+    const int32_t *kv_len;     /* (batch) cached positions of each sequence, its new rows included */
+    void *out;                 /* (rows, ld_out) in dtype */
+    float *lse;                /* optional (rows, heads): natural log of the softmax sum */
+    void *workspace;           /* qw_op_chunk_attn_workspace bytes, 256-byte aligned, zeroed before its first call */
+    int32_t *err;              /* optional device word, set non-zero when a bounded device wait gave up */
+    int64_t ld_q, ld_out;      /* row strides in elements, multiples of 16 bytes; 0 = heads * head_dim */
+    uint64_t workspace_bytes;
+    int32_t dtype;             /* QW_DTYPE_BF16 (tensor cores) or QW_DTYPE_F32: q, cache and out */
+    int32_t batch, rows;       /* rows = row_start[batch] */
+    int32_t heads, kv_heads, head_dim; /* heads 1..16 per KV head; head_dim 64 or 128 */
+    int32_t page_size, num_pages, max_pages;
+    int32_t window;            /* 0, or how many positions a row sees at most, its own included */
+    float scale;               /* 0 = 1 / sqrt(head_dim) */
+    int32_t reserved;
+} qw_chunk_attn_args;
+
+/* Causal attention of a ragged batch of new rows over the paged cache, in one launch: sequences of any numbers of
+ * new rows (none and one included) over any numbers of cached positions.  Row i of a sequence's n new rows stands at
+ * position p = kv_len - n + i and sees positions max(0, p - window + 1) .. p (all up to p without a window); a row
+ * that sees nothing gives zeros and an lse of -infinity.  What lies in the cache outside the positions that some row
+ * of the sequence sees is never used, whatever it holds.  fp32 accumulation and softmax.  The lengths are read on the
+ * device: nothing in the call depends on them, so a captured call follows new ones.  The workspace carries no results
+ * between calls, but calls that overlap on the GPU need one each.  batch <= 1024.  Stands in for the scores, mask,
+ * softmax and value sum of the reference's attention block (AttentionFeatures.java:531-616, 906-917), which takes one
+ * row of one sequence. */
+qw_status qw_op_chunk_attn(const qw_chunk_attn_args *args, void *stream);
+
+/* Workspace bytes of qw_op_chunk_attn on any batch of this geometry (0: unsupported geometry). */
+uint64_t qw_op_chunk_attn_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim);
+
+/* The pages of every layer: k and v are [layer][page][kv_head][page_size][head_dim] in dtype (BF16 or F32). */
+typedef struct qw_kv_pool {
+    void *k, *v;
+    int32_t layers, num_pages, kv_heads, page_size, head_dim, dtype;
+} qw_kv_pool;
+
+/* Copy pages in every layer, keys and values: rows [0, rows[i]) (all of the page when rows is NULL) of page src[i]
+ * to page dst[i], i < n.  src, dst and rows are device arrays; a pair with a number outside the pool, or of a page
+ * with itself, is skipped.  No page may be both a source and a destination, or twice a destination, in one call. */
+qw_status qw_op_kv_copy_pages(const qw_kv_pool *pool, const int32_t *src, const int32_t *dst, const int32_t *rows,
+                              int32_t n, void *stream);
+
+/* Close the gaps that dropped positions leave: position dst_base[b] + i of sequence b in dst_table (dst_base NULL = 0)
+ * receives position keep[keep_start[b] + i] of src_table, in every layer; keep is ascending within a sequence.  With
+ * `rope` (rope_len, head_dim / 2, 2) = (cos, sin) per position, keys are turned back by the distance they move (in
+ * fp32, rounded once), so that they lie as if they had been written at their new position; NULL copies them as they
+ * are.  Tables are (batch, max_pages); rows = keep_start[batch]; all arrays are device arrays.  The destination pages
+ * must not be among the source pages. */
+qw_status qw_op_kv_compact(const qw_kv_pool *pool, const int32_t *src_table, const int32_t *dst_table,
+                           int32_t max_pages, const int32_t *keep, const int32_t *keep_start, const int32_t *dst_base,
+                           int32_t batch, int32_t rows, const float *rope, int32_t rope_len, void *stream);
+
 /* Human-readable description of the last error on this model (never NULL).  With m == NULL:
  * the last error of an op-level entry point on this thread. */
 const char *qw_last_error(const qw_model *m);
