@@ -21,6 +21,6 @@ struct ChunkArgs {
 };
 
 cudaError_t chunk_attn_launch(const ChunkArgs &a, int dtype, cudaStream_t st);
-size_t chunk_attn_workspace(int heads, int kv_heads, int head_dim);
+size_t chunk_attn_workspace(int head_dim);
 
 }  // namespace qw

@@ -627,6 +627,22 @@ cudaError_t tma_map_bf16_sw128(CUtensorMap *m, const void *base, long long rows,
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t tma_map_bf16_sw128_3d(CUtensorMap *m, const void *base, int n0, int n1, long long n2, long long s1,
+                                  long long s2, int b1, int b2) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return cudaErrorNotSupported;
+    if ((reinterpret_cast<uintptr_t>(base) & 15) || (s1 % 8) || (s2 % 8) || b1 < 1 || b2 < 1 || b1 > 256 || b2 > 256)
+        return cudaErrorMisalignedAddress;
+    cuuint64_t dims[3] = {(cuuint64_t)n0, (cuuint64_t)n1, (cuuint64_t)n2};
+    cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+    cuuint32_t box[3] = {64u, (cuuint32_t)b1, (cuuint32_t)b2};
+    cuuint32_t es[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <int EPI>
 static cudaError_t prepare_epi() {
     const void *fns[] = {(const void *)qw_tc_gemm_kernel<64, EPI>, (const void *)qw_tc_gemm_kernel<128, EPI>,

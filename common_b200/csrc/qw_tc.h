@@ -48,6 +48,11 @@ cudaError_t tc_gemm_launch(const void *W, const void *X, const TcArgs &a, int ep
 // columns (128 bytes), 128-byte swizzle, zero fill out of bounds.  base 16-byte aligned, ld a multiple of 8.
 cudaError_t tma_map_bf16_sw128(CUtensorMap *m, const void *base, long long rows, int cols, int ld, int box_rows);
 
+// The same for a bf16 (n2, n1, n0) array whose innermost axis is contiguous, strides s1 and s2 elements (multiples of
+// 8): boxes of b2 x b1 x 64.
+cudaError_t tma_map_bf16_sw128_3d(CUtensorMap *m, const void *base, int n0, int n1, long long n2, long long s1,
+                                  long long s2, int b1, int b2);
+
 // Opt every GEMM variant in to its shared memory (once per device, outside of stream capture).
 cudaError_t tc_prepare();
 
