@@ -20,7 +20,8 @@ struct ChunkArgs {
     float sl2;  // scale * log2(e)
 };
 
-cudaError_t chunk_attn_launch(const ChunkArgs &a, int dtype, cudaStream_t st);
-size_t chunk_attn_workspace(int head_dim);
+cudaError_t chunk_attn_tc_launch(const ChunkArgs &a, cudaStream_t st);    // bf16 (qw_chunk_attn_tc.cu)
+cudaError_t chunk_attn_simt_launch(const ChunkArgs &a, cudaStream_t st);  // fp32 (qw_chunk_attn.cu)
+size_t chunk_attn_tc_workspace(int head_dim);
 
 }  // namespace qw

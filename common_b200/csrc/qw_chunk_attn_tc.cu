@@ -1,0 +1,1003 @@
+// qw_chunk_attn_tc.cu -- attention of a ragged batch of new tokens over the paged bf16 cache on the 5th-generation
+// tensor cores (the semantics are those of qw_chunk_attn.cu).
+//
+// The G query heads of a KV head share its keys, so the rows of a query tile are (position, head of the group) pairs:
+// P = floor(128 / G) positions of all G heads, at most 128 rows, one row per TMEM lane.  An item is two such tiles of
+// one sequence and KV head; a K / V block of 128 keys serves both.  The key blocks of all items, in the order
+// sequence, KV head, tiles, form one line that is cut into equal shares, one per CTA (one CTA per SM): every SM gets
+// the same number of blocks whatever the lengths are.  An item cut by a share's end leaves partial results (O, maximum,
+// sum) in the workspace, and the CTAs that share it join them, each a part of its rows, once all are there.
+//
+// An item with one tile only (decoding: G rows; the last rows of a chunk) gives its blocks to the two tile slots in
+// turn, so that one slot's softmax still runs while the tensor cores work on the other; the slots' results are joined
+// at the item's end.
+//
+// Warps (three warpgroups):
+//   0     K and V: TMA boxes of min(page, 128) rows into rings of tc_stages tiles each, one lane per box
+//   1     TMEM and the MMAs: S_t = Q_t K^T, then O_t += P_t V as soon as slot t's softmax has written P_t over S_t;
+//         it also clears the rows of a V block that the sequence never sees (0 x NaN is NaN)
+//   2     Q: one box of (64 columns, G heads, P positions) per 64 columns
+//   3     walks the CTA's share of the line and hands its pieces to the other warps through a ring
+//   4..7  softmax and result of slot 0, one row per thread; 8..11 of slot 1
+// Every wait is bounded; one that runs out sets the error word and ends the CTA (its copies landed, its TMEM freed).
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <mutex>
+
+#include "../../include/qwen3_b200.h"
+#include "qw_chunk_attn.h"
+#include "qw_internal.cuh"
+#include "qw_tc.h"
+#include "qw_tc_util.cuh"
+
+namespace qw {
+namespace {
+
+constexpr int kThreads = 384, kRows = 128, kKeys = 128, kMaxStages = 5;
+constexpr float kRescale = 8.f;  // the running maximum is raised only when it grows by more than 2^8: p stays below 2^8
+constexpr int kPieces = 4;       // ring of pieces
+constexpr int kMinShare = 5;     // units that a CTA beyond one per item is worth: splitting an item costs about as much
+constexpr int kCounterWords = 512;  // arrivals | departures, 256 words each
+
+__host__ __device__ constexpr int tc_stages(int d) { return d == 128 ? 2 : 5; }
+__host__ __device__ constexpr int tc_tile_bytes(int d) { return kRows * d * 2; }
+__host__ __device__ constexpr size_t part_bytes(int d) { return (size_t)kRows * d * 4 + kRows * 8; }
+
+struct Seq {
+    int n, kv, r0;  // new rows, cached positions, first row
+};
+
+// one piece of an item, as the scheduler hands it out
+struct Piece {
+    int flags;       // kEnd, kPair, ...
+    int blk0, nblk;  // key blocks (absolute number of the first)
+    int r0;          // ring index of the first block
+    int q0;          // Q ring index of its first tile
+    int alt;         // parity of the single-tile blocks before it: which slot takes its first block
+    int row0, pos0;  // first row of the item and its position
+    int n0, n1;      // positions in its tiles
+    int kvh, slot;   // KV head, page-table row
+    int lo, hi;      // positions that its rows see
+    int clo, chi;    // positions that some row of the sequence sees: the cache holds something there
+};
+enum { kEnd = 1, kPair = 2, kWhole = 4, kHead = 8 };  // kHead: the item begins in this share
+
+// an item that several CTAs share
+struct Shared {
+    int on, c0, np, pair, rows0, rows, row, head;
+};
+
+struct __align__(16) Smem {
+    unsigned pre[kChunkMaxBatch + 1];  // units of the line before each sequence
+    Seq seq[kChunkMaxBatch];
+    Piece piece[kPieces];
+    Shared shared[2];
+    uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages], q_full[2], q_empty[2],
+        s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], done;
+    uint32_t tmem;
+    int abort, go;
+    int empty;  // some rows stand before their sequence's first position
+};
+
+// one item's keys
+struct Item {
+    int nsub, f, pf, pl, klo, j0, nb;  // tiles; first new row; positions of the first and last row; first seen; blocks
+    __device__ __forceinline__ unsigned units() const { return nb ? nb + 1 : 0; }  // an item that sees nothing is not on the line
+};
+__device__ __forceinline__ Item make_item(const Seq &s, int i, int P, int window) {
+    Item it;
+    it.f = i * 2 * P;
+    const int l = min(s.n, it.f + 2 * P) - 1, p0 = s.kv - s.n;
+    it.nsub = s.n - it.f > P ? 2 : 1;
+    it.pf = p0 + it.f;
+    it.pl = p0 + l;
+    it.klo = window ? max(0, it.pf - window + 1) : 0;
+    it.j0 = it.klo / kKeys;
+    it.nb = it.pl < 0 ? 0 : it.pl / kKeys - it.j0 + 1;
+    return it;
+}
+
+// the line of W units in Ge shares: the first W % Ge of them one unit longer
+struct Line {
+    unsigned q, rem;
+    __device__ __forceinline__ unsigned start(unsigned c) const { return c * q + min(c, rem); }
+    __device__ __forceinline__ unsigned owner(unsigned u) const {
+        const unsigned head = rem * (q + 1);
+        return u < head ? u / (q + 1) : rem + (u - head) / q;
+    }
+};
+
+// K-major or MN-major 128-byte-swizzled operand descriptor; lbo / sbo in bytes
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
+           (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// The MMAs and commits are predicated on the elected lane inside the instruction sequence, not branched around: the
+// whole warp computes their operands, which the compiler then keeps in uniform registers.
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc,
+                                       uint32_t elect) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(elect)
+        : "memory");
+}
+// with the A operand (P) in tensor memory: two bf16 per 32-bit column along K
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc,
+                                       uint32_t elect) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(elect)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar, uint32_t elect) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "setp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(elect)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(smem_u32(dst)),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t taddr, float *v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t *o) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
+          "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void red_release(unsigned *p) {
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory");
+}
+// a bounded wait that ends the same way for every lane of the warp
+__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag, int *err) {
+    return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, err));
+}
+
+// A partial result: O as float4 columns [D / 4][128 rows], then (maximum in log2 units, sum) per row.
+template <int D>
+struct Part {
+    char *p;
+    __device__ __forceinline__ float4 *o(int c4, int row) const { return reinterpret_cast<float4 *>(p) + c4 * kRows + row; }
+    __device__ __forceinline__ float2 *ml(int row) const { return reinterpret_cast<float2 *>(p + (size_t)kRows * D * 4) + row; }
+};
+// which: 0 the share's first piece, 1 its last, 2 the exchange between the slots; k: tile, or slot in turn
+template <int D>
+__device__ __forceinline__ Part<D> part_of(const ChunkArgs &a, int cta, int which, int k) {
+    return Part<D>{(char *)a.workspace + kCounterWords * 4 + ((size_t)cta * 6 + which * 2 + k) * part_bytes(D)};
+}
+
+template <int D>
+__device__ __forceinline__ void put_row(const ChunkArgs &a, const Shared &m, int r, int c4, const float4 &o, float M, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const size_t grow = (size_t)(m.row + r / a.G);
+    const int head = m.head + r % a.G;
+    *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + grow * a.ld_out + (size_t)head * D + c4 * 4) =
+        make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
+    if (c4 == 0 && a.lse) a.lse[grow * a.H + head] = l == 0.f ? -INFINITY : (M + __log2f(l)) * 0.69314718055994531f;
+}
+
+// Rows [lo, lo + nr) of a shared item: sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, m = max m_p, over its parts.
+template <int D>
+__device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, int lo, int nr, int tid, float *red) {
+    const int nparts = m.pair ? m.np : 2 * m.np;
+    auto part = [&](int p, int tile) {
+        const int k = m.pair ? p : p >> 1;
+        return part_of<D>(a, m.c0 + k, k == 0 ? 1 : 0, m.pair ? tile : p & 1);
+    };
+    if (nr >= 16) {
+        // lanes take rows (the parts' columns are contiguous over rows), a warp 8 float4 columns of 32 rows at a time
+        const int lane = tid & 31, ntask = (nr + 31) / 32 * (D / 32);
+        for (int task = tid >> 5; task < ntask; task += 8) {
+            const int r = lo + task / (D / 32) * 32 + lane, c0 = task % (D / 32) * 8;
+            if (r >= lo + nr) continue;
+            const int tile = r >= m.rows0, row = r - (tile ? m.rows0 : 0);
+            float M = -INFINITY, l = 0.f;
+            float4 o[8];
+#pragma unroll
+            for (int c = 0; c < 8; c++) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int p = 0; p < nparts; p++) {
+                const Part<D> px = part(p, tile);
+                const float2 ml = __ldcg(px.ml(row));
+                float4 x[8];
+#pragma unroll
+                for (int c = 0; c < 8; c++) x[c] = __ldcg(px.o(c0 + c, row));
+                if (ml.x == -INFINITY) continue;  // nothing seen there (O may not have been written)
+                const float mn = fmaxf(M, ml.x), wo = ex2(M - mn), wx = ex2(ml.x - mn);
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    o[c].x = o[c].x * wo + x[c].x * wx; o[c].y = o[c].y * wo + x[c].y * wx;
+                    o[c].z = o[c].z * wo + x[c].z * wx; o[c].w = o[c].w * wo + x[c].w * wx;
+                }
+                l = l * wo + ml.y * wx;
+                M = mn;
+            }
+#pragma unroll
+            for (int c = 0; c < 8; c++) put_row<D>(a, m, r, c0 + c, o[c], M, l);
+        }
+        return;
+    }
+    // few rows: a thread takes 4 columns of a row, several threads share the parts
+    const int E = nr * (D / 4), ng = max(1, 256 / E);
+    for (int e0 = 0; e0 < E; e0 += 256) {
+        const int g = E < 256 ? tid / E : 0, e = E < 256 ? tid % E : e0 + tid;
+        const bool on = g < ng && e < E;
+        const int r = lo + e % nr, c4 = e / nr;
+        const int tile = r >= m.rows0, row = r - (tile ? m.rows0 : 0);
+        float M = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (on) {
+#pragma unroll 4
+            for (int p = g; p < nparts; p += ng) {
+                const Part<D> px = part(p, tile);
+                const float2 ml = __ldcg(px.ml(row));
+                const float4 x = __ldcg(px.o(c4, row));
+                if (ml.x == -INFINITY) continue;
+                const float mn = fmaxf(M, ml.x), wo = ex2(M - mn), wx = ex2(ml.x - mn);
+                o.x = o.x * wo + x.x * wx; o.y = o.y * wo + x.y * wx;
+                o.z = o.z * wo + x.z * wx; o.w = o.w * wo + x.w * wx;
+                l = l * wo + ml.y * wx;
+                M = mn;
+            }
+        }
+        if (ng > 1) {  // E < 256: one round
+            float *mine = red + tid * 8;
+            if (on) { mine[0] = M; mine[1] = l; mine[2] = o.x; mine[3] = o.y; mine[4] = o.z; mine[5] = o.w; }
+            bar_softmax();
+            if (on && g == 0)
+                for (int h = 1; h < ng; h++) {
+                    const float *x = red + (h * E + e) * 8;
+                    if (x[0] == -INFINITY) continue;
+                    const float mn = fmaxf(M, x[0]), wo = ex2(M - mn), wx = ex2(x[0] - mn);
+                    o.x = o.x * wo + x[2] * wx; o.y = o.y * wo + x[3] * wx;
+                    o.z = o.z * wo + x[4] * wx; o.w = o.w * wo + x[5] * wx;
+                    l = l * wo + x[1] * wx;
+                    M = mn;
+                }
+        }
+        if (on && g == 0) put_row<D>(a, m, r, c4, o, M, l);
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    qw_chunk_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                            const __grid_constant__ CUtensorMap tmV, const ChunkArgs a) {
+    constexpr int NST = tc_stages(D), TILE = tc_tile_bytes(D), HALF = kRows * 128, NH = D / 64;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Smem sh;
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *sQ = sm, *sK = sm + 2 * TILE, *sV = sK + NST * TILE;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *abort_flag = &sh.abort;
+    const int G = a.G, P = kRows / G;
+
+    // ---- units of every sequence: an item costs its blocks and one more ----
+    if (threadIdx.x == 0) sh.empty = 0;
+    __syncthreads();
+    for (int b0 = warp * 32; b0 < a.batch; b0 += kThreads) {
+        const int b = b0 + lane;
+        Seq s{0, 0, 0};
+        if (b < a.batch) {
+            const int r0 = a.row_start[b], r1 = a.row_start[b + 1], kv = a.kv_len[b];
+            s.r0 = min(max(r0, 0), a.rows);
+            s.n = max(0, min(r1, a.rows) - s.r0);
+            s.kv = min(max(kv, 0), a.max_pages << a.log2_ps);
+            sh.seq[b] = s;
+            if (s.n > s.kv) sh.empty = 1;
+        }
+        const int items = (s.n + 2 * P - 1) / (2 * P);
+        unsigned units = 0;
+        if (items <= 4)
+            for (int i = 0; i < items; i++) units += make_item(s, i, P, a.window).units();
+        // long chunks: the whole warp on one sequence after the other
+        for (unsigned m = __ballot_sync(0xffffffffu, items > 4); m; m &= m - 1) {
+            const int l = __ffs(m) - 1;
+            const Seq t{__shfl_sync(0xffffffffu, s.n, l), __shfl_sync(0xffffffffu, s.kv, l), 0};
+            const int ni = __shfl_sync(0xffffffffu, items, l);
+            unsigned u = 0;
+            for (int i = lane; i < ni; i += 32) u += make_item(t, i, P, a.window).units();
+            u = __reduce_add_sync(0xffffffffu, u);
+            if (lane == l) units = u;
+        }
+        if (b < a.batch) sh.pre[b + 1] = units * a.Hkv;
+    }
+    if (warp == 2 && lane == 0) {
+        for (int i = 0; i < NST; i++) {
+            mbar_init(&sh.k_full[i], 1);
+            mbar_init(&sh.k_empty[i], 2);
+            mbar_init(&sh.v_full[i], 1);
+            mbar_init(&sh.v_empty[i], 2);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.q_full[i], 1);
+            mbar_init(&sh.q_empty[i], 2);
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_full[i], 4);
+            mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.x_full[i], 4);
+            mbar_init(&sh.x_empty[i], 4);
+            sh.shared[i].on = 0;
+        }
+        for (int i = 0; i < kPieces; i++) {
+            mbar_init(&sh.w_full[i], 1);
+            mbar_init(&sh.w_empty[i], 12);  // K / V, Q, the MMA warp for each slot, eight softmax warps
+        }
+        mbar_init(&sh.done, 1);
+        sh.abort = 0;
+        sh.pre[0] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmQ) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmK) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmV) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const int cta = blockIdx.x;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 3) {
+            // ---------------- the scheduler ----------------
+            unsigned W = 0;
+            int items = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += 32) {
+                const int b = b0 + lane;
+                unsigned v = b < a.batch ? sh.pre[b + 1] : 0;
+                int ni = 0;  // items that see something
+                if (b < a.batch && sh.seq[b].kv > 0) {
+                    const Seq s = sh.seq[b];
+                    ni = (s.n + 2 * P - 1) / (2 * P) - max(0, s.n - s.kv) / (2 * P);
+                }
+                items += __reduce_add_sync(0xffffffffu, ni * a.Hkv);
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned w = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v += w;
+                }
+                if (b < a.batch) sh.pre[b + 1] = W + v;
+                W += __shfl_sync(0xffffffffu, v, 31);
+            }
+            __syncwarp();
+            // one CTA per item at least, and more where the shares stay long enough to be worth joining
+            const int Ge = min((int)gridDim.x, max(items, (int)((W + kMinShare - 1) / kMinShare)));
+            Line line{0, 0};
+            unsigned at = 0, end = 0;
+            int b = 0, h = 0, i = 0, off = 0;
+            if (cta < Ge) {  // Ge <= W: an item has two units at least
+                line.q = W / Ge;
+                line.rem = W % Ge;
+                at = line.start(cta);
+                end = line.start(cta + 1);
+                int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before the share
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (sh.pre[mid] <= at) lo = mid;
+                    else hi = mid - 1;
+                }
+                b = lo;
+                const unsigned per = (sh.pre[lo + 1] - sh.pre[lo]) / a.Hkv;
+                unsigned rem = at - sh.pre[lo];
+                h = (int)(rem / per);
+                rem -= h * per;
+                const Seq s = sh.seq[lo];
+                for (; i * 2 * P < s.n; i += 32) {  // the item that holds unit rem of this head
+                    unsigned v = (i + lane) * 2 * P < s.n ? make_item(s, i + lane, P, a.window).units() : 0;
+                    const unsigned mine = v;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const unsigned w = __shfl_up_sync(0xffffffffu, v, o);
+                        if (lane >= o) v += w;
+                    }
+                    const unsigned m = __ballot_sync(0xffffffffu, v > rem);
+                    if (m) {
+                        const int k = __ffs(m) - 1;
+                        i += k;
+                        off = (int)(rem - __shfl_sync(0xffffffffu, v - mine, k));
+                        break;
+                    }
+                    rem -= __shfl_sync(0xffffffffu, v, 31);
+                }
+            }
+            int np = 0, rn = 0, qn = 0, alt = 0;
+            bool ok = true;
+            for (;;) {
+                Piece pc;
+                pc.flags = kEnd;
+                Item it;
+                Seq s;
+                unsigned u0 = 0;
+                int ch = 0, cb = 0;
+                while (at < end) {
+                    s = sh.seq[b];
+                    if (s.n <= 0) { b++; continue; }
+                    it = make_item(s, i, P, a.window);
+                    const int units = (int)it.units();
+                    const int take = min(units - off, (int)(end - at));
+                    const int ja = min(off, it.nb), jb = min(off + take, it.nb);
+                    u0 = at - off;
+                    cb = b; ch = h;
+                    at += take;
+                    off += take;
+                    if (off == units) {
+                        off = 0;
+                        if ((++i) * 2 * P >= s.n) {
+                            i = 0;
+                            if (++h == a.Hkv) { h = 0; b++; }
+                        }
+                    }
+                    if (ja < jb) {
+                        pc.flags = (it.nsub == 2 ? kPair : 0) | (ja == 0 && jb == it.nb ? kWhole : 0) | (ja == 0 ? kHead : 0);
+                        pc.blk0 = it.j0 + ja;
+                        pc.nblk = jb - ja;
+                        break;
+                    }
+                }
+                ok = warp_wait(&sh.w_empty[np % kPieces], (uint32_t)(np / kPieces + 1) & 1u, abort_flag, a.err);
+                if (!ok) break;
+                if (!(pc.flags & kEnd)) {
+                    pc.r0 = rn; pc.q0 = qn; pc.alt = alt & 1;
+                    rn += pc.nblk;
+                    qn += it.nsub;
+                    if (it.nsub == 1) alt += pc.nblk;
+                    pc.row0 = s.r0 + it.f; pc.pos0 = it.pf;
+                    pc.n0 = min(P, s.n - it.f); pc.n1 = it.nsub == 2 ? min(P, s.n - it.f - P) : 0;
+                    pc.kvh = ch; pc.slot = a.slots ? a.slots[cb] : cb;
+                    pc.lo = it.klo; pc.hi = it.pl;
+                    pc.clo = a.window ? max(0, s.kv - s.n - a.window + 1) : 0;
+                    pc.chi = s.kv;
+                    if (!(pc.flags & kWhole) && lane == 0) {
+                        Shared &m = sh.shared[pc.flags & kHead ? 1 : 0];
+                        m.on = 1;
+                        m.c0 = (int)line.owner(u0);
+                        m.np = (int)line.owner(u0 + it.nb - 1) - m.c0 + 1;
+                        m.pair = it.nsub == 2;
+                        m.rows0 = pc.n0 * G;
+                        m.rows = (pc.n0 + pc.n1) * G;
+                        m.row = pc.row0;
+                        m.head = ch * G;
+                    }
+                }
+                if (lane == 0) {
+                    sh.piece[np % kPieces] = pc;
+                    mbar_arrive(&sh.w_full[np % kPieces]);
+                }
+                __syncwarp();
+                np++;
+                if (pc.flags & kEnd) break;
+            }
+        } else if (warp == 0) {
+            // ---------------- K and V ----------------
+            const int br = min(a.ps, kKeys), nbox = kKeys / br;
+            const int box = lane / NH, half = lane % NH;
+            int r = 0;
+            bool ok = true;
+            for (int np = 0; ok; np++) {
+                if (!warp_wait(&sh.w_full[np % kPieces], (uint32_t)(np / kPieces) & 1u, abort_flag, a.err)) break;
+                const Piece &pc = sh.piece[np % kPieces];
+                const int flags = pc.flags, blk0 = pc.blk0, nblk = pc.nblk, lo = pc.lo, hi = pc.hi, kvh = pc.kvh;
+                const int *table = a.page_table + (size_t)pc.slot * a.max_pages;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.w_empty[np % kPieces]);
+                if (flags & kEnd) break;
+                auto page_row = [&](int j) -> int {  // first cache row of this lane's box; none outside what is seen
+                    const int t = (blk0 + j) * kKeys + box * br;
+                    if (j >= nblk || box >= nbox || t > hi || t + br <= lo) return -br;
+                    const int pg = table[t >> a.log2_ps];
+                    return (unsigned)pg < (unsigned)a.num_pages ? (pg * a.Hkv + kvh) * a.ps + (t & (a.ps - 1)) : -br;
+                };
+                int y = page_row(0);
+                for (int j = 0; j < nblk; j++, r++) {
+                    const int yn = page_row(j + 1);
+                    const int st = r % NST;
+                    const uint32_t ph = (uint32_t)(r / NST) & 1u;
+#pragma unroll
+                    for (int kv = 0; kv < 2; kv++) {
+                        uint64_t *full = kv ? &sh.v_full[st] : &sh.k_full[st];
+                        ok = warp_wait(kv ? &sh.v_empty[st] : &sh.k_empty[st], ph ^ 1u, abort_flag, a.err);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(full, TILE);
+                        __syncwarp();
+                        if (box < nbox)
+                            tma_load_2d((kv ? sV : sK) + st * TILE + half * HALF + box * br * 128, kv ? &tmV : &tmK, full,
+                                        half * 64, y);
+                    }
+                    if (!ok) break;
+                    y = yn;
+                }
+            }
+            if (*abort_flag) {  // copies in flight land before the shared memory goes away
+                const uint64_t t0 = gtime_ns();
+                for (int q = max(0, r - NST); q <= r; q++) {
+                    const int k = q % NST;
+                    while (!mbar_try(smem_u32(&sh.k_full[k]), (uint32_t)(q / NST) & 1u) && gtime_ns() - t0 < kTcuWaitCycles / 8) {
+                    }
+                    while (!mbar_try(smem_u32(&sh.v_full[k]), (uint32_t)(q / NST) & 1u) && gtime_ns() - t0 < kTcuWaitCycles / 8) {
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            // ---------------- MMAs ----------------
+            constexpr uint32_t IDS = tc_idesc_f16(kRows, kKeys, 0), IDP = tc_idesc_f16(kRows, D, 1);
+            const uint32_t elect = lane == 0 ? 1u : 0u;
+            const uint64_t dQ = desc_sw128(smem_u32(sQ), 16, 1024), dK = desc_sw128(smem_u32(sK), 16, 1024),
+                           dV = desc_sw128(smem_u32(sV), HALF, 1024);
+            struct Slot {
+                int np, left;         // next piece; visits left in the current one
+                int r, step, q;       // ring index of the visit's block, and of the tile
+                int blk, clo, chi;    // the block's number, and the positions that hold something
+                int visits;           // so far: phase of p_full
+                bool first, one;      // first visit of the piece; single-tile piece
+                bool alone;           // the other slot has no visit in it
+            };
+            Slot sl[2];
+            bool ok = true;
+            auto next_piece = [&](Slot &s, int t) {
+                for (;;) {
+                    ok = warp_wait(&sh.w_full[s.np % kPieces], (uint32_t)(s.np / kPieces) & 1u, abort_flag, a.err);
+                    if (!ok) { s.left = 0; return; }
+                    const Piece &pc = sh.piece[s.np % kPieces];
+                    const int flags = pc.flags, nblk = pc.nblk;
+                    const int j = flags & kPair ? 0 : pc.alt ^ t;  // the slot's first block
+                    s.one = !(flags & kPair);
+                    s.step = s.one ? 2 : 1;
+                    s.left = flags & kEnd ? 0 : (nblk - j + s.step - 1) / s.step;
+                    s.r = pc.r0 + j;
+                    s.q = pc.q0 + (s.one ? 0 : t);
+                    s.blk = pc.blk0 + j;
+                    s.clo = pc.clo;
+                    s.chi = pc.chi;
+                    s.first = true;
+                    s.alone = nblk == 1;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.w_empty[s.np % kPieces]);
+                    s.np++;
+                    if ((flags & kEnd) || s.left > 0) return;
+                }
+            };
+            // S_t = Q_t K^T of the slot's current visit into TMEM columns [128 t, 128 t + 128)
+            auto issue_s = [&](Slot &s, int t) {
+                const int st = __shfl_sync(0xffffffffu, s.r % NST, 0), qe = __shfl_sync(0xffffffffu, s.q & 1, 0);
+                ok = warp_wait(&sh.q_full[qe], (uint32_t)(s.q >> 1) & 1u, abort_flag, a.err) &&
+                     warp_wait(&sh.k_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
+                if (!ok) return;
+                tc_fence_after();
+                const uint64_t da = dQ + (uint64_t)(qe * (TILE >> 4)), db = dK + (uint64_t)(st * (TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const uint64_t off = (uint64_t)(((kk >> 2) * HALF + (kk & 3) * 32) >> 4);
+                    mma_ss(tmem + (uint32_t)(t * kKeys), da + off, db + off, IDS, kk > 0 ? 1u : 0u, elect);
+                }
+                commit(&sh.s_full[t], elect);  // also covers the slot's PV before it: O_t may be rescaled
+                commit(&sh.k_empty[st], elect);
+                if (s.one) commit(&sh.k_empty[st], elect);
+                if (s.left == 1) {
+                    commit(&sh.q_empty[qe], elect);
+                    if (!s.one || s.alone) commit(&sh.q_empty[qe], elect);
+                }
+            };
+            // O_t (+)= P_t V of the slot's current visit
+            auto issue_pv = [&](Slot &s, int t) {
+                const int st = __shfl_sync(0xffffffffu, s.r % NST, 0);
+                ok = warp_wait(&sh.v_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
+                if (!ok) return;
+                const int k0 = s.blk * kKeys;
+                if (s.chi < k0 + kKeys || s.clo > k0) {
+                    // rows that no row of the sequence sees: P is 0 there, and V must be finite (both slots of a pair
+                    // write the same zeros)
+                    const int z0 = min(kKeys, max(0, s.clo - k0)) * 128, z1 = min(kKeys, max(0, s.chi - k0)) * 128;
+#pragma unroll
+                    for (int hf = 0; hf < NH; hf++) {
+                        uint8_t *v = sV + st * TILE + hf * HALF;
+                        for (int x = lane * 16; x < z0; x += 512) *reinterpret_cast<uint4 *>(v + x) = make_uint4(0, 0, 0, 0);
+                        for (int x = z1 + lane * 16; x < HALF; x += 512) *reinterpret_cast<uint4 *>(v + x) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                ok = warp_wait(&sh.p_full[t], (uint32_t)s.visits & 1u, abort_flag, a.err);
+                if (!ok) return;
+                s.visits++;
+                tc_fence_after();
+                const uint64_t db = dV + (uint64_t)(st * (TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; kk++)
+                    mma_ts(tmem + 256u + (uint32_t)(t * 128), tmem + (uint32_t)(t * kKeys + kk * 8),
+                           db + (uint64_t)(kk * 2048 >> 4), IDP, kk > 0 ? 1u : (s.first ? 0u : 1u), elect);
+                commit(&sh.v_empty[st], elect);
+                if (s.one) commit(&sh.v_empty[st], elect);
+                if (s.left == 1) commit(&sh.o_full[t], elect);
+                s.first = false;
+                s.r += s.step;
+                s.blk += s.step;
+                s.left--;
+            };
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                sl[t].np = sl[t].visits = sl[t].left = 0;
+                if (ok) next_piece(sl[t], t);
+                if (ok && sl[t].left) issue_s(sl[t], t);
+            }
+            while (ok && (sl[0].left || sl[1].left)) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    Slot &s = sl[t];
+                    if (!ok || !s.left) continue;
+                    issue_pv(s, t);
+                    if (ok && !s.left) next_piece(s, t);
+                    if (ok && s.left) issue_s(s, t);
+                }
+            }
+            // every MMA of this CTA has completed before the TMEM is freed
+            commit(&sh.done, elect);
+            const uint64_t t0 = gtime_ns();
+            while (!mbar_try(smem_u32(&sh.done), 0) && gtime_ns() - t0 < kTcuWaitCycles) {
+            }
+        } else {
+            // ---------------- Q ----------------
+            int q = 0;
+            bool ok = true;
+            if (lane == 0) {
+                for (int np = 0; ok; np++) {
+                    if (!mbar_wait(&sh.w_full[np % kPieces], (uint32_t)(np / kPieces) & 1u, abort_flag, a.err)) break;
+                    const Piece &pc = sh.piece[np % kPieces];
+                    const int flags = pc.flags, row0 = pc.row0, kvh = pc.kvh;
+                    mbar_arrive(&sh.w_empty[np % kPieces]);
+                    if (flags & kEnd) break;
+                    for (int t = 0; t < (flags & kPair ? 2 : 1); t++, q++) {
+                        const int e = q & 1;
+                        ok = mbar_wait(&sh.q_empty[e], ((uint32_t)(q >> 1) & 1u) ^ 1u, abort_flag, a.err);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&sh.q_full[e], (uint32_t)(NH * G * P * 128));
+                        for (int c = 0; c < NH; c++)
+                            tma_load_3d(sQ + e * TILE + c * HALF, &tmQ, &sh.q_full[e], c * 64, kvh * G, row0 + t * P);
+                    }
+                }
+                if (*abort_flag) {
+                    const uint64_t t0 = gtime_ns();
+                    for (int k = max(0, q - 2); k < q; k++)
+                        while (!mbar_try(smem_u32(&sh.q_full[k & 1]), (uint32_t)(k >> 1) & 1u) && gtime_ns() - t0 < kTcuWaitCycles / 8) {
+                        }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ---------------- softmax and results ----------------
+        const int t = (warp - 4) >> 2, qq = warp & 3, row = qq * 32 + lane;
+        const int rpos = row / G, rhead = row % G;
+        const uint32_t trow = tmem + ((uint32_t)(qq * 32) << 16);
+        const uint32_t ts = trow + (uint32_t)(t * kKeys), to = trow + 256u + (uint32_t)(t * 128);
+        if (sh.empty) {
+            // rows of items whose every row stands before the first position
+            for (int b = 0; b < a.batch; b++) {
+                const Seq s = sh.seq[b];
+                const int before = s.n - s.kv;
+                if (before <= 0) continue;
+                const int rows = s.kv == 0 ? s.n : before / (2 * P) * 2 * P;
+                const int vec = a.H * D / 8;
+                for (int e = blockIdx.x * 256 + threadIdx.x - 128; e < rows * vec; e += gridDim.x * 256) {
+                    const int r = s.r0 + e / vec, c = e % vec * 8;
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)r * a.ld_out + c) = make_uint4(0, 0, 0, 0);
+                    if (a.lse && c % D == 0) a.lse[(size_t)r * a.H + c / D] = -INFINITY;
+                }
+            }
+        }
+        int nv = 0, no = 0, nx[2] = {0, 0};  // visits, pieces with visits, exchanges by writing slot
+        bool ok = true;
+        for (int np = 0; ok; np++) {
+            ok = warp_wait(&sh.w_full[np % kPieces], (uint32_t)(np / kPieces) & 1u, abort_flag, a.err);
+            if (!ok) break;
+            const Piece &pc = sh.piece[np % kPieces];
+            const int flags = pc.flags, nblk = pc.nblk, alt = pc.alt;
+            const bool pair = flags & kPair, whole = flags & kWhole;
+            const int tp = pair ? t * P : 0;                           // first position of the slot's tile in the item
+            const int rows = (pair && t ? pc.n1 : pc.n0) * G;          // valid rows of the tile
+            const int pos = pc.pos0 + tp + rpos;
+            const int grow = pc.row0 + tp + rpos, head = pc.kvh * G + rhead;
+            const int jj = pair ? 0 : alt ^ t, step = pair ? 1 : 2;    // the slot's first block of the piece
+            int k0 = (pc.blk0 + jj) * kKeys;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.w_empty[np % kPieces]);
+            if (flags & kEnd) break;
+            const bool valid = row < rows, warp_on = qq * 32 < rows;
+            __nv_bfloat16 *orow = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)grow * a.ld_out + (size_t)head * D;
+            const int mine = (nblk - jj + step - 1) / step;
+            const bool exchange = whole && !pair && nblk > 1;
+            const bool finish = whole && (!exchange || ((alt + nblk - 1) & 1) == t);  // the slot of the last block
+            const int which = flags & kHead ? 1 : 0, part = pair ? t : jj;
+            if (mine <= 0) {
+                if (!whole && valid) __stcg(part_of<D>(a, cta, which, part).ml(row), make_float2(-INFINITY, 0.f));
+                continue;
+            }
+            float m_use = -INFINITY, l = 0.f;
+            for (int v = 0; v < mine; v++, nv++, k0 += step * kKeys) {
+                ok = warp_wait(&sh.s_full[t], (uint32_t)nv & 1u, abort_flag, a.err);
+                if (!ok) break;
+                tc_fence_after();
+                if (warp_on) {
+                    float x[kKeys];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) ld32(ts + (uint32_t)(c * 32), x + c * 32);
+                    wait_ld();
+                    const int hi = valid ? pos - k0 : kKeys, lo = valid && a.window ? pos - a.window + 1 - k0 : 0;
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (__any_sync(0xffffffffu, hi < kKeys - 1 || lo > 0)) {
+#pragma unroll
+                        for (int e = 0; e < kKeys; e++)
+                            if (e > hi || e < lo) x[e] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int e = 0; e < kKeys; e++) m4[e & 3] = fmaxf(m4[e & 3], x[e]);
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.sl2;
+                    float alpha = 1.f;
+                    bool need = false;
+                    if (v == 0) {
+                        m_use = mx;
+                    } else if (mx > m_use + kRescale) {
+                        alpha = ex2(m_use - mx);
+                        m_use = mx;
+                        need = true;
+                    }
+                    const float off = m_use == -INFINITY ? 0.f : m_use;
+                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const float p0 = ex2(fmaf(x[c * 32 + e], a.sl2, -off)), p1 = ex2(fmaf(x[c * 32 + e + 1], a.sl2, -off));
+                            s4[(e >> 1) & 3] += p0 + p1;
+                            pk[e / 2] = pack2(p0, p1);
+                        }
+                        st16(ts + (uint32_t)(c * 16), pk);
+                    }
+                    l = l * alpha + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+                    if (v > 0 && __any_sync(0xffffffffu, need)) {
+#pragma unroll
+                        for (int c = 0; c < D / 16; c++) {
+                            uint32_t o[16];
+                            ld16(to + (uint32_t)(c * 16), o);
+                            wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            st16(to + (uint32_t)(c * 16), o);
+                        }
+                    }
+                    wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[t]);
+            }
+            if (!ok) break;
+            ok = warp_wait(&sh.o_full[t], (uint32_t)no & 1u, abort_flag, a.err);
+            if (!ok) break;
+            no++;
+            tc_fence_after();
+            if (finish) {
+                // the item's result; of a single-tile item, joined with the other slot's
+                float wo = 1.f, wx = 0.f;
+                Part<D> px = part_of<D>(a, cta, 2, t ^ 1);
+                if (exchange) {
+                    ok = warp_wait(&sh.x_full[t ^ 1], (uint32_t)nx[t ^ 1] & 1u, abort_flag, a.err);
+                    if (!ok) break;
+                    nx[t ^ 1]++;
+                    if (valid) {
+                        const float2 o = __ldcg(px.ml(row));
+                        const float M = fmaxf(m_use, o.x);
+                        wo = M == -INFINITY ? 0.f : ex2(m_use - M);
+                        wx = M == -INFINITY ? 0.f : ex2(o.x - M);
+                        l = l * wo + o.y * wx;
+                        m_use = M;
+                    }
+                }
+                if (warp_on) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    const float io = wo * inv, ix = wx * inv;
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        float o[32];
+                        ld32(to + (uint32_t)(c * 32), o);
+                        wait_ld();
+                        if (valid) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (exchange) z = __ldcg(px.o((c * 32 + e) / 4, row));
+                                o[e] = fmaf(z.x, ix, o[e] * io);
+                                o[e + 1] = fmaf(z.y, ix, o[e + 1] * io);
+                                o[e + 2] = fmaf(z.z, ix, o[e + 2] * io);
+                                o[e + 3] = fmaf(z.w, ix, o[e + 3] * io);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8)
+                                *reinterpret_cast<uint4 *>(orow + c * 32 + e) =
+                                    make_uint4(pack2(o[e], o[e + 1]), pack2(o[e + 2], o[e + 3]), pack2(o[e + 4], o[e + 5]),
+                                               pack2(o[e + 6], o[e + 7]));
+                        }
+                    }
+                    if (valid && a.lse)
+                        a.lse[(size_t)grow * a.H + head] = l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994531f;
+                }
+                if (exchange) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.x_empty[t ^ 1]);
+                }
+            } else {
+                // a partial result: for the other slot, or for the CTAs that share the item
+                Part<D> pp = part_of<D>(a, cta, whole ? 2 : which, whole ? t : part);
+                if (whole) {
+                    ok = warp_wait(&sh.x_empty[t], ((uint32_t)nx[t] & 1u) ^ 1u, abort_flag, a.err);
+                    if (!ok) break;
+                    nx[t]++;
+                }
+                if (warp_on) {
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        float o[32];
+                        ld32(to + (uint32_t)(c * 32), o);
+                        wait_ld();
+                        if (valid) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                __stcg(pp.o((c * 32 + e) / 4, row), make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                        }
+                    }
+                    if (valid) __stcg(pp.ml(row), make_float2(m_use, l));
+                }
+                if (whole) {
+                    __threadfence_block();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.x_full[t]);
+                }
+            }
+        }
+        // ---- items shared with other CTAs: every CTA joins a part of the rows once all pieces are there ----
+        const int tid = threadIdx.x - 128;
+        unsigned *arrived = reinterpret_cast<unsigned *>(a.workspace), *left = arrived + kCounterWords / 2;
+        bar_softmax();
+        if (tid < 2 && sh.shared[tid].on) {
+            __threadfence();
+            red_release(arrived + sh.shared[tid].c0);
+        }
+        for (int k = 0; k < 2; k++) {
+            const Shared m = sh.shared[k];
+            if (!m.on) continue;
+            const int me = cta - m.c0;
+            const int lo = (int)((long long)m.rows * me / m.np), nr = (int)((long long)m.rows * (me + 1) / m.np) - lo;
+            if (nr > 0) {
+                if (tid == 0) {
+                    const uint64_t t0 = gtime_ns();
+                    bool there = !*abort_flag;
+                    while (there && ld_acquire(arrived + m.c0) < (unsigned)m.np)
+                        if (gtime_ns() - t0 > kTcuWaitCycles) {
+                            there = false;
+                            if (a.err) atomicExch(a.err, TC_DEVERR_TIMEOUT);
+                        }
+                    sh.go = there;
+                }
+                bar_softmax();
+                if (sh.go) join_rows<D>(a, m, lo, nr, tid, reinterpret_cast<float *>(sQ));
+                bar_softmax();
+            }
+            if (tid == 0 && atomicAdd(left + m.c0, 1u) == (unsigned)m.np - 1u) {
+                arrived[m.c0] = 0u;  // the last to leave: ready for the next launch
+                left[m.c0] = 0u;
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int D>
+cudaError_t launch(const ChunkArgs &a, cudaStream_t st) {
+    constexpr int smem = (2 + 2 * tc_stages(D)) * tc_tile_bytes(D) + 1024;
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    {
+        static std::mutex mu;
+        static bool prepared[64] = {};
+        std::lock_guard<std::mutex> lk(mu);
+        if (!prepared[dev]) {
+            e = cudaFuncSetAttribute(qw_chunk_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e != cudaSuccess) return e;
+            prepared[dev] = true;
+        }
+    }
+    CUtensorMap mq, mk, mv;
+    const int P = kRows / a.G, br = a.ps < kKeys ? a.ps : kKeys;
+    const long long crow = (long long)a.num_pages * a.Hkv * a.ps;
+    if ((e = tma_map_bf16_sw128_3d(&mq, a.q, a.d, a.H, a.rows, a.d, a.ld_q, a.G, P)) != cudaSuccess) return e;
+    if ((e = tma_map_bf16_sw128(&mk, a.k, crow, a.d, a.d, br)) != cudaSuccess) return e;
+    if ((e = tma_map_bf16_sw128(&mv, a.v, crow, a.d, a.d, br)) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms < kNumSMsB200 ? sms : kNumSMsB200);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeCooperative;  // CTAs that share an item wait for one another
+    at[0].val.cooperative = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, qw_chunk_attn_tc_kernel<D>, mq, mk, mv, a);
+}
+
+}  // namespace
+
+cudaError_t chunk_attn_tc_launch(const ChunkArgs &a, cudaStream_t st) {
+    return a.d == 128 ? launch<128>(a, st) : launch<64>(a, st);
+}
+
+size_t chunk_attn_tc_workspace(int head_dim) { return kCounterWords * 4 + (size_t)kNumSMsB200 * 6 * part_bytes(head_dim); }
+
+}  // namespace qw
