@@ -12,13 +12,14 @@
 // turn, so that one slot's softmax still runs while the tensor cores work on the other; the slots' results are joined
 // at the item's end.
 //
-// Warps (three warpgroups):
+// Warps (five warpgroups):
 //   0     K and V: TMA boxes of min(page, 128) rows into rings of tc_stages tiles each, one lane per box
 //   1     TMEM and the MMAs: S_t = Q_t K^T, then O_t += P_t V as soon as slot t's softmax has written P_t over S_t;
 //         it also clears the rows of a V block that the sequence never sees (0 x NaN is NaN)
 //   2     Q: one box of (64 columns, G heads, P positions) per 64 columns
 //   3     walks the CTA's share of the line and hands its pieces to the other warps through a ring
-//   4..7  softmax and result of slot 0, one row per thread; 8..11 of slot 1
+//   4..11 softmax and result of slot 0, two threads per row (64 keys, and half of the columns of O, each), so that one
+//         warp's loads, maxima and stores run beside the other's exponentials; 12..19 of slot 1
 // Every wait is bounded; one that runs out sets the error word and ends the CTA (its copies landed, its TMEM freed).
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -33,11 +34,11 @@
 namespace qw {
 namespace {
 
-constexpr int kThreads = 384, kRows = 128, kKeys = 128, kMaxStages = 5;
+constexpr int kThreads = 640, kSoftThreads = 512, kRows = 128, kKeys = 128, kMaxStages = 5;
 constexpr float kRescale = 8.f;  // the running maximum is raised only when it grows by more than 2^8: p stays below 2^8
 constexpr int kPieces = 4;       // ring of pieces
 constexpr int kMinShare = 5;     // units that a CTA beyond one per item is worth: splitting an item costs about as much
-constexpr int kCounterWords = 512;  // arrivals | departures, 256 words each
+constexpr int kCounterWords = 256;  // arrivals | departures | arrivals at items cut once, one word per CTA each
 
 __host__ __device__ constexpr int tc_stages(int d) { return d == 128 ? 2 : 5; }
 __host__ __device__ constexpr int tc_tile_bytes(int d) { return kRows * d * 2; }
@@ -60,7 +61,7 @@ struct Piece {
     int lo, hi;      // positions that its rows see
     int clo, chi;    // positions that some row of the sequence sees: the cache holds something there
 };
-enum { kEnd = 1, kPair = 2, kWhole = 4, kHead = 8 };  // kHead: the item begins in this share
+enum { kEnd = 1, kPair = 2, kWhole = 4, kHead = 8, kTwo = 16 };  // kHead: the item begins in this share; kTwo: and is cut once
 
 // an item that several CTAs share
 struct Shared {
@@ -75,6 +76,7 @@ struct __align__(16) Smem {
     uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages], q_full[2], q_empty[2],
         s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], done;
     uint32_t tmem;
+    float mx[2][2][kRows], sum[2][2][kRows];  // [slot][half][row]
     int abort, go;
     int empty;  // some rows stand before their sequence's first position
 };
@@ -186,12 +188,34 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unf2(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory"); }
+// The two warps that share 32 rows of a slot.  One whose wait ran out still arrives for the other, which may have seen
+// the wait end in time; that one's next wait needs the missing results and runs out too.
+__device__ __forceinline__ void leave_pair(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void bar_pair(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
     unsigned v;
     asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
@@ -200,6 +224,7 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
 __device__ __forceinline__ void red_release(unsigned *p) {
     asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory");
 }
+__device__ __forceinline__ int uni(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 // a bounded wait that ends the same way for every lane of the warp
 __device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag, int *err) {
     return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, err));
@@ -215,7 +240,7 @@ struct Part {
 // which: 0 the share's first piece, 1 its last, 2 the exchange between the slots; k: tile, or slot in turn
 template <int D>
 __device__ __forceinline__ Part<D> part_of(const ChunkArgs &a, int cta, int which, int k) {
-    return Part<D>{(char *)a.workspace + kCounterWords * 4 + ((size_t)cta * 6 + which * 2 + k) * part_bytes(D)};
+    return Part<D>{(char *)a.workspace + 3 * kCounterWords * 4 + ((size_t)cta * 6 + which * 2 + k) * part_bytes(D)};
 }
 
 template <int D>
@@ -239,7 +264,7 @@ __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, i
     if (nr >= 16) {
         // lanes take rows (the parts' columns are contiguous over rows), a warp 8 float4 columns of 32 rows at a time
         const int lane = tid & 31, ntask = (nr + 31) / 32 * (D / 32);
-        for (int task = tid >> 5; task < ntask; task += 8) {
+        for (int task = tid >> 5; task < ntask; task += kSoftThreads / 32) {
             const int r = lo + task / (D / 32) * 32 + lane, c0 = task % (D / 32) * 8;
             if (r >= lo + nr) continue;
             const int tile = r >= m.rows0, row = r - (tile ? m.rows0 : 0);
@@ -269,9 +294,9 @@ __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, i
         return;
     }
     // few rows: a thread takes 4 columns of a row, several threads share the parts
-    const int E = nr * (D / 4), ng = max(1, 256 / E);
-    for (int e0 = 0; e0 < E; e0 += 256) {
-        const int g = E < 256 ? tid / E : 0, e = E < 256 ? tid % E : e0 + tid;
+    const int E = nr * (D / 4), ng = max(1, kSoftThreads / E);
+    for (int e0 = 0; e0 < E; e0 += kSoftThreads) {
+        const int g = E < kSoftThreads ? tid / E : 0, e = E < kSoftThreads ? tid % E : e0 + tid;
         const bool on = g < ng && e < E;
         const int r = lo + e % nr, c4 = e / nr;
         const int tile = r >= m.rows0, row = r - (tile ? m.rows0 : 0);
@@ -291,7 +316,7 @@ __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, i
                 M = mn;
             }
         }
-        if (ng > 1) {  // E < 256: one round
+        if (ng > 1) {  // one round
             float *mine = red + tid * 8;
             if (on) { mine[0] = M; mine[1] = l; mine[2] = o.x; mine[3] = o.y; mine[4] = o.z; mine[5] = o.w; }
             bar_softmax();
@@ -319,7 +344,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ Smem sh;
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sQ = sm, *sK = sm + 2 * TILE, *sV = sK + NST * TILE;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (values shuffled from lane 0 are known to be the same in the whole warp: what is computed from them stays in
+    // uniform registers, where the MMA's operands have to be)
+    const int warp = uni(threadIdx.x >> 5), lane = threadIdx.x & 31;
     volatile int *abort_flag = &sh.abort;
     const int G = a.G, P = kRows / G;
 
@@ -356,23 +383,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 2 && lane == 0) {
         for (int i = 0; i < NST; i++) {
             mbar_init(&sh.k_full[i], 1);
-            mbar_init(&sh.k_empty[i], 2);
+            mbar_init(&sh.k_empty[i], 1);
             mbar_init(&sh.v_full[i], 1);
-            mbar_init(&sh.v_empty[i], 2);
+            mbar_init(&sh.v_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.q_full[i], 1);
-            mbar_init(&sh.q_empty[i], 2);
+            mbar_init(&sh.q_empty[i], 1);
             mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_full[i], 4);
+            mbar_init(&sh.p_full[i], 8);
             mbar_init(&sh.o_full[i], 1);
-            mbar_init(&sh.x_full[i], 4);
-            mbar_init(&sh.x_empty[i], 4);
+            mbar_init(&sh.x_full[i], 8);
+            mbar_init(&sh.x_empty[i], 8);
             sh.shared[i].on = 0;
         }
         for (int i = 0; i < kPieces; i++) {
             mbar_init(&sh.w_full[i], 1);
-            mbar_init(&sh.w_empty[i], 12);  // K / V, Q, the MMA warp for each slot, eight softmax warps
+            mbar_init(&sh.w_empty[i], 20);  // K / V, Q, the MMA warp for each slot, sixteen softmax warps
         }
         mbar_init(&sh.done, 1);
         sh.abort = 0;
@@ -390,11 +417,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: the allocation begins at column 0
     const int cta = blockIdx.x;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 3) {
             // ---------------- the scheduler ----------------
             unsigned W = 0;
@@ -504,11 +531,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     pc.lo = it.klo; pc.hi = it.pl;
                     pc.clo = a.window ? max(0, s.kv - s.n - a.window + 1) : 0;
                     pc.chi = s.kv;
-                    if (!(pc.flags & kWhole) && lane == 0) {
+                    const int c0 = pc.flags & kHead ? cta : (int)line.owner(u0);
+                    const int ni = pc.flags & kWhole ? 1 : (int)line.owner(u0 + it.nb - 1) - c0 + 1;
+                    if (ni == 2) pc.flags |= kTwo;
+                    if (ni > 2 && lane == 0) {
                         Shared &m = sh.shared[pc.flags & kHead ? 1 : 0];
                         m.on = 1;
-                        m.c0 = (int)line.owner(u0);
-                        m.np = (int)line.owner(u0 + it.nb - 1) - m.c0 + 1;
+                        m.c0 = c0;
+                        m.np = ni;
                         m.pair = it.nsub == 2;
                         m.rows0 = pc.n0 * G;
                         m.rows = (pc.n0 + pc.n1) * G;
@@ -590,21 +620,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             Slot sl[2];
             bool ok = true;
+            unsigned k_used = 0, v_used = 0, q_used = 0;  // ring entries that one of two slots has used
             auto next_piece = [&](Slot &s, int t) {
                 for (;;) {
                     ok = warp_wait(&sh.w_full[s.np % kPieces], (uint32_t)(s.np / kPieces) & 1u, abort_flag, a.err);
                     if (!ok) { s.left = 0; return; }
                     const Piece &pc = sh.piece[s.np % kPieces];
-                    const int flags = pc.flags, nblk = pc.nblk;
-                    const int j = flags & kPair ? 0 : pc.alt ^ t;  // the slot's first block
+                    const int flags = uni(pc.flags), nblk = uni(pc.nblk);
+                    const int j = flags & kPair ? 0 : uni(pc.alt) ^ t;  // the slot's first block
                     s.one = !(flags & kPair);
                     s.step = s.one ? 2 : 1;
                     s.left = flags & kEnd ? 0 : (nblk - j + s.step - 1) / s.step;
-                    s.r = pc.r0 + j;
-                    s.q = pc.q0 + (s.one ? 0 : t);
-                    s.blk = pc.blk0 + j;
-                    s.clo = pc.clo;
-                    s.chi = pc.chi;
+                    s.r = uni(pc.r0) + j;
+                    s.q = uni(pc.q0) + (s.one ? 0 : t);
+                    s.blk = uni(pc.blk0) + j;
+                    s.clo = uni(pc.clo);
+                    s.chi = uni(pc.chi);
                     s.first = true;
                     s.alone = nblk == 1;
                     __syncwarp();
@@ -615,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             // S_t = Q_t K^T of the slot's current visit into TMEM columns [128 t, 128 t + 128)
             auto issue_s = [&](Slot &s, int t) {
-                const int st = __shfl_sync(0xffffffffu, s.r % NST, 0), qe = __shfl_sync(0xffffffffu, s.q & 1, 0);
+                const int st = s.r % NST, qe = s.q & 1;
                 ok = warp_wait(&sh.q_full[qe], (uint32_t)(s.q >> 1) & 1u, abort_flag, a.err) &&
                      warp_wait(&sh.k_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
                 if (!ok) return;
@@ -627,16 +658,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mma_ss(tmem + (uint32_t)(t * kKeys), da + off, db + off, IDS, kk > 0 ? 1u : 0u, elect);
                 }
                 commit(&sh.s_full[t], elect);  // also covers the slot's PV before it: O_t may be rescaled
-                commit(&sh.k_empty[st], elect);
-                if (s.one) commit(&sh.k_empty[st], elect);
-                if (s.left == 1) {
-                    commit(&sh.q_empty[qe], elect);
-                    if (!s.one || s.alone) commit(&sh.q_empty[qe], elect);
+                k_used ^= 1u << st;  // a pair's block is released by the second of its two slots
+                if (s.one) k_used &= ~(1u << st);
+                if (!(k_used >> st & 1u)) commit(&sh.k_empty[st], elect);
+                if (s.left == 1) {  // a single tile serves both slots, where both have visits
+                    if (s.one && !s.alone) q_used ^= 1u << qe;
+                    if (!(q_used >> qe & 1u)) commit(&sh.q_empty[qe], elect);
                 }
             };
             // O_t (+)= P_t V of the slot's current visit
             auto issue_pv = [&](Slot &s, int t) {
-                const int st = __shfl_sync(0xffffffffu, s.r % NST, 0);
+                const int st = s.r % NST;
                 ok = warp_wait(&sh.v_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
                 if (!ok) return;
                 const int k0 = s.blk * kKeys;
@@ -655,15 +687,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 ok = warp_wait(&sh.p_full[t], (uint32_t)s.visits & 1u, abort_flag, a.err);
                 if (!ok) return;
-                s.visits++;
                 tc_fence_after();
                 const uint64_t db = dV + (uint64_t)(st * (TILE >> 4));
 #pragma unroll
-                for (int kk = 0; kk < kKeys / 16; kk++)
-                    mma_ts(tmem + 256u + (uint32_t)(t * 128), tmem + (uint32_t)(t * kKeys + kk * 8),
+                for (int kk = 0; kk < kKeys / 16; kk++)  // P's halves lie over their own halves of S
+                    mma_ts(tmem + 256u + (uint32_t)(t * 128), tmem + (uint32_t)(t * kKeys + (kk & 3) * 8 + (kk >> 2) * 64),
                            db + (uint64_t)(kk * 2048 >> 4), IDP, kk > 0 ? 1u : (s.first ? 0u : 1u), elect);
-                commit(&sh.v_empty[st], elect);
-                if (s.one) commit(&sh.v_empty[st], elect);
+                s.visits++;
+                v_used ^= 1u << st;
+                if (s.one) v_used &= ~(1u << st);
+                if (!(v_used >> st & 1u)) commit(&sh.v_empty[st], elect);
                 if (s.left == 1) commit(&sh.o_full[t], elect);
                 s.first = false;
                 s.r += s.step;
@@ -720,12 +753,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
         // ---------------- softmax and results ----------------
-        const int t = (warp - 4) >> 2, qq = warp & 3, row = qq * 32 + lane;
+        const int t = (warp - 4) >> 3, hf = ((warp - 4) >> 2) & 1, qq = warp & 3, row = qq * 32 + lane, pair_id = 2 + t * 4 + qq;
         const int rpos = row / G, rhead = row % G;
         const uint32_t trow = tmem + ((uint32_t)(qq * 32) << 16);
-        const uint32_t ts = trow + (uint32_t)(t * kKeys), to = trow + 256u + (uint32_t)(t * 128);
+        const uint32_t ts = trow + (uint32_t)(t * kKeys + hf * 64), to = trow + 256u + (uint32_t)(t * 128 + hf * (D / 2));
         if (sh.empty) {
             // rows of items whose every row stands before the first position
             for (int b = 0; b < a.batch; b++) {
@@ -734,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (before <= 0) continue;
                 const int rows = s.kv == 0 ? s.n : before / (2 * P) * 2 * P;
                 const int vec = a.H * D / 8;
-                for (int e = blockIdx.x * 256 + threadIdx.x - 128; e < rows * vec; e += gridDim.x * 256) {
+                for (int e = blockIdx.x * kSoftThreads + threadIdx.x - 128; e < rows * vec; e += gridDim.x * kSoftThreads) {
                     const int r = s.r0 + e / vec, c = e % vec * 8;
                     *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)r * a.ld_out + c) = make_uint4(0, 0, 0, 0);
                     if (a.lse && c % D == 0) a.lse[(size_t)r * a.H + c / D] = -INFINITY;
@@ -759,35 +792,59 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(&sh.w_empty[np % kPieces]);
             if (flags & kEnd) break;
             const bool valid = row < rows, warp_on = qq * 32 < rows;
-            __nv_bfloat16 *orow = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)grow * a.ld_out + (size_t)head * D;
+            __nv_bfloat16 *orow = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)grow * a.ld_out + (size_t)head * D + hf * (D / 2);
             const int mine = (nblk - jj + step - 1) / step;
-            const bool exchange = whole && !pair && nblk > 1;
-            const bool finish = whole && (!exchange || ((alt + nblk - 1) & 1) == t);  // the slot of the last block
+            // An item cut once is finished by the CTA in which it begins, at the end of its share, from the other's part:
+            // that came first in the next share and has long been there.
+            const bool two = flags & kTwo, closes = whole || (two && (flags & kHead));
+            const bool exchange = closes && !pair && nblk > 1;
+            const bool finish = closes && (!exchange || ((alt + nblk - 1) & 1) == t);  // the slot of the last block
             const int which = flags & kHead ? 1 : 0, part = pair ? t : jj;
+            unsigned *arrived2 = reinterpret_cast<unsigned *>(a.workspace) + kCounterWords + (flags & kHead ? cta : cta - 1);
             if (mine <= 0) {
-                if (!whole && valid) __stcg(part_of<D>(a, cta, which, part).ml(row), make_float2(-INFINITY, 0.f));
+                if (!closes) {
+                    if (valid && hf == 0) __stcg(part_of<D>(a, cta, which, part).ml(row), make_float2(-INFINITY, 0.f));
+                    if (two) {
+                        __threadfence();
+                        __syncwarp();
+                        if (lane == 0) red_release(arrived2);
+                    }
+                }
                 continue;
             }
-            float m_use = -INFINITY, l = 0.f;
+            float m_use = -INFINITY, l = 0.f;  // running maximum (log2 units), sum of this half's probabilities
             for (int v = 0; v < mine; v++, nv++, k0 += step * kKeys) {
                 ok = warp_wait(&sh.s_full[t], (uint32_t)nv & 1u, abort_flag, a.err);
-                if (!ok) break;
+                if (!ok) {
+                    if (warp_on) leave_pair(pair_id);
+                    break;
+                }
                 tc_fence_after();
                 if (warp_on) {
-                    float x[kKeys];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) ld32(ts + (uint32_t)(c * 32), x + c * 32);
+                    float x[64];
+                    ld32(ts, x);
+                    ld32(ts + 32u, x + 32);
                     wait_ld();
-                    const int hi = valid ? pos - k0 : kKeys, lo = valid && a.window ? pos - a.window + 1 - k0 : 0;
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (__any_sync(0xffffffffu, hi < kKeys - 1 || lo > 0)) {
+                    const int hi = valid ? pos - k0 - hf * 64 : 64;
+                    if (hi < 63) {
 #pragma unroll
-                        for (int e = 0; e < kKeys; e++)
-                            if (e > hi || e < lo) x[e] = -INFINITY;
+                        for (int e = 0; e < 64; e++)
+                            if (e > hi) x[e] = -INFINITY;
                     }
+                    if (a.window && valid && hi >= a.window) {
+                        const int lo = hi - a.window;
 #pragma unroll
-                    for (int e = 0; e < kKeys; e++) m4[e & 3] = fmaxf(m4[e & 3], x[e]);
-                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.sl2;
+                        for (int e = 0; e < 64; e++)
+                            if (e <= lo) x[e] = -INFINITY;
+                    }
+                    // maximum of the raw scores (the scale is positive), with that of the row's other half
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) m4[(e >> 1) & 3] = fmaxf(m4[(e >> 1) & 3], fmaxf(x[e], x[e + 1]));
+                    float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    sh.mx[t][hf][row] = mx;
+                    bar_pair(pair_id);
+                    mx = fmaxf(mx, sh.mx[t][hf ^ 1][row]) * a.sl2;
                     float alpha = 1.f;
                     bool need = false;
                     if (v == 0) {
@@ -797,23 +854,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                         m_use = mx;
                         need = true;
                     }
-                    const float off = m_use == -INFINITY ? 0.f : m_use;
-                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                    // p = 2^(s scale log2 e - m); P goes to TMEM as packed bf16 pairs over the first half of this half's
+                    // columns of S, and its sum is taken before that rounding
+                    const float off = m_use == -INFINITY ? 0.f : -m_use;
+                    const uint64_t off2 = f2(off, off), sl2 = f2(a.sl2, a.sl2);
+                    uint64_t s2[2] = {0, 0};
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
+                    for (int c = 0; c < 2; c++) {
                         uint32_t pk[16];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float p0 = ex2(fmaf(x[c * 32 + e], a.sl2, -off)), p1 = ex2(fmaf(x[c * 32 + e + 1], a.sl2, -off));
-                            s4[(e >> 1) & 3] += p0 + p1;
-                            pk[e / 2] = pack2(p0, p1);
+                        for (int e = 0; e < 16; e++) {
+                            float p0, p1;
+                            unf2(fma2(f2(x[c * 32 + 2 * e], x[c * 32 + 2 * e + 1]), sl2, off2), p0, p1);
+                            p0 = ex2(p0);
+                            p1 = ex2(p1);
+                            s2[e & 1] = add2(s2[e & 1], f2(p0, p1));
+                            pk[e] = pack2(p0, p1);
                         }
                         st16(ts + (uint32_t)(c * 16), pk);
                     }
-                    l = l * alpha + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
-                    if (v > 0 && __any_sync(0xffffffffu, need)) {
+                    float s0, s1;
+                    unf2(add2(s2[0], s2[1]), s0, s1);
+                    l = l * alpha + (s0 + s1);
+                    // this half of O's columns (the slot's PV before has completed: s_full came after it)
+                    if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
-                        for (int c = 0; c < D / 16; c++) {
+                        for (int c = 0; c < D / 32; c++) {
                             uint32_t o[16];
                             ld16(to + (uint32_t)(c * 16), o);
                             wait_ld();
@@ -830,52 +896,102 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!ok) break;
             ok = warp_wait(&sh.o_full[t], (uint32_t)no & 1u, abort_flag, a.err);
-            if (!ok) break;
+            if (!ok) {
+                if (warp_on) leave_pair(pair_id);
+                break;
+            }
             no++;
             tc_fence_after();
+            if (warp_on) {  // the row's sum, of both halves
+                sh.sum[t][hf][row] = l;
+                bar_pair(pair_id);
+                l += sh.sum[t][hf ^ 1][row];
+            }
             if (finish) {
-                // the item's result; of a single-tile item, joined with the other slot's
-                float wo = 1.f, wx = 0.f;
-                Part<D> px = part_of<D>(a, cta, 2, t ^ 1);
+                // the item's result, joined with the other slot's (of a single-tile item) and the other CTA's parts
+                float wo = 1.f, w[3] = {0.f, 0.f, 0.f};
+                const Part<D> px[3] = {part_of<D>(a, cta, 2, t ^ 1), part_of<D>(a, cta + 1, 0, pair ? t : 0), part_of<D>(a, cta + 1, 0, 1)};
+                const bool have[3] = {exchange, !whole, !whole && !pair};
                 if (exchange) {
                     ok = warp_wait(&sh.x_full[t ^ 1], (uint32_t)nx[t ^ 1] & 1u, abort_flag, a.err);
                     if (!ok) break;
                     nx[t ^ 1]++;
-                    if (valid) {
-                        const float2 o = __ldcg(px.ml(row));
-                        const float M = fmaxf(m_use, o.x);
-                        wo = M == -INFINITY ? 0.f : ex2(m_use - M);
-                        wx = M == -INFINITY ? 0.f : ex2(o.x - M);
-                        l = l * wo + o.y * wx;
-                        m_use = M;
+                }
+                if (!whole) {
+                    // all sixteen softmax warps of the other CTA
+                    if (lane == 0) {
+                        const uint64_t t0 = gtime_ns();
+                        while (ld_acquire(arrived2) < 16u && !*abort_flag)
+                            if (gtime_ns() - t0 > kTcuWaitCycles) {
+                                *abort_flag = 1;
+                                if (a.err) atomicExch(a.err, TC_DEVERR_TIMEOUT);
+                            }
+                        // the last of the item's finishing warps leaves the counter as it was
+                        if (atomicAdd(arrived2, 0x100u) >> 8 == (pair ? 15u : 7u)) *arrived2 = 0u;
                     }
+                    __syncwarp();
+                }
+                if (valid) {
+                    float2 o[3];
+                    float M = m_use;
+#pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        o[i] = have[i] ? __ldcg(px[i].ml(row)) : make_float2(-INFINITY, 0.f);
+                        M = fmaxf(M, o[i].x);
+                    }
+                    const float Mu = M == -INFINITY ? 0.f : M;
+                    wo = ex2(m_use - Mu);
+                    l *= wo;
+#pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        w[i] = ex2(o[i].x - Mu);
+                        l += o[i].y * w[i];
+                    }
+                    m_use = M;
                 }
                 if (warp_on) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-                    const float io = wo * inv, ix = wx * inv;
+                    wo *= inv;
 #pragma unroll
                     for (int c = 0; c < D / 32; c++) {
-                        float o[32];
-                        ld32(to + (uint32_t)(c * 32), o);
-                        wait_ld();
-                        if (valid) {
+                        uint32_t u[16];
+                        ld16(to + (uint32_t)(c * 16), u);
+                        float o[16];
+                        float4 z[4];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
-                                float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                                if (exchange) z = __ldcg(px.o((c * 32 + e) / 4, row));
-                                o[e] = fmaf(z.x, ix, o[e] * io);
-                                o[e + 1] = fmaf(z.y, ix, o[e + 1] * io);
-                                o[e + 2] = fmaf(z.z, ix, o[e + 2] * io);
-                                o[e + 3] = fmaf(z.w, ix, o[e + 3] * io);
+                        for (int e = 0; e < 4; e++) z[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int i = 0; i < 3; i++) {
+                            if (!valid || w[i] == 0.f) continue;  // nothing seen there (O may not have been written)
+                            const float wi = w[i] * inv;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float4 q = __ldcg(px[i].o(hf * (D / 8) + c * 4 + e, row));
+                                z[e].x = fmaf(q.x, wi, z[e].x); z[e].y = fmaf(q.y, wi, z[e].y);
+                                z[e].z = fmaf(q.z, wi, z[e].z); z[e].w = fmaf(q.w, wi, z[e].w);
+                            }
+                        }
+                        wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            o[4 * e] = fmaf(__uint_as_float(u[4 * e]), wo, z[e].x);
+                            o[4 * e + 1] = fmaf(__uint_as_float(u[4 * e + 1]), wo, z[e].y);
+                            o[4 * e + 2] = fmaf(__uint_as_float(u[4 * e + 2]), wo, z[e].z);
+                            o[4 * e + 3] = fmaf(__uint_as_float(u[4 * e + 3]), wo, z[e].w);
+                        }
+                        if (valid) {
+                            if (l == 0.f) {  // saw nothing
+#pragma unroll
+                                for (int e = 0; e < 16; e++) o[e] = 0.f;
                             }
 #pragma unroll
-                            for (int e = 0; e < 32; e += 8)
-                                *reinterpret_cast<uint4 *>(orow + c * 32 + e) =
+                            for (int e = 0; e < 16; e += 8)
+                                *reinterpret_cast<uint4 *>(orow + c * 16 + e) =
                                     make_uint4(pack2(o[e], o[e + 1]), pack2(o[e + 2], o[e + 3]), pack2(o[e + 4], o[e + 5]),
                                                pack2(o[e + 6], o[e + 7]));
                         }
                     }
-                    if (valid && a.lse)
+                    if (valid && hf == 0 && a.lse)
                         a.lse[(size_t)grow * a.H + head] = l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994531f;
                 }
                 if (exchange) {
@@ -884,36 +1000,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
                 // a partial result: for the other slot, or for the CTAs that share the item
-                Part<D> pp = part_of<D>(a, cta, whole ? 2 : which, whole ? t : part);
-                if (whole) {
+                const Part<D> pp = part_of<D>(a, cta, closes ? 2 : which, closes ? t : part);
+                if (closes) {
                     ok = warp_wait(&sh.x_empty[t], ((uint32_t)nx[t] & 1u) ^ 1u, abort_flag, a.err);
                     if (!ok) break;
                     nx[t]++;
                 }
                 if (warp_on) {
 #pragma unroll
-                    for (int c = 0; c < D / 32; c++) {
+                    for (int c = 0; c < D / 64; c++) {
                         float o[32];
                         ld32(to + (uint32_t)(c * 32), o);
                         wait_ld();
                         if (valid) {
 #pragma unroll
                             for (int e = 0; e < 32; e += 4)
-                                __stcg(pp.o((c * 32 + e) / 4, row), make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                                __stcg(pp.o(hf * (D / 8) + (c * 32 + e) / 4, row), make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
                         }
                     }
-                    if (valid) __stcg(pp.ml(row), make_float2(m_use, l));
+                    if (valid && hf == 0) __stcg(pp.ml(row), make_float2(m_use, l));
                 }
-                if (whole) {
+                if (closes) {
                     __threadfence_block();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.x_full[t]);
+                } else if (two) {
+                    __threadfence();
+                    __syncwarp();
+                    if (lane == 0) red_release(arrived2);
                 }
             }
         }
-        // ---- items shared with other CTAs: every CTA joins a part of the rows once all pieces are there ----
+        // ---- items in three pieces and more: every CTA joins a part of the rows once all pieces are there ----
         const int tid = threadIdx.x - 128;
-        unsigned *arrived = reinterpret_cast<unsigned *>(a.workspace), *left = arrived + kCounterWords / 2;
+        unsigned *arrived = reinterpret_cast<unsigned *>(a.workspace), *left = arrived + 2 * kCounterWords;
         bar_softmax();
         if (tid < 2 && sh.shared[tid].on) {
             __threadfence();
@@ -998,6 +1118,6 @@ cudaError_t chunk_attn_tc_launch(const ChunkArgs &a, cudaStream_t st) {
     return a.d == 128 ? launch<128>(a, st) : launch<64>(a, st);
 }
 
-size_t chunk_attn_tc_workspace(int head_dim) { return kCounterWords * 4 + (size_t)kNumSMsB200 * 6 * part_bytes(head_dim); }
+size_t chunk_attn_tc_workspace(int head_dim) { return 3 * kCounterWords * 4 + (size_t)kNumSMsB200 * 6 * part_bytes(head_dim); }
 
 }  // namespace qw
