@@ -37,6 +37,7 @@ namespace {
 constexpr int kThreads = 640, kSoftThreads = 512, kRows = 128, kKeys = 128, kMaxStages = 5;
 constexpr float kRescale = 8.f;  // the running maximum is raised only when it grows by more than 2^8: p stays below 2^8
 constexpr int kPieces = 4;       // ring of pieces
+constexpr int kFewRows = 8;      // rows of an exchange in shared memory: a token's heads of one KV head
 constexpr int kMinShare = 5;     // units that a CTA beyond one per item is worth: splitting an item costs about as much
 constexpr int kCounterWords = 256;  // arrivals | departures | arrivals at items cut once, one word per CTA each
 
@@ -77,6 +78,8 @@ struct __align__(16) Smem {
         s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], done;
     uint32_t tmem;
     float mx[2][2][kRows], sum[2][2][kRows];  // [slot][half][row]
+    float4 xo[2][128 / 4 * kFewRows];  // [slot]: O as float4 columns of kFewRows rows (16-byte aligned by its type)
+    float2 xml[2][kFewRows];
     int abort, go;
     int empty;  // some rows stand before their sequence's first position
 };
@@ -211,6 +214,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// 32 bytes: a whole sector of a row per lane
+__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory"); }
 // The two warps that share 32 rows of a slot.  One whose wait ran out still arrives for the other, which may have seen
 // the wait end in time; that one's next wait needs the missing results and runs out too.
@@ -225,6 +234,18 @@ __device__ __forceinline__ void red_release(unsigned *p) {
     asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory");
 }
 __device__ __forceinline__ int uni(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+// whether a phase is over, without the pause of a wait
+__device__ __forceinline__ bool mbar_test(uint32_t addr, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // a bounded wait that ends the same way for every lane of the warp
 __device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag, int *err) {
     return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, err));
@@ -237,7 +258,8 @@ struct Part {
     __device__ __forceinline__ float4 *o(int c4, int row) const { return reinterpret_cast<float4 *>(p) + c4 * kRows + row; }
     __device__ __forceinline__ float2 *ml(int row) const { return reinterpret_cast<float2 *>(p + (size_t)kRows * D * 4) + row; }
 };
-// which: 0 the share's first piece, 1 its last, 2 the exchange between the slots; k: tile, or slot in turn
+// which: 0 the share's first piece, 1 its last, 2 the exchange between the slots (of more than kFewRows rows; fewer go
+// through shared memory); k: tile, or slot in turn
 template <int D>
 __device__ __forceinline__ Part<D> part_of(const ChunkArgs &a, int cta, int which, int k) {
     return Part<D>{(char *)a.workspace + 3 * kCounterWords * 4 + ((size_t)cta * 6 + which * 2 + k) * part_bytes(D)};
@@ -617,6 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int visits;           // so far: phase of p_full
                 bool first, one;      // first visit of the piece; single-tile piece
                 bool alone;           // the other slot has no visit in it
+                bool ready;           // the next block's keys have been seen
             };
             Slot sl[2];
             bool ok = true;
@@ -637,6 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     s.clo = uni(pc.clo);
                     s.chi = uni(pc.chi);
                     s.first = true;
+                    s.ready = false;
                     s.alone = nblk == 1;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.w_empty[s.np % kPieces]);
@@ -647,8 +671,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             // S_t = Q_t K^T of the slot's current visit into TMEM columns [128 t, 128 t + 128)
             auto issue_s = [&](Slot &s, int t) {
                 const int st = s.r % NST, qe = s.q & 1;
-                ok = warp_wait(&sh.q_full[qe], (uint32_t)(s.q >> 1) & 1u, abort_flag, a.err) &&
-                     warp_wait(&sh.k_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
+                if (s.first) ok = warp_wait(&sh.q_full[qe], (uint32_t)(s.q >> 1) & 1u, abort_flag, a.err);
+                if (ok && !s.ready) ok = warp_wait(&sh.k_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
                 if (!ok) return;
                 tc_fence_after();
                 const uint64_t da = dQ + (uint64_t)(qe * (TILE >> 4)), db = dK + (uint64_t)(st * (TILE >> 4));
@@ -685,6 +709,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
+                // (looked at now, so that S of the slot's next block follows this PV at once)
+                const int rn = s.r + s.step;
+                s.ready = s.left > 1 && __all_sync(0xffffffffu, mbar_test(smem_u32(&sh.k_full[rn % NST]), (uint32_t)(rn / NST) & 1u));
                 ok = warp_wait(&sh.p_full[t], (uint32_t)s.visits & 1u, abort_flag, a.err);
                 if (!ok) return;
                 tc_fence_after();
@@ -799,6 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool two = flags & kTwo, closes = whole || (two && (flags & kHead));
             const bool exchange = closes && !pair && nblk > 1;
             const bool finish = closes && (!exchange || ((alt + nblk - 1) & 1) == t);  // the slot of the last block
+            const bool few = rows <= kFewRows;  // (of a single tile)
             const int which = flags & kHead ? 1 : 0, part = pair ? t : jj;
             unsigned *arrived2 = reinterpret_cast<unsigned *>(a.workspace) + kCounterWords + (flags & kHead ? cta : cta - 1);
             if (mine <= 0) {
@@ -878,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l = l * alpha + (s0 + s1);
                     // this half of O's columns (the slot's PV before has completed: s_full came after it)
                     if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[16];
                             ld16(to + (uint32_t)(c * 16), o);
@@ -908,92 +936,94 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l += sh.sum[t][hf ^ 1][row];
             }
             if (finish) {
-                // the item's result, joined with the other slot's (of a single-tile item) and the other CTA's parts
-                float wo = 1.f, w[3] = {0.f, 0.f, 0.f};
-                const Part<D> px[3] = {part_of<D>(a, cta, 2, t ^ 1), part_of<D>(a, cta + 1, 0, pair ? t : 0), part_of<D>(a, cta + 1, 0, 1)};
-                const bool have[3] = {exchange, !whole, !whole && !pair};
-                if (exchange) {
-                    ok = warp_wait(&sh.x_full[t ^ 1], (uint32_t)nx[t ^ 1] & 1u, abort_flag, a.err);
-                    if (!ok) break;
-                    nx[t ^ 1]++;
-                }
-                if (!whole) {
-                    // all sixteen softmax warps of the other CTA
-                    if (lane == 0) {
-                        const uint64_t t0 = gtime_ns();
-                        while (ld_acquire(arrived2) < 16u && !*abort_flag)
-                            if (gtime_ns() - t0 > kTcuWaitCycles) {
-                                *abort_flag = 1;
-                                if (a.err) atomicExch(a.err, TC_DEVERR_TIMEOUT);
+                if (!exchange && whole) {
+                    // the item's result
+                    if (warp_on) {
+                        const float inv = l == 0.f ? 0.f : 1.f / l;
+                        float o[D / 2];
+#pragma unroll
+                        for (int c = 0; c < D / 64; c++) ld32(to + (uint32_t)(c * 32), o + c * 32);
+                        wait_ld();
+                        if (valid) {
+#pragma unroll
+                            for (int c = 0; c < D / 2; c += 16) {
+                                uint32_t pk[8];
+#pragma unroll
+                                for (int e = 0; e < 8; e++) pk[e] = pack2(o[c + 2 * e] * inv, o[c + 2 * e + 1] * inv);
+                                store32(orow + c, pk);
                             }
-                        // the last of the item's finishing warps leaves the counter as it was
-                        if (atomicAdd(arrived2, 0x100u) >> 8 == (pair ? 15u : 7u)) *arrived2 = 0u;
+                        }
                     }
-                    __syncwarp();
-                }
-                if (valid) {
-                    float2 o[3];
-                    float M = m_use;
-#pragma unroll
-                    for (int i = 0; i < 3; i++) {
-                        o[i] = have[i] ? __ldcg(px[i].ml(row)) : make_float2(-INFINITY, 0.f);
-                        M = fmaxf(M, o[i].x);
+                } else {
+                    // joined with the other slot's (of a single-tile item) and the other CTA's parts
+                    const Part<D> p0 = few ? Part<D>{nullptr} : part_of<D>(a, cta, 2, t ^ 1);
+                    const float4 *xo = few ? sh.xo[t ^ 1] + row : p0.o(0, row);
+                    const float2 *xml = few ? &sh.xml[t ^ 1][row & (kFewRows - 1)] : p0.ml(row);
+                    const int xs = few ? kFewRows : kRows;  // float4 columns lie this far apart
+                    const Part<D> p1 = part_of<D>(a, cta + 1, 0, pair ? t : 0), p2 = part_of<D>(a, cta + 1, 0, 1);
+                    if (exchange) {
+                        ok = warp_wait(&sh.x_full[t ^ 1], (uint32_t)nx[t ^ 1] & 1u, abort_flag, a.err);
+                        if (!ok) break;
+                        nx[t ^ 1]++;
                     }
-                    const float Mu = M == -INFINITY ? 0.f : M;
-                    wo = ex2(m_use - Mu);
-                    l *= wo;
-#pragma unroll
-                    for (int i = 0; i < 3; i++) {
-                        w[i] = ex2(o[i].x - Mu);
-                        l += o[i].y * w[i];
+                    if (!whole) {
+                        // all sixteen softmax warps of the other CTA
+                        if (lane == 0) {
+                            const uint64_t t0 = gtime_ns();
+                            while (ld_acquire(arrived2) < 16u && !*abort_flag)
+                                if (gtime_ns() - t0 > kTcuWaitCycles) {
+                                    *abort_flag = 1;
+                                    if (a.err) atomicExch(a.err, TC_DEVERR_TIMEOUT);
+                                }
+                            // the last of the item's finishing warps leaves the counter as it was
+                            if (atomicAdd(arrived2, 0x100u) >> 8 == (pair ? 15u : 7u)) *arrived2 = 0u;
+                        }
+                        __syncwarp();
                     }
-                    m_use = M;
-                }
-                if (warp_on) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    wo *= inv;
-#pragma unroll
-                    for (int c = 0; c < D / 32; c++) {
-                        uint32_t u[16];
-                        ld16(to + (uint32_t)(c * 16), u);
-                        float o[16];
-                        float4 z[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) z[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                        for (int i = 0; i < 3; i++) {
-                            if (!valid || w[i] == 0.f) continue;  // nothing seen there (O may not have been written)
-                            const float wi = w[i] * inv;
+                    if (warp_on) {
+                        const float2 none = make_float2(-INFINITY, 0.f);
+                        const float2 o0 = valid && exchange ? *xml : none, o1 = valid && !whole ? __ldcg(p1.ml(row)) : none,
+                                     o2 = valid && !whole && !pair ? __ldcg(p2.ml(row)) : none;
+                        const float M = fmaxf(fmaxf(m_use, o0.x), fmaxf(o1.x, o2.x)), Mu = M == -INFINITY ? 0.f : M;
+                        float wo = ex2(m_use - Mu), w0 = ex2(o0.x - Mu), w1 = ex2(o1.x - Mu), w2 = ex2(o2.x - Mu);
+                        l = l * wo + o0.y * w0 + o1.y * w1 + o2.y * w2;
+                        m_use = M;
+                        const float inv = l == 0.f ? 0.f : 1.f / l;
+                        wo *= inv; w0 *= inv; w1 *= inv; w2 *= inv;
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; c++) {
+                            uint32_t u[16];
+                            ld16(to + (uint32_t)(c * 16), u);
+                            const int c4 = hf * (D / 8) + c * 4;
+                            float4 q0[4], q1[4], q2[4];
+                            // a part of weight 0 saw nothing (its O may not have been written)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const float4 q = __ldcg(px[i].o(hf * (D / 8) + c * 4 + e, row));
-                                z[e].x = fmaf(q.x, wi, z[e].x); z[e].y = fmaf(q.y, wi, z[e].y);
-                                z[e].z = fmaf(q.z, wi, z[e].z); z[e].w = fmaf(q.w, wi, z[e].w);
+                                const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                                q0[e] = w0 != 0.f ? xo[(c4 + e) * xs] : z;
+                                q1[e] = w1 != 0.f ? __ldcg(p1.o(c4 + e, row)) : z;
+                                q2[e] = w2 != 0.f ? __ldcg(p2.o(c4 + e, row)) : z;
                             }
-                        }
-                        wait_ld();
+                            wait_ld();
+                            float o[16];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            o[4 * e] = fmaf(__uint_as_float(u[4 * e]), wo, z[e].x);
-                            o[4 * e + 1] = fmaf(__uint_as_float(u[4 * e + 1]), wo, z[e].y);
-                            o[4 * e + 2] = fmaf(__uint_as_float(u[4 * e + 2]), wo, z[e].z);
-                            o[4 * e + 3] = fmaf(__uint_as_float(u[4 * e + 3]), wo, z[e].w);
-                        }
-                        if (valid) {
-                            if (l == 0.f) {  // saw nothing
-#pragma unroll
-                                for (int e = 0; e < 16; e++) o[e] = 0.f;
+                            for (int e = 0; e < 4; e++) {
+                                o[4 * e] = __uint_as_float(u[4 * e]) * wo + q0[e].x * w0 + q1[e].x * w1 + q2[e].x * w2;
+                                o[4 * e + 1] = __uint_as_float(u[4 * e + 1]) * wo + q0[e].y * w0 + q1[e].y * w1 + q2[e].y * w2;
+                                o[4 * e + 2] = __uint_as_float(u[4 * e + 2]) * wo + q0[e].z * w0 + q1[e].z * w1 + q2[e].z * w2;
+                                o[4 * e + 3] = __uint_as_float(u[4 * e + 3]) * wo + q0[e].w * w0 + q1[e].w * w1 + q2[e].w * w2;
                             }
+                            if (valid) {
+                                uint32_t pk[8];
 #pragma unroll
-                            for (int e = 0; e < 16; e += 8)
-                                *reinterpret_cast<uint4 *>(orow + c * 16 + e) =
-                                    make_uint4(pack2(o[e], o[e + 1]), pack2(o[e + 2], o[e + 3]), pack2(o[e + 4], o[e + 5]),
-                                               pack2(o[e + 6], o[e + 7]));
+                                for (int e = 0; e < 8; e++) pk[e] = pack2(o[2 * e], o[2 * e + 1]);
+                                store32(orow + c * 16, pk);
+                            }
                         }
                     }
-                    if (valid && hf == 0 && a.lse)
-                        a.lse[(size_t)grow * a.H + head] = l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994531f;
                 }
+                if (valid && hf == 0 && a.lse)
+                    a.lse[(size_t)grow * a.H + head] = l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994531f;
                 if (exchange) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.x_empty[t ^ 1]);
@@ -1001,24 +1031,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
                 // a partial result: for the other slot, or for the CTAs that share the item
                 const Part<D> pp = part_of<D>(a, cta, closes ? 2 : which, closes ? t : part);
+                float4 *po = closes && few ? sh.xo[t] + row : pp.o(0, row);
+                const int ps = closes && few ? kFewRows : kRows;
                 if (closes) {
                     ok = warp_wait(&sh.x_empty[t], ((uint32_t)nx[t] & 1u) ^ 1u, abort_flag, a.err);
                     if (!ok) break;
                     nx[t]++;
                 }
                 if (warp_on) {
-#pragma unroll
-                    for (int c = 0; c < D / 64; c++) {
-                        float o[32];
-                        ld32(to + (uint32_t)(c * 32), o);
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t o[16];
+                        ld16(to + (uint32_t)(c * 16), o);
                         wait_ld();
                         if (valid) {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4)
-                                __stcg(pp.o(hf * (D / 8) + (c * 32 + e) / 4, row), make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                            for (int e = 0; e < 4; e++)
+                                reinterpret_cast<uint4 *>(po)[(hf * (D / 8) + c * 4 + e) * ps] =
+                                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                         }
                     }
-                    if (valid && hf == 0) __stcg(pp.ml(row), make_float2(m_use, l));
+                    if (valid && hf == 0) *(closes && few ? &sh.xml[t][row & (kFewRows - 1)] : pp.ml(row)) = make_float2(m_use, l);
                 }
                 if (closes) {
                     __threadfence_block();
