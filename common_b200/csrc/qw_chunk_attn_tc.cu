@@ -372,35 +372,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int *abort_flag = &sh.abort;
     const int G = a.G, P = kRows / G;
 
-    // ---- units of every sequence: an item costs its blocks and one more ----
-    if (threadIdx.x == 0) sh.empty = 0;
-    __syncthreads();
-    for (int b0 = warp * 32; b0 < a.batch; b0 += kThreads) {
-        const int b = b0 + lane;
-        Seq s{0, 0, 0};
-        if (b < a.batch) {
-            const int r0 = a.row_start[b], r1 = a.row_start[b + 1], kv = a.kv_len[b];
-            s.r0 = min(max(r0, 0), a.rows);
-            s.n = max(0, min(r1, a.rows) - s.r0);
-            s.kv = min(max(kv, 0), a.max_pages << a.log2_ps);
-            sh.seq[b] = s;
-            if (s.n > s.kv) sh.empty = 1;
-        }
-        const int items = (s.n + 2 * P - 1) / (2 * P);
-        unsigned units = 0;
-        if (items <= 4)
-            for (int i = 0; i < items; i++) units += make_item(s, i, P, a.window).units();
-        // long chunks: the whole warp on one sequence after the other
-        for (unsigned m = __ballot_sync(0xffffffffu, items > 4); m; m &= m - 1) {
-            const int l = __ffs(m) - 1;
-            const Seq t{__shfl_sync(0xffffffffu, s.n, l), __shfl_sync(0xffffffffu, s.kv, l), 0};
-            const int ni = __shfl_sync(0xffffffffu, items, l);
-            unsigned u = 0;
-            for (int i = lane; i < ni; i += 32) u += make_item(t, i, P, a.window).units();
-            u = __reduce_add_sync(0xffffffffu, u);
-            if (lane == l) units = u;
-        }
-        if (b < a.batch) sh.pre[b + 1] = units * a.Hkv;
+    // the scheduler's first lengths are on their way while the rest is set up
+    int len0 = 0, len1 = 0, len2 = 0;
+    if (warp == 3 && lane < a.batch) {
+        len0 = a.row_start[lane];
+        len1 = a.row_start[lane + 1];
+        len2 = a.kv_len[lane];
     }
     if (warp == 2 && lane == 0) {
         for (int i = 0; i < NST; i++) {
@@ -425,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_init(&sh.done, 1);
         sh.abort = 0;
+        sh.empty = 0;
         sh.pre[0] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmQ) : "memory");
@@ -446,17 +424,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 3) {
             // ---------------- the scheduler ----------------
+            // units of every sequence (an item costs its blocks and one more) and their running sum
             unsigned W = 0;
-            int items = 0;
+            int items = 0;  // that see something
             for (int b0 = 0; b0 < a.batch; b0 += 32) {
                 const int b = b0 + lane;
-                unsigned v = b < a.batch ? sh.pre[b + 1] : 0;
-                int ni = 0;  // items that see something
-                if (b < a.batch && sh.seq[b].kv > 0) {
-                    const Seq s = sh.seq[b];
-                    ni = (s.n + 2 * P - 1) / (2 * P) - max(0, s.n - s.kv) / (2 * P);
+                Seq s{0, 0, 0};
+                if (b < a.batch) {
+                    s.r0 = min(max(len0, 0), a.rows);
+                    s.n = max(0, min(len1, a.rows) - s.r0);
+                    s.kv = min(max(len2, 0), a.max_pages << a.log2_ps);
+                    sh.seq[b] = s;
                 }
-                items += __reduce_add_sync(0xffffffffu, ni * a.Hkv);
+                if (b + 32 < a.batch) {
+                    len0 = a.row_start[b + 32];
+                    len1 = a.row_start[b + 33];
+                    len2 = a.kv_len[b + 32];
+                }
+                if (s.n > s.kv) sh.empty = 1;
+                const int ni = s.n <= 2 * P ? s.n > 0 : (s.n + 2 * P - 1) / (2 * P);
+                unsigned units = 0;
+                if (ni <= 2)
+                    for (int i = 0; i < ni; i++) units += make_item(s, i, P, a.window).units();
+                // long chunks: the whole warp on one sequence after the other
+                for (unsigned m = __ballot_sync(0xffffffffu, ni > 2); m; m &= m - 1) {
+                    const int l = __ffs(m) - 1;
+                    const Seq t{__shfl_sync(0xffffffffu, s.n, l), __shfl_sync(0xffffffffu, s.kv, l), 0};
+                    const int n = __shfl_sync(0xffffffffu, ni, l);
+                    unsigned u = 0;
+                    for (int i = lane; i < n; i += 32) u += make_item(t, i, P, a.window).units();
+                    u = __reduce_add_sync(0xffffffffu, u);
+                    if (lane == l) units = u;
+                }
+                const int gone = s.n > s.kv ? (s.n - s.kv) / (2 * P) : 0;  // items before the first position
+                items += __reduce_add_sync(0xffffffffu, s.kv > 0 ? (ni - gone) * a.Hkv : 0);
+                unsigned v = units * a.Hkv;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const unsigned w = __shfl_up_sync(0xffffffffu, v, o);
@@ -473,23 +475,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             int b = 0, h = 0, i = 0, off = 0;
             if (cta < Ge) {  // Ge <= W: an item has two units at least
                 line.q = W / Ge;
-                line.rem = W % Ge;
+                line.rem = W - line.q * Ge;
                 at = line.start(cta);
                 end = line.start(cta + 1);
-                int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before the share
-                while (lo < hi) {
-                    const int mid = (lo + hi + 1) >> 1;
-                    if (sh.pre[mid] <= at) lo = mid;
-                    else hi = mid - 1;
+                unsigned rem = 0, per = 1;
+                for (int b0 = 0; b0 < a.batch; b0 += 32) {  // the sequence that holds unit `at`
+                    const unsigned p0 = b0 + lane < a.batch ? sh.pre[b0 + lane] : 0xffffffffu;
+                    const unsigned p1 = b0 + lane < a.batch ? sh.pre[b0 + lane + 1] : 0xffffffffu;
+                    const unsigned m = __ballot_sync(0xffffffffu, p0 <= at && at < p1);
+                    if (m) {
+                        const int l = __ffs(m) - 1;
+                        b = b0 + l;
+                        rem = at - __shfl_sync(0xffffffffu, p0, l);
+                        per = __shfl_sync(0xffffffffu, p1 - p0, l) / a.Hkv;
+                        break;
+                    }
                 }
-                b = lo;
-                const unsigned per = (sh.pre[lo + 1] - sh.pre[lo]) / a.Hkv;
-                unsigned rem = at - sh.pre[lo];
-                h = (int)(rem / per);
-                rem -= h * per;
-                const Seq s = sh.seq[lo];
+                if (rem >= per) {
+                    h = (int)(rem / per);
+                    rem -= h * per;
+                }
+                const Seq s = sh.seq[b];
                 for (; i * 2 * P < s.n; i += 32) {  // the item that holds unit rem of this head
                     unsigned v = (i + lane) * 2 * P < s.n ? make_item(s, i + lane, P, a.window).units() : 0;
+                    if (s.n <= 2 * P) {  // the only one
+                        off = (int)rem;
+                        break;
+                    }
                     const unsigned mine = v;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
@@ -553,8 +565,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     pc.lo = it.klo; pc.hi = it.pl;
                     pc.clo = a.window ? max(0, s.kv - s.n - a.window + 1) : 0;
                     pc.chi = s.kv;
-                    const int c0 = pc.flags & kHead ? cta : (int)line.owner(u0);
-                    const int ni = pc.flags & kWhole ? 1 : (int)line.owner(u0 + it.nb - 1) - c0 + 1;
+                    // the CTAs that the item lies in: mostly this one and its neighbour
+                    int c0 = cta, ni = 1;
+                    if (!(pc.flags & kWhole)) {
+                        if (!(pc.flags & kHead)) c0 = u0 >= line.start(cta - 1) ? cta - 1 : (int)line.owner(u0);
+                        const unsigned last = u0 + it.nb - 1;
+                        const int c1 = last < line.start(cta + 1) ? cta : last < line.start(cta + 2) ? cta + 1 : (int)line.owner(last);
+                        ni = c1 - c0 + 1;
+                    }
                     if (ni == 2) pc.flags |= kTwo;
                     if (ni > 2 && lane == 0) {
                         Shared &m = sh.shared[pc.flags & kHead ? 1 : 0];
@@ -786,21 +804,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rpos = row / G, rhead = row % G;
         const uint32_t trow = tmem + ((uint32_t)(qq * 32) << 16);
         const uint32_t ts = trow + (uint32_t)(t * kKeys + hf * 64), to = trow + 256u + (uint32_t)(t * 128 + hf * (D / 2));
-        if (sh.empty) {
-            // rows of items whose every row stands before the first position
-            for (int b = 0; b < a.batch; b++) {
-                const Seq s = sh.seq[b];
-                const int before = s.n - s.kv;
-                if (before <= 0) continue;
-                const int rows = s.kv == 0 ? s.n : before / (2 * P) * 2 * P;
-                const int vec = a.H * D / 8;
-                for (int e = blockIdx.x * kSoftThreads + threadIdx.x - 128; e < rows * vec; e += gridDim.x * kSoftThreads) {
-                    const int r = s.r0 + e / vec, c = e % vec * 8;
-                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)r * a.ld_out + c) = make_uint4(0, 0, 0, 0);
-                    if (a.lse && c % D == 0) a.lse[(size_t)r * a.H + c / D] = -INFINITY;
-                }
-            }
-        }
         int nv = 0, no = 0, nx[2] = {0, 0};  // visits, pieces with visits, exchanges by writing slot
         bool ok = true;
         for (int np = 0; ok; np++) {
@@ -826,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool two = flags & kTwo, closes = whole || (two && (flags & kHead));
             const bool exchange = closes && !pair && nblk > 1;
             const bool finish = closes && (!exchange || ((alt + nblk - 1) & 1) == t);  // the slot of the last block
-            const bool few = rows <= kFewRows;  // (of a single tile)
+            const bool few = !pair && rows <= kFewRows;
             const int which = flags & kHead ? 1 : 0, part = pair ? t : jj;
             unsigned *arrived2 = reinterpret_cast<unsigned *>(a.workspace) + kCounterWords + (flags & kHead ? cta : cta - 1);
             if (mine <= 0) {
@@ -935,6 +938,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bar_pair(pair_id);
                 l += sh.sum[t][hf ^ 1][row];
             }
+            auto put_few = [&](int slot) {  // this half of O's columns of the valid rows
+                float o[D / 2];
+#pragma unroll
+                for (int c = 0; c < D / 64; c++) ld32(to + (uint32_t)(c * 32), o + c * 32);
+                wait_ld();
+                if (valid) {
+#pragma unroll
+                    for (int c = 0; c < D / 8; c++)
+                        sh.xo[slot][(hf * (D / 8) + c) * kFewRows + row] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                }
+                __syncwarp();
+            };
             if (finish) {
                 if (!exchange && whole) {
                     // the item's result
@@ -956,11 +971,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 } else {
                     // joined with the other slot's (of a single-tile item) and the other CTA's parts
-                    const Part<D> p0 = few ? Part<D>{nullptr} : part_of<D>(a, cta, 2, t ^ 1);
-                    const float4 *xo = few ? sh.xo[t ^ 1] + row : p0.o(0, row);
-                    const float2 *xml = few ? &sh.xml[t ^ 1][row & (kFewRows - 1)] : p0.ml(row);
-                    const int xs = few ? kFewRows : kRows;  // float4 columns lie this far apart
-                    const Part<D> p1 = part_of<D>(a, cta + 1, 0, pair ? t : 0), p2 = part_of<D>(a, cta + 1, 0, 1);
+                    const Part<D> p0 = part_of<D>(a, cta, 2, t ^ 1), p1 = part_of<D>(a, cta + 1, 0, pair ? t : 0), p2 = part_of<D>(a, cta + 1, 0, 1);
+                    if (few) {  // this slot's own O beside the other's
+                        ok = warp_wait(&sh.x_empty[t], ((uint32_t)nx[t] & 1u) ^ 1u, abort_flag, a.err);
+                        if (!ok) break;
+                        if (warp_on) put_few(t);
+                    }
                     if (exchange) {
                         ok = warp_wait(&sh.x_full[t ^ 1], (uint32_t)nx[t ^ 1] & 1u, abort_flag, a.err);
                         if (!ok) break;
@@ -980,9 +996,47 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         __syncwarp();
                     }
-                    if (warp_on) {
-                        const float2 none = make_float2(-INFINITY, 0.f);
-                        const float2 o0 = valid && exchange ? *xml : none, o1 = valid && !whole ? __ldcg(p1.ml(row)) : none,
+                    const float2 none = make_float2(-INFINITY, 0.f);
+                    if (few) {
+                        if (warp_on) {
+                            // few rows: every lane takes one of them and some columns of it
+                            const int r = lane & (kFewRows - 1), src = min(r, rows - 1);
+                            const float2 own = make_float2(__shfl_sync(0xffffffffu, m_use, src), __shfl_sync(0xffffffffu, l, src));
+                            const float2 o0 = exchange ? sh.xml[t ^ 1][src] : none, o1 = whole ? none : __ldcg(p1.ml(src)),
+                                         o2 = whole ? none : __ldcg(p2.ml(src));
+                            const float M = fmaxf(fmaxf(own.x, o0.x), fmaxf(o1.x, o2.x)), Mu = M == -INFINITY ? 0.f : M;
+                            float wo = ex2(own.x - Mu), w0 = ex2(o0.x - Mu), w1 = ex2(o1.x - Mu), w2 = ex2(o2.x - Mu);
+                            l = own.y * wo + o0.y * w0 + o1.y * w1 + o2.y * w2;
+                            m_use = M;
+                            const float inv = l == 0.f ? 0.f : 1.f / l;
+                            wo *= inv; w0 *= inv; w1 *= inv; w2 *= inv;
+                            const int rg = __shfl_sync(0xffffffffu, grow, src), rh = __shfl_sync(0xffffffffu, head, src);
+                            __nv_bfloat16 *to_row = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)rg * a.ld_out + (size_t)rh * D;
+                            float4 q[4][D / 32];
+#pragma unroll
+                            for (int c = 0; c < D / 32; c++) {
+                                const int c4 = hf * (D / 8) + (lane >> 3) + 4 * c;
+                                const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                                q[0][c] = sh.xo[t][c4 * kFewRows + src];
+                                q[1][c] = exchange ? sh.xo[t ^ 1][c4 * kFewRows + src] : z;
+                                // (a part of weight 0 saw nothing: its O may not have been written)
+                                q[2][c] = w1 != 0.f ? __ldcg(p1.o(c4, src)) : z;
+                                q[3][c] = w2 != 0.f ? __ldcg(p2.o(c4, src)) : z;
+                            }
+                            if (r < rows) {
+#pragma unroll
+                                for (int c = 0; c < D / 32; c++) {
+                                    const float4 o = make_float4(q[0][c].x * wo + q[1][c].x * w0 + q[2][c].x * w1 + q[3][c].x * w2,
+                                                                 q[0][c].y * wo + q[1][c].y * w0 + q[2][c].y * w1 + q[3][c].y * w2,
+                                                                 q[0][c].z * wo + q[1][c].z * w0 + q[2][c].z * w1 + q[3][c].z * w2,
+                                                                 q[0][c].w * wo + q[1][c].w * w0 + q[2][c].w * w1 + q[3][c].w * w2);
+                                    const int c4 = hf * (D / 8) + (lane >> 3) + 4 * c;
+                                    *reinterpret_cast<uint2 *>(to_row + c4 * 4) = make_uint2(pack2(o.x, o.y), pack2(o.z, o.w));
+                                }
+                            }
+                        }
+                    } else if (warp_on) {
+                        const float2 o0 = valid && exchange ? __ldcg(p0.ml(row)) : none, o1 = valid && !whole ? __ldcg(p1.ml(row)) : none,
                                      o2 = valid && !whole && !pair ? __ldcg(p2.ml(row)) : none;
                         const float M = fmaxf(fmaxf(m_use, o0.x), fmaxf(o1.x, o2.x)), Mu = M == -INFINITY ? 0.f : M;
                         float wo = ex2(m_use - Mu), w0 = ex2(o0.x - Mu), w1 = ex2(o1.x - Mu), w2 = ex2(o2.x - Mu);
@@ -1000,7 +1054,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                                q0[e] = w0 != 0.f ? xo[(c4 + e) * xs] : z;
+                                q0[e] = w0 != 0.f ? __ldcg(p0.o(c4 + e, row)) : z;
                                 q1[e] = w1 != 0.f ? __ldcg(p1.o(c4 + e, row)) : z;
                                 q2[e] = w2 != 0.f ? __ldcg(p2.o(c4 + e, row)) : z;
                             }
@@ -1031,14 +1085,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
                 // a partial result: for the other slot, or for the CTAs that share the item
                 const Part<D> pp = part_of<D>(a, cta, closes ? 2 : which, closes ? t : part);
-                float4 *po = closes && few ? sh.xo[t] + row : pp.o(0, row);
-                const int ps = closes && few ? kFewRows : kRows;
                 if (closes) {
                     ok = warp_wait(&sh.x_empty[t], ((uint32_t)nx[t] & 1u) ^ 1u, abort_flag, a.err);
                     if (!ok) break;
                     nx[t]++;
                 }
-                if (warp_on) {
+                if (warp_on && closes && few) {
+                    put_few(t);
+                    if (valid && hf == 0) sh.xml[t][row] = make_float2(m_use, l);
+                } else if (warp_on) {
 #pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
                         uint32_t o[16];
@@ -1047,11 +1102,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (valid) {
 #pragma unroll
                             for (int e = 0; e < 4; e++)
-                                reinterpret_cast<uint4 *>(po)[(hf * (D / 8) + c * 4 + e) * ps] =
+                                *reinterpret_cast<uint4 *>(pp.o(hf * (D / 8) + c * 4 + e, row)) =
                                     make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                         }
                     }
-                    if (valid && hf == 0) *(closes && few ? &sh.xml[t][row & (kFewRows - 1)] : pp.ml(row)) = make_float2(m_use, l);
+                    if (valid && hf == 0) *pp.ml(row) = make_float2(m_use, l);
                 }
                 if (closes) {
                     __threadfence_block();
@@ -1061,6 +1116,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __threadfence();
                     __syncwarp();
                     if (lane == 0) red_release(arrived2);
+                }
+            }
+        }
+        if (sh.empty) {
+            // rows of items whose every row stands before the first position
+            for (int b = 0; b < a.batch; b++) {
+                const Seq s = sh.seq[b];
+                const int before = s.n - s.kv;
+                if (before <= 0) continue;
+                const int rows = s.kv == 0 ? s.n : before / (2 * P) * 2 * P;
+                const int vec = a.H * D / 8;
+                for (int e = blockIdx.x * kSoftThreads + threadIdx.x - 128; e < rows * vec; e += gridDim.x * kSoftThreads) {
+                    const int r = s.r0 + e / vec, c = e % vec * 8;
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)r * a.ld_out + c) = make_uint4(0, 0, 0, 0);
+                    if (a.lse && c % D == 0) a.lse[(size_t)r * a.H + c / D] = -INFINITY;
                 }
             }
         }
