@@ -76,11 +76,15 @@ struct CompactArgs {
     int rope_len;
 };
 
-// One warp per (kept row, layer): the row of every head, keys turned back, values as they are.
-template <typename T>
-__global__ void __launch_bounds__(kCompactThreads) qw_kv_compact_kernel(const CompactArgs a) {
-    const int r = blockIdx.x * (kCompactThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= a.rows) return;
+// where a kept row lies and where it goes, as element offsets within one layer and head 0
+struct RowMove {
+    long long from, to;
+    int delta;  // positions it moves down; -1: nothing to do
+};
+
+__device__ __forceinline__ RowMove row_move(const CompactArgs &a, int r) {
+    RowMove m{0, 0, -1};
+    if (r >= a.rows) return m;
     // the sequence that row r belongs to: the last b with keep_start[b] <= r
     int lo = 0, hi = a.batch - 1;
     while (lo < hi) {
@@ -89,36 +93,127 @@ __global__ void __launch_bounds__(kCompactThreads) qw_kv_compact_kernel(const Co
         else hi = mid - 1;
     }
     const int i = r - a.keep_start[lo];
-    if (i < 0 || r >= a.keep_start[lo + 1]) return;
+    if (i < 0 || r >= a.keep_start[lo + 1]) return m;
     const int come = a.keep[r], to = (a.dst_base ? a.dst_base[lo] : 0) + i;
     const int cp = come >> a.log2_ps, tp = to >> a.log2_ps;
-    if (come < 0 || to < 0 || cp >= a.max_pages || tp >= a.max_pages) return;
+    if (come < 0 || to < 0 || cp >= a.max_pages || tp >= a.max_pages) return m;
     const int sp = a.src_table[(size_t)lo * a.max_pages + cp], dp = a.dst_table[(size_t)lo * a.max_pages + tp];
-    if ((unsigned)sp >= (unsigned)a.num_pages || (unsigned)dp >= (unsigned)a.num_pages) return;
-    const int layer = blockIdx.y, d = a.d, half = d / 2, hv = half / 8;
-    const size_t head_elems = (size_t)a.ps * d;
-    const size_t from = ((size_t)layer * a.num_pages + sp) * a.heads * head_elems + (size_t)(come & (a.ps - 1)) * d;
-    const size_t dest = ((size_t)layer * a.num_pages + dp) * a.heads * head_elems + (size_t)(to & (a.ps - 1)) * d;
-    T *k = reinterpret_cast<T *>(a.k), *v = reinterpret_cast<T *>(a.v);
-    const int delta = come - to;
-    const bool turn = a.rope && delta > 0 && delta < a.rope_len;
-    for (int u = lane; u < a.heads * hv; u += 32) {
-        const int h = u / hv, c = (u % hv) * 8;
-        const T *p = k + from + h * head_elems + c;
-        T *o = k + dest + h * head_elems + c;
-        float x[8], y[8];
-        load8(p, x);
-        load8(p + half, y);
-        if (turn) turn_back(x, y, a.rope + (size_t)delta * half + c);
-        put8(o, x);
-        put8(o + half, y);
-        const T *pv = v + from + h * head_elems + c;
-        T *ov = v + dest + h * head_elems + c;
-        load8(pv, x);
-        load8(pv + half, y);
-        put8(ov, x);
-        put8(ov + half, y);
+    if ((unsigned)sp >= (unsigned)a.num_pages || (unsigned)dp >= (unsigned)a.num_pages) return m;
+    const long long page = (long long)a.heads * a.ps * a.d;
+    m.from = sp * page + (long long)(come & (a.ps - 1)) * a.d;
+    m.to = dp * page + (long long)(to & (a.ps - 1)) * a.d;
+    m.delta = max(0, come - to);
+    return m;
+}
+
+// 8 elements as they lie in memory
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16> &r, float (&v)[8]) {
+    const uint4 u = r.v[0];
+    v[0] = bf16lo(u.x); v[1] = bf16hi(u.x); v[2] = bf16lo(u.y); v[3] = bf16hi(u.y);
+    v[4] = bf16lo(u.z); v[5] = bf16hi(u.z); v[6] = bf16lo(u.w); v[7] = bf16hi(u.w);
+}
+__device__ __forceinline__ void unpack8(const Raw8<float> &r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        v[4 * i] = __uint_as_float(r.v[i].x); v[4 * i + 1] = __uint_as_float(r.v[i].y);
+        v[4 * i + 2] = __uint_as_float(r.v[i].z); v[4 * i + 3] = __uint_as_float(r.v[i].w);
     }
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw(const T *p) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.v[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_raw(T *p, const Raw8<T> &r) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(p)[i] = r.v[i];
+}
+
+// One CTA per (64 kept rows, layer).  The rows' places are looked up once; a warp then takes a head at a time: its 64 rows
+// are one contiguous piece of a destination page (mostly of a source page too).  A lane takes 8 elements of a row's first
+// half and the matching 8 of its second (the rotary pairs), HV lanes a row, and has U rows of keys and values on the way.
+template <typename T, int HV, int U>
+__global__ void __launch_bounds__(kCompactThreads, 2) qw_kv_compact_kernel(const CompactArgs a) {
+    constexpr int ROWS = 64, STEP = 32 / HV, HALF = HV * 8;
+    __shared__ RowMove moves[ROWS];
+    for (int i = threadIdx.x; i < ROWS; i += blockDim.x) moves[i] = row_move(a, blockIdx.x * ROWS + i);
+    __syncthreads();
+    const int lane = threadIdx.x & 31, c = (lane % HV) * 8;
+    const size_t layer = (size_t)blockIdx.y * a.num_pages * a.heads * a.ps * a.d, head = (size_t)a.ps * a.d;
+    for (int h = threadIdx.x >> 5; h < a.heads; h += blockDim.x >> 5) {
+        T *k = reinterpret_cast<T *>(a.k) + layer + h * head + c, *v = reinterpret_cast<T *>(a.v) + layer + h * head + c;
+        for (int r0 = lane / HV; r0 < ROWS; r0 += U * STEP) {
+            Raw8<T> q[U][4];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const RowMove &m = moves[r0 + u * STEP];
+                if (m.delta < 0) continue;
+                q[u][0] = load_raw(k + m.from);
+                q[u][1] = load_raw(k + m.from + HALF);
+                q[u][2] = load_raw(v + m.from);
+                q[u][3] = load_raw(v + m.from + HALF);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const RowMove &m = moves[r0 + u * STEP];
+                if (m.delta < 0) continue;
+                store_raw(v + m.to, q[u][2]);
+                store_raw(v + m.to + HALF, q[u][3]);
+                if (a.rope && m.delta > 0 && m.delta < a.rope_len) {
+                    float x[8], y[8];
+                    unpack8(q[u][0], x);
+                    unpack8(q[u][1], y);
+                    turn_back(x, y, a.rope + (size_t)m.delta * HALF + c);
+                    put8(k + m.to, x);
+                    put8(k + m.to + HALF, y);
+                } else {
+                    store_raw(k + m.to, q[u][0]);
+                    store_raw(k + m.to + HALF, q[u][1]);
+                }
+            }
+        }
+    }
+}
+
+// Head sizes other than 64 and 128: one warp per (kept row, layer).
+template <typename T>
+__global__ void __launch_bounds__(kCompactThreads) qw_kv_compact_any_kernel(const CompactArgs a) {
+    const RowMove m = row_move(a, blockIdx.x * (kCompactThreads / 32) + (threadIdx.x >> 5));
+    if (m.delta < 0) return;
+    const int lane = threadIdx.x & 31, half = a.d / 2, hv = half / 8;
+    const size_t layer = (size_t)blockIdx.y * a.num_pages * a.heads * a.ps * a.d, head = (size_t)a.ps * a.d;
+    T *k = reinterpret_cast<T *>(a.k) + layer, *v = reinterpret_cast<T *>(a.v) + layer;
+    const bool turn = a.rope && m.delta > 0 && m.delta < a.rope_len;
+    for (int u = lane; u < a.heads * hv; u += 32) {
+        const size_t at = (u / hv) * head + (u % hv) * 8;
+        float x[8], y[8], vx[8], vy[8];
+        load8(k + m.from + at, x);
+        load8(k + m.from + at + half, y);
+        load8(v + m.from + at, vx);
+        load8(v + m.from + at + half, vy);
+        if (turn) turn_back(x, y, a.rope + (size_t)m.delta * half + (u % hv) * 8);
+        put8(k + m.to + at, x);
+        put8(k + m.to + at + half, y);
+        put8(v + m.to + at, vx);
+        put8(v + m.to + at + half, vy);
+    }
+}
+
+template <typename T>
+void compact_launch(const CompactArgs &a, cudaStream_t st) {
+    constexpr int U = sizeof(T) == 2 ? 4 : 2;
+    const int threads = 32 * (a.heads < kCompactThreads / 32 ? a.heads : kCompactThreads / 32);
+    if (a.d == 128)
+        qw_kv_compact_kernel<T, 8, U><<<dim3((a.rows + 63) / 64, a.layers), threads, 0, st>>>(a);
+    else if (a.d == 64)
+        qw_kv_compact_kernel<T, 4, U><<<dim3((a.rows + 63) / 64, a.layers), threads, 0, st>>>(a);
+    else
+        qw_kv_compact_any_kernel<T><<<dim3((a.rows + kCompactThreads / 32 - 1) / (kCompactThreads / 32), a.layers),
+                                      kCompactThreads, 0, st>>>(a);
 }
 
 int log2_exact(int x) {
@@ -177,10 +272,8 @@ extern "C" qw_status qw_op_kv_compact(const qw_kv_pool *pool, const int32_t *src
     a.src_table = src_table; a.dst_table = dst_table; a.max_pages = max_pages;
     a.keep = keep; a.keep_start = keep_start; a.dst_base = dst_base; a.batch = batch; a.rows = rows;
     a.rope = (const float2 *)rope; a.rope_len = rope_len;
-    const int per = kCompactThreads / 32;
-    const dim3 grid((rows + per - 1) / per, pool->layers);
-    if (pool->dtype == QW_DTYPE_F32) qw_kv_compact_kernel<float><<<grid, kCompactThreads, 0, (cudaStream_t)stream>>>(a);
-    else qw_kv_compact_kernel<__nv_bfloat16><<<grid, kCompactThreads, 0, (cudaStream_t)stream>>>(a);
+    if (pool->dtype == QW_DTYPE_F32) compact_launch<float>(a, (cudaStream_t)stream);
+    else compact_launch<__nv_bfloat16>(a, (cudaStream_t)stream);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return op_fail(QW_ERR_CUDA, std::string("compaction launch: ") + cudaGetErrorString(e));
     return QW_OK;
