@@ -15,7 +15,7 @@ namespace qw {
 namespace {
 
 constexpr int kCopyThreads = 256;
-constexpr int kCompactThreads = 256;
+constexpr int kCompactThreads = 256, kCompactRows = 32;
 
 // One CTA per (page pair, layer, K or V, head): rows [0, n) of the head are contiguous in both pages.
 __global__ void __launch_bounds__(kCopyThreads)
@@ -133,12 +133,12 @@ __device__ __forceinline__ void store_raw(T *p, const Raw8<T> &r) {
     for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(p)[i] = r.v[i];
 }
 
-// One CTA per (64 kept rows, layer).  The rows' places are looked up once; a warp then takes a head at a time: its 64 rows
+// One CTA per (kCompactRows kept rows, layer).  The rows' places are looked up once; a warp then takes a head at a time: its rows
 // are one contiguous piece of a destination page (mostly of a source page too).  A lane takes 8 elements of a row's first
 // half and the matching 8 of its second (the rotary pairs), HV lanes a row, and has U rows of keys and values on the way.
 template <typename T, int HV, int U>
 __global__ void __launch_bounds__(kCompactThreads, 2) qw_kv_compact_kernel(const CompactArgs a) {
-    constexpr int ROWS = 64, STEP = 32 / HV, HALF = HV * 8;
+    constexpr int ROWS = kCompactRows, STEP = 32 / HV, HALF = HV * 8;
     __shared__ RowMove moves[ROWS];
     for (int i = threadIdx.x; i < ROWS; i += blockDim.x) moves[i] = row_move(a, blockIdx.x * ROWS + i);
     __syncthreads();
@@ -208,9 +208,9 @@ void compact_launch(const CompactArgs &a, cudaStream_t st) {
     constexpr int U = sizeof(T) == 2 ? 4 : 2;
     const int threads = 32 * (a.heads < kCompactThreads / 32 ? a.heads : kCompactThreads / 32);
     if (a.d == 128)
-        qw_kv_compact_kernel<T, 8, U><<<dim3((a.rows + 63) / 64, a.layers), threads, 0, st>>>(a);
+        qw_kv_compact_kernel<T, 8, U><<<dim3((a.rows + kCompactRows - 1) / kCompactRows, a.layers), threads, 0, st>>>(a);
     else if (a.d == 64)
-        qw_kv_compact_kernel<T, 4, U><<<dim3((a.rows + 63) / 64, a.layers), threads, 0, st>>>(a);
+        qw_kv_compact_kernel<T, 4, U><<<dim3((a.rows + kCompactRows - 1) / kCompactRows, a.layers), threads, 0, st>>>(a);
     else
         qw_kv_compact_any_kernel<T><<<dim3((a.rows + kCompactThreads / 32 - 1) / (kCompactThreads / 32), a.layers),
                                       kCompactThreads, 0, st>>>(a);
