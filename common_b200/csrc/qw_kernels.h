@@ -38,6 +38,8 @@ cudaError_t qk_sumsq_launch(const float *qkv, int ld, int qw, int kw, int B, flo
 cudaError_t hold_launch(unsigned long long ns, cudaStream_t st);
 cudaError_t add_launch(float *out, const float *a, const float *b, size_t n, cudaStream_t st);
 cudaError_t zero_launch(float *out, size_t n, cudaStream_t st);  // programmatically launched; memset when unaligned
+// out[i] = x[row[i]] (+ part[row[i]]) for rows of D floats (a multiple of 4); row[i] < 0 leaves out[i] as it is
+cudaError_t gather_rows_launch(float *out, const float *x, const float *part, const int *row, int n, int D, cudaStream_t st);
 cudaError_t swiglu_rows_launch(float *gu, int T, int F, __nv_bfloat16 *h, cudaStream_t st);  // zeroes gu after reading
 
 struct NormRowsArgs {

@@ -190,4 +190,22 @@ cudaError_t hold_launch(unsigned long long ns, cudaStream_t st) {
     return cudaGetLastError();
 }
 
+__global__ void qw_gather_rows_kernel(float *out, const float *x, const float *part, const int *row, int D) {
+    const int r = row[blockIdx.x];
+    if (r < 0) return;
+    for (int i = threadIdx.x * 4; i < D; i += blockDim.x * 4) {
+        float4 v = *reinterpret_cast<const float4 *>(x + (size_t)r * D + i);
+        if (part) {
+            const float4 p = *reinterpret_cast<const float4 *>(part + (size_t)r * D + i);
+            v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+        }
+        *reinterpret_cast<float4 *>(out + (size_t)blockIdx.x * D + i) = v;
+    }
+}
+
+cudaError_t gather_rows_launch(float *out, const float *x, const float *part, const int *row, int n, int D, cudaStream_t st) {
+    qw_gather_rows_kernel<<<n, 256, 0, st>>>(out, x, part, row, D);
+    return cudaGetLastError();
+}
+
 }  // namespace qw

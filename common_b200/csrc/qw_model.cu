@@ -21,6 +21,7 @@
 #include "qw_ops.h"
 #include "qw_tc.h"
 #include "qw_ar.h"
+#include "qw_chunk_attn.h"
 
 using namespace qw;
 
@@ -71,6 +72,9 @@ struct qw_model {
     int *d_page_table = nullptr;
     std::vector<int> h_page_table, free_pages;
     std::vector<std::vector<int>> slot_pages;
+    std::vector<int> page_refs;  // slots that hold each page
+    int *d_cache = nullptr;      // arguments of the page operators and of qw_extend (cache_words)
+    void *chunk_ws = nullptr;    // workspace of the chunk attention (qw_extend)
     // activations
     int T = 0, B = 0, maxsplit = 64;
     float *xa = nullptr, *xb = nullptr, *part = nullptr, *qkv = nullptr, *attn = nullptr, *hbuf = nullptr;
@@ -316,6 +320,17 @@ qw_status place(qw_model *m, const Target &t, const void *src, int src_dtype, in
 // ------------------------------------------------------------------------------------------
 // paged KV
 // ------------------------------------------------------------------------------------------
+int take_page(qw_model *m) {
+    const int pg = m->free_pages.back();
+    m->free_pages.pop_back();
+    m->page_refs[pg] = 1;
+    return pg;
+}
+
+void drop_page(qw_model *m, int pg) {
+    if (--m->page_refs[pg] == 0) m->free_pages.push_back(pg);
+}
+
 qw_status reserve_pages(qw_model *m, int slot, int npos) {
     if (slot < 0 || slot >= m->B) return fail(m, QW_ERR_ARG, "slot %d out of range [0,%d)", slot, m->B);
     if (npos > m->c.seq_len) return fail(m, QW_ERR_SHAPE, "position %d beyond seq_len %d", npos, m->c.seq_len);
@@ -327,8 +342,7 @@ qw_status reserve_pages(qw_model *m, int slot, int npos) {
         return fail(m, QW_ERR_OOM, "KV cache exhausted: slot %d needs %d more pages, %zu free", slot, need - have,
                     m->free_pages.size());
     for (int i = have; i < need; i++) {
-        int pg = m->free_pages.back();
-        m->free_pages.pop_back();
+        int pg = take_page(m);
         sp.push_back(pg);
         m->h_page_table[(size_t)slot * m->max_pages + i] = pg;
     }
@@ -340,8 +354,74 @@ qw_status reserve_pages(qw_model *m, int slot, int npos) {
 
 void release_slot(qw_model *m, int slot) {
     auto &sp = m->slot_pages[slot];
-    for (int pg : sp) m->free_pages.push_back(pg);
+    for (int pg : sp) drop_page(m, pg);
     sp.clear();
+}
+
+// device ints for the page operators: page moves (3 per page) or a compaction's table, base, start and kept
+// positions, or qw_extend's sequences (4 per slot)
+size_t cache_words(const qw_model *m) {
+    return std::max({(size_t)3 * std::max(m->max_pages, m->B), (size_t)m->max_pages + m->c.seq_len + 8, (size_t)4 * m->B + 8});
+}
+qw_status cache_buffer(qw_model *m) {
+    if (!m->d_cache) AL(m->d_cache, cache_words(m));
+    return QW_OK;
+}
+qw_kv_pool cache_pool(const qw_model *m) {
+    return qw_kv_pool{m->kpool, m->vpool, m->c.layers, m->num_pages, m->Hkvl, m->page_size, m->c.head_dim,
+                      m->bf16kv ? QW_DTYPE_BF16 : QW_DTYPE_F32};
+}
+// the slot's table row from page `from` on, after the work already on the stream
+qw_status send_table(qw_model *m, int slot, size_t from) {
+    auto &sp = m->slot_pages[slot];
+    if (from >= sp.size()) return QW_OK;
+    int *row = m->h_page_table.data() + (size_t)slot * m->max_pages;
+    for (size_t i = from; i < sp.size(); i++) row[i] = sp[i];
+    CK(cudaMemcpyAsync(m->d_page_table + (size_t)slot * m->max_pages + from, row + from, sizeof(int) * (sp.size() - from),
+                       cudaMemcpyHostToDevice, m->st));
+    return QW_OK;
+}
+// copies rows [0, rows[i]) of page src[i] to page dst[i] in every layer
+qw_status copy_pages(qw_model *m, const std::vector<int> &src, const std::vector<int> &dst, const std::vector<int> &rows) {
+    const size_t n = src.size();
+    if (!n) return QW_OK;
+    qw_status s = cache_buffer(m);
+    if (s) return s;
+    std::vector<int> all(src);
+    all.insert(all.end(), dst.begin(), dst.end());
+    all.insert(all.end(), rows.begin(), rows.end());
+    CK(cudaMemcpyAsync(m->d_cache, all.data(), sizeof(int) * 3 * n, cudaMemcpyHostToDevice, m->st));
+    const qw_kv_pool pool = cache_pool(m);
+    s = qw_op_kv_copy_pages(&pool, m->d_cache, m->d_cache + n, m->d_cache + 2 * n, (int)n, m->st);
+    return s ? fail(m, s, "%s", op_last_error()) : QW_OK;
+}
+
+// pages for positions [0, to), and those of [from, to) this slot's own: a page that other slots hold too is copied first
+qw_status own_pages(qw_model *m, int slot, int from, int to) {
+    qw_status s = reserve_pages(m, slot, to);
+    if (s) return s;
+    auto &sp = m->slot_pages[slot];
+    std::vector<int> src, dst, rows;
+    size_t first = 0;
+    for (int i = from / m->page_size; i < (int)sp.size() && i * m->page_size < to; i++)
+        if (m->page_refs[sp[i]] > 1) {
+            if (src.empty()) first = i;
+            src.push_back(i);
+        }
+    if (src.empty()) return QW_OK;
+    if (m->free_pages.size() < src.size())
+        return fail(m, QW_ERR_OOM, "KV cache exhausted: slot %d writes to %zu shared pages, %zu free", slot, src.size(),
+                    m->free_pages.size());
+    for (int &i : src) {
+        const int pg = sp[i];
+        sp[i] = take_page(m);
+        m->page_refs[pg]--;
+        dst.push_back(sp[i]);
+        rows.push_back(m->page_size);
+        i = pg;
+    }
+    if ((s = copy_pages(m, src, dst, rows))) return s;
+    return send_table(m, slot, first);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -562,13 +642,20 @@ qw_status tc_gemm(qw_model *m, int kind, const void *W, const void *X, int M, in
         if (s_) return s_;         \
     } while (0)
 
+// the sequences of a ragged pass (device arrays): rows row_start[i] .. row_start[i + 1] - 1 end at position kv_len[i] - 1
+// of slot slots[i]
+struct ChunkSeqs {
+    int n;
+    const int *row_start, *kv_len, *slots;
+};
+
 // All layers for T token rows (row r: token tokens[r] or hidden x_in row r, at slot row_slot[r] and
 // position row_pos[r]).  prefill: the rows are nseq sequences of L consecutive positions from p0
-// (flash attention); otherwise T single-token sequences (paged decode attention).  Leaves the
-// residual stream in m->xa and, under tensor parallelism, the last all-reduced partial in *pending.
+// (flash attention), or with `chunk` its ragged sequences (chunk attention); otherwise T single-token
+// sequences (paged decode attention).  Leaves the residual stream in m->xa and, under tensor parallelism, the last all-reduced partial in *pending.
 qw_status tc_layers(qw_model *m, int T, const int *tokens, const float *x_in, const int *row_slot, const int *row_pos,
                     bool prefill, int nseq, int p0, int L, const int *seq_slots, const float **pending_out,
-                    bool *final_normed = nullptr, bool *seq_par = nullptr) {
+                    bool *final_normed = nullptr, bool *seq_par = nullptr, const ChunkSeqs *chunk = nullptr) {
     const qw_config &c = m->c;
     PrefillBuffers &pf = m->pf;
     const int D = m->D, d = c.head_dim;
@@ -582,7 +669,7 @@ qw_status tc_layers(qw_model *m, int T, const int *tokens, const float *x_in, co
     // (each rank gets its block of T / tp rows summed), the residual update and rmsnorm run on that block only, and
     // the normalised bf16 rows are all-gathered as the next projection's operand: 3/4 of an fp32 all-reduce's bytes
     // and 1/tp of the row work.  The residual stream is then current only in this rank's row block.
-    const bool sp = tpm && prefill && m->prefill_sp && T % m->tp == 0;
+    const bool sp = tpm && prefill && !chunk && m->prefill_sp && T % m->tp == 0;
     if (seq_par) *seq_par = sp;
     const int Tl = sp ? T / m->tp : T, rb = sp ? m->rank * Tl : 0;  // this rank's row block
     auto sp_norm = [&](const float *part, const float *w, const int *tok) -> qw_status {
@@ -652,7 +739,15 @@ qw_status tc_layers(qw_model *m, int T, const int *tokens, const float *x_in, co
             }
             LK(qkv_post_launch(qa, T, m->bf16kv, m->st));
         }
-        if (prefill) {
+        if (chunk) {
+            ChunkArgs ca{};
+            ca.q = pf.q; ca.ld_q = m->Ql; ca.k = kc; ca.v = vc; ca.page_table = m->d_page_table; ca.max_pages = m->max_pages;
+            ca.slots = chunk->slots; ca.row_start = chunk->row_start; ca.kv_len = chunk->kv_len; ca.batch = chunk->n;
+            ca.rows = T; ca.out = pf.act; ca.ld_out = m->Ql; ca.err = pf.d_err; ca.workspace = m->chunk_ws;
+            ca.H = m->Hl; ca.Hkv = m->Hkvl; ca.G = m->Hl / m->Hkvl; ca.d = d; ca.ps = m->page_size; ca.log2_ps = m->log2_page;
+            ca.num_pages = m->num_pages; ca.sl2 = (float)(1.4426950408889634 / sqrt((double)d));
+            LKK(QW_KERNEL_ATTN, chunk_attn_tc_launch(ca, m->st));
+        } else if (prefill) {
             FlashArgs fa{};
             fa.q = pf.q; fa.ld_q = m->Ql; fa.kcache = kc; fa.vcache = vc; fa.page_table = m->d_page_table;
             fa.max_pages = m->max_pages; fa.page_size = m->page_size; fa.log2_page = m->log2_page;
@@ -730,16 +825,13 @@ qw_status tc_layers(qw_model *m, int T, const int *tokens, const float *x_in, co
     return QW_OK;
 }
 
-// Decode step for B > kGemvMaxB sequences: batched layers, then rmsnorm + lm_head GEMM + row argmax.
-qw_status tc_decode(qw_model *m, int *tokens, const float *x_in, const int *slots, int *positions, int B,
-                    float *logits_out_dev, int *argmax_dev, int advance, int *hist, int hist_ld) {
-    const float *pending = nullptr;
-    bool normed = false;
-    TRY(tc_layers(m, B, tokens, x_in, slots, positions, false, 0, 0, 1, nullptr, &pending, &normed));
+// The end of a batched step: final rmsnorm of the B rows of x (unless it has been applied), lm_head GEMM, row argmax.
+qw_status tc_head(qw_model *m, float *x, const float *pending, bool normed, int *tokens, int *positions, int B,
+                  float *logits_out_dev, int *argmax_dev, int advance, int *hist, int hist_ld) {
     const bool tpm = m->tp > 1;
     if (!normed) {
         NormRowsArgs na{};
-        na.x = m->xa; na.ld_x = m->D; na.part = const_cast<float *>(pending); na.ld_part = m->D; na.zero_part = pending == m->part_split;
+        na.x = x; na.ld_x = m->D; na.part = const_cast<float *>(pending); na.ld_part = m->D; na.zero_part = pending == m->part_split;
         na.w = m->norm_final; na.eps = (float)m->c.eps; na.out = m->pf.act; na.ld_out = m->D; na.K = m->D;
         LK(norm_rows_launch(na, B, m->st));
     }
@@ -764,6 +856,15 @@ qw_status tc_decode(qw_model *m, int *tokens, const float *x_in, const int *slot
     LKK(QW_KERNEL_LM_HEAD, rows_argmax_launch(ra, B, m->st));
     if (tpm) return tp_merge_argmax(m, B, logits_out_dev, argmax_dev, tokens, positions, advance, hist, hist_ld);
     return QW_OK;
+}
+
+// Decode step for B > kGemvMaxB sequences: batched layers, then rmsnorm + lm_head GEMM + row argmax.
+qw_status tc_decode(qw_model *m, int *tokens, const float *x_in, const int *slots, int *positions, int B,
+                    float *logits_out_dev, int *argmax_dev, int advance, int *hist, int hist_ld) {
+    const float *pending = nullptr;
+    bool normed = false;
+    TRY(tc_layers(m, B, tokens, x_in, slots, positions, false, 0, 0, 1, nullptr, &pending, &normed));
+    return tc_head(m, m->xa, pending, normed, tokens, positions, B, logits_out_dev, argmax_dev, advance, hist, hist_ld);
 }
 
 // full device step for any B (chunks of kGemvMaxB rows through the GEMV path)
@@ -799,7 +900,7 @@ qw_status check_positions(qw_model *m, const int32_t *slots, const int32_t *posi
             if ((slots ? slots[b2] : b2) == s) return fail(m, QW_ERR_ARG, "slot %d used twice in one batch", s);
         if (positions[b] < 0 || positions[b] >= m->c.seq_len)
             return fail(m, QW_ERR_SHAPE, "position %d outside [0,%d)", positions[b], m->c.seq_len);
-        qw_status st = reserve_pages(m, s, positions[b] + 1);
+        qw_status st = own_pages(m, s, positions[b], positions[b] + 1);
         if (st) return st;
     }
     return QW_OK;
@@ -852,7 +953,7 @@ qw_status tc_prefill(qw_model *m, const int32_t *tokens, const int32_t *slots, i
             int t = tokens[(size_t)b * seq_len + p];
             if (t < 0 || t >= m->c.vocab) return fail(m, QW_ERR_ARG, "token %d outside vocab", t);
         }
-        TRY(reserve_pages(m, sl[b], seq_len));
+        TRY(own_pages(m, sl[b], 0, seq_len));
     }
     const int Lc = std::max(1, std::min(seq_len, m->T / batch));
     const int Tmax = m->T;
@@ -916,6 +1017,73 @@ qw_status tc_prefill(qw_model *m, const int32_t *tokens, const int32_t *slots, i
     CK(cudaStreamSynchronize(m->st));
     derr = pin[0];
     if (derr) return fail(m, QW_ERR_TIMEOUT, "tensor-core kernel gave up waiting (device error %d)", derr);
+    if (argmax_out) memcpy(argmax_out, hp, sizeof(int) * batch);
+    return QW_OK;
+}
+
+// New tokens of a ragged batch on the tensor cores: sequence b's rows row_start[b] .. row_start[b + 1] - 1 stand at
+// positions start[b] .. of its slot.  Passes of up to T rows, in order; every sequence's last hidden row is kept for the
+// head.
+qw_status tc_extend(qw_model *m, const int32_t *tokens, const int32_t *row_start, const int32_t *sl, const int32_t *start,
+                    int batch, float *logits_out, int32_t *argmax_out) {
+    PrefillBuffers &pf = m->pf;
+    TRY(cache_buffer(m));
+    if (!m->chunk_ws) {
+        const size_t n = qw_op_chunk_attn_workspace(m->Hl, m->Hkvl, m->c.head_dim);
+        ALB(m->chunk_ws, n);
+        CK(cudaMemsetAsync(m->chunk_ws, 0, n, m->st));
+    }
+    const int Tmax = m->T, rows = row_start[batch];
+    int *pin = pf.h_pin, *d_start = m->d_cache, *d_kv = d_start + m->B + 1, *d_sl = d_kv + m->B, *d_last = d_sl + m->B;
+    std::vector<int> ext;
+    m->launches = 0;
+    int b = 0;
+    for (int r0 = 0; r0 < rows; r0 += Tmax) {
+        const int T = std::min(Tmax, rows - r0);
+        CK(cudaStreamSynchronize(m->st));  // the pinned staging of the previous pass has been consumed
+        std::vector<int> first, kv, slot, last(m->B, -1);
+        while (b < batch && row_start[b] < r0 + T) {
+            const int a = std::max(row_start[b], r0), e = std::min(row_start[b + 1], r0 + T);
+            first.push_back(a - r0);
+            kv.push_back(start[b] + e - row_start[b]);
+            slot.push_back(sl[b]);
+            for (int r = a; r < e; r++) {
+                pin[r - r0] = sl[b];
+                pin[Tmax + r - r0] = start[b] + r - row_start[b];
+                pin[2 * Tmax + r - r0] = tokens[r];
+            }
+            if (e < row_start[b + 1]) break;  // goes on in the next pass
+            last[b] = e - 1 - r0;
+            b++;
+        }
+        const int n = (int)first.size();
+        first.push_back(T);
+        ext.assign((size_t)4 * m->B + 1, 0);
+        std::copy(first.begin(), first.end(), ext.begin());
+        std::copy(kv.begin(), kv.end(), ext.begin() + m->B + 1);
+        std::copy(slot.begin(), slot.end(), ext.begin() + 2 * m->B + 1);
+        std::copy(last.begin(), last.end(), ext.begin() + 3 * m->B + 1);
+        CK(cudaMemcpyAsync(m->d_cache, ext.data(), sizeof(int) * ext.size(), cudaMemcpyHostToDevice, m->st));
+        CK(cudaMemcpyAsync(pf.row_slot, pin, sizeof(int) * (size_t)3 * Tmax, cudaMemcpyHostToDevice, m->st));
+        const ChunkSeqs cs{n, d_start, d_kv, d_sl};
+        const float *pending = nullptr;
+        TRY(tc_layers(m, T, pf.row_tok, nullptr, pf.row_slot, pf.row_pos, true, n, 0, 0, nullptr, &pending, nullptr, nullptr,
+                      &cs));
+        LK(gather_rows_launch(pf.x_host_stage, m->xa, pending, d_last, batch, m->D, m->st));
+    }
+    float *dlog = nullptr;
+    if (logits_out) dlog = m->logits_all ? m->logits_all + (size_t)m->tp * m->B * m->Vl : m->logits;
+    if (batch > kGemvMaxB)
+        TRY(tc_head(m, pf.x_host_stage, nullptr, false, nullptr, nullptr, batch, dlog, m->d_argmax, 0, nullptr, 0));
+    else
+        TRY(lm_head_gemv(m, pf.x_host_stage, m->D, nullptr, 0, batch, dlog, m->d_argmax, nullptr, nullptr, 0, nullptr, 0));
+    int *hp = m->h_pin_i + 3 * m->B;
+    CK(cudaMemcpyAsync(hp, m->d_argmax, sizeof(int) * batch, cudaMemcpyDeviceToHost, m->st));
+    if (logits_out)
+        CK(cudaMemcpyAsync(logits_out, dlog, sizeof(float) * (size_t)batch * m->c.vocab, cudaMemcpyDeviceToHost, m->st));
+    CK(cudaMemcpyAsync(&pin[0], pf.d_err, sizeof(int), cudaMemcpyDeviceToHost, m->st));
+    CK(cudaStreamSynchronize(m->st));
+    if (pin[0]) return fail(m, QW_ERR_TIMEOUT, "tensor-core kernel gave up waiting (device error %d)", pin[0]);
     if (argmax_out) memcpy(argmax_out, hp, sizeof(int) * batch);
     return QW_OK;
 }
@@ -1096,6 +1264,7 @@ static qw_status create_impl(qw_model *m, const qw_config *cfg, int device, int 
     CK(cudaMemsetAsync(m->d_page_table, 0, sizeof(int) * m->B * m->max_pages, m->st));
     m->slot_pages.assign(m->B, {});
     for (int p = m->num_pages - 1; p >= 0; p--) m->free_pages.push_back(p);
+    m->page_refs.assign(m->num_pages, 0);
     // ---- activations ----
     const int T = m->T, B = m->B;
     AL(m->xa, (size_t)T * D);
@@ -1416,6 +1585,156 @@ qw_status qw_prefill(qw_model *m, const int32_t *tokens, const int32_t *slots, i
     return QW_OK;
 }
 
+qw_status qw_extend(qw_model *m, const int32_t *tokens, const int32_t *row_start, const int32_t *slots,
+                    const int32_t *start, int32_t batch, float *logits_out, int32_t *argmax_out) {
+    if (!m) return QW_ERR_ARG;
+    if (!tokens || !row_start || !start) return fail(m, QW_ERR_ARG, "null tokens / row_start / start");
+    if (batch < 1 || batch > m->B) return fail(m, QW_ERR_SHAPE, "batch %d outside [1,%d]", batch, m->B);
+    if (!m->finalized) return fail(m, QW_ERR_STATE, "weights not finalized");
+    CK(cudaSetDevice(m->dev));
+    if (row_start[0] != 0) return fail(m, QW_ERR_ARG, "row_start begins with %d", row_start[0]);
+    std::vector<int> sl(batch);
+    for (int b = 0; b < batch; b++) {
+        const int n = row_start[b + 1] - row_start[b];
+        sl[b] = slots ? slots[b] : b;
+        if (sl[b] < 0 || sl[b] >= m->B) return fail(m, QW_ERR_ARG, "slot %d out of range", sl[b]);
+        for (int b2 = 0; b2 < b; b2++)
+            if (sl[b2] == sl[b]) return fail(m, QW_ERR_ARG, "slot %d used twice in one batch", sl[b]);
+        if (n < 1) return fail(m, QW_ERR_SHAPE, "sequence %d brings %d tokens", b, n);
+        if (start[b] < 0 || start[b] > m->c.seq_len - n)
+            return fail(m, QW_ERR_SHAPE, "positions %d + %d outside [0,%d)", start[b], n, m->c.seq_len);
+        for (int r = row_start[b]; r < row_start[b + 1]; r++)
+            if (tokens[r] < 0 || tokens[r] >= m->c.vocab) return fail(m, QW_ERR_ARG, "token %d outside vocab", tokens[r]);
+    }
+    for (int b = 0; b < batch; b++) {
+        qw_status s = own_pages(m, sl[b], start[b], start[b] + row_start[b + 1] - row_start[b]);
+        if (s) return s;
+    }
+    if (m->pf.tc && m->Hl / m->Hkvl <= 16 && batch <= kChunkMaxBatch)
+        return tc_extend(m, tokens, row_start, sl.data(), start, batch, logits_out, argmax_out);
+    // token by token through the decode kernels (fp32 weights or cache): the sequences that have one left
+    for (int i = 0;; i++) {
+        std::vector<int> seq, tok, pos, slot;
+        bool last = false;
+        for (int b = 0; b < batch; b++) {
+            const int n = row_start[b + 1] - row_start[b];
+            if (i >= n) continue;
+            seq.push_back(b);
+            tok.push_back(tokens[row_start[b] + i]);
+            pos.push_back(start[b] + i);
+            slot.push_back(sl[b]);
+            last |= i == n - 1;
+        }
+        const int n = (int)seq.size();
+        if (!n) return QW_OK;
+        std::vector<float> lg(last && logits_out ? (size_t)n * m->c.vocab : 0);
+        std::vector<int> am(n);
+        qw_status s = host_step(m, tok.data(), nullptr, slot.data(), pos.data(), n, lg.empty() ? nullptr : lg.data(), am.data());
+        if (s) return s;
+        for (int k = 0; k < n; k++) {
+            const int b = seq[k];
+            if (i != row_start[b + 1] - row_start[b] - 1) continue;
+            if (logits_out) memcpy(logits_out + (size_t)b * m->c.vocab, lg.data() + (size_t)k * m->c.vocab, sizeof(float) * m->c.vocab);
+            if (argmax_out) argmax_out[b] = am[k];
+        }
+    }
+}
+
+qw_status qw_fork(qw_model *m, int32_t src, const int32_t *dst, int32_t n, int32_t n_positions) {
+    if (!m) return QW_ERR_ARG;
+    if (n < 0 || (n && !dst)) return fail(m, QW_ERR_ARG, "fork into %d slots", n);
+    if (src < 0 || src >= m->B) return fail(m, QW_ERR_ARG, "slot %d out of range", src);
+    if (n_positions < 0 || n_positions > (int)m->slot_pages[src].size() * m->page_size)
+        return fail(m, QW_ERR_SHAPE, "slot %d holds pages for %zu positions, not %d", src,
+                    m->slot_pages[src].size() * m->page_size, n_positions);
+    for (int i = 0; i < n; i++) {
+        if (dst[i] < 0 || dst[i] >= m->B || dst[i] == src) return fail(m, QW_ERR_ARG, "fork of slot %d into %d", src, dst[i]);
+        for (int k = 0; k < i; k++)
+            if (dst[k] == dst[i]) return fail(m, QW_ERR_ARG, "slot %d named twice", dst[i]);
+    }
+    CK(cudaSetDevice(m->dev));
+    for (int i = 0; i < n; i++) release_slot(m, dst[i]);
+    const int full = n_positions / m->page_size, tail = n_positions % m->page_size;
+    if (tail && (int)m->free_pages.size() < n)
+        return fail(m, QW_ERR_OOM, "KV cache exhausted: %d forks need a page each, %zu free", n, m->free_pages.size());
+    std::vector<int> from, to, rows;
+    const std::vector<int> sp = m->slot_pages[src];
+    for (int i = 0; i < n; i++) {
+        auto &dp = m->slot_pages[dst[i]];
+        dp.assign(sp.begin(), sp.begin() + full);
+        for (int pg : dp) m->page_refs[pg]++;
+        if (tail) {
+            dp.push_back(take_page(m));
+            from.push_back(sp[full]);
+            to.push_back(dp.back());
+            rows.push_back(tail);
+        }
+    }
+    qw_status s = copy_pages(m, from, to, rows);
+    for (int i = 0; i < n && !s; i++) s = send_table(m, dst[i], 0);
+    return s;
+}
+
+qw_status qw_truncate(qw_model *m, int32_t slot, int32_t n_positions) {
+    if (!m) return QW_ERR_ARG;
+    if (slot < 0 || slot >= m->B || n_positions < 0) return fail(m, QW_ERR_ARG, "slot %d, %d positions", slot, n_positions);
+    auto &sp = m->slot_pages[slot];
+    const size_t need = ((size_t)n_positions + m->page_size - 1) / m->page_size;
+    while (sp.size() > need) {
+        drop_page(m, sp.back());
+        sp.pop_back();
+    }
+    return QW_OK;
+}
+
+qw_status qw_compact(qw_model *m, int32_t slot, const int32_t *keep, int32_t n_keep) {
+    if (!m) return QW_ERR_ARG;
+    if (slot < 0 || slot >= m->B) return fail(m, QW_ERR_ARG, "slot %d out of range", slot);
+    if (n_keep < 0 || (n_keep && !keep)) return fail(m, QW_ERR_ARG, "%d positions to keep", n_keep);
+    auto &sp = m->slot_pages[slot];
+    const int ps = m->page_size, held = (int)std::min<size_t>(sp.size() * ps, m->c.seq_len);
+    int same = 0;  // leading positions that stay where they are
+    for (int i = 0; i < n_keep; i++) {
+        if (keep[i] < 0 || keep[i] >= held || (i && keep[i] <= keep[i - 1]))
+            return fail(m, QW_ERR_ARG, "positions to keep must ascend within [0,%d): %d", held, keep[i]);
+        if (same == i && keep[i] == i) same++;
+    }
+    if (same == n_keep) return qw_truncate(m, slot, n_keep);
+    CK(cudaSetDevice(m->dev));
+    const int base = same / ps;  // whole pages before stay, shared or not; the rest is gathered into new ones
+    const int fresh = (n_keep + ps - 1) / ps - base;
+    if ((int)m->free_pages.size() < fresh)
+        return fail(m, QW_ERR_OOM, "KV cache exhausted: compacting slot %d needs %d pages, %zu free", slot, fresh,
+                    m->free_pages.size());
+    qw_status s = cache_buffer(m);
+    if (s) return s;
+    const int rows = n_keep - base * ps;
+    std::vector<int> arg(m->max_pages, -1);  // destination table | base | start | kept positions
+    std::vector<int> np(sp.begin(), sp.begin() + base);
+    for (int i = 0; i < fresh; i++) {
+        np.push_back(take_page(m));
+        arg[base + i] = np.back();
+    }
+    arg.push_back(base * ps);
+    arg.push_back(0);
+    arg.push_back(rows);
+    arg.insert(arg.end(), keep + base * ps, keep + n_keep);
+    CK(cudaMemcpyAsync(m->d_cache, arg.data(), sizeof(int) * arg.size(), cudaMemcpyHostToDevice, m->st));
+    const qw_kv_pool pool = cache_pool(m);
+    const int *d = m->d_cache;
+    s = qw_op_kv_compact(&pool, m->d_page_table + (size_t)slot * m->max_pages, d, m->max_pages, d + m->max_pages + 3,
+                         d + m->max_pages + 1, d + m->max_pages, 1, rows, (const float *)m->freq, m->c.seq_len, m->st);
+    if (s) {
+        for (int i = 0; i < fresh; i++) drop_page(m, np[base + i]);
+        return fail(m, s, "%s", op_last_error());
+    }
+    for (size_t i = base; i < sp.size(); i++) drop_page(m, sp[i]);
+    sp = np;
+    return send_table(m, slot, base);
+}
+
+int32_t qw_free_pages(const qw_model *m) { return m ? (int32_t)m->free_pages.size() : 0; }
+
 // Sampled generation (AutoregressiveModel.next with a temperature): the prompt's last logits give the
 // first generated token; every later step writes its logits and the sampling kernel feeds the drawn token
 // back and advances the position, all on the device.
@@ -1692,7 +2011,7 @@ void qw_destroy(qw_model *m) {
     }
     if (!m->lm_alias) cudaFree(m->lm);
     cudaFree(m->embed); cudaFree(m->norm_final); cudaFree(m->freq);
-    cudaFree(m->kpool); cudaFree(m->vpool); cudaFree(m->d_page_table);
+    cudaFree(m->kpool); cudaFree(m->vpool); cudaFree(m->d_page_table); cudaFree(m->d_cache); cudaFree(m->chunk_ws);
     cudaFree(m->xa); cudaFree(m->xb); cudaFree(m->part); cudaFree(m->qkv); cudaFree(m->attn); cudaFree(m->hbuf);
     cudaFree(m->part_o); cudaFree(m->part_ml); cudaFree(m->qk_ss); cudaFree(m->counters); cudaFree(m->am_counter);
     cudaFree(m->am_pval); cudaFree(m->am_pidx); cudaFree(m->am_val); cudaFree(m->am_idx); cudaFree(m->am_val_all);

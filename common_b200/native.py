@@ -27,7 +27,8 @@ EXPORTS = ("qw_abi_version", "qw_build_info", "qw_get_unique_id", "qw_create", "
            "qw_generate", "qw_decode_step_device", "qw_capture_decode", "qw_replay_decode", "qw_synchronize",
            "qw_stream", "qw_last_launch_count", "qw_last_error", "qw_destroy", "qw_profile_decode",
            "qw_set_device_inputs", "qw_profile_prefill", "qw_op_lm_head_argmax", "qw_op_lm_head_argmax_static", "qw_op_linear", "qw_set_sampling", "qw_decode_sample", "qw_op_sample",
-           "qw_op_chunk_attn", "qw_op_chunk_attn_workspace", "qw_op_kv_copy_pages", "qw_op_kv_compact")
+           "qw_op_chunk_attn", "qw_op_chunk_attn_workspace", "qw_op_kv_copy_pages", "qw_op_kv_compact",
+           "qw_extend", "qw_fork", "qw_truncate", "qw_compact", "qw_free_pages")
 KERNEL_NAMES = {0: "other", 1: "qkv", 2: "attn", 3: "o_proj", 4: "gate_up", 5: "down", 6: "lm_head", 7: "step"}
 
 
@@ -89,6 +90,11 @@ def load() -> C.CDLL:
         "qw_decode_step": (I32, [P, PI, PI, PI, I32, PF, PI]),
         "qw_forward_hidden": (I32, [P, PF, PI, PI, I32, PF, PI]),
         "qw_prefill": (I32, [P, PI, PI, I32, I32, PF, PI]),
+        "qw_extend": (I32, [P, PI, PI, PI, PI, I32, PF, PI]),
+        "qw_fork": (I32, [P, I32, PI, I32, I32]),
+        "qw_truncate": (I32, [P, I32, I32]),
+        "qw_compact": (I32, [P, I32, PI, I32]),
+        "qw_free_pages": (I32, [P]),
         "qw_generate": (I32, [P, PI, I32, I32, I32, PI]),
         "qw_decode_step_device": (I32, [P, P, P, P, I32, P, P, I32]),
         "qw_capture_decode": (I32, [P, P, P, P, I32, P, P]),
@@ -335,6 +341,37 @@ class NativeModel:
         am = np.zeros(B, np.int32)
         self._check(self.L.qw_prefill(self.h, _ip(t), _ip(s), B, S, _fp(logits), _ip(am)))
         return logits, am
+
+    def extend(self, tokens, start, slots=None, want_logits=True):
+        """New tokens for a ragged batch: tokens is a list of sequences, start their first positions; returns the logits
+        and greedy token of each sequence's last new position."""
+        rows = [np.ascontiguousarray(t, np.int32).reshape(-1) for t in tokens]
+        B = len(rows)
+        flat = np.concatenate(rows) if rows else np.zeros(0, np.int32)
+        row_start = np.cumsum([0] + [r.size for r in rows]).astype(np.int32)
+        p = np.ascontiguousarray(start, np.int32)
+        s = None if slots is None else np.ascontiguousarray(slots, np.int32)
+        if p.size != B or (s is not None and s.size != B):
+            raise QwenError(2, f"{B} sequences, {p.size} start positions" + ("" if s is None else f", {s.size} slots"))
+        logits = np.zeros((B, self.cfg.vocab), np.float32) if want_logits else None
+        am = np.zeros(B, np.int32)
+        self._check(self.L.qw_extend(self.h, _ip(flat), _ip(row_start), _ip(s), _ip(p), B, _fp(logits), _ip(am)))
+        return logits, am
+
+    def fork(self, src: int, dst, n_positions: int):
+        d = np.ascontiguousarray(dst, np.int32).reshape(-1)
+        self._check(self.L.qw_fork(self.h, src, _ip(d), d.size, n_positions))
+
+    def truncate(self, slot: int, n_positions: int):
+        self._check(self.L.qw_truncate(self.h, slot, n_positions))
+
+    def compact(self, slot: int, keep):
+        k = np.ascontiguousarray(keep, np.int32).reshape(-1)
+        self._check(self.L.qw_compact(self.h, slot, _ip(k), k.size))
+
+    @property
+    def free_pages(self) -> int:
+        return self.L.qw_free_pages(self.h)
 
     def set_sampling(self, temperature: float, top_p: float = 1.0, seed: int = 0, mode: int = 0):
         self._check(self.L.qw_set_sampling(self.h, temperature, top_p, seed, mode))

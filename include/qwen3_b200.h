@@ -167,6 +167,41 @@ qw_status qw_forward_hidden(qw_model *m, const float *x_in, const int32_t *slots
 qw_status qw_prefill(qw_model *m, const int32_t *tokens, const int32_t *slots, int32_t batch,
                      int32_t seq_len, float *logits_out, int32_t *argmax_out);
 
+/* New tokens for a ragged batch on top of what the slots hold: sequence b's tokens
+ * tokens[row_start[b] .. row_start[b + 1] - 1] (row_start has batch + 1 entries and begins with 0; one token at least
+ * each) stand at positions start[b], start[b] + 1, ... of slot slots[b] (NULL = 0..batch-1), whose positions before
+ * start[b] have been written.  One call serves the next turns of conversations, chunks of long prompts, and single
+ * tokens beside them.  Writes the logits / greedy token of each sequence's last new position (either may be NULL).
+ * Results equal feeding the tokens one by one, within the bf16 tolerance.  With bf16 weights and cache all rows go
+ * through the layers together (passes of max_tokens rows) and qw_op_chunk_attn's kernel; otherwise token by token.
+ * The reference feeds one token per forward (AutoregressiveModel.java:295-308). */
+qw_status qw_extend(qw_model *m, const int32_t *tokens, const int32_t *row_start, const int32_t *slots,
+                    const int32_t *start, int32_t batch, float *logits_out, int32_t *argmax_out);
+
+/* ---- pages of a slot: shared, copied, compacted, freed ----------------------------------------
+ * A page may be held by several slots.  A call that writes to a position inside a shared page (qw_decode_step,
+ * qw_prefill, qw_extend and those built on them) gives the slot a copy of its own first; the device-resident calls
+ * (qw_decode_step_device, captured steps) write where the table points, so they must not write to positions that were
+ * there when the slot was forked.  The reference has one cache per model and no counterpart to these. */
+
+/* Clear slots dst[0..n-1] and let each hold the first n_positions of slot src: whole pages are shared, the last, partly
+ * filled one is copied (in every layer, one launch).  QW_ERR_OOM when there is no page for a copy: the destination slots
+ * are then empty. */
+qw_status qw_fork(qw_model *m, int32_t src, const int32_t *dst, int32_t n, int32_t n_positions);
+
+/* Drop the positions from n_positions on: their whole pages are given up, and free when no other slot holds them. */
+qw_status qw_truncate(qw_model *m, int32_t slot, int32_t n_positions);
+
+/* Keep only the positions keep[0] < keep[1] < ... < keep[n_keep - 1] of a slot, moved together to positions
+ * 0 .. n_keep - 1, their keys turned to the rotary angles of their new positions (for bf16 caches rounded once more); the
+ * next token stands at position n_keep.  Pages before the first dropped position stay as they are, shared or not; the
+ * rest is gathered into new pages (QW_ERR_OOM, and nothing changed, when there are not enough) and the old ones are given
+ * up. */
+qw_status qw_compact(qw_model *m, int32_t slot, const int32_t *keep, int32_t n_keep);
+
+/* Pages that no slot holds. */
+int32_t qw_free_pages(const qw_model *m);
+
 /* Greedy autoregressive generation (AutoregressiveModel.next loop,
  * AutoregressiveModel.java:295-308): prompts (batch x prompt_len) are fed first,
  * then each step feeds the argmax of the previous step's logits.  tokens_out
