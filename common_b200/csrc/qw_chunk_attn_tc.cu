@@ -18,8 +18,8 @@
 //         it also clears the rows of a V block that the sequence never sees (0 x NaN is NaN)
 //   2     Q: one box of (64 columns, G heads, P positions) per 64 columns
 //   3     walks the CTA's share of the line and hands its pieces to the other warps through a ring
-//   4..11 softmax and result of slot 0, two threads per row (64 keys, and half of the columns of O, each), so that one
-//         warp's loads, maxima and stores run beside the other's exponentials; 12..19 of slot 1
+//   4..11 softmax and result of slot 0: a warp has 16 rows, two threads per row (64 keys, and half of the columns of O,
+//         each), so that one warp's loads, maxima and stores run beside another's exponentials; 12..19 of slot 1
 // Every wait is bounded; one that runs out sets the error word and ends the CTA (its copies landed, its TMEM freed).
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -38,6 +38,7 @@ constexpr int kThreads = 640, kSoftThreads = 512, kRows = 128, kKeys = 128, kMax
 constexpr float kRescale = 8.f;  // the running maximum is raised only when it grows by more than 2^8: p stays below 2^8
 constexpr int kPieces = 4;       // ring of pieces
 constexpr int kFewRows = 8;      // rows of an exchange in shared memory: a token's heads of one KV head
+constexpr int kItemUnits = 2;    // what a tile costs beside its blocks
 constexpr int kMinShare = 5;     // units that a CTA beyond one per item is worth: splitting an item costs about as much
 constexpr int kCounterWords = 256;  // arrivals | departures | arrivals at items cut once, one word per CTA each
 
@@ -77,7 +78,6 @@ struct __align__(16) Smem {
     uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages], q_full[2], q_empty[2],
         s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], done;
     uint32_t tmem;
-    float mx[2][2][kRows], sum[2][2][kRows];  // [slot][half][row]
     float4 xo[2][128 / 4 * kFewRows];  // [slot]: O as float4 columns of kFewRows rows (16-byte aligned by its type)
     float2 xml[2][kFewRows];
     int abort, go;
@@ -87,7 +87,10 @@ struct __align__(16) Smem {
 // one item's keys
 struct Item {
     int nsub, f, pf, pl, klo, j0, nb;  // tiles; first new row; positions of the first and last row; first seen; blocks
-    __device__ __forceinline__ unsigned units() const { return nb ? nb + 1 : 0; }  // an item that sees nothing is not on the line
+    // a visit of a slot is a unit: a block costs as many as the item has tiles, and its queries and results kItemUnits
+    // per tile; an item that sees nothing is not on the line
+    __device__ __forceinline__ unsigned units() const { return nb ? (nb + kItemUnits) * nsub : 0; }
+    __device__ __forceinline__ int blocks_before(int u) const { return min(nb, nsub == 2 ? (u + 1) >> 1 : u); }
 };
 __device__ __forceinline__ Item make_item(const Seq &s, int i, int P, int window) {
     Item it;
@@ -155,33 +158,37 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, u
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
+// 16 TMEM lanes in two column groups: threads 0..15 take column taddr + i, threads 16..31 column taddr + SPLIT + i
+template <int SPLIT>
 __device__ __forceinline__ void ld32(uint32_t taddr, float *v) {
     uint32_t r[32];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "tcgen05.ld.sync.aligned.16x32bx2.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32], %33;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
+        : "r"(taddr), "n"(SPLIT));
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
+template <int SPLIT>
 __device__ __forceinline__ void ld16(uint32_t taddr, uint32_t *o) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        "tcgen05.ld.sync.aligned.16x32bx2.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16], %17;"
         : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
           "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-        : "r"(taddr));
+        : "r"(taddr), "n"(SPLIT));
 }
+template <int SPLIT>
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t *r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "tcgen05.st.sync.aligned.16x32bx2.x16.b32 [%0], %17, "
         "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "n"(SPLIT)
         : "memory");
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -221,10 +228,6 @@ __device__ __forceinline__ void store32(void *p, const uint32_t *v) {
                  : "memory");
 }
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory"); }
-// The two warps that share 32 rows of a slot.  One whose wait ran out still arrives for the other, which may have seen
-// the wait end in time; that one's next wait needs the missing results and runs out too.
-__device__ __forceinline__ void leave_pair(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void bar_pair(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
     unsigned v;
     asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
@@ -424,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 3) {
             // ---------------- the scheduler ----------------
-            // units of every sequence (an item costs its blocks and one more) and their running sum
+            // units of every sequence and their running sum
             unsigned W = 0;
             int items = 0;  // that see something
             for (int b0 = 0; b0 < a.batch; b0 += 32) {
@@ -473,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Line line{0, 0};
             unsigned at = 0, end = 0;
             int b = 0, h = 0, i = 0, off = 0;
-            if (cta < Ge) {  // Ge <= W: an item has two units at least
+            if (cta < Ge) {  // W / Ge >= 2: an item has three units at least
                 line.q = W / Ge;
                 line.rem = W - line.q * Ge;
                 at = line.start(cta);
@@ -533,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     it = make_item(s, i, P, a.window);
                     const int units = (int)it.units();
                     const int take = min(units - off, (int)(end - at));
-                    const int ja = min(off, it.nb), jb = min(off + take, it.nb);
+                    const int ja = it.blocks_before(off), jb = it.blocks_before(off + take);
                     u0 = at - off;
                     cb = b; ch = h;
                     at += take;
@@ -569,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     int c0 = cta, ni = 1;
                     if (!(pc.flags & kWhole)) {
                         if (!(pc.flags & kHead)) c0 = u0 >= line.start(cta - 1) ? cta - 1 : (int)line.owner(u0);
-                        const unsigned last = u0 + it.nb - 1;
+                        const unsigned last = u0 + (it.nb - 1) * it.nsub;  // where its last block begins
                         const int c1 = last < line.start(cta + 1) ? cta : last < line.start(cta + 2) ? cta + 1 : (int)line.owner(last);
                         ni = c1 - c0 + 1;
                     }
@@ -800,10 +803,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
         // ---------------- softmax and results ----------------
-        const int t = (warp - 4) >> 3, hf = ((warp - 4) >> 2) & 1, qq = warp & 3, row = qq * 32 + lane, pair_id = 2 + t * 4 + qq;
+        const int t = (warp - 4) >> 3, hf = lane >> 4, w0 = (warp & 3) * 32 + ((warp - 4) & 4) * 4, row = w0 + (lane & 15);
         const int rpos = row / G, rhead = row % G;
-        const uint32_t trow = tmem + ((uint32_t)(qq * 32) << 16);
-        const uint32_t ts = trow + (uint32_t)(t * kKeys + hf * 64), to = trow + 256u + (uint32_t)(t * 128 + hf * (D / 2));
+        const uint32_t trow = tmem + ((uint32_t)w0 << 16);
+        const uint32_t ts = trow + (uint32_t)(t * kKeys), to = trow + 256u + (uint32_t)(t * 128);
         int nv = 0, no = 0, nx[2] = {0, 0};  // visits, pieces with visits, exchanges by writing slot
         bool ok = true;
         for (int np = 0; ok; np++) {
@@ -821,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.w_empty[np % kPieces]);
             if (flags & kEnd) break;
-            const bool valid = row < rows, warp_on = qq * 32 < rows;
+            const bool valid = row < rows, warp_on = w0 < rows;
             __nv_bfloat16 *orow = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)grow * a.ld_out + (size_t)head * D + hf * (D / 2);
             const int mine = (nblk - jj + step - 1) / step;
             // An item cut once is finished by the CTA in which it begins, at the end of its share, from the other's part:
@@ -846,15 +849,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m_use = -INFINITY, l = 0.f;  // running maximum (log2 units), sum of this half's probabilities
             for (int v = 0; v < mine; v++, nv++, k0 += step * kKeys) {
                 ok = warp_wait(&sh.s_full[t], (uint32_t)nv & 1u, abort_flag, a.err);
-                if (!ok) {
-                    if (warp_on) leave_pair(pair_id);
-                    break;
-                }
+                if (!ok) break;
                 tc_fence_after();
                 if (warp_on) {
                     float x[64];
-                    ld32(ts, x);
-                    ld32(ts + 32u, x + 32);
+                    ld32<64>(ts, x);
+                    ld32<64>(ts + 32u, x + 32);
                     wait_ld();
                     const int hi = valid ? pos - k0 - hf * 64 : 64;
                     if (hi < 63) {
@@ -873,9 +873,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 64; e += 2) m4[(e >> 1) & 3] = fmaxf(m4[(e >> 1) & 3], fmaxf(x[e], x[e + 1]));
                     float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                    sh.mx[t][hf][row] = mx;
-                    bar_pair(pair_id);
-                    mx = fmaxf(mx, sh.mx[t][hf ^ 1][row]) * a.sl2;
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) * a.sl2;
                     float alpha = 1.f;
                     bool need = false;
                     if (v == 0) {
@@ -902,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             s2[e & 1] = add2(s2[e & 1], f2(p0, p1));
                             pk[e] = pack2(p0, p1);
                         }
-                        st16(ts + (uint32_t)(c * 16), pk);
+                        st16<64>(ts + (uint32_t)(c * 16), pk);
                     }
                     float s0, s1;
                     unf2(add2(s2[0], s2[1]), s0, s1);
@@ -912,11 +910,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[16];
-                            ld16(to + (uint32_t)(c * 16), o);
+                            ld16<D / 2>(to + (uint32_t)(c * 16), o);
                             wait_ld();
 #pragma unroll
                             for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                            st16(to + (uint32_t)(c * 16), o);
+                            st16<D / 2>(to + (uint32_t)(c * 16), o);
                         }
                     }
                     wait_st();
@@ -927,21 +925,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!ok) break;
             ok = warp_wait(&sh.o_full[t], (uint32_t)no & 1u, abort_flag, a.err);
-            if (!ok) {
-                if (warp_on) leave_pair(pair_id);
-                break;
-            }
+            if (!ok) break;
             no++;
             tc_fence_after();
-            if (warp_on) {  // the row's sum, of both halves
-                sh.sum[t][hf][row] = l;
-                bar_pair(pair_id);
-                l += sh.sum[t][hf ^ 1][row];
-            }
+            l += __shfl_xor_sync(0xffffffffu, l, 16);  // the row's sum, of both halves
             auto put_few = [&](int slot) {  // this half of O's columns of the valid rows
                 float o[D / 2];
 #pragma unroll
-                for (int c = 0; c < D / 64; c++) ld32(to + (uint32_t)(c * 32), o + c * 32);
+                for (int c = 0; c < D / 64; c++) ld32<D / 2>(to + (uint32_t)(c * 32), o + c * 32);
                 wait_ld();
                 if (valid) {
 #pragma unroll
@@ -957,7 +948,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float inv = l == 0.f ? 0.f : 1.f / l;
                         float o[D / 2];
 #pragma unroll
-                        for (int c = 0; c < D / 64; c++) ld32(to + (uint32_t)(c * 32), o + c * 32);
+                        for (int c = 0; c < D / 64; c++) ld32<D / 2>(to + (uint32_t)(c * 32), o + c * 32);
                         wait_ld();
                         if (valid) {
 #pragma unroll
@@ -1005,33 +996,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const float2 o0 = exchange ? sh.xml[t ^ 1][src] : none, o1 = whole ? none : __ldcg(p1.ml(src)),
                                          o2 = whole ? none : __ldcg(p2.ml(src));
                             const float M = fmaxf(fmaxf(own.x, o0.x), fmaxf(o1.x, o2.x)), Mu = M == -INFINITY ? 0.f : M;
-                            float wo = ex2(own.x - Mu), w0 = ex2(o0.x - Mu), w1 = ex2(o1.x - Mu), w2 = ex2(o2.x - Mu);
-                            l = own.y * wo + o0.y * w0 + o1.y * w1 + o2.y * w2;
+                            float wo = ex2(own.x - Mu), w0e = ex2(o0.x - Mu), w1 = ex2(o1.x - Mu), w2 = ex2(o2.x - Mu);
+                            l = own.y * wo + o0.y * w0e + o1.y * w1 + o2.y * w2;
                             m_use = M;
                             const float inv = l == 0.f ? 0.f : 1.f / l;
-                            wo *= inv; w0 *= inv; w1 *= inv; w2 *= inv;
+                            wo *= inv; w0e *= inv; w1 *= inv; w2 *= inv;
                             const int rg = __shfl_sync(0xffffffffu, grow, src), rh = __shfl_sync(0xffffffffu, head, src);
                             __nv_bfloat16 *to_row = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)rg * a.ld_out + (size_t)rh * D;
-                            float4 q[4][D / 32];
+#pragma unroll 1
+                            for (int g = 0; g < D / 4; g += 16) {
+                                float4 q[4][4];
 #pragma unroll
-                            for (int c = 0; c < D / 32; c++) {
-                                const int c4 = hf * (D / 8) + (lane >> 3) + 4 * c;
-                                const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                                q[0][c] = sh.xo[t][c4 * kFewRows + src];
-                                q[1][c] = exchange ? sh.xo[t ^ 1][c4 * kFewRows + src] : z;
-                                // (a part of weight 0 saw nothing: its O may not have been written)
-                                q[2][c] = w1 != 0.f ? __ldcg(p1.o(c4, src)) : z;
-                                q[3][c] = w2 != 0.f ? __ldcg(p2.o(c4, src)) : z;
-                            }
-                            if (r < rows) {
+                                for (int c = 0; c < 4; c++) {
+                                    const int c4 = g + (lane >> 3) + 4 * c;
+                                    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                                    q[0][c] = sh.xo[t][c4 * kFewRows + src];
+                                    q[1][c] = exchange ? sh.xo[t ^ 1][c4 * kFewRows + src] : z;
+                                    // (a part of weight 0 saw nothing: its O may not have been written)
+                                    q[2][c] = w1 != 0.f ? __ldcg(p1.o(c4, src)) : z;
+                                    q[3][c] = w2 != 0.f ? __ldcg(p2.o(c4, src)) : z;
+                                }
+                                if (r < rows) {
 #pragma unroll
-                                for (int c = 0; c < D / 32; c++) {
-                                    const float4 o = make_float4(q[0][c].x * wo + q[1][c].x * w0 + q[2][c].x * w1 + q[3][c].x * w2,
-                                                                 q[0][c].y * wo + q[1][c].y * w0 + q[2][c].y * w1 + q[3][c].y * w2,
-                                                                 q[0][c].z * wo + q[1][c].z * w0 + q[2][c].z * w1 + q[3][c].z * w2,
-                                                                 q[0][c].w * wo + q[1][c].w * w0 + q[2][c].w * w1 + q[3][c].w * w2);
-                                    const int c4 = hf * (D / 8) + (lane >> 3) + 4 * c;
-                                    *reinterpret_cast<uint2 *>(to_row + c4 * 4) = make_uint2(pack2(o.x, o.y), pack2(o.z, o.w));
+                                    for (int c = 0; c < 4; c++) {
+                                        const float4 o = make_float4(q[0][c].x * wo + q[1][c].x * w0e + q[2][c].x * w1 + q[3][c].x * w2,
+                                                                     q[0][c].y * wo + q[1][c].y * w0e + q[2][c].y * w1 + q[3][c].y * w2,
+                                                                     q[0][c].z * wo + q[1][c].z * w0e + q[2][c].z * w1 + q[3][c].z * w2,
+                                                                     q[0][c].w * wo + q[1][c].w * w0e + q[2][c].w * w1 + q[3][c].w * w2);
+                                        *reinterpret_cast<uint2 *>(to_row + (g + (lane >> 3) + 4 * c) * 4) = make_uint2(pack2(o.x, o.y), pack2(o.z, o.w));
+                                    }
                                 }
                             }
                         }
@@ -1039,22 +1032,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float2 o0 = valid && exchange ? __ldcg(p0.ml(row)) : none, o1 = valid && !whole ? __ldcg(p1.ml(row)) : none,
                                      o2 = valid && !whole && !pair ? __ldcg(p2.ml(row)) : none;
                         const float M = fmaxf(fmaxf(m_use, o0.x), fmaxf(o1.x, o2.x)), Mu = M == -INFINITY ? 0.f : M;
-                        float wo = ex2(m_use - Mu), w0 = ex2(o0.x - Mu), w1 = ex2(o1.x - Mu), w2 = ex2(o2.x - Mu);
-                        l = l * wo + o0.y * w0 + o1.y * w1 + o2.y * w2;
+                        float wo = ex2(m_use - Mu), w0e = ex2(o0.x - Mu), w1 = ex2(o1.x - Mu), w2 = ex2(o2.x - Mu);
+                        l = l * wo + o0.y * w0e + o1.y * w1 + o2.y * w2;
                         m_use = M;
                         const float inv = l == 0.f ? 0.f : 1.f / l;
-                        wo *= inv; w0 *= inv; w1 *= inv; w2 *= inv;
+                        wo *= inv; w0e *= inv; w1 *= inv; w2 *= inv;
 #pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t u[16];
-                            ld16(to + (uint32_t)(c * 16), u);
+                            ld16<D / 2>(to + (uint32_t)(c * 16), u);
                             const int c4 = hf * (D / 8) + c * 4;
                             float4 q0[4], q1[4], q2[4];
                             // a part of weight 0 saw nothing (its O may not have been written)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                                q0[e] = w0 != 0.f ? __ldcg(p0.o(c4 + e, row)) : z;
+                                q0[e] = w0e != 0.f ? __ldcg(p0.o(c4 + e, row)) : z;
                                 q1[e] = w1 != 0.f ? __ldcg(p1.o(c4 + e, row)) : z;
                                 q2[e] = w2 != 0.f ? __ldcg(p2.o(c4 + e, row)) : z;
                             }
@@ -1062,10 +1055,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             float o[16];
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                o[4 * e] = __uint_as_float(u[4 * e]) * wo + q0[e].x * w0 + q1[e].x * w1 + q2[e].x * w2;
-                                o[4 * e + 1] = __uint_as_float(u[4 * e + 1]) * wo + q0[e].y * w0 + q1[e].y * w1 + q2[e].y * w2;
-                                o[4 * e + 2] = __uint_as_float(u[4 * e + 2]) * wo + q0[e].z * w0 + q1[e].z * w1 + q2[e].z * w2;
-                                o[4 * e + 3] = __uint_as_float(u[4 * e + 3]) * wo + q0[e].w * w0 + q1[e].w * w1 + q2[e].w * w2;
+                                o[4 * e] = __uint_as_float(u[4 * e]) * wo + q0[e].x * w0e + q1[e].x * w1 + q2[e].x * w2;
+                                o[4 * e + 1] = __uint_as_float(u[4 * e + 1]) * wo + q0[e].y * w0e + q1[e].y * w1 + q2[e].y * w2;
+                                o[4 * e + 2] = __uint_as_float(u[4 * e + 2]) * wo + q0[e].z * w0e + q1[e].z * w1 + q2[e].z * w2;
+                                o[4 * e + 3] = __uint_as_float(u[4 * e + 3]) * wo + q0[e].w * w0e + q1[e].w * w1 + q2[e].w * w2;
                             }
                             if (valid) {
                                 uint32_t pk[8];
@@ -1097,7 +1090,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
                         uint32_t o[16];
-                        ld16(to + (uint32_t)(c * 16), o);
+                        ld16<D / 2>(to + (uint32_t)(c * 16), o);
                         wait_ld();
                         if (valid) {
 #pragma unroll
