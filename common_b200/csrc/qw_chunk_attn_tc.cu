@@ -14,10 +14,10 @@
 //
 // Warps (five warpgroups):
 //   0     K and V: TMA boxes of min(page, 128) rows into rings of tc_stages tiles each, one lane per box
-//   1     TMEM and the MMAs: S_t = Q_t K^T, then O_t += P_t V as soon as slot t's softmax has written P_t over S_t;
-//         it also clears the rows of a V block that the sequence never sees (0 x NaN is NaN)
-//   2     Q: one box of (64 columns, G heads, P positions) per 64 columns
-//   3     walks the CTA's share of the line and hands its pieces to the other warps through a ring
+//   1, 2  the MMAs of a slot each: S_t = Q_t K^T, then O_t += P_t V as soon as slot t's softmax has written P_t over S_t;
+//         they also clear the rows of a V block that the sequence never sees (0 x NaN is NaN)
+//   3     walks the CTA's share of the line, hands its pieces to the other warps through a ring, and loads their queries:
+//         one box of (64 columns, G heads, P positions) per 64 columns
 //   4..11 softmax and result of slot 0: a warp has 16 rows, two threads per row (64 keys, and half of the columns of O,
 //         each), so that one warp's loads, maxima and stores run beside another's exponentials; 12..19 of slot 1
 // Every wait is bounded; one that runs out sets the error word and ends the CTA (its copies landed, its TMEM freed).
@@ -76,7 +76,7 @@ struct __align__(16) Smem {
     Piece piece[kPieces];
     Shared shared[2];
     uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages], q_full[2], q_empty[2],
-        s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], done;
+        s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], turn[2], done[2];
     uint32_t tmem;
     float4 xo[2][128 / 4 * kFewRows];  // [slot]: O as float4 columns of kFewRows rows (16-byte aligned by its type)
     float2 xml[2][kFewRows];
@@ -238,14 +238,14 @@ __device__ __forceinline__ void red_release(unsigned *p) {
 }
 __device__ __forceinline__ int uni(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 // whether a phase is over, without the pause of a wait
-__device__ __forceinline__ bool mbar_test(uint32_t addr, uint32_t parity) {
+__device__ __forceinline__ bool mbar_test(uint64_t *b, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(addr), "r"(parity)
+        : "r"(smem_u32(b)), "r"(parity)
         : "memory");
     return ok != 0;
 }
@@ -385,13 +385,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 2 && lane == 0) {
         for (int i = 0; i < NST; i++) {
             mbar_init(&sh.k_full[i], 1);
-            mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.k_empty[i], 2);
             mbar_init(&sh.v_full[i], 1);
-            mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.v_empty[i], 2);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.q_full[i], 1);
-            mbar_init(&sh.q_empty[i], 1);
+            mbar_init(&sh.q_empty[i], 2);
+            mbar_init(&sh.turn[i], 1);
+            mbar_init(&sh.done[i], 1);
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.p_full[i], 8);
             mbar_init(&sh.o_full[i], 1);
@@ -401,9 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < kPieces; i++) {
             mbar_init(&sh.w_full[i], 1);
-            mbar_init(&sh.w_empty[i], 20);  // K / V, Q, the MMA warp for each slot, sixteen softmax warps
+            mbar_init(&sh.w_empty[i], 19);  // K / V, two MMA warps, sixteen softmax warps
         }
-        mbar_init(&sh.done, 1);
         sh.abort = 0;
         sh.empty = 0;
         sh.pre[0] = 0;
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     rem -= __shfl_sync(0xffffffffu, v, 31);
                 }
             }
-            int np = 0, rn = 0, qn = 0, alt = 0;
+            int np = 0, rn = 0, qn = 0, alt = 0, q_sent = 0;
             bool ok = true;
             for (;;) {
                 Piece pc;
@@ -596,6 +597,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 np++;
                 if (pc.flags & kEnd) break;
+                // the piece's queries
+                for (int q = pc.q0; q < pc.q0 + it.nsub && ok; q++) {
+                    const int e = q & 1;
+                    ok = warp_wait(&sh.q_empty[e], ((uint32_t)(q >> 1) & 1u) ^ 1u, abort_flag, a.err);
+                    if (ok && lane == 0) {
+                        mbar_arrive_expect_tx(&sh.q_full[e], (uint32_t)(NH * G * P * 128));
+                        for (int c = 0; c < NH; c++)
+                            tma_load_3d(sQ + e * TILE + c * HALF, &tmQ, &sh.q_full[e], c * 64, ch * G, pc.row0 + (q - pc.q0) * P);
+                        q_sent = q + 1;
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+            }
+            if (*abort_flag && lane == 0) {  // copies in flight land before the shared memory goes away
+                const uint64_t t0 = gtime_ns();
+                for (int k = max(0, q_sent - 2); k < q_sent; k++)
+                    while (!mbar_try(smem_u32(&sh.q_full[k & 1]), (uint32_t)(k >> 1) & 1u) && gtime_ns() - t0 < kTcuWaitCycles / 8) {
+                    }
             }
         } else if (warp == 0) {
             // ---------------- K and V ----------------
@@ -647,157 +667,113 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-        } else if (warp == 1) {
-            // ---------------- MMAs ----------------
+        } else {
+            // ---------------- MMAs: a warp per slot, so that one's waits and commits run beside the other's MMAs ----------------
             constexpr uint32_t IDS = tc_idesc_f16(kRows, kKeys, 0), IDP = tc_idesc_f16(kRows, D, 1);
+            const int t = warp - 1;
             const uint32_t elect = lane == 0 ? 1u : 0u;
             const uint64_t dQ = desc_sw128(smem_u32(sQ), 16, 1024), dK = desc_sw128(smem_u32(sK), 16, 1024),
                            dV = desc_sw128(smem_u32(sV), HALF, 1024);
-            struct Slot {
-                int np, left;         // next piece; visits left in the current one
-                int r, step, q;       // ring index of the visit's block, and of the tile
-                int blk, clo, chi;    // the block's number, and the positions that hold something
-                int visits;           // so far: phase of p_full
-                bool first, one;      // first visit of the piece; single-tile piece
-                bool alone;           // the other slot has no visit in it
-                bool ready;           // the next block's keys have been seen
-            };
-            Slot sl[2];
+            const uint32_t ts = tmem + (uint32_t)(t * kKeys), to = tmem + 256u + (uint32_t)(t * 128);
             bool ok = true;
-            unsigned k_used = 0, v_used = 0, q_used = 0;  // ring entries that one of two slots has used
-            auto next_piece = [&](Slot &s, int t) {
-                for (;;) {
-                    ok = warp_wait(&sh.w_full[s.np % kPieces], (uint32_t)(s.np / kPieces) & 1u, abort_flag, a.err);
-                    if (!ok) { s.left = 0; return; }
-                    const Piece &pc = sh.piece[s.np % kPieces];
-                    const int flags = uni(pc.flags), nblk = uni(pc.nblk);
-                    const int j = flags & kPair ? 0 : uni(pc.alt) ^ t;  // the slot's first block
-                    s.one = !(flags & kPair);
-                    s.step = s.one ? 2 : 1;
-                    s.left = flags & kEnd ? 0 : (nblk - j + s.step - 1) / s.step;
-                    s.r = uni(pc.r0) + j;
-                    s.q = uni(pc.q0) + (s.one ? 0 : t);
-                    s.blk = uni(pc.blk0) + j;
-                    s.clo = uni(pc.clo);
-                    s.chi = uni(pc.chi);
-                    s.first = true;
-                    s.ready = false;
-                    s.alone = nblk == 1;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.w_empty[s.np % kPieces]);
-                    s.np++;
-                    if ((flags & kEnd) || s.left > 0) return;
-                }
+            int visits = 0;  // phase of p_full
+            // A ring entry's barrier says something about use `phase` only after the use before has been released.
+            auto filled = [&](uint64_t *empty, uint64_t *full, int phase) {
+                return warp_wait(empty, ((uint32_t)phase & 1u) ^ 1u, abort_flag, a.err) &&
+                       warp_wait(full, (uint32_t)phase & 1u, abort_flag, a.err);
             };
-            // S_t = Q_t K^T of the slot's current visit into TMEM columns [128 t, 128 t + 128)
-            auto issue_s = [&](Slot &s, int t) {
-                const int st = s.r % NST, qe = s.q & 1;
-                if (s.first) ok = warp_wait(&sh.q_full[qe], (uint32_t)(s.q >> 1) & 1u, abort_flag, a.err);
-                if (ok && !s.ready) ok = warp_wait(&sh.k_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
-                if (!ok) return;
-                tc_fence_after();
-                const uint64_t da = dQ + (uint64_t)(qe * (TILE >> 4)), db = dK + (uint64_t)(st * (TILE >> 4));
-#pragma unroll
-                for (int kk = 0; kk < D / 16; kk++) {
-                    const uint64_t off = (uint64_t)(((kk >> 2) * HALF + (kk & 3) * 32) >> 4);
-                    mma_ss(tmem + (uint32_t)(t * kKeys), da + off, db + off, IDS, kk > 0 ? 1u : 0u, elect);
-                }
-                commit(&sh.s_full[t], elect);  // also covers the slot's PV before it: O_t may be rescaled
-                k_used ^= 1u << st;  // a pair's block is released by the second of its two slots
-                if (s.one) k_used &= ~(1u << st);
-                if (!(k_used >> st & 1u)) commit(&sh.k_empty[st], elect);
-                if (s.left == 1) {  // a single tile serves both slots, where both have visits
-                    if (s.one && !s.alone) q_used ^= 1u << qe;
-                    if (!(q_used >> qe & 1u)) commit(&sh.q_empty[qe], elect);
-                }
+            // On the blocks of two tiles the slots take turns, slot 0 first: interleaved, the MMAs of both would take as long
+            // together, and each slot's softmax would wait for the end of both.  (A single tile is bound by its loads.)
+            int turns = 0;
+            auto take_turn = [&]() {
+                return warp_wait(&sh.turn[t], (uint32_t)(t == 0 ? turns + 1 : turns) & 1u, abort_flag, a.err);
             };
-            // O_t (+)= P_t V of the slot's current visit
-            auto issue_pv = [&](Slot &s, int t) {
-                const int st = s.r % NST;
-                ok = warp_wait(&sh.v_full[st], (uint32_t)(s.r / NST) & 1u, abort_flag, a.err);
-                if (!ok) return;
-                const int k0 = s.blk * kKeys;
-                if (s.chi < k0 + kKeys || s.clo > k0) {
-                    // rows that no row of the sequence sees: P is 0 there, and V must be finite (both slots of a pair
-                    // write the same zeros)
-                    const int z0 = min(kKeys, max(0, s.clo - k0)) * 128, z1 = min(kKeys, max(0, s.chi - k0)) * 128;
+            auto end_turn = [&]() {
+                if (lane == 0) mbar_arrive(&sh.turn[t ^ 1]);
+                turns++;
+            };
+            for (int np = 0; ok; np++) {
+                ok = warp_wait(&sh.w_full[np % kPieces], (uint32_t)(np / kPieces) & 1u, abort_flag, a.err);
+                if (!ok) break;
+                const Piece &pc = sh.piece[np % kPieces];
+                const int flags = uni(pc.flags), nblk = uni(pc.nblk);
+                const bool one = !(flags & kPair);
+                const int j0 = one ? uni(pc.alt) ^ t : 0, step = one ? 2 : 1;  // the slot's first block
+                const int q = uni(pc.q0) + (one ? 0 : t), qe = q & 1, clo = uni(pc.clo), chi = uni(pc.chi);
+                int r = uni(pc.r0) + j0, k0 = (uni(pc.blk0) + j0) * kKeys;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.w_empty[np % kPieces]);
+                if (flags & kEnd) break;
+                if (j0 >= nblk) continue;
+                // S = Q K^T of block j (ring index rs)
+                auto issue_s = [&](int j, int rs) {
+                    const int st = rs % NST;
+                    const uint64_t da = dQ + (uint64_t)(qe * (TILE >> 4)), db = dK + (uint64_t)(st * (TILE >> 4));
 #pragma unroll
-                    for (int hf = 0; hf < NH; hf++) {
-                        uint8_t *v = sV + st * TILE + hf * HALF;
-                        for (int x = lane * 16; x < z0; x += 512) *reinterpret_cast<uint4 *>(v + x) = make_uint4(0, 0, 0, 0);
-                        for (int x = z1 + lane * 16; x < HALF; x += 512) *reinterpret_cast<uint4 *>(v + x) = make_uint4(0, 0, 0, 0);
+                    for (int kk = 0; kk < D / 16; kk++) {
+                        const uint64_t off = (uint64_t)(((kk >> 2) * HALF + (kk & 3) * 32) >> 4);
+                        mma_ss(ts, da + off, db + off, IDS, kk > 0 ? 1u : 0u, elect);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                // (looked at now, so that S of the slot's next block follows this PV at once)
-                const int rn = s.r + s.step;
-                s.ready = s.left > 1 && __all_sync(0xffffffffu, mbar_test(smem_u32(&sh.k_full[rn % NST]), (uint32_t)(rn / NST) & 1u));
-                ok = warp_wait(&sh.p_full[t], (uint32_t)s.visits & 1u, abort_flag, a.err);
-                if (!ok) return;
+                    commit(&sh.s_full[t], elect);  // also covers the slot's PV before it: O may be rescaled
+                    // two arrivals release an entry: of both slots, where both use it
+                    commit(&sh.k_empty[st], elect);
+                    if (one) commit(&sh.k_empty[st], elect);
+                    if (j + step >= nblk) {
+                        commit(&sh.q_empty[qe], elect);
+                        if (!one || nblk == 1) commit(&sh.q_empty[qe], elect);
+                    }
+                };
+                ok = filled(&sh.q_empty[qe], &sh.q_full[qe], q >> 1) && filled(&sh.k_empty[r % NST], &sh.k_full[r % NST], r / NST);
+                if (!ok) break;
                 tc_fence_after();
-                const uint64_t db = dV + (uint64_t)(st * (TILE >> 4));
+                issue_s(j0, r);
+                for (int j = j0; j < nblk; j += step, r += step, k0 += step * kKeys) {
+                    const int st = r % NST, ph = r / NST, rn = r + step, sn = rn % NST, pn = rn / NST;
+                    const bool last = j + step >= nblk;
+                    ok = filled(&sh.v_empty[st], &sh.v_full[st], ph);
+                    if (!ok) break;
+                    if (chi < k0 + kKeys || clo > k0) {
+                        // rows that no row of the sequence sees: P is 0 there, and V must be finite (both slots of a
+                        // pair write the same zeros)
+                        const int z0 = min(kKeys, max(0, clo - k0)) * 128, z1 = min(kKeys, max(0, chi - k0)) * 128;
 #pragma unroll
-                for (int kk = 0; kk < kKeys / 16; kk++)  // P's halves lie over their own halves of S
-                    mma_ts(tmem + 256u + (uint32_t)(t * 128), tmem + (uint32_t)(t * kKeys + (kk & 3) * 8 + (kk >> 2) * 64),
-                           db + (uint64_t)(kk * 2048 >> 4), IDP, kk > 0 ? 1u : (s.first ? 0u : 1u), elect);
-                s.visits++;
-                v_used ^= 1u << st;
-                if (s.one) v_used &= ~(1u << st);
-                if (!(v_used >> st & 1u)) commit(&sh.v_empty[st], elect);
-                if (s.left == 1) commit(&sh.o_full[t], elect);
-                s.first = false;
-                s.r += s.step;
-                s.blk += s.step;
-                s.left--;
-            };
+                        for (int hf = 0; hf < NH; hf++) {
+                            uint8_t *v = sV + st * TILE + hf * HALF;
+                            for (int x = lane * 16; x < z0; x += 512) *reinterpret_cast<uint4 *>(v + x) = make_uint4(0, 0, 0, 0);
+                            for (int x = z1 + lane * 16; x < HALF; x += 512) *reinterpret_cast<uint4 *>(v + x) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    // the next block's keys, if they are there already: S then follows this PV at once
+                    bool next = !last && mbar_test(&sh.k_empty[sn], ((uint32_t)pn & 1u) ^ 1u) && mbar_test(&sh.k_full[sn], (uint32_t)pn & 1u);
+                    next = __all_sync(0xffffffffu, next);
+                    ok = warp_wait(&sh.p_full[t], (uint32_t)visits++ & 1u, abort_flag, a.err) && (one || take_turn());
+                    if (!ok) break;
+                    tc_fence_after();
+                    // O (+)= P V
+                    const uint64_t dv = dV + (uint64_t)(st * (TILE >> 4));
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                sl[t].np = sl[t].visits = sl[t].left = 0;
-                if (ok) next_piece(sl[t], t);
-                if (ok && sl[t].left) issue_s(sl[t], t);
-            }
-            while (ok && (sl[0].left || sl[1].left)) {
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    Slot &s = sl[t];
-                    if (!ok || !s.left) continue;
-                    issue_pv(s, t);
-                    if (ok && !s.left) next_piece(s, t);
-                    if (ok && s.left) issue_s(s, t);
+                    for (int kk = 0; kk < kKeys / 16; kk++)  // P's halves lie over their own halves of S
+                        mma_ts(to, ts + (uint32_t)((kk & 3) * 8 + (kk >> 2) * 64), dv + (uint64_t)(kk * 2048 >> 4), IDP,
+                               kk > 0 ? 1u : (j > j0 ? 1u : 0u), elect);
+                    if (next) issue_s(j + step, rn);
+                    commit(&sh.v_empty[st], elect);
+                    if (one) commit(&sh.v_empty[st], elect);
+                    if (last) commit(&sh.o_full[t], elect);
+                    if (!one) end_turn();
+                    if (!last && !next) {
+                        ok = filled(&sh.k_empty[sn], &sh.k_full[sn], pn);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_s(j + step, rn);
+                    }
                 }
             }
             // every MMA of this CTA has completed before the TMEM is freed
-            commit(&sh.done, elect);
+            commit(&sh.done[t], elect);
             const uint64_t t0 = gtime_ns();
-            while (!mbar_try(smem_u32(&sh.done), 0) && gtime_ns() - t0 < kTcuWaitCycles) {
-            }
-        } else {
-            // ---------------- Q ----------------
-            int q = 0;
-            bool ok = true;
-            if (lane == 0) {
-                for (int np = 0; ok; np++) {
-                    if (!mbar_wait(&sh.w_full[np % kPieces], (uint32_t)(np / kPieces) & 1u, abort_flag, a.err)) break;
-                    const Piece &pc = sh.piece[np % kPieces];
-                    const int flags = pc.flags, row0 = pc.row0, kvh = pc.kvh;
-                    mbar_arrive(&sh.w_empty[np % kPieces]);
-                    if (flags & kEnd) break;
-                    for (int t = 0; t < (flags & kPair ? 2 : 1); t++, q++) {
-                        const int e = q & 1;
-                        ok = mbar_wait(&sh.q_empty[e], ((uint32_t)(q >> 1) & 1u) ^ 1u, abort_flag, a.err);
-                        if (!ok) break;
-                        mbar_arrive_expect_tx(&sh.q_full[e], (uint32_t)(NH * G * P * 128));
-                        for (int c = 0; c < NH; c++)
-                            tma_load_3d(sQ + e * TILE + c * HALF, &tmQ, &sh.q_full[e], c * 64, kvh * G, row0 + t * P);
-                    }
-                }
-                if (*abort_flag) {
-                    const uint64_t t0 = gtime_ns();
-                    for (int k = max(0, q - 2); k < q; k++)
-                        while (!mbar_try(smem_u32(&sh.q_full[k & 1]), (uint32_t)(k >> 1) & 1u) && gtime_ns() - t0 < kTcuWaitCycles / 8) {
-                        }
-                }
+            while (!mbar_try(smem_u32(&sh.done[t]), 0) && gtime_ns() - t0 < kTcuWaitCycles) {
             }
         }
     } else {
