@@ -18,15 +18,22 @@ namespace qw {
 namespace {
 
 constexpr int kSiRows = 64, kSiKeys = 64, kSiThreads = 256;
+constexpr int kSiMaxCtas = 2 * kNumSMsB200;  // of a launch that splits keys: its partial results lie in the workspace
 
-// One CTA per (64 rows of a sequence's (position, head of the group) list, KV head): q, K and V tiles in shared memory
-// as fp32, a 4 x 4 block of scores and 4 x (D / 16) of the output per thread.
-template <typename T, int D>
-__global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const ChunkArgs a) {
+__host__ __device__ constexpr size_t si_part_bytes(int d) { return (size_t)kSiRows * (d + 2) * 4; }
+
+// One CTA per (64 rows of a sequence's (position, head of the group) list, KV head, range of its keys): q, K and V tiles
+// in shared memory, a 4 x 4 block of scores and 4 x (D / 16) of the output per thread.  Where the rows alone do not fill
+// the GPU the keys are split, and the last CTA of a tile to finish joins the ranges in their order (no sum depends on who
+// came when).  fp32 caches have no tensor-core path in this library; the arithmetic of 64 x 64 x D tiles bounds this
+// kernel: 13.5 TFLOP/s (512 rows over 4000 positions, 32 heads).
+template <int D>
+__global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const ChunkArgs a, int nsplit) {
     extern __shared__ float si_smem[];
     constexpr int LD = D + 4;
     float *sq = si_smem, *sk = sq + kSiRows * LD, *sv = sk + kSiKeys * LD, *sp = sv + kSiKeys * LD;
     __shared__ float s_m[kSiRows], s_l[kSiRows], s_alpha[kSiRows];
+    __shared__ bool s_last;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int G = a.G, kvh = blockIdx.y;
     int b = 0, tile = blockIdx.x, n = 0;
@@ -40,16 +47,17 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const Ch
     const int r0 = a.row_start[b], kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps);
     const int p0 = kv - n, first = tile * kSiRows, last = min(first + kSiRows, n * G) - 1;
     const int *table = a.page_table + (size_t)(a.slots ? a.slots[b] : b) * a.max_pages;
-    const T *q = reinterpret_cast<const T *>(a.q);
-    const T *kc = reinterpret_cast<const T *>(a.k), *vc = reinterpret_cast<const T *>(a.v);
+    const float *q = (const float *)a.q, *kc = (const float *)a.k, *vc = (const float *)a.v;
     for (int i = tid; i < kSiRows * D; i += kSiThreads) {
         const int r = i / D, c = i % D, pr = first + r;
-        sq[r * LD + c] = pr <= last ? Elt<T>::load(q + (size_t)(r0 + pr / G) * a.ld_q + (size_t)(kvh * G + pr % G) * D + c) : 0.f;
+        sq[r * LD + c] = pr <= last ? q[(size_t)(r0 + pr / G) * a.ld_q + (size_t)(kvh * G + pr % G) * D + c] : 0.f;
     }
     if (tid < kSiRows) { s_m[tid] = -INFINITY; s_l[tid] = 0.f; }
     float o[4][D / 16] = {};
     const int lo = a.window ? max(0, p0 + first / G - a.window + 1) : 0;
-    for (int k0 = lo / kSiKeys * kSiKeys; k0 <= p0 + last / G; k0 += kSiKeys) {
+    const int b0 = lo / kSiKeys, nb = p0 + last / G < 0 ? 0 : (p0 + last / G) / kSiKeys + 1 - b0;
+    const int kend = (b0 + (int)((long long)nb * (blockIdx.z + 1) / nsplit)) * kSiKeys;
+    for (int k0 = (b0 + (int)((long long)nb * blockIdx.z / nsplit)) * kSiKeys; k0 < kend; k0 += kSiKeys) {
         __syncthreads();
         for (int i = tid; i < kSiKeys * D; i += kSiThreads) {
             const int r = i / D, c = i % D, pos = k0 + r;
@@ -58,8 +66,8 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const Ch
                 const int pg = table[pos >> a.log2_ps];
                 if ((unsigned)pg < (unsigned)a.num_pages) {
                     const size_t at = (((size_t)pg * a.Hkv + kvh) * a.ps + (pos & (a.ps - 1))) * D + c;
-                    kx = Elt<T>::load(kc + at);
-                    vx = Elt<T>::load(vc + at);
+                    kx = kc[at];
+                    vx = vc[at];
                 }
             }
             sk[r * LD + c] = kx;
@@ -120,35 +128,248 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const Ch
             }
     }
     __syncthreads();
+    if (nsplit > 1) {
+        // partial results: O [row][D], then maximum and sum
+        const int tile_id = blockIdx.y * gridDim.x + blockIdx.x;
+        unsigned *counter = reinterpret_cast<unsigned *>(a.workspace) + tile_id;
+        char *parts = (char *)a.workspace + kChunkCounterBytes + (size_t)tile_id * nsplit * si_part_bytes(D);
+        float *mine = reinterpret_cast<float *>(parts + blockIdx.z * si_part_bytes(D));
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int c = 0; c < D / 16; c++) mine[(ty * 4 + i) * D + tx + 16 * c] = o[i][c];
+        if (tid < kSiRows) {
+            mine[kSiRows * D + tid] = s_m[tid];
+            mine[kSiRows * (D + 1) + tid] = s_l[tid];
+        }
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            s_last = atomicAdd(counter, 1u) == (unsigned)nsplit - 1u;
+            if (s_last) *counter = 0u;
+        }
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        if (tid < kSiRows) s_m[tid] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = ty * 4 + i;
+            float m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 16; c++) o[i][c] = 0.f;
+            for (int z = 0; z < nsplit; z++) {
+                const float *p = reinterpret_cast<const float *>(parts + z * si_part_bytes(D));
+                const float pm = __ldcg(p + kSiRows * D + r);
+                if (pm == -INFINITY) continue;  // this range showed the row nothing
+                const float mn = fmaxf(m, pm), wo = exp2f(m - mn), wp = exp2f(pm - mn);
+                l = l * wo + __ldcg(p + kSiRows * (D + 1) + r) * wp;
+#pragma unroll
+                for (int c = 0; c < D / 16; c++) o[i][c] = o[i][c] * wo + __ldcg(p + r * D + tx + 16 * c) * wp;
+                m = mn;
+            }
+            __syncwarp();
+            if (tx == 0) { s_m[r] = m; s_l[r] = l; }
+        }
+        __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int pr = first + ty * 4 + i;
         if (pr > last) continue;
         const float l = s_l[ty * 4 + i], inv = l > 0.f ? 1.f / l : 0.f;
         const size_t row = (size_t)(r0 + pr / G), head = (size_t)(kvh * G + pr % G);
-        T *out = reinterpret_cast<T *>(a.out) + row * a.ld_out + head * D;
+        float *out = (float *)a.out + row * a.ld_out + head * D;
 #pragma unroll
-        for (int c = 0; c < D / 16; c++) Elt<T>::store(out + tx + 16 * c, l == 0.f ? 0.f : o[i][c] * inv);
+        for (int c = 0; c < D / 16; c++) out[tx + 16 * c] = l == 0.f ? 0.f : o[i][c] * inv;
         if (a.lse && tx == 0)
             a.lse[row * a.H + head] = l > 0.f ? (s_m[ty * 4 + i] + log2f(l)) * 0.69314718055994531f : l == 0.f ? -INFINITY : l;
     }
 }
 
-template <typename T, int D>
+// Few rows per sequence (decoding): one CTA per (row, KV head, range of its keys).  A warp takes 4 steps of 32 / (D / 4) keys
+// at a time, D / 4 lanes a key (its 16 bytes per lane are one coalesced row of the cache), the dot products of the group's R
+// heads are summed across those lanes, and every lane keeps its columns of the R outputs.  Bound by HBM: the lanes' sums
+// are about 5 R shuffles a key for 8 D bytes.
+template <int D, int R>
+__global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_rows_kernel(const ChunkArgs a, int nsplit) {
+    constexpr int LK = D / 4, KPS = 32 / LK, W = kSiThreads / 32;
+    __shared__ float4 s_o[W][R][32];
+    __shared__ float s_m[W][R], s_l[W][R];
+    __shared__ bool s_last;
+    const int row = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int sub = lane / LK, c = (lane % LK) * 4, G = a.G;
+    int b = 0, e = a.batch - 1;  // the sequence that the row belongs to: the last that begins at or before it
+    while (b < e) {
+        const int mid = (b + e + 1) >> 1;
+        if (a.row_start[mid] <= row) b = mid;
+        else e = mid - 1;
+    }
+    if (a.row_start[b] > row || a.row_start[b + 1] <= row) return;
+    const int kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps);
+    const int pos = kv - (min(a.row_start[b + 1], a.rows) - row);
+    const int lo = a.window ? max(0, pos - a.window + 1) : 0, n = pos + 1 - lo;
+    const int k_begin = n > 0 ? lo + (int)((long long)n * blockIdx.z / nsplit) : 0;
+    const int k_end = n > 0 ? lo + (int)((long long)n * (blockIdx.z + 1) / nsplit) : 0;
+    const int *table = a.page_table + (size_t)(a.slots ? a.slots[b] : b) * a.max_pages;
+    const float *kc = (const float *)a.k, *vc = (const float *)a.v;
+    float4 q[R], o[R];
+    float m[R], l[R];
+#pragma unroll
+    for (int h = 0; h < R; h++) {
+        q[h] = o[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h < G) q[h] = *reinterpret_cast<const float4 *>((const float *)a.q + (size_t)row * a.ld_q + (size_t)(kvh * G + h) * D + c);
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+    }
+    for (int k0 = k_begin + warp * 4 * KPS; k0 < k_end; k0 += W * 4 * KPS) {
+        float4 k[4], v[4];
+        bool sees[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int key = k0 + u * KPS + sub;
+            sees[u] = key < k_end;
+            k[u] = v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int pg = sees[u] ? table[key >> a.log2_ps] : -1;
+            if ((unsigned)pg < (unsigned)a.num_pages) {
+                const size_t at = (((size_t)pg * a.Hkv + kvh) * a.ps + (key & (a.ps - 1))) * D + c;
+                k[u] = *reinterpret_cast<const float4 *>(kc + at);
+                v[u] = *reinterpret_cast<const float4 *>(vc + at);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < R; h++) {
+            float s[4], mx = m[h];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                s[u] = q[h].x * k[u].x + q[h].y * k[u].y + q[h].z * k[u].z + q[h].w * k[u].w;
+#pragma unroll
+                for (int w = LK / 2; w > 0; w >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+                s[u] = sees[u] ? s[u] * a.sl2 : -INFINITY;
+                mx = fmaxf(mx, s[u]);
+            }
+            const float mu = mx == -INFINITY ? 0.f : mx, al = exp2f(m[h] - mu);
+            l[h] *= al;
+            o[h].x *= al; o[h].y *= al; o[h].z *= al; o[h].w *= al;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float p = exp2f(s[u] - mu);
+                l[h] += p;
+                o[h].x += p * v[u].x; o[h].y += p * v[u].y; o[h].z += p * v[u].z; o[h].w += p * v[u].w;
+            }
+            m[h] = mx;
+        }
+    }
+    // join the lanes that took different keys, then the warps, then (the last CTA of the row) the ranges
+    auto join = [](float &m0, float &l0, float4 &o0, float m1, float l1, const float4 &o1) {
+        if (m1 == -INFINITY) return;
+        const float mn = fmaxf(m0, m1), w0 = exp2f(m0 - mn), w1 = exp2f(m1 - mn);
+        l0 = l0 * w0 + l1 * w1;
+        o0 = make_float4(o0.x * w0 + o1.x * w1, o0.y * w0 + o1.y * w1, o0.z * w0 + o1.z * w1, o0.w * w0 + o1.w * w1);
+        m0 = mn;
+    };
+#pragma unroll
+    for (int h = 0; h < R; h++) {
+#pragma unroll
+        for (int w = LK; w < 32; w <<= 1) {
+            const float m1 = __shfl_xor_sync(0xffffffffu, m[h], w), l1 = __shfl_xor_sync(0xffffffffu, l[h], w);
+            const float4 o1 = make_float4(__shfl_xor_sync(0xffffffffu, o[h].x, w), __shfl_xor_sync(0xffffffffu, o[h].y, w),
+                                          __shfl_xor_sync(0xffffffffu, o[h].z, w), __shfl_xor_sync(0xffffffffu, o[h].w, w));
+            join(m[h], l[h], o[h], m1, l1, o1);
+        }
+        s_o[warp][h][lane] = o[h];
+        if (lane == 0) { s_m[warp][h] = m[h]; s_l[warp][h] = l[h]; }
+    }
+    __syncthreads();
+    const int id = blockIdx.y * gridDim.x + blockIdx.x;
+    unsigned *counter = reinterpret_cast<unsigned *>(a.workspace) + id;
+    float *parts = reinterpret_cast<float *>((char *)a.workspace + kChunkCounterBytes) + (size_t)id * nsplit * R * (D + 2);
+    for (int h = warp; h < R; h += W) {
+        float mm = -INFINITY, ll = 0.f;
+        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < W; w++) join(mm, ll, oo, s_m[w][h], s_l[w][h], s_o[w][h][lane]);
+        if (nsplit > 1) {
+            float *p = parts + ((size_t)blockIdx.z * R + h) * (D + 2);
+            if (lane < LK) {
+                p[c] = oo.x; p[c + 1] = oo.y; p[c + 2] = oo.z; p[c + 3] = oo.w;
+            }
+            if (lane == 0) { p[D] = mm; p[D + 1] = ll; }
+        } else {
+            s_o[0][h][lane] = oo;
+            if (lane == 0) { s_m[0][h] = mm; s_l[0][h] = ll; }
+        }
+    }
+    if (nsplit > 1) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            s_last = atomicAdd(counter, 1u) == (unsigned)nsplit - 1u;
+            if (s_last) *counter = 0u;
+        }
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+    }
+    for (int h = warp; h < G; h += W) {
+        float mm = -INFINITY, ll = 0.f;
+        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (nsplit > 1) {
+            for (int z = 0; z < nsplit; z++) {
+                const float *p = parts + ((size_t)z * R + h) * (D + 2);
+                join(mm, ll, oo, __ldcg(p + D), __ldcg(p + D + 1),
+                     make_float4(__ldcg(p + c), __ldcg(p + c + 1), __ldcg(p + c + 2), __ldcg(p + c + 3)));
+            }
+        } else {
+            mm = s_m[0][h]; ll = s_l[0][h]; oo = s_o[0][h][lane];
+        }
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        const size_t head = (size_t)(kvh * G + h);
+        if (lane < LK)
+            *reinterpret_cast<float4 *>((float *)a.out + (size_t)row * a.ld_out + head * D + c) =
+                ll == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(oo.x * inv, oo.y * inv, oo.z * inv, oo.w * inv);
+        if (a.lse && lane == 0) a.lse[(size_t)row * a.H + head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+    }
+}
+
+template <int D, int R>
+cudaError_t rows_launch(const ChunkArgs &a, cudaStream_t st) {
+    // ranges of 128 keys at least, and as many CTAs as fill the GPU four times
+    const long long ctas = (long long)a.rows * a.Hkv, blocks = ((long long)a.max_pages * a.ps + 127) / 128;
+    long long nsplit = 4 * kSiMaxCtas / 2 / ctas;
+    if (nsplit > blocks) nsplit = blocks;
+    if (nsplit < 1) nsplit = 1;
+    qw_chunk_attn_rows_kernel<D, R><<<dim3(a.rows, a.Hkv, (unsigned)nsplit), kSiThreads, 0, st>>>(a, (int)nsplit);
+    return cudaGetLastError();
+}
+
+template <int D>
 cudaError_t simt_launch(const ChunkArgs &a, cudaStream_t st) {
+    // Up to two rows a sequence: the rows' kernel reads the cache once per row; above, the tiles' once per 64 / G rows.
+    // 8 sequences of one row at 4000 positions, 4 heads per KV head: 987 us by tiles, 87 us (3.0 TB/s)
+    // by rows.
+    if (a.G <= 8 && a.rows <= 2 * (long long)a.batch) {
+        if (a.G == 1) return rows_launch<D, 1>(a, st);
+        if (a.G == 2) return rows_launch<D, 2>(a, st);
+        if (a.G <= 4) return rows_launch<D, 4>(a, st);
+        return rows_launch<D, 8>(a, st);
+    }
     const int smem = (3 * kSiRows * (D + 4) + kSiRows * (kSiKeys + 1)) * (int)sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(qw_chunk_attn_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(qw_chunk_attn_simt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     // at most one tile more than the whole ones for every sequence
     const long long tiles = (long long)a.rows * a.G / kSiRows + a.batch;
-    qw_chunk_attn_simt_kernel<T, D><<<dim3((unsigned)tiles, a.Hkv), kSiThreads, smem, st>>>(a);
+    const long long blocks = ((long long)a.max_pages * a.ps + kSiKeys - 1) / kSiKeys;
+    long long nsplit = kSiMaxCtas / (tiles * a.Hkv);
+    if (nsplit > blocks) nsplit = blocks;
+    if (nsplit < 1) nsplit = 1;
+    qw_chunk_attn_simt_kernel<D><<<dim3((unsigned)tiles, a.Hkv, (unsigned)nsplit), kSiThreads, smem, st>>>(a, (int)nsplit);
     return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t chunk_attn_simt_launch(const ChunkArgs &a, cudaStream_t st) {
-    return a.d == 128 ? simt_launch<float, 128>(a, st) : simt_launch<float, 64>(a, st);
+    return a.d == 128 ? simt_launch<128>(a, st) : simt_launch<64>(a, st);
 }
 
 }  // namespace qw

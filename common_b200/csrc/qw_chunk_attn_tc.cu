@@ -23,7 +23,7 @@
 // Every wait is bounded; one that runs out sets the error word and ends the CTA (its copies landed, its TMEM freed).
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <mutex>
+#include <atomic>
 
 #include "../../include/qwen3_b200.h"
 #include "qw_chunk_attn.h"
@@ -40,7 +40,8 @@ constexpr int kPieces = 4;       // ring of pieces
 constexpr int kFewRows = 8;      // rows of an exchange in shared memory: a token's heads of one KV head
 constexpr int kItemUnits = 2;    // what a tile costs beside its blocks
 constexpr int kMinShare = 5;     // units that a CTA beyond one per item is worth: splitting an item costs about as much
-constexpr int kCounterWords = 256;  // arrivals | departures | arrivals at items cut once, one word per CTA each
+constexpr int kCounterWords = 256;  // arrivals | arrivals at items cut once | departures, one word per CTA each
+static_assert(3 * kCounterWords * 4 == kChunkCounterBytes && kNumSMsB200 <= kCounterWords, "counters");
 
 __host__ __device__ constexpr int tc_stages(int d) { return d == 128 ? 2 : 5; }
 __host__ __device__ constexpr int tc_tile_bytes(int d) { return kRows * d * 2; }
@@ -265,7 +266,7 @@ struct Part {
 // through shared memory); k: tile, or slot in turn
 template <int D>
 __device__ __forceinline__ Part<D> part_of(const ChunkArgs &a, int cta, int which, int k) {
-    return Part<D>{(char *)a.workspace + 3 * kCounterWords * 4 + ((size_t)cta * 6 + which * 2 + k) * part_bytes(D)};
+    return Part<D>{(char *)a.workspace + kChunkCounterBytes + ((size_t)cta * 6 + which * 2 + k) * part_bytes(D)};
 }
 
 template <int D>
@@ -1149,21 +1150,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int D>
 cudaError_t launch(const ChunkArgs &a, cudaStream_t st) {
     constexpr int smem = (2 + 2 * tc_stages(D)) * tc_tile_bytes(D) + 1024;
-    int dev = 0, sms = 0;
+    int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    {
-        static std::mutex mu;
-        static bool prepared[64] = {};
-        std::lock_guard<std::mutex> lk(mu);
-        if (!prepared[dev]) {
-            e = cudaFuncSetAttribute(qw_chunk_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-            if (e != cudaSuccess) return e;
-            prepared[dev] = true;
-        }
+    static std::atomic<int> grids[64];  // CTAs of a launch on each device, once its kernel has been prepared
+    int grid = grids[dev].load(std::memory_order_acquire);
+    if (!grid) {
+        e = cudaFuncSetAttribute(qw_chunk_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        e = cudaDeviceGetAttribute(&grid, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+        grid = grid < kNumSMsB200 ? grid : kNumSMsB200;
+        grids[dev].store(grid, std::memory_order_release);
     }
     CUtensorMap mq, mk, mv;
     const int P = kRows / a.G, br = a.ps < kKeys ? a.ps : kKeys;
@@ -1172,7 +1171,7 @@ cudaError_t launch(const ChunkArgs &a, cudaStream_t st) {
     if ((e = tma_map_bf16_sw128(&mk, a.k, crow, a.d, a.d, br)) != cudaSuccess) return e;
     if ((e = tma_map_bf16_sw128(&mv, a.v, crow, a.d, a.d, br)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms < kNumSMsB200 ? sms : kNumSMsB200);
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -1190,6 +1189,6 @@ cudaError_t chunk_attn_tc_launch(const ChunkArgs &a, cudaStream_t st) {
     return a.d == 128 ? launch<128>(a, st) : launch<64>(a, st);
 }
 
-size_t chunk_attn_tc_workspace(int head_dim) { return 3 * kCounterWords * 4 + (size_t)kNumSMsB200 * 6 * part_bytes(head_dim); }
+size_t chunk_attn_tc_workspace(int head_dim) { return kChunkCounterBytes + (size_t)kNumSMsB200 * 6 * part_bytes(head_dim); }
 
 }  // namespace qw

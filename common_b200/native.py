@@ -229,7 +229,7 @@ class ChunkAttention:
 
 def op_kv_copy_pages(pool: KvPool, src_ptr: int, dst_ptr: int, rows_ptr: int, n: int, stream: int = 0) -> None:
     """qw_op_kv_copy_pages over raw device pointers (rows_ptr 0: whole pages)."""
-    st = load().qw_op_kv_copy_pages(C.byref(pool), src_ptr, dst_ptr, rows_ptr or None, n, stream or None)
+    st = (_lib or load()).qw_op_kv_copy_pages(pool, src_ptr, dst_ptr, rows_ptr, n, stream)
     if st:
         raise QwenError(st, op_error())
 
@@ -237,8 +237,8 @@ def op_kv_copy_pages(pool: KvPool, src_ptr: int, dst_ptr: int, rows_ptr: int, n:
 def op_kv_compact(pool: KvPool, src_table: int, dst_table: int, max_pages: int, keep: int, keep_start: int, batch: int,
                   rows: int, rope: int = 0, rope_len: int = 0, dst_base: int = 0, stream: int = 0) -> None:
     """qw_op_kv_compact over raw device pointers."""
-    st = load().qw_op_kv_compact(C.byref(pool), src_table, dst_table, max_pages, keep, keep_start, dst_base or None,
-                                 batch, rows, rope or None, rope_len, stream or None)
+    st = (_lib or load()).qw_op_kv_compact(pool, src_table, dst_table, max_pages, keep, keep_start, dst_base, batch, rows,
+                                           rope, rope_len, stream)
     if st:
         raise QwenError(st, op_error())
 

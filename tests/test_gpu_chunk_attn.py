@@ -237,3 +237,43 @@ def test_without_lse():
     assert bool((c.lse == -7.0).all())
     c.run()
     c.check()
+
+
+def test_a_cache_past_32_bit_offsets():
+    """More than 2^32 bytes of keys (and of values): sequences in the pool's first and last pages."""
+    torch = _torch()
+    c = Case([1, 40], [200, 300], 32, 8, 128, 64, seed=9)
+    pages = 36000
+    k = torch.zeros((pages, 8, 64, 128), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    assert k.numel() * 2 > 2 ** 32
+    used = sorted({int(x) for x in c.table.flatten().tolist() if x >= 0})
+    where = {p: (i if i % 2 else pages - 1 - i) for i, p in enumerate(used)}
+    for p, to in where.items():
+        k[to], v[to] = c.k[p], c.v[p]
+    table = c.table.tolist()
+    c.table = torch.tensor([[where.get(x, -1) for x in r] for r in table], dtype=torch.int32, device="cuda")
+    c.k, c.v = k, v
+    c.attn.args.num_pages = pages
+    c.run()
+    c.check()
+
+
+def test_lengths_beyond_the_table_and_wild_page_numbers_stay_in_bounds():
+    torch = _torch()
+    c = Case([3, 2], [100, 60], 16, 8, 128, 64, seed=10)
+    c.kv_len[0] = 1 << 30                       # clamped to what the table can name
+    c.table[1, 0] = 1 << 30                     # slot of sequence 1: not a page, read as zeros
+    c.run()
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 0 and bool((c.obuf[5:] == -7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_many_sequences(dtype):
+    """More sequences than CTAs and than one warp's lanes, some without rows."""
+    new = [i % 3 for i in range(300)]
+    kv = [n and n + (37 * i) % 500 for i, n in enumerate(new)]
+    c = Case(new, kv, 16, 8, 128, 64, dtype=dtype, seed=11)
+    c.run()
+    c.check()
