@@ -415,9 +415,12 @@ extern "C" qw_status qw_op_chunk_attn(const qw_chunk_attn_args *p, void *stream)
     a.workspace = p->workspace;
     a.ld_q = ld_q; a.ld_out = ld_out;
     a.batch = p->batch; a.rows = p->rows; a.H = p->heads; a.Hkv = p->kv_heads; a.G = p->heads / p->kv_heads;
-    a.d = p->head_dim; a.ps = p->page_size; a.num_pages = p->num_pages; a.max_pages = p->max_pages; a.window = p->window;
+    a.d = p->head_dim; a.ps = p->page_size; a.num_pages = p->num_pages; a.max_pages = p->max_pages;
+    a.window = p->window < (long long)p->max_pages * p->page_size ? p->window : 0;  // as long as a slot: it cuts nothing off
     a.log2_ps = 0;
     while ((1 << a.log2_ps) < a.ps) a.log2_ps++;
+    if (p->dtype == QW_DTYPE_BF16 && chunk_attn_tc_most_units(a) > 0xFFFFFFFFull)
+        return op_fail(QW_ERR_SHAPE, "rows over max_pages pages are too many key blocks for one call");
     const float scale = p->scale > 0.f ? p->scale : (float)(1.0 / sqrt((double)p->head_dim));
     a.sl2 = scale * 1.4426950408889634f;
     cudaError_t e = p->dtype == QW_DTYPE_BF16 ? chunk_attn_tc_launch(a, (cudaStream_t)stream)

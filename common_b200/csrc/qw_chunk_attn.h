@@ -24,5 +24,7 @@ struct ChunkArgs {
 cudaError_t chunk_attn_tc_launch(const ChunkArgs &a, cudaStream_t st);    // bf16 (qw_chunk_attn_tc.cu)
 cudaError_t chunk_attn_simt_launch(const ChunkArgs &a, cudaStream_t st);  // fp32 (qw_chunk_attn.cu)
 size_t chunk_attn_tc_workspace(int head_dim);
+// more units than the line of any lengths of these arguments has (the kernel numbers them in 32 bits)
+uint64_t chunk_attn_tc_most_units(const ChunkArgs &a);
 
 }  // namespace qw

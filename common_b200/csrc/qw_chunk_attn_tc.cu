@@ -106,6 +106,30 @@ __device__ __forceinline__ Item make_item(const Seq &s, int i, int P, int window
     return it;
 }
 
+// sum of floor((a i + b) / 128) over i in [0, n), a even and positive, b >= 0: floor(x / 128) = (x - x mod 128) / 128, and the
+// remainders repeat every 128 / gcd(a, 128) terms
+__device__ __forceinline__ unsigned floor_sum(unsigned n, unsigned a, unsigned b) {
+    const unsigned g = min(a & (0u - a), (unsigned)kKeys), p = kKeys / g, r = n & (p - 1);
+    unsigned long long rest = (unsigned long long)((n - r) / p) * (p * (b & (g - 1)) + g * p * (p - 1) / 2);
+    for (unsigned i = 0, x = b & (kKeys - 1); i < r; i++, x = (x + a) & (kKeys - 1)) rest += x;
+    return (unsigned)(((unsigned long long)n * (n - 1) / 2 * a + (unsigned long long)n * b - rest) / kKeys);
+}
+// units of a sequence of ni > 0 items and one KV head: all items but the last have two whole tiles
+__device__ __forceinline__ unsigned seq_units(const Seq &s, int ni, int gone, int P, int window) {
+    const int p0 = s.kv - s.n, m = max(0, ni - 1 - gone), step = 2 * P;  // m whole items from item `gone` on see something
+    unsigned u = make_item(s, ni - 1, P, window).units();
+    if (m > 0) {
+        unsigned blocks = floor_sum(m, step, p0 + step * (gone + 1) - 1) + m * (1 + kItemUnits);
+        if (window) {
+            const int before = window - 1 - p0;  // rows that see from the first position on
+            const int i = max(gone, before > 0 ? (before + step - 1) / step : 0);
+            if (i < ni - 1) blocks -= floor_sum(ni - 1 - i, step, step * i - before);
+        }
+        u += 2 * blocks;
+    }
+    return u;
+}
+
 // the line of W units in Ge shares: the first W % Ge of them one unit longer
 struct Line {
     unsigned q, rem;
@@ -448,20 +472,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (s.n > s.kv) sh.empty = 1;
                 const int ni = s.n <= 2 * P ? s.n > 0 : (s.n + 2 * P - 1) / (2 * P);
-                unsigned units = 0;
-                if (ni <= 2)
-                    for (int i = 0; i < ni; i++) units += make_item(s, i, P, a.window).units();
-                // long chunks: the whole warp on one sequence after the other
-                for (unsigned m = __ballot_sync(0xffffffffu, ni > 2); m; m &= m - 1) {
-                    const int l = __ffs(m) - 1;
-                    const Seq t{__shfl_sync(0xffffffffu, s.n, l), __shfl_sync(0xffffffffu, s.kv, l), 0};
-                    const int n = __shfl_sync(0xffffffffu, ni, l);
-                    unsigned u = 0;
-                    for (int i = lane; i < n; i += 32) u += make_item(t, i, P, a.window).units();
-                    u = __reduce_add_sync(0xffffffffu, u);
-                    if (lane == l) units = u;
-                }
                 const int gone = s.n > s.kv ? (s.n - s.kv) / (2 * P) : 0;  // items before the first position
+                const unsigned units = ni ? seq_units(s, ni, gone, P, a.window) : 0;
                 items += __reduce_add_sync(0xffffffffu, s.kv > 0 ? (ni - gone) * a.Hkv : 0);
                 unsigned v = units * a.Hkv;
 #pragma unroll
@@ -1187,6 +1199,12 @@ cudaError_t launch(const ChunkArgs &a, cudaStream_t st) {
 
 cudaError_t chunk_attn_tc_launch(const ChunkArgs &a, cudaStream_t st) {
     return a.d == 128 ? launch<128>(a, st) : launch<64>(a, st);
+}
+
+uint64_t chunk_attn_tc_most_units(const ChunkArgs &a) {
+    const uint64_t step = 2 * (kRows / a.G), items = a.rows / step + a.batch, cap = (uint64_t)a.max_pages << a.log2_ps;
+    const uint64_t seen = a.window && a.window + step < cap ? a.window + step : cap;
+    return items * 2 * (seen / kKeys + 2 + kItemUnits) * a.Hkv;
 }
 
 size_t chunk_attn_tc_workspace(int head_dim) { return kChunkCounterBytes + (size_t)kNumSMsB200 * 6 * part_bytes(head_dim); }

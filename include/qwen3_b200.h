@@ -369,9 +369,11 @@ typedef struct qw_chunk_attn_args {
  * that sees nothing gives zeros and an lse of -infinity.  What lies in the cache outside the positions that some row
  * of the sequence sees is never used, whatever it holds.  fp32 accumulation and softmax.  The lengths are read on the
  * device: nothing in the call depends on them, so a captured call follows new ones.  The workspace carries no results
- * between calls, but calls that overlap on the GPU need one each.  batch <= 1024.  Stands in for the scores, mask,
- * softmax and value sum of the reference's attention block (AttentionFeatures.java:531-616, 906-917), which takes one
- * row of one sequence. */
+ * between calls, but calls that overlap on the GPU need one each.  batch <= 1024, and in bf16 rows x heads x max_pages x
+ * page_size below about 2^46 (QW_ERR_SHAPE beyond).  A row's own masked positions that others of its sequence see (those
+ * after it in its chunk, those before its window) may hold any finite values, and any keys; an infinite or NaN value there
+ * can reach it, as 0 x infinity does.  Stands in for the scores, mask, softmax and value sum of the reference's attention
+ * block (AttentionFeatures.java:531-616, 906-917), which takes one row of one sequence. */
 qw_status qw_op_chunk_attn(const qw_chunk_attn_args *args, void *stream);
 
 /* Workspace bytes of qw_op_chunk_attn on any batch of this geometry (0: unsupported geometry). */

@@ -35,6 +35,13 @@ def test_chunk_attention_refuses(status, over):
     assert e.value.status == status and str(e.value)
 
 
+def test_chunk_attention_refuses_more_key_blocks_than_it_can_number():
+    # 2^22 rows over 2^22 positions: 2^16 items of 2^15 blocks, two tiles, 8 KV heads
+    with pytest.raises(native.QwenError) as e:
+        attention(rows=1 << 22, max_pages=1 << 16)
+    assert e.value.status == SHAPE and "key blocks" in str(e.value)
+
+
 def test_chunk_attention_of_nothing_is_done():
     attention(rows=0, q=0)
     attention(batch=0, row_start=0)

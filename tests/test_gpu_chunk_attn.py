@@ -229,6 +229,22 @@ def test_runs_on_its_own_stream_and_in_a_graph_that_follows_new_lengths():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_a_window_longer_than_any_sequence_cuts_nothing_off(dtype):
+    """The longest window there is, on rows before the first position, in the first pages and far beyond them."""
+    c = Case([40, 130, 300, 3], [25, 130, 1500, 0], 8, 2, 64, 16, window=2 ** 31 - 1, dtype=dtype, seed=12)
+    c.run()
+    c.check()
+
+
+def test_long_chunks_of_every_group_size():
+    """The place of every item of many-item sequences: group sizes whose tiles are no power of two among them."""
+    for G, window in ((1, 0), (3, 0), (5, 200), (6, 1), (7, 333), (11, 0), (13, 90), (16, 2000)):
+        c = Case([700, 1, 451, 90], [2111, 300, 451, 60], 2 * G, 2, 64, 16, window=window, seed=G)
+        c.run()
+        c.check()
+
+
 def test_without_lse():
     c = Case([40, 1], [400, 1200], 16, 8, 128, 64, seed=8)
     c.run(lse=False)
