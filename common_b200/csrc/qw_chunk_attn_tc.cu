@@ -246,11 +246,16 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// 32 bytes: a whole sector of a row per lane
-__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
+// 32 bytes, a whole sector of a row per lane, where the rows are so aligned (16 bytes are all that is asked of them)
+__device__ __forceinline__ void store32(void *p, const uint32_t *v, bool aligned32) {
+    if (aligned32) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                     "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4 *>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<uint4 *>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
 }
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory"); }
 __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
@@ -796,6 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rpos = row / G, rhead = row % G;
         const uint32_t trow = tmem + ((uint32_t)w0 << 16);
         const uint32_t ts = trow + (uint32_t)(t * kKeys), to = trow + 256u + (uint32_t)(t * 128);
+        const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)a.ld_out * 2) & 31) == 0;
         int nv = 0, no = 0, nx[2] = {0, 0};  // visits, pieces with visits, exchanges by writing slot
         bool ok = true;
         for (int np = 0; ok; np++) {
@@ -945,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 uint32_t pk[8];
 #pragma unroll
                                 for (int e = 0; e < 8; e++) pk[e] = pack2(o[c + 2 * e] * inv, o[c + 2 * e + 1] * inv);
-                                store32(orow + c, pk);
+                                store32(orow + c, pk, wide);
                             }
                         }
                     }
@@ -1053,7 +1059,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 uint32_t pk[8];
 #pragma unroll
                                 for (int e = 0; e < 8; e++) pk[e] = pack2(o[2 * e], o[2 * e + 1]);
-                                store32(orow + c * 16, pk);
+                                store32(orow + c * 16, pk, wide);
                             }
                         }
                     }

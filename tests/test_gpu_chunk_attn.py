@@ -169,6 +169,14 @@ def test_rows_inside_wider_buffers():
     c.check()
 
 
+@pytest.mark.parametrize("d,window", [(128, 0), (64, 0), (128, 70)])
+def test_rows_aligned_to_16_bytes_and_no_more(d, window):
+    """Rows of q and out that begin on odd multiples of 16 bytes, in whole items, cut ones and single tokens."""
+    c = Case([300, 1, 9, 130, 1], [2500, 300, 1000, 130, 4000], 16, 4, d, 64, window=window, fused=8, gap=8, seed=13)
+    c.run()
+    c.check()
+
+
 def test_large_scores_and_a_late_maximum():
     """Scores over a wide range in which every later block holds a larger one: the running maximum is raised."""
     torch = _torch()
