@@ -5,12 +5,24 @@
 // P = floor(128 / G) positions of all G heads, at most 128 rows, one row per TMEM lane.  An item is two such tiles of
 // one sequence and KV head; a K / V block of 128 keys serves both.  The key blocks of all items, in the order
 // sequence, KV head, tiles, form one line that is cut into equal shares, one per CTA (one CTA per SM): every SM gets
-// the same number of blocks whatever the lengths are.  An item cut by a share's end leaves partial results (O, maximum,
-// sum) in the workspace, and the CTAs that share it join them, each a part of its rows, once all are there.
+// the same number of blocks whatever the lengths are.  An item cut once is finished by the CTA in which it begins, from
+// the other's partial result (O, maximum, sum) in the workspace; the CTAs that share an item cut more often join its
+// rows, each a part of them, once all are there.  Where there are no more items than SMs and none much longer than a
+// share would be, a CTA takes each item whole.
 //
 // An item with one tile only (decoding: G rows; the last rows of a chunk) gives its blocks to the two tile slots in
 // turn, so that one slot's softmax still runs while the tensor cores work on the other; the slots' results are joined
 // at the item's end.
+//
+// What bounds it (32 heads over 8 KV heads of 128 where not said otherwise):
+//   long chunks: a slot's chain S (690 clocks), softmax (1900, of which the exponentials of two slots on the 16 a clock of
+//     an SM take 1024 each), P V (560) and the commits between them, beside the other slot's: a pair of blocks every 3700
+//     clocks.  4096 rows over 20096 positions: 1005 us, 1.21 PFLOP/s (0.73 of what cuBLAS reaches); 1120 us once the power
+//     limit holds the clock down
+//   single tokens: HBM.  64 sequences over 3900..4250 positions: 174 us, 6.15 TB/s; one over 120001: 89 us, 5.5 TB/s
+//   short ones: the way to the first scores (11000 clocks: lengths, schedule, page table, first keys), a visit of a block
+//     after the other (1800 clocks of softmax each), the join of cut items; a token on 300 positions 10 us
+// 16 softmax warps with two threads per row against 8 with one: 1187 against 1441 us (4096 rows over 20096 positions).
 //
 // Warps (five warpgroups):
 //   0     K and V: TMA boxes of min(page, 128) rows into rings of tc_stages tiles each, one lane per box
@@ -35,11 +47,23 @@ namespace qw {
 namespace {
 
 constexpr int kThreads = 640, kSoftThreads = 512, kRows = 128, kKeys = 128, kMaxStages = 5;
-constexpr float kRescale = 8.f;  // the running maximum is raised only when it grows by more than 2^8: p stays below 2^8
+// The running maximum is raised only when it grows by more than 8 (in log2 units): p stays below 2^8, and O is seldom
+// rescaled.  4096 rows over 20096 positions 1005 us, 1104 with every maximum; 8 chunks on old sequences 127 and 138.
+constexpr float kRescale = 8.f;
 constexpr int kPieces = 4;       // ring of pieces
-constexpr int kFewRows = 8;      // rows of an exchange in shared memory: a token's heads of one KV head
-constexpr int kItemUnits = 2;    // what a tile costs beside its blocks
-constexpr int kMinShare = 5;     // units that a CTA beyond one per item is worth: splitting an item costs about as much
+// Rows of an exchange between the slots in shared memory: a token's heads of one KV head.  Through the workspace, as more
+// rows go, 64 single tokens take 184 instead of 174 us, 32 of them beside a chunk 96 instead of 84.
+constexpr int kFewRows = 8;
+// What a tile costs beside its blocks, in blocks: its queries and results.  8 prompts of 1420..1962 tokens take 214 us, 216
+// with 1 and 228 with 4 (32 tokens beside a chunk 84, 86, 86; 8 chunks on old sequences 127, 127, 125).
+constexpr int kItemUnits = 2;
+// Units of a share at least; with fewer it might hold no block of an item that it lies in.  A token on 2000 positions, 8 KV
+// heads: 13.2 us; with 3 units 14.1, with 5 15.6, with 10 22.0.
+constexpr int kMinShare = 2;
+// What a cut costs in units: items are left whole where the longest has at most so many more than a share.  5 tokens on
+// 100..1500 positions take 12.7 instead of 18.6 us, 6 chunks under a window 30.8 instead of 35.2.  With 4, 17 tokens on
+// 100..1500 positions take 22.3 instead of 19.6; with 8, one on 900 takes 14.8 instead of 12.6.
+constexpr int kJoinUnits = 6;
 constexpr int kCounterWords = 256;  // arrivals | arrivals at items cut once | departures, one word per CTA each
 static_assert(3 * kCounterWords * 4 == kChunkCounterBytes && kNumSMsB200 <= kCounterWords, "counters");
 
@@ -72,7 +96,8 @@ struct Shared {
 };
 
 struct __align__(16) Smem {
-    unsigned pre[kChunkMaxBatch + 1];  // units of the line before each sequence
+    unsigned pre[kChunkMaxBatch + 1];   // units of the line before each sequence
+    unsigned whole[kChunkMaxBatch + 1]; // items of the line before each sequence
     Seq seq[kChunkMaxBatch];
     Piece piece[kPieces];
     Shared shared[2];
@@ -91,7 +116,11 @@ struct Item {
     // a visit of a slot is a unit: a block costs as many as the item has tiles, and its queries and results kItemUnits
     // per tile; an item that sees nothing is not on the line
     __device__ __forceinline__ unsigned units() const { return nb ? (nb + kItemUnits) * nsub : 0; }
-    __device__ __forceinline__ int blocks_before(int u) const { return min(nb, nsub == 2 ? (u + 1) >> 1 : u); }
+    // on a line of whole items, each is one unit
+    __device__ __forceinline__ unsigned units(bool flat) const { return flat ? nb > 0 : units(); }
+    __device__ __forceinline__ int blocks_before(int u, bool flat) const {
+        return flat && u ? nb : min(nb, nsub == 2 ? (u + 1) >> 1 : u);
+    }
 };
 __device__ __forceinline__ Item make_item(const Seq &s, int i, int P, int window) {
     Item it;
@@ -437,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         sh.abort = 0;
         sh.empty = 0;
-        sh.pre[0] = 0;
+        sh.pre[0] = sh.whole[0] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmQ) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmK) : "memory");
@@ -460,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---------------- the scheduler ----------------
             // units of every sequence and their running sum
             unsigned W = 0;
-            int items = 0;  // that see something
+            unsigned items = 0, most = 0;  // that see something; units of the largest
             for (int b0 = 0; b0 < a.batch; b0 += 32) {
                 const int b = b0 + lane;
                 Seq s{0, 0, 0};
@@ -479,31 +508,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int ni = s.n <= 2 * P ? s.n > 0 : (s.n + 2 * P - 1) / (2 * P);
                 const int gone = s.n > s.kv ? (s.n - s.kv) / (2 * P) : 0;  // items before the first position
                 const unsigned units = ni ? seq_units(s, ni, gone, P, a.window) : 0;
-                items += __reduce_add_sync(0xffffffffu, s.kv > 0 ? (ni - gone) * a.Hkv : 0);
-                unsigned v = units * a.Hkv;
+                unsigned big = ni ? make_item(s, ni - 1, P, a.window).units() : 0;
+                if (ni > 1) big = max(big, make_item(s, ni - 2, P, a.window).units());
+                most = max(most, __reduce_max_sync(0xffffffffu, big));
+                unsigned v = units * a.Hkv, c = s.kv > 0 ? (ni - gone) * a.Hkv : 0;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned w = __shfl_up_sync(0xffffffffu, v, o);
-                    if (lane >= o) v += w;
+                    const unsigned w = __shfl_up_sync(0xffffffffu, v, o), x = __shfl_up_sync(0xffffffffu, c, o);
+                    if (lane >= o) {
+                        v += w;
+                        c += x;
+                    }
                 }
-                if (b < a.batch) sh.pre[b + 1] = W + v;
+                if (b < a.batch) {
+                    sh.pre[b + 1] = W + v;
+                    sh.whole[b + 1] = items + c;
+                }
                 W += __shfl_sync(0xffffffffu, v, 31);
+                items += __shfl_sync(0xffffffffu, c, 31);
             }
             __syncwarp();
-            // one CTA per item at least, and more where the shares stay long enough to be worth joining
-            const int Ge = min((int)gridDim.x, max(items, (int)((W + kMinShare - 1) / kMinShare)));
+            // Cut items save time only where the longest one is well above a share; otherwise a CTA takes each item whole.
+            const unsigned grid = gridDim.x;
+            const bool flat = items <= grid && most <= max((unsigned)kMinShare, W / grid) + kJoinUnits;
+            if (flat) W = items;
+            const int Ge = flat ? items : min(grid, max(items, W / kMinShare));
+            const unsigned *pre = flat ? sh.whole : sh.pre;
             Line line{0, 0};
             unsigned at = 0, end = 0;
             int b = 0, h = 0, i = 0, off = 0;
-            if (cta < Ge) {  // W / Ge >= 2: an item has three units at least
+            if (cta < Ge) {  // W / Ge >= kMinShare where items are cut: an item has three units at least
                 line.q = W / Ge;
                 line.rem = W - line.q * Ge;
                 at = line.start(cta);
                 end = line.start(cta + 1);
                 unsigned rem = 0, per = 1;
                 for (int b0 = 0; b0 < a.batch; b0 += 32) {  // the sequence that holds unit `at`
-                    const unsigned p0 = b0 + lane < a.batch ? sh.pre[b0 + lane] : 0xffffffffu;
-                    const unsigned p1 = b0 + lane < a.batch ? sh.pre[b0 + lane + 1] : 0xffffffffu;
+                    const unsigned p0 = b0 + lane < a.batch ? pre[b0 + lane] : 0xffffffffu;
+                    const unsigned p1 = b0 + lane < a.batch ? pre[b0 + lane + 1] : 0xffffffffu;
                     const unsigned m = __ballot_sync(0xffffffffu, p0 <= at && at < p1);
                     if (m) {
                         const int l = __ffs(m) - 1;
@@ -519,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const Seq s = sh.seq[b];
                 for (; i * 2 * P < s.n; i += 32) {  // the item that holds unit rem of this head
-                    unsigned v = (i + lane) * 2 * P < s.n ? make_item(s, i + lane, P, a.window).units() : 0;
+                    unsigned v = (i + lane) * 2 * P < s.n ? make_item(s, i + lane, P, a.window).units(flat) : 0;
                     if (s.n <= 2 * P) {  // the only one
                         off = (int)rem;
                         break;
@@ -553,9 +595,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     s = sh.seq[b];
                     if (s.n <= 0) { b++; continue; }
                     it = make_item(s, i, P, a.window);
-                    const int units = (int)it.units();
+                    const int units = (int)it.units(flat);
                     const int take = min(units - off, (int)(end - at));
-                    const int ja = it.blocks_before(off), jb = it.blocks_before(off + take);
+                    const int ja = it.blocks_before(off, flat), jb = it.blocks_before(off + take, flat);
                     u0 = at - off;
                     cb = b; ch = h;
                     at += take;
@@ -701,7 +743,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                        warp_wait(full, (uint32_t)phase & 1u, abort_flag, a.err);
             };
             // On the blocks of two tiles the slots take turns, slot 0 first: interleaved, the MMAs of both would take as long
-            // together, and each slot's softmax would wait for the end of both.  (A single tile is bound by its loads.)
+            // together, and each slot's softmax would wait for the end of both (4096 rows over 20096 positions: 1204 us, and
+            // 1021 with turns).  (A single tile's blocks are in both slots already, and bound by their loads.)
             int turns = 0;
             auto take_turn = [&]() {
                 return warp_wait(&sh.turn[t], (uint32_t)(t == 0 ? turns + 1 : turns) & 1u, abort_flag, a.err);
