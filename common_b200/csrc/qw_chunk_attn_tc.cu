@@ -19,7 +19,7 @@
 //     an SM take 1024 each), P V (560) and the commits between them, beside the other slot's: a pair of blocks every 3700
 //     clocks.  4096 rows over 20096 positions: 1005 us, 1.21 PFLOP/s (0.73 of what cuBLAS reaches); 1120 us once the power
 //     limit holds the clock down
-//   single tokens: HBM.  64 sequences over 3900..4250 positions: 174 us, 6.15 TB/s; one over 120001: 89 us, 5.5 TB/s
+//   single tokens: HBM.  64 sequences over 3900..4250 positions: 169 us, 6.3 TB/s; one over 120001: 86 us, 5.7 TB/s
 //   short ones: the way to the first scores (11000 clocks: lengths, schedule, page table, first keys), a visit of a block
 //     after the other (1800 clocks of softmax each), the join of cut items; a token on 300 positions 10 us
 // 16 softmax warps with two threads per row against 8 with one: 1187 against 1441 us (4096 rows over 20096 positions).
@@ -52,7 +52,7 @@ constexpr int kThreads = 640, kSoftThreads = 512, kRows = 128, kKeys = 128, kMax
 constexpr float kRescale = 8.f;
 constexpr int kPieces = 4;       // ring of pieces
 // Rows of an exchange between the slots in shared memory: a token's heads of one KV head.  Through the workspace, as more
-// rows go, 64 single tokens take 184 instead of 174 us, 32 of them beside a chunk 96 instead of 84.
+// rows go, 64 single tokens took 184 instead of 174 us, 32 of them beside a chunk 96 instead of 84.
 constexpr int kFewRows = 8;
 // What a tile costs beside its blocks, in blocks: its queries and results.  8 prompts of 1420..1962 tokens take 214 us, 216
 // with 1 and 228 with 4 (32 tokens beside a chunk 84, 86, 86; 8 chunks on old sequences 127, 127, 125).
@@ -88,7 +88,8 @@ struct Piece {
     int lo, hi;      // positions that its rows see
     int clo, chi;    // positions that some row of the sequence sees: the cache holds something there
 };
-enum { kEnd = 1, kPair = 2, kWhole = 4, kHead = 8, kTwo = 16 };  // kHead: the item begins in this share; kTwo: and is cut once
+// kHead: the item begins in this share; kTwo: and is cut once; kOnce: no other item has its sequence's keys
+enum { kEnd = 1, kPair = 2, kWhole = 4, kHead = 8, kTwo = 16, kOnce = 32 };
 
 // an item that several CTAs share
 struct Shared {
@@ -203,6 +204,13 @@ __device__ __forceinline__ void commit(uint64_t *bar, uint32_t elect) {
         "setp.ne.b32 e, %1, 0;\n\t"
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
         "r"(elect)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_hint(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], "
+        "[%4], %5;" ::"r"(smem_u32(dst)),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
@@ -610,7 +618,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     if (ja < jb) {
-                        pc.flags = (it.nsub == 2 ? kPair : 0) | (ja == 0 && jb == it.nb ? kWhole : 0) | (ja == 0 ? kHead : 0);
+                        pc.flags = (it.nsub == 2 ? kPair : 0) | (ja == 0 && jb == it.nb ? kWhole : 0) | (ja == 0 ? kHead : 0) |
+                                   (s.n <= 2 * P ? kOnce : 0);
                         pc.blk0 = it.j0 + ja;
                         pc.nblk = jb - ja;
                         break;
@@ -681,6 +690,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---------------- K and V ----------------
             const int br = min(a.ps, kKeys), nbox = kKeys / br;
             const int box = lane / NH, half = lane % NH;
+            // Keys that one item alone reads pass through L2 without pushing out what others use: 64 tokens over 3900..4250
+            // positions 169 us, 174 without; one over 120001 86 us, 89, and behind an L2 full of written lines 96 and 105.
+            // (Sequences whose pages are the same ones lose by it: 64 tokens over the same 4000 positions 129 us, 123 without.)
+            uint64_t once;
+            asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
             int r = 0;
             bool ok = true;
             for (int np = 0; ok; np++) {
@@ -709,9 +723,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!ok) break;
                         if (lane == 0) mbar_arrive_expect_tx(full, TILE);
                         __syncwarp();
-                        if (box < nbox)
-                            tma_load_2d((kv ? sV : sK) + st * TILE + half * HALF + box * br * 128, kv ? &tmV : &tmK, full,
-                                        half * 64, y);
+                        if (box < nbox) {
+                            uint8_t *to = (kv ? sV : sK) + st * TILE + half * HALF + box * br * 128;
+                            if (flags & kOnce) tma_load_2d_hint(to, kv ? &tmV : &tmK, full, half * 64, y, once);
+                            else tma_load_2d(to, kv ? &tmV : &tmK, full, half * 64, y);
+                        }
                     }
                     if (!ok) break;
                     y = yn;
