@@ -19,7 +19,8 @@
 //     an SM take 1024 each), P V (560) and the commits between them, beside the other slot's: a pair of blocks every 3700
 //     clocks.  4096 rows over 20096 positions: 1005 us, 1.21 PFLOP/s (0.73 of what cuBLAS reaches); 1120 us once the power
 //     limit holds the clock down
-//   single tokens: HBM.  64 sequences over 3900..4250 positions: 169 us, 6.3 TB/s; one over 120001: 86 us, 5.7 TB/s
+//   single tokens: HBM.  64 sequences over 3900..4250 positions: 168 us, 6.4 TB/s (176 under the
+//     power limit); one over 120001: 86 us, 5.7 TB/s
 //   short ones: the way to the first scores (11000 clocks: lengths, schedule, page table, first keys), a visit of a block
 //     after the other (1800 clocks of softmax each), the join of cut items; a token on 300 positions 10 us
 // 16 softmax warps with two threads per row against 8 with one: 1187 against 1441 us (4096 rows over 20096 positions).
@@ -88,8 +89,9 @@ struct Piece {
     int lo, hi;      // positions that its rows see
     int clo, chi;    // positions that some row of the sequence sees: the cache holds something there
 };
-// kHead: the item begins in this share; kTwo: and is cut once; kOnce: no other item has its sequence's keys
-enum { kEnd = 1, kPair = 2, kWhole = 4, kHead = 8, kTwo = 16, kOnce = 32 };
+// kHead: the item begins in this share; kTwo: and is cut once; kOnce: no other item has its sequence's keys; kLow: one tile
+// of 16 rows at most
+enum { kEnd = 1, kPair = 2, kWhole = 4, kHead = 8, kTwo = 16, kOnce = 32, kLow = 64 };
 
 // an item that several CTAs share
 struct Shared {
@@ -103,7 +105,7 @@ struct __align__(16) Smem {
     Piece piece[kPieces];
     Shared shared[2];
     uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages], q_full[2], q_empty[2],
-        s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], turn[2], done[2];
+        s_full[2], p_full[2], o_full[2], x_full[2], x_empty[2], w_full[kPieces], w_empty[kPieces], turn[2], done[2], zeroed;
     uint32_t tmem;
     float4 xo[2][128 / 4 * kFewRows];  // [slot]: O as float4 columns of kFewRows rows (16-byte aligned by its type)
     float2 xml[2][kFewRows];
@@ -429,8 +431,9 @@ __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, i
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    qw_chunk_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                            const __grid_constant__ CUtensorMap tmV, const ChunkArgs a) {
+    qw_chunk_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQ1,
+                            const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                            const ChunkArgs a) {
     constexpr int NST = tc_stages(D), TILE = tc_tile_bytes(D), HALF = kRows * 128, NH = D / 64;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Smem sh;
@@ -468,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sh.x_empty[i], 8);
             sh.shared[i].on = 0;
         }
+        mbar_init(&sh.zeroed, kSoftThreads / 32);
         for (int i = 0; i < kPieces; i++) {
             mbar_init(&sh.w_full[i], 1);
             mbar_init(&sh.w_empty[i], 19);  // K / V, two MMA warps, sixteen softmax warps
@@ -590,9 +594,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     rem -= __shfl_sync(0xffffffffu, v, 31);
                 }
             }
-            int np = 0, rn = 0, qn = 0, alt = 0, q_sent = 0;
-            bool ok = true;
-            for (;;) {
+            int np = 0, rn = 0, qn = 0, alt = 0, q_sent = 0, clean = 3;  // clean: query tiles whose rows from G on are zero
+            bool ok = warp_wait(&sh.zeroed, 0, abort_flag, a.err);
+            while (ok) {
                 Piece pc;
                 pc.flags = kEnd;
                 Item it;
@@ -619,7 +623,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (ja < jb) {
                         pc.flags = (it.nsub == 2 ? kPair : 0) | (ja == 0 && jb == it.nb ? kWhole : 0) | (ja == 0 ? kHead : 0) |
-                                   (s.n <= 2 * P ? kOnce : 0);
+                                   (s.n <= 2 * P ? kOnce : 0) |
+                                   (it.nsub == 1 && (s.n - it.f) * G <= 16 ? kLow : 0);
                         pc.blk0 = it.j0 + ja;
                         pc.nblk = jb - ja;
                         break;
@@ -666,14 +671,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 np++;
                 if (pc.flags & kEnd) break;
-                // the piece's queries
+                // The piece's queries.  Of a single token only its own rows are fetched, as long as the tile's others are the
+                // zeros of the start: rows of other sequences would cost their way here and, multiplied with every key, power
+                // (64 tokens over 3900..4250 positions, for seconds, the power limit holding the clock down: 184 us, 194 with them).
+                const bool token = pc.n0 == 1 && it.nsub == 1;
                 for (int q = pc.q0; q < pc.q0 + it.nsub && ok; q++) {
                     const int e = q & 1;
                     ok = warp_wait(&sh.q_empty[e], ((uint32_t)(q >> 1) & 1u) ^ 1u, abort_flag, a.err);
-                    if (ok && lane == 0) {
-                        mbar_arrive_expect_tx(&sh.q_full[e], (uint32_t)(NH * G * P * 128));
+                    if (!ok) break;
+                    const bool own = token && clean >> e & 1;
+                    if (!own) clean &= ~(1 << e);
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.q_full[e], (uint32_t)(NH * G * (own ? 1 : P) * 128));
                         for (int c = 0; c < NH; c++)
-                            tma_load_3d(sQ + e * TILE + c * HALF, &tmQ, &sh.q_full[e], c * 64, ch * G, pc.row0 + (q - pc.q0) * P);
+                            tma_load_3d(sQ + e * TILE + c * HALF, own ? &tmQ1 : &tmQ, &sh.q_full[e], c * 64, ch * G,
+                                        pc.row0 + (q - pc.q0) * P);
                         q_sent = q + 1;
                     }
                     __syncwarp();
@@ -746,6 +758,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
             // ---------------- MMAs: a warp per slot, so that one's waits and commits run beside the other's MMAs ----------------
             constexpr uint32_t IDS = tc_idesc_f16(kRows, kKeys, 0), IDP = tc_idesc_f16(kRows, D, 1);
+            // Rows 0..15 of a product of 64 rows lie in the same TMEM lanes as of 128: a token's heads take half the tensor
+            // cores' work, and power (64 tokens over 3900..4250 positions, under the power limit: 176 us, 184 with 128 rows).
+            constexpr uint32_t IDS64 = tc_idesc_f16(64, kKeys, 0), IDP64 = tc_idesc_f16(64, D, 1);
             const int t = warp - 1;
             const uint32_t elect = lane == 0 ? 1u : 0u;
             const uint64_t dQ = desc_sw128(smem_u32(sQ), 16, 1024), dK = desc_sw128(smem_u32(sK), 16, 1024),
@@ -789,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++) {
                         const uint64_t off = (uint64_t)(((kk >> 2) * HALF + (kk & 3) * 32) >> 4);
-                        mma_ss(ts, da + off, db + off, IDS, kk > 0 ? 1u : 0u, elect);
+                        mma_ss(ts, da + off, db + off, flags & kLow ? IDS64 : IDS, kk > 0 ? 1u : 0u, elect);
                     }
                     commit(&sh.s_full[t], elect);  // also covers the slot's PV before it: O may be rescaled
                     // two arrivals release an entry: of both slots, where both use it
@@ -832,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint64_t dv = dV + (uint64_t)(st * (TILE >> 4));
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; kk++)  // P's halves lie over their own halves of S
-                        mma_ts(to, ts + (uint32_t)((kk & 3) * 8 + (kk >> 2) * 64), dv + (uint64_t)(kk * 2048 >> 4), IDP,
+                        mma_ts(to, ts + (uint32_t)((kk & 3) * 8 + (kk >> 2) * 64), dv + (uint64_t)(kk * 2048 >> 4), flags & kLow ? IDP64 : IDP,
                                kk > 0 ? 1u : (j > j0 ? 1u : 0u), elect);
                     if (next) issue_s(j + step, rn);
                     commit(&sh.v_empty[st], elect);
@@ -855,6 +870,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        // zeros for the rows that a single token's queries leave (before the first of them are fetched)
+        for (int i = threadIdx.x - 128; i < 2 * TILE / 16; i += kSoftThreads) reinterpret_cast<uint4 *>(sQ)[i] = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.zeroed);
         // ---------------- softmax and results ----------------
         const int t = (warp - 4) >> 3, hf = lane >> 4, w0 = (warp & 3) * 32 + ((warp - 4) & 4) * 4, row = w0 + (lane & 15);
         const int rpos = row / G, rhead = row % G;
@@ -1241,10 +1261,11 @@ cudaError_t launch(const ChunkArgs &a, cudaStream_t st) {
         grid = grid < kNumSMsB200 ? grid : kNumSMsB200;
         grids[dev].store(grid, std::memory_order_release);
     }
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mq1, mk, mv;
     const int P = kRows / a.G, br = a.ps < kKeys ? a.ps : kKeys;
     const long long crow = (long long)a.num_pages * a.Hkv * a.ps;
     if ((e = tma_map_bf16_sw128_3d(&mq, a.q, a.d, a.H, a.rows, a.d, a.ld_q, a.G, P)) != cudaSuccess) return e;
+    if ((e = tma_map_bf16_sw128_3d(&mq1, a.q, a.d, a.H, a.rows, a.d, a.ld_q, a.G, 1)) != cudaSuccess) return e;
     if ((e = tma_map_bf16_sw128(&mk, a.k, crow, a.d, a.d, br)) != cudaSuccess) return e;
     if ((e = tma_map_bf16_sw128(&mv, a.v, crow, a.d, a.d, br)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -1257,7 +1278,7 @@ cudaError_t launch(const ChunkArgs &a, cudaStream_t st) {
     at[0].val.cooperative = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, qw_chunk_attn_tc_kernel<D>, mq, mk, mv, a);
+    return cudaLaunchKernelEx(&cfg, qw_chunk_attn_tc_kernel<D>, mq, mq1, mk, mv, a);
 }
 
 }  // namespace
