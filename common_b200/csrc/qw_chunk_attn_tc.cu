@@ -758,8 +758,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
             // ---------------- MMAs: a warp per slot, so that one's waits and commits run beside the other's MMAs ----------------
             constexpr uint32_t IDS = tc_idesc_f16(kRows, kKeys, 0), IDP = tc_idesc_f16(kRows, D, 1);
-            // Rows 0..15 of a product of 64 rows lie in the same TMEM lanes as of 128: a token's heads take half the tensor
-            // cores' work, and power (64 tokens over 3900..4250 positions, under the power limit: 176 us, 184 with 128 rows).
+            // Rows 0..15 of a product of 64 rows lie in the same TMEM lanes as of 128.  For a token's heads it takes as long, at
+            // less power (64 tokens over 3900..4250 positions, under the power limit: 176 us, 184 with 128 rows).
             constexpr uint32_t IDS64 = tc_idesc_f16(64, kKeys, 0), IDP64 = tc_idesc_f16(64, D, 1);
             const int t = warp - 1;
             const uint32_t elect = lane == 0 ? 1u : 0u;
