@@ -253,6 +253,24 @@ def test_long_chunks_of_every_group_size():
         c.check()
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(seed):
+    """Batches of random shapes: items left whole, cut once and cut often, empty rows and sequences, every group size."""
+    import random
+    rng = random.Random(seed)
+    for _ in range(6):
+        G, kv_heads, d = rng.choice([1, 2, 3, 4, 5, 6, 7, 8, 12, 16]), rng.choice([1, 2, 4, 8]), rng.choice([64, 128])
+        B, longest = rng.choice([(1, 9000), (2, 6000), (3, 3000), (7, 2000), (30, 900)])
+        single = rng.random() < 0.4
+        new = [1 if single else rng.choice([0, 1, 2, rng.randint(1, 40), rng.randint(1, 300)]) for _ in range(B)]
+        kv = [max(0, n + rng.choice([0, -1, -5, rng.randint(0, longest), rng.randint(0, longest)])) for n in new]
+        c = Case(new, kv, G * kv_heads, kv_heads, d, rng.choice([16, 64, 256]), window=rng.choice([0, 0, 1, 130, 1500]),
+                 seed=seed, fused=rng.choice([0, 64]), gap=rng.choice([0, 8]))
+        c.run()
+        c.run()
+        c.check()
+
+
 def test_without_lse():
     c = Case([40, 1], [400, 1200], 16, 8, 128, 64, seed=8)
     c.run(lse=False)
