@@ -15,7 +15,7 @@ namespace qw {
 namespace {
 
 constexpr int kCopyThreads = 256;
-constexpr int kCompactThreads = 256, kCompactRows = 16;
+constexpr int kCompactThreads = 128, kCompactRows = 8;
 
 // One CTA per (page pair, layer, K or V, head): rows [0, n) of the head are contiguous in both pages.  Bound by HBM: 6.7 TB/s
 // where whole pages move (453 us for 3.0 GB), the launch where a few do (4.7 us for 4 pages of 28 layers).
@@ -137,13 +137,15 @@ __device__ __forceinline__ void store_raw(T *p, const Raw8<T> &r) {
 // One CTA per (kCompactRows kept rows, layer).  The rows' places are looked up once; a warp then takes a head at a time: its rows
 // are one contiguous piece of a destination page (mostly of a source page too).  A lane takes 8 elements of a row's first
 // half and the matching 8 of its second (the rotary pairs), HV lanes a row, and has U rows of keys and values on the way.
-// Bound by HBM: 3.74 GB moved at 6.2 TB/s (604 us; 28 layers, 8 heads of 128, bf16), 337 MB at 5.9 TB/s (57 us), where the last
-// CTAs and the launch show.  What counts is loads in flight per SM: 2 rows a lane in 4 CTAs of an SM (64 registers)
-// against 4 rows in 2 CTAs (113 registers) take 604 against 724 us and 57 against 57; 32 rows a CTA instead of 16
-// take 594 and 59.5, 64 take 602 and 65; the turns' arithmetic hides behind the loads.
+// Bound by HBM: 3.74 GB moved at 6.3 TB/s (592 us; 28 layers, 8 heads of 128, bf16), 337 MB at 5.9 TB/s (57 us), where the last
+// CTAs and the launch show.  What counts is loads in flight per SM and small CTAs to end on: 2 rows a lane in 4 CTAs of
+// 256 threads (64 registers) against 4 rows in 2 CTAs (113 registers) take 604 against 724 us; 128 threads and 8 rows a
+// CTA 592 and 57.3, 256 threads and 16 rows 604 and 57.3, 128 and 16 590 and 59.8, 256 and 8 652 and 56.7; the
+// turns' arithmetic hides behind the loads.
 template <typename T, int HV, int U>
-__global__ void __launch_bounds__(kCompactThreads, 4) qw_kv_compact_kernel(const CompactArgs a) {
+__global__ void __launch_bounds__(kCompactThreads, 8) qw_kv_compact_kernel(const CompactArgs a) {
     constexpr int ROWS = kCompactRows, STEP = 32 / HV, HALF = HV * 8;
+    static_assert(ROWS % (U * STEP) == 0, "rows of a warp's round");
     __shared__ RowMove moves[ROWS];
     for (int i = threadIdx.x; i < ROWS; i += blockDim.x) moves[i] = row_move(a, blockIdx.x * ROWS + i);
     __syncthreads();
@@ -210,12 +212,11 @@ __global__ void __launch_bounds__(kCompactThreads) qw_kv_compact_any_kernel(cons
 
 template <typename T>
 void compact_launch(const CompactArgs &a, cudaStream_t st) {
-    constexpr int U = sizeof(T) == 2 ? 2 : 1;
     const int threads = 32 * (a.heads < kCompactThreads / 32 ? a.heads : kCompactThreads / 32);
     if (a.d == 128)
-        qw_kv_compact_kernel<T, 8, U><<<dim3((a.rows + kCompactRows - 1) / kCompactRows, a.layers), threads, 0, st>>>(a);
+        qw_kv_compact_kernel<T, 8, sizeof(T) == 2 ? 2 : 1><<<dim3((a.rows + kCompactRows - 1) / kCompactRows, a.layers), threads, 0, st>>>(a);
     else if (a.d == 64)
-        qw_kv_compact_kernel<T, 4, U><<<dim3((a.rows + kCompactRows - 1) / kCompactRows, a.layers), threads, 0, st>>>(a);
+        qw_kv_compact_kernel<T, 4, 1><<<dim3((a.rows + kCompactRows - 1) / kCompactRows, a.layers), threads, 0, st>>>(a);
     else
         qw_kv_compact_any_kernel<T><<<dim3((a.rows + kCompactThreads / 32 - 1) / (kCompactThreads / 32), a.layers),
                                       kCompactThreads, 0, st>>>(a);
