@@ -331,6 +331,18 @@ void drop_page(qw_model *m, int pg) {
     if (--m->page_refs[pg] == 0) m->free_pages.push_back(pg);
 }
 
+// The slot's table row from page `from` on.  Every write of the table goes through the model's stream: kernels queued
+// there (a compaction, steps on the device) still read the row as it was, and a later write follows an earlier one.
+qw_status send_table(qw_model *m, int slot, size_t from) {
+    auto &sp = m->slot_pages[slot];
+    if (from >= sp.size()) return QW_OK;
+    int *row = m->h_page_table.data() + (size_t)slot * m->max_pages;
+    for (size_t i = from; i < sp.size(); i++) row[i] = sp[i];
+    CK(cudaMemcpyAsync(m->d_page_table + (size_t)slot * m->max_pages + from, row + from, sizeof(int) * (sp.size() - from),
+                       cudaMemcpyHostToDevice, m->st));
+    return QW_OK;
+}
+
 qw_status reserve_pages(qw_model *m, int slot, int npos) {
     if (slot < 0 || slot >= m->B) return fail(m, QW_ERR_ARG, "slot %d out of range [0,%d)", slot, m->B);
     if (npos > m->c.seq_len) return fail(m, QW_ERR_SHAPE, "position %d beyond seq_len %d", npos, m->c.seq_len);
@@ -341,15 +353,8 @@ qw_status reserve_pages(qw_model *m, int slot, int npos) {
     if ((int)m->free_pages.size() < need - have)
         return fail(m, QW_ERR_OOM, "KV cache exhausted: slot %d needs %d more pages, %zu free", slot, need - have,
                     m->free_pages.size());
-    for (int i = have; i < need; i++) {
-        int pg = take_page(m);
-        sp.push_back(pg);
-        m->h_page_table[(size_t)slot * m->max_pages + i] = pg;
-    }
-    CK(cudaMemcpy(m->d_page_table + (size_t)slot * m->max_pages + have,
-                  m->h_page_table.data() + (size_t)slot * m->max_pages + have, sizeof(int) * (need - have),
-                  cudaMemcpyHostToDevice));
-    return QW_OK;
+    for (int i = have; i < need; i++) sp.push_back(take_page(m));
+    return send_table(m, slot, have);
 }
 
 void release_slot(qw_model *m, int slot) {
@@ -370,16 +375,6 @@ qw_status cache_buffer(qw_model *m) {
 qw_kv_pool cache_pool(const qw_model *m) {
     return qw_kv_pool{m->kpool, m->vpool, m->c.layers, m->num_pages, m->Hkvl, m->page_size, m->c.head_dim,
                       m->bf16kv ? QW_DTYPE_BF16 : QW_DTYPE_F32};
-}
-// the slot's table row from page `from` on, after the work already on the stream
-qw_status send_table(qw_model *m, int slot, size_t from) {
-    auto &sp = m->slot_pages[slot];
-    if (from >= sp.size()) return QW_OK;
-    int *row = m->h_page_table.data() + (size_t)slot * m->max_pages;
-    for (size_t i = from; i < sp.size(); i++) row[i] = sp[i];
-    CK(cudaMemcpyAsync(m->d_page_table + (size_t)slot * m->max_pages + from, row + from, sizeof(int) * (sp.size() - from),
-                       cudaMemcpyHostToDevice, m->st));
-    return QW_OK;
 }
 // copies rows [0, rows[i]) of page src[i] to page dst[i] in every layer
 qw_status copy_pages(qw_model *m, const std::vector<int> &src, const std::vector<int> &dst, const std::vector<int> &rows) {
