@@ -151,7 +151,6 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const Ch
         __syncthreads();
         if (!s_last) return;
         __threadfence();
-        if (tid < kSiRows) s_m[tid] = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = ty * 4 + i;
