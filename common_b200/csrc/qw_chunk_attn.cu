@@ -283,50 +283,47 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_rows_kernel(const Ch
     const int id = blockIdx.y * gridDim.x + blockIdx.x;
     unsigned *counter = reinterpret_cast<unsigned *>(a.workspace) + id;
     float *parts = reinterpret_cast<float *>((char *)a.workspace + kChunkCounterBytes) + (size_t)id * nsplit * R * (D + 2);
-    for (int h = warp; h < R; h += W) {
-        float mm = -INFINITY, ll = 0.f;
-        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < W; w++) join(mm, ll, oo, s_m[w][h], s_l[w][h], s_o[w][h][lane]);
-        if (nsplit > 1) {
-            float *p = parts + ((size_t)blockIdx.z * R + h) * (D + 2);
-            if (lane < LK) {
-                p[c] = oo.x; p[c + 1] = oo.y; p[c + 2] = oo.z; p[c + 3] = oo.w;
-            }
-            if (lane == 0) { p[D] = mm; p[D + 1] = ll; }
-        } else {
-            s_o[0][h][lane] = oo;
-            if (lane == 0) { s_m[0][h] = mm; s_l[0][h] = ll; }
-        }
-    }
-    if (nsplit > 1) {
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            s_last = atomicAdd(counter, 1u) == (unsigned)nsplit - 1u;
-            if (s_last) *counter = 0u;
-        }
-        __syncthreads();
-        if (!s_last) return;
-        __threadfence();
-    }
-    for (int h = warp; h < G; h += W) {
-        float mm = -INFINITY, ll = 0.f;
-        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (nsplit > 1) {
-            for (int z = 0; z < nsplit; z++) {
-                const float *p = parts + ((size_t)z * R + h) * (D + 2);
-                join(mm, ll, oo, __ldcg(p + D), __ldcg(p + D + 1),
-                     make_float4(__ldcg(p + c), __ldcg(p + c + 1), __ldcg(p + c + 2), __ldcg(p + c + 3)));
-            }
-        } else {
-            mm = s_m[0][h]; ll = s_l[0][h]; oo = s_o[0][h][lane];
-        }
+    auto result = [&](int h, float mm, float ll, const float4 &oo) {
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         const size_t head = (size_t)(kvh * G + h);
         if (lane < LK)
             *reinterpret_cast<float4 *>((float *)a.out + (size_t)row * a.ld_out + head * D + c) =
                 ll == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(oo.x * inv, oo.y * inv, oo.z * inv, oo.w * inv);
         if (a.lse && lane == 0) a.lse[(size_t)row * a.H + head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+    };
+    for (int h = warp; h < G; h += W) {
+        float mm = -INFINITY, ll = 0.f;
+        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < W; w++) join(mm, ll, oo, s_m[w][h], s_l[w][h], s_o[w][h][lane]);
+        if (nsplit == 1) {
+            result(h, mm, ll, oo);
+            continue;
+        }
+        float *p = parts + ((size_t)blockIdx.z * R + h) * (D + 2);
+        if (lane < LK) {
+            p[c] = oo.x; p[c + 1] = oo.y; p[c + 2] = oo.z; p[c + 3] = oo.w;
+        }
+        if (lane == 0) { p[D] = mm; p[D + 1] = ll; }
+    }
+    if (nsplit == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+        s_last = atomicAdd(counter, 1u) == (unsigned)nsplit - 1u;
+        if (s_last) *counter = 0u;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    for (int h = warp; h < G; h += W) {
+        float mm = -INFINITY, ll = 0.f;
+        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int z = 0; z < nsplit; z++) {
+            const float *p = parts + ((size_t)z * R + h) * (D + 2);
+            join(mm, ll, oo, __ldcg(p + D), __ldcg(p + D + 1),
+                 make_float4(__ldcg(p + c), __ldcg(p + c + 1), __ldcg(p + c + 2), __ldcg(p + c + 3)));
+        }
+        result(h, mm, ll, oo);
     }
 }
 

@@ -27,3 +27,9 @@ def _repeats(c, times):
 def test_tiles_whose_keys_are_split_repeat_bit_for_bit(new, kv, heads, kv_heads, d):
     """Many rows a sequence and few tiles: the last CTA of a tile joins its ranges of keys."""
     _repeats(Case(new, kv, heads, kv_heads, d, 64, dtype="fp32", seed=21), 300)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,d", [(200, 16, 8, 128), (320, 6, 2, 64), (8, 8, 2, 128)])
+def test_single_rows_repeat_bit_for_bit(batch, heads, kv_heads, d):
+    """One row a sequence: rows enough to fill the GPU, whose keys one CTA takes, and few, whose keys are split."""
+    _repeats(Case([1] * batch, [1 + 37 * i % 700 for i in range(batch)], heads, kv_heads, d, 64, dtype="fp32", seed=22), 100)
