@@ -36,15 +36,16 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const Ch
     __shared__ bool s_last;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int G = a.G, kvh = blockIdx.y;
-    int b = 0, tile = blockIdx.x, n = 0;
+    int b = 0, tile = blockIdx.x, r0 = 0, n = 0;
     for (; b < a.batch; b++) {
-        n = max(0, min(a.row_start[b + 1], a.rows) - max(a.row_start[b], 0));
+        r0 = min(max(a.row_start[b], 0), a.rows);
+        n = max(0, min(a.row_start[b + 1], a.rows) - r0);
         const int t = (n * G + kSiRows - 1) / kSiRows;
         if (tile < t) break;
         tile -= t;
     }
     if (b >= a.batch) return;
-    const int r0 = a.row_start[b], kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps);
+    const int kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps);
     const int p0 = kv - n, first = tile * kSiRows, last = min(first + kSiRows, n * G) - 1;
     const int *table = a.page_table + (size_t)(a.slots ? a.slots[b] : b) * a.max_pages;
     const float *q = (const float *)a.q, *kc = (const float *)a.k, *vc = (const float *)a.v;
