@@ -1193,11 +1193,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int before = s.n - s.kv;
                 if (before <= 0) continue;
                 const int rows = s.kv == 0 ? s.n : before / (2 * P) * 2 * P;
-                const int vec = a.H * D / 8;
-                for (int e = blockIdx.x * kSoftThreads + threadIdx.x - 128; e < rows * vec; e += gridDim.x * kSoftThreads) {
-                    const int r = s.r0 + e / vec, c = e % vec * 8;
-                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)r * a.ld_out + c) = make_uint4(0, 0, 0, 0);
-                    if (a.lse && c % D == 0) a.lse[(size_t)r * a.H + c / D] = -INFINITY;
+                for (unsigned r = blockIdx.x; r < (unsigned)rows; r += gridDim.x) {
+                    const size_t grow = (size_t)s.r0 + r;
+                    uint4 *to_row = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + grow * a.ld_out);
+                    for (int c = threadIdx.x - 128; c < a.H * (D / 8); c += kSoftThreads) to_row[c] = make_uint4(0, 0, 0, 0);
+                    for (int h = threadIdx.x - 128; a.lse && h < a.H; h += kSoftThreads) a.lse[grow * a.H + h] = -INFINITY;
                 }
             }
         }

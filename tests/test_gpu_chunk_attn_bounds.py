@@ -41,3 +41,25 @@ def test_row_starts_outside_the_rows_are_clamped(dtype, new, lengths):
     c.row_start = torch.tensor(lengths, dtype=torch.int32, device="cuda")
     c.run()
     _check(c, bufs)
+
+
+def test_more_rows_that_see_nothing_than_32_bits_count_vectors_of():
+    """2^21 rows of 64 heads of 128 are 2^31 vectors of 16 bytes (34 GB): a sequence with nothing cached."""
+    import torch
+    from common_b200 import native
+    rows, H, d = 2 ** 21 + 1000, 64, 128
+    out = torch.full((rows, H * d), -7.0, dtype=torch.bfloat16, device="cuda")
+    lse = torch.full((rows, H), -7.0, device="cuda")
+    cache = torch.zeros((1, 8, 64, d), dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    kv_len = torch.zeros(1, dtype=torch.int32, device="cuda")
+    n = native.chunk_attn_workspace(H, 8, d)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    attn = native.ChunkAttention(H, 8, d, 64, 1, 1, ws.data_ptr(), n)
+    attn(out.data_ptr(), cache.data_ptr(), cache.data_ptr(), table.data_ptr(), start.data_ptr(), kv_len.data_ptr(), 1, rows,
+         out.data_ptr(), lse=lse.data_ptr())
+    torch.cuda.synchronize()
+    for part in out.split(2 ** 18):
+        assert not bool(part.any())
+    assert bool((lse == -float("inf")).all())
