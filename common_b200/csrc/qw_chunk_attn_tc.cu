@@ -111,6 +111,7 @@ struct __align__(16) Smem {
     float2 xml[2][kFewRows];
     int abort, go;
     int empty;  // some rows stand before their sequence's first position
+    int unordered;  // row_start does not ascend
 };
 
 // one item's keys
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sh.w_empty[i], 19);  // K / V, two MMA warps, sixteen softmax warps
         }
         sh.abort = 0;
-        sh.empty = 0;
+        sh.empty = sh.unordered = 0;
         sh.pre[0] = sh.whole[0] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmQ) : "memory");
@@ -510,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     s.n = max(0, min(len1, a.rows) - s.r0);
                     s.kv = min(max(len2, 0), a.max_pages << a.log2_ps);
                     sh.seq[b] = s;
+                    if (len1 < len0) sh.unordered = 1;
                 }
                 if (b + 32 < a.batch) {
                     len0 = a.row_start[b + 32];
@@ -540,6 +542,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 items += __shfl_sync(0xffffffffu, c, 31);
             }
             __syncwarp();
+            if (sh.unordered) {
+                // Sequences that overlap may name more units than the host allowed for, and than 32 bits number: then
+                // nothing is scheduled.  (Units in 2^16, rounded down for each sequence.)
+                unsigned t = 0;
+                for (int b = lane; b < a.batch; b += 32) t += (sh.pre[b + 1] - sh.pre[b]) >> 16;
+                if (__reduce_add_sync(0xffffffffu, t) >= 0x10000u - kChunkMaxBatch) {
+                    W = items = 0;
+                    if (lane == 0 && a.err) atomicExch(a.err, TC_DEVERR_LENGTHS);
+                }
+            }
             // Cut items save time only where the longest one is well above a share; otherwise a CTA takes each item whole.
             const unsigned grid = gridDim.x;
             const bool flat = items <= grid && most <= max((unsigned)kMinShare, W / grid) + kJoinUnits;

@@ -21,7 +21,7 @@ enum TcEpi {
 };
 
 // device-side error codes written to TcArgs::err
-enum { TC_DEVERR_TIMEOUT = 1 };
+enum { TC_DEVERR_TIMEOUT = 1, TC_DEVERR_LENGTHS = 2 };
 
 struct TcArgs {
     int M;       // output features (rows of W)

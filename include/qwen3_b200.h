@@ -351,7 +351,8 @@ typedef struct qw_chunk_attn_args {
     void *out;                 /* (rows, ld_out) in dtype */
     float *lse;                /* optional (rows, heads): natural log of the softmax sum */
     void *workspace;           /* qw_op_chunk_attn_workspace bytes, 256-byte aligned, zeroed before its first call */
-    int32_t *err;              /* optional device word, set non-zero when a bounded device wait gave up */
+    int32_t *err;              /* optional device word, set non-zero when a bounded device wait gave up, or (bf16) when
+                                  a row_start that does not ascend names more work than 32 bits number: none is done */
     int64_t ld_q, ld_out;      /* row strides in elements, multiples of 16 bytes; 0 = heads * head_dim */
     uint64_t workspace_bytes;
     int32_t dtype;             /* QW_DTYPE_BF16 (tensor cores) or QW_DTYPE_F32: q, cache and out */

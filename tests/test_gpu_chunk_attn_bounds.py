@@ -63,3 +63,31 @@ def test_more_rows_that_see_nothing_than_32_bits_count_vectors_of():
     for part in out.split(2 ** 18):
         assert not bool(part.any())
     assert bool((lse == -float("inf")).all())
+
+
+def test_overlapping_sequences_of_more_work_than_32_bits_number_do_nothing():
+    """512 sequences that all name the same 2^20 rows over 2^22 positions: 2^40 units of work; some are empty."""
+    import torch
+    from common_b200 import native
+    rows, H, d, B = 2 ** 20, 8, 64, 1024
+    out = torch.full((rows, H * d), -7.0, dtype=torch.bfloat16, device="cuda")
+    cache = torch.zeros((1, H, 256, d), dtype=torch.bfloat16, device="cuda")
+    table = torch.full((B, 2 ** 14), -1, dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, rows] * (B // 2) + [0], dtype=torch.int32, device="cuda")
+    kv_len = torch.full((B,), 2 ** 22, dtype=torch.int32, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    n = native.chunk_attn_workspace(H, H, d)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    attn = native.ChunkAttention(H, H, d, 256, 1, 2 ** 14, ws.data_ptr(), n)
+
+    def call(batch, rows):
+        attn(out.data_ptr(), cache.data_ptr(), cache.data_ptr(), table.data_ptr(), start.data_ptr(), kv_len.data_ptr(), batch,
+             rows, out.data_ptr(), err=err.data_ptr())
+        torch.cuda.synchronize()
+
+    call(B, rows)
+    assert int(err.item()) != 0 and bool((out == -7.0).all())
+    err.zero_()
+    start[: 2] = torch.tensor([0, 1], dtype=torch.int32)
+    call(1, 1)                                # the workspace is as it was: one row over pages that are not there
+    assert int(err.item()) == 0 and not bool(out[0].any()) and bool((out[1:] == -7.0).all())
