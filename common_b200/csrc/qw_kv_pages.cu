@@ -35,13 +35,14 @@ __global__ void __launch_bounds__(kCopyThreads)
     for (int i = threadIdx.x; i < n; i += kCopyThreads) to[i] = from[i];
 }
 
-// turn 8 pairs (x, y) back by the table's angle: (x cos + y sin, y cos - x sin), in fp32, rounded once
-__device__ __forceinline__ void turn_back(float (&x)[8], float (&y)[8], const float2 *cs) {
+// turn 8 pairs (x, y) back by the table's angles: (x cos + y sin, y cos - x sin), in fp32, rounded once; `up` holds the sign bit
+// alone where they turn forward
+__device__ __forceinline__ void turn_back(float (&x)[8], float (&y)[8], const float2 *cs, int up) {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const float2 c = cs[e];
-        const float a = x[e] * c.x + y[e] * c.y;
-        y[e] = y[e] * c.x - x[e] * c.y;
+        const float s = __int_as_float(__float_as_int(c.y) ^ up), a = x[e] * c.x + y[e] * s;
+        y[e] = y[e] * c.x - x[e] * s;
         x[e] = a;
     }
 }
@@ -80,11 +81,13 @@ struct CompactArgs {
 // where a kept row lies and where it goes, as element offsets within one layer and head 0
 struct RowMove {
     long long from, to;
-    int delta;  // positions it moves down; -1: nothing to do
+    const float2 *turn;  // the table's angles of the distance; null: keys stay as they are
+    int up;              // the sign bit where it moves up
+    int skip;            // nothing to do
 };
 
 __device__ __forceinline__ RowMove row_move(const CompactArgs &a, int r) {
-    RowMove m{0, 0, -1};
+    RowMove m{0, 0, nullptr, 0, 1};
     if (r >= a.rows) return m;
     // the sequence that row r belongs to: the last b with keep_start[b] <= r
     int lo = 0, hi = a.batch - 1;
@@ -100,10 +103,14 @@ __device__ __forceinline__ RowMove row_move(const CompactArgs &a, int r) {
     if (come < 0 || to < 0 || cp >= a.max_pages || tp >= a.max_pages) return m;
     const int sp = a.src_table[(size_t)lo * a.max_pages + cp], dp = a.dst_table[(size_t)lo * a.max_pages + tp];
     if ((unsigned)sp >= (unsigned)a.num_pages || (unsigned)dp >= (unsigned)a.num_pages) return m;
+    const int distance = abs(come - to);
+    if (a.rope && distance >= a.rope_len) return m;  // the table has no angle for it
+    if (a.rope && distance) m.turn = a.rope + (size_t)distance * (a.d / 2);
+    m.skip = 0;
+    m.up = (come - to) & (int)0x80000000;
     const long long page = (long long)a.heads * a.ps * a.d;
     m.from = sp * page + (long long)(come & (a.ps - 1)) * a.d;
     m.to = dp * page + (long long)(to & (a.ps - 1)) * a.d;
-    m.delta = max(0, come - to);
     return m;
 }
 
@@ -158,7 +165,7 @@ __global__ void __launch_bounds__(kCompactThreads, 8) qw_kv_compact_kernel(const
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const RowMove &m = moves[r0 + u * STEP];
-                if (m.delta < 0) continue;
+                if (m.skip) continue;
                 q[u][0] = load_raw(k + m.from);
                 q[u][1] = load_raw(k + m.from + HALF);
                 q[u][2] = load_raw(v + m.from);
@@ -167,14 +174,14 @@ __global__ void __launch_bounds__(kCompactThreads, 8) qw_kv_compact_kernel(const
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const RowMove &m = moves[r0 + u * STEP];
-                if (m.delta < 0) continue;
+                if (m.skip) continue;
                 store_raw(v + m.to, q[u][2]);
                 store_raw(v + m.to + HALF, q[u][3]);
-                if (a.rope && m.delta > 0 && m.delta < a.rope_len) {
+                if (m.turn) {
                     float x[8], y[8];
                     unpack8(q[u][0], x);
                     unpack8(q[u][1], y);
-                    turn_back(x, y, a.rope + (size_t)m.delta * HALF + c);
+                    turn_back(x, y, m.turn + c, m.up);
                     put8(k + m.to, x);
                     put8(k + m.to + HALF, y);
                 } else {
@@ -190,11 +197,10 @@ __global__ void __launch_bounds__(kCompactThreads, 8) qw_kv_compact_kernel(const
 template <typename T>
 __global__ void __launch_bounds__(kCompactThreads) qw_kv_compact_any_kernel(const CompactArgs a) {
     const RowMove m = row_move(a, blockIdx.x * (kCompactThreads / 32) + (threadIdx.x >> 5));
-    if (m.delta < 0) return;
+    if (m.skip) return;
     const int lane = threadIdx.x & 31, half = a.d / 2, hv = half / 8;
     const size_t layer = (size_t)blockIdx.y * a.num_pages * a.heads * a.ps * a.d, head = (size_t)a.ps * a.d;
     T *k = reinterpret_cast<T *>(a.k) + layer, *v = reinterpret_cast<T *>(a.v) + layer;
-    const bool turn = a.rope && m.delta > 0 && m.delta < a.rope_len;
     for (int u = lane; u < a.heads * hv; u += 32) {
         const size_t at = (u / hv) * head + (u % hv) * 8;
         float x[8], y[8], vx[8], vy[8];
@@ -202,7 +208,7 @@ __global__ void __launch_bounds__(kCompactThreads) qw_kv_compact_any_kernel(cons
         load8(k + m.from + at + half, y);
         load8(v + m.from + at, vx);
         load8(v + m.from + at + half, vy);
-        if (turn) turn_back(x, y, a.rope + (size_t)m.delta * half + (u % hv) * 8);
+        if (m.turn) turn_back(x, y, m.turn + (u % hv) * 8, m.up);
         put8(k + m.to + at, x);
         put8(k + m.to + at + half, y);
         put8(v + m.to + at, vx);

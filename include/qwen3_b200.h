@@ -394,9 +394,11 @@ qw_status qw_op_kv_copy_pages(const qw_kv_pool *pool, const int32_t *src, const 
 
 /* Close the gaps that dropped positions leave: position dst_base[b] + i of sequence b in dst_table (dst_base NULL = 0)
  * receives position keep[keep_start[b] + i] of src_table, in every layer; keep is ascending within a sequence.  With
- * `rope` (rope_len, head_dim / 2, 2) = (cos, sin) per position, keys are turned back by the distance they move (in
- * fp32, rounded once), so that they lie as if they had been written at their new position; NULL copies them as they
- * are.  Tables are (batch, max_pages); rows = keep_start[batch]; all arrays are device arrays.  The destination pages
+ * `rope`, keys are turned by the distance they move, back when they move down and forward when they move up (in fp32,
+ * rounded once), so that they lie as if they had been written at their new position; row d of the table, (rope_len,
+ * head_dim / 2, 2) = (cos, sin), is the angle of a distance of d positions, and a row that moves by rope_len or more is left
+ * out.  NULL copies the keys as they are.  Rows whose old or new position is outside the tables, or has no page there, are left
+ * out too.  Tables are (batch, max_pages); rows = keep_start[batch]; all arrays are device arrays.  The destination pages
  * must not be among the source pages. */
 qw_status qw_op_kv_compact(const qw_kv_pool *pool, const int32_t *src_table, const int32_t *dst_table,
                            int32_t max_pages, const int32_t *keep, const int32_t *keep_start, const int32_t *dst_base,
