@@ -65,6 +65,7 @@ struct qw_model {
     uint32_t top_loaded = 0;
     bool finalized = false;
     float2 *freq = nullptr;
+    bool freq_by_distance = true;  // row a + b of the table turns by the angles of rows a and b together (qw_compact)
     // paged KV
     int page_size = 64, log2_page = 6, num_pages = 0, max_pages = 0;
     void *kpool = nullptr, *vpool = nullptr;
@@ -1458,6 +1459,28 @@ qw_status qw_init_synthetic(qw_model *m, uint64_t seed, float stdv) {
     return QW_OK;
 }
 
+// Whether a loaded RoPE table turns a key by an angle that grows evenly with its position, as one computed from a theta does
+// (a table scaled in length or with angles of another form does not).  Row p is compared with the product of rows p / 2 and
+// p - p / 2, so that row 1 fixes all of them; entries may be rounded to bf16 (three by 2^-9 in each component), and angles
+// computed in fp32 (2^-24 of an angle up to p, three times).
+static qw_status check_freq(qw_model *m) {
+    const int half = m->c.head_dim / 2;
+    std::vector<float2> t((size_t)m->c.seq_len * half);
+    CK(cudaMemcpyAsync(t.data(), m->freq, sizeof(float2) * t.size(), cudaMemcpyDeviceToHost, m->st));
+    CK(cudaStreamSynchronize(m->st));
+    m->freq_by_distance = true;
+    for (int p = 0; p < m->c.seq_len && m->freq_by_distance; p++) {
+        const float2 *x = t.data() + (size_t)p * half, *a = t.data() + (size_t)(p / 2) * half, *b = t.data() + (size_t)(p - p / 2) * half;
+        const float tol = 0x1p-6f + 0x1p-22f * p;
+        for (int i = 0; i < half; i++) {
+            const float re = p > 1 ? a[i].x * b[i].x - a[i].y * b[i].y : p ? x[i].x / hypotf(x[i].x, x[i].y) : 1.f;
+            const float im = p > 1 ? a[i].x * b[i].y + a[i].y * b[i].x : p ? x[i].y / hypotf(x[i].x, x[i].y) : 0.f;
+            if (!(fabsf(x[i].x - re) <= tol && fabsf(x[i].y - im) <= tol)) m->freq_by_distance = false;
+        }
+    }
+    return QW_OK;
+}
+
 qw_status qw_finalize_weights(qw_model *m) {
     if (!m) return QW_ERR_ARG;
     CK(cudaSetDevice(m->dev));
@@ -1492,6 +1515,10 @@ qw_status qw_finalize_weights(qw_model *m) {
         m->step.embed = (const __nv_bfloat16 *)m->embed;
     }
     CK(cudaStreamSynchronize(m->st));
+    if (m->top_loaded >> K_FREQ & 1) {
+        qw_status s = check_freq(m);
+        if (s) return s;
+    }
     m->finalized = true;
     return QW_OK;
 }
@@ -1695,6 +1722,8 @@ qw_status qw_compact(qw_model *m, int32_t slot, const int32_t *keep, int32_t n_k
         if (same == i && keep[i] == i) same++;
     }
     if (same == n_keep) return qw_truncate(m, slot, n_keep);
+    if (!m->freq_by_distance)
+        return fail(m, QW_ERR_UNSUPPORTED, "rope.freq_cis is not a table of angles that grow evenly with the position: keys cannot be moved");
     CK(cudaSetDevice(m->dev));
     const int base = same / ps;  // whole pages before stay, shared or not; the rest is gathered into new ones
     const int fresh = (n_keep + ps - 1) / ps - base;

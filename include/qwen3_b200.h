@@ -196,7 +196,9 @@ qw_status qw_truncate(qw_model *m, int32_t slot, int32_t n_positions);
  * 0 .. n_keep - 1, their keys turned to the rotary angles of their new positions (for bf16 caches rounded once more); the
  * next token stands at position n_keep.  Pages before the first dropped position stay as they are, shared or not; the
  * rest is gathered into new pages (QW_ERR_OOM, and nothing changed, when there are not enough) and the old ones are given
- * up. */
+ * up.  A key turns by the angle of the distance that it moves: with a loaded "rope.freq_cis" whose angles do not grow evenly
+ * with the position (or whose entries do not lie on the unit circle) the call returns QW_ERR_UNSUPPORTED, and nothing
+ * changes, unless the kept positions are the first ones. */
 qw_status qw_compact(qw_model *m, int32_t slot, const int32_t *keep, int32_t n_keep);
 
 /* Pages that no slot holds. */
