@@ -160,10 +160,10 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_simt_kernel(const Ch
             for (int c = 0; c < D / 16; c++) o[i][c] = 0.f;
             for (int z = 0; z < nsplit; z++) {
                 const float *p = reinterpret_cast<const float *>(parts + z * si_part_bytes(D));
-                const float pm = __ldcg(p + kSiRows * D + r);
-                if (pm == -INFINITY) continue;  // this range showed the row nothing
+                const float pm = __ldcg(p + kSiRows * D + r), pl = __ldcg(p + kSiRows * (D + 1) + r);
+                if (pl == 0.f) continue;  // this range showed the row nothing (NaN scores have no maximum, but a sum)
                 const float mn = fmaxf(m, pm), wo = exp2f(m - mn), wp = exp2f(pm - mn);
-                l = l * wo + __ldcg(p + kSiRows * (D + 1) + r) * wp;
+                l = l * wo + pl * wp;
 #pragma unroll
                 for (int c = 0; c < D / 16; c++) o[i][c] = o[i][c] * wo + __ldcg(p + r * D + tx + 16 * c) * wp;
                 m = mn;
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kSiThreads) qw_chunk_attn_rows_kernel(const Ch
     }
     // join the lanes that took different keys, then the warps, then (the last CTA of the row) the ranges
     auto join = [](float &m0, float &l0, float4 &o0, float m1, float l1, const float4 &o1) {
-        if (m1 == -INFINITY) return;
+        if (l1 == 0.f) return;  // nothing seen (NaN scores have no maximum, but a sum)
         const float mn = fmaxf(m0, m1), w0 = exp2f(m0 - mn), w1 = exp2f(m1 - mn);
         l0 = l0 * w0 + l1 * w1;
         o0 = make_float4(o0.x * w0 + o1.x * w1, o0.y * w0 + o1.y * w1, o0.z * w0 + o1.z * w1, o0.w * w0 + o1.w * w1);

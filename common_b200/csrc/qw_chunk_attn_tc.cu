@@ -348,7 +348,8 @@ __device__ __forceinline__ void put_row(const ChunkArgs &a, const Shared &m, int
     if (c4 == 0 && a.lse) a.lse[grow * a.H + head] = l == 0.f ? -INFINITY : (M + __log2f(l)) * 0.69314718055994531f;
 }
 
-// Rows [lo, lo + nr) of a shared item: sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, m = max m_p, over its parts.
+// Rows [lo, lo + nr) of a shared item: sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, m = max m_p, over its parts.  (A part
+// of NaN scores has no maximum, but a sum of NaN.)
 template <int D>
 __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, int lo, int nr, int tid, float *red) {
     const int nparts = m.pair ? m.np : 2 * m.np;
@@ -373,7 +374,7 @@ __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, i
                 float4 x[8];
 #pragma unroll
                 for (int c = 0; c < 8; c++) x[c] = __ldcg(px.o(c0 + c, row));
-                if (ml.x == -INFINITY) continue;  // nothing seen there (O may not have been written)
+                if (ml.y == 0.f) continue;  // nothing seen there (O may not have been written)
                 const float mn = fmaxf(M, ml.x), wo = ex2(M - mn), wx = ex2(ml.x - mn);
 #pragma unroll
                 for (int c = 0; c < 8; c++) {
@@ -403,7 +404,7 @@ __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, i
                 const Part<D> px = part(p, tile);
                 const float2 ml = __ldcg(px.ml(row));
                 const float4 x = __ldcg(px.o(c4, row));
-                if (ml.x == -INFINITY) continue;
+                if (ml.y == 0.f) continue;
                 const float mn = fmaxf(M, ml.x), wo = ex2(M - mn), wx = ex2(ml.x - mn);
                 o.x = o.x * wo + x.x * wx; o.y = o.y * wo + x.y * wx;
                 o.z = o.z * wo + x.z * wx; o.w = o.w * wo + x.w * wx;
@@ -418,7 +419,7 @@ __device__ __forceinline__ void join_rows(const ChunkArgs &a, const Shared &m, i
             if (on && g == 0)
                 for (int h = 1; h < ng; h++) {
                     const float *x = red + (h * E + e) * 8;
-                    if (x[0] == -INFINITY) continue;
+                    if (x[1] == 0.f) continue;
                     const float mn = fmaxf(M, x[0]), wo = ex2(M - mn), wx = ex2(x[0] - mn);
                     o.x = o.x * wo + x[2] * wx; o.y = o.y * wo + x[3] * wx;
                     o.z = o.z * wo + x[4] * wx; o.w = o.w * wo + x[5] * wx;
