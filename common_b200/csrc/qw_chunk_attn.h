@@ -8,6 +8,7 @@ namespace qw {
 
 constexpr int kChunkMaxBatch = 1024;  // sequences of one call (their schedule lies in shared memory)
 constexpr int kChunkCounterBytes = 3 * 256 * 4;  // the workspace begins with counters, zero between calls
+                                                 // (but for one whose bounded wait gave up)
 
 struct ChunkArgs {
     const void *q, *k, *v;  // q (rows, ld_q): heads side by side; k, v: one layer's pages

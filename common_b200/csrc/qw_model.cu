@@ -1079,7 +1079,10 @@ qw_status tc_extend(qw_model *m, const int32_t *tokens, const int32_t *row_start
         CK(cudaMemcpyAsync(logits_out, dlog, sizeof(float) * (size_t)batch * m->c.vocab, cudaMemcpyDeviceToHost, m->st));
     CK(cudaMemcpyAsync(&pin[0], pf.d_err, sizeof(int), cudaMemcpyDeviceToHost, m->st));
     CK(cudaStreamSynchronize(m->st));
-    if (pin[0]) return fail(m, QW_ERR_TIMEOUT, "tensor-core kernel gave up waiting (device error %d)", pin[0]);
+    if (pin[0]) {  // the attention may have left counts of its own in its workspace
+        CK(cudaMemsetAsync(m->chunk_ws, 0, qw_op_chunk_attn_workspace(m->Hl, m->Hkvl, m->c.head_dim), m->st));
+        return fail(m, QW_ERR_TIMEOUT, "tensor-core kernel gave up waiting (device error %d)", pin[0]);
+    }
     if (argmax_out) memcpy(argmax_out, hp, sizeof(int) * batch);
     return QW_OK;
 }

@@ -203,8 +203,9 @@ def chunk_attn_workspace(heads: int, kv_heads: int, head_dim: int) -> int:
 
 class ChunkAttention:
     """qw_op_chunk_attn over raw device pointers: the geometry and the workspace once, then one call per layer and
-    step.  The workspace (chunk_attn_workspace bytes, zeroed by the caller before the first call) serves one call at a
-    time: calls that overlap on the GPU need a ChunkAttention with a workspace of its own."""
+    step.  The workspace (chunk_attn_workspace bytes, zeroed by the caller before the first call, and again after a call
+    that set the err word) serves one call at a time: calls that overlap on the GPU need a ChunkAttention with a workspace
+    of its own."""
 
     def __init__(self, heads: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, max_pages: int,
                  workspace_ptr: int, workspace_bytes: int, window: int = 0, scale: float = 0.0,

@@ -352,7 +352,8 @@ typedef struct qw_chunk_attn_args {
     const int32_t *kv_len;     /* (batch) cached positions of each sequence, its new rows included */
     void *out;                 /* (rows, ld_out) in dtype */
     float *lse;                /* optional (rows, heads): natural log of the softmax sum */
-    void *workspace;           /* qw_op_chunk_attn_workspace bytes, 256-byte aligned, zeroed before its first call */
+    void *workspace;           /* qw_op_chunk_attn_workspace bytes, 256-byte aligned, zeroed before its first call and
+                                  again after a call that set err */
     int32_t *err;              /* optional device word, set non-zero when a bounded device wait gave up, or (bf16) when
                                   a row_start that does not ascend names more work than 32 bits number: none is done */
     int64_t ld_q, ld_out;      /* row strides in elements, multiples of 16 bytes; 0 = heads * head_dim */
@@ -372,7 +373,8 @@ typedef struct qw_chunk_attn_args {
  * that sees nothing gives zeros and an lse of -infinity.  What lies in the cache outside the positions that some row
  * of the sequence sees is never used, whatever it holds.  fp32 accumulation and softmax.  The lengths are read on the
  * device: nothing in the call depends on them, so a captured call follows new ones.  The workspace carries no results
- * between calls, but calls that overlap on the GPU need one each.  batch <= 1024, and in bf16 rows x heads x max_pages x
+ * between calls, but calls that overlap on the GPU need one each; a call whose wait gave up leaves counts in it that a
+ * later call would take for its own, so pass err, and zero the workspace before the next call where it was set.  batch <= 1024, and in bf16 rows x heads x max_pages x
  * page_size below about 2^46 (QW_ERR_SHAPE beyond).  A row's own masked positions that others of its sequence see (those
  * after it in its chunk, those before its window) may hold any finite values, and any keys; an infinite or NaN value there
  * can reach it, as 0 x infinity does.  Stands in for the scores, mask, softmax and value sum of the reference's attention
