@@ -43,6 +43,56 @@ def test_row_starts_outside_the_rows_are_clamped(dtype, new, lengths):
     _check(c, bufs)
 
 
+def _reference(c, kv):
+    """(out, A, lse) in 64 bits with the lengths `kv` (within the table), where a page that is none reads as zeros."""
+    import torch
+    G, d, r = c.H // c.Hkv, c.d, 0
+    out = torch.zeros((c.rows, c.H, d), dtype=torch.float64, device="cuda")
+    A, lse = torch.zeros_like(out), torch.zeros((c.rows, c.H), dtype=torch.float64, device="cuda")
+    for b, (n, m) in enumerate(zip(c.new, kv)):
+        p = torch.arange(m, device="cuda")
+        pg = c.table[len(c.new) - b].long()[p // c.page]
+        there = ((pg >= 0) & (pg < c.num_pages))[:, None, None]
+        pg = torch.where(there[:, 0, 0], pg, 0)
+        k = torch.where(there, c.k[pg, :, p % c.page].double(), 0.0)
+        v = torch.where(there, c.v[pg, :, p % c.page].double(), 0.0)
+        q = c.q[r : r + n].double().view(n, c.Hkv, G, d)
+        x = torch.einsum("nhgd,lhd->hgnl", q, k) / d ** 0.5
+        x = x.masked_fill(p[None] > torch.arange(m - n, m, device="cuda")[:, None], -float("inf"))
+        w = torch.softmax(x, -1)
+        out[r : r + n] = torch.einsum("hgnl,lhd->nhgd", w, v).reshape(n, c.H, d)
+        A[r : r + n] = torch.einsum("hgnl,lhd->nhgd", w, v.abs()).reshape(n, c.H, d)
+        lse[r : r + n] = torch.logsumexp(x, -1).permute(2, 0, 1).reshape(n, c.H)
+        r += n
+    return out, A, lse
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("new,kv", [([3, 2, 7], [100, 60, 500]), ([1, 1, 1], [100, 60, 500]), ([40, 90, 1], [100, 130, 9000])])
+def test_lengths_beyond_the_table_are_clamped_and_pages_that_are_none_read_as_zeros(dtype, new, kv):
+    """Sequence 0 is said to be longer than its slot, sequence 1's first page and sequence 2's second one have numbers outside
+    the pool; the third is itself in order beyond that."""
+    import torch
+    c = Case(new, kv, 16, 8, 128, 64, dtype=dtype, seed=10)
+    g = torch.Generator(device="cuda").manual_seed(32)
+    c.k = torch.randn(c.k.shape, device="cuda", generator=g).to(c.dt)  # all of the pool: the clamped length reaches further
+    c.v = torch.randn(c.v.shape, device="cuda", generator=g).to(c.dt)
+    c.kv_len[0] = 1 << 30
+    c.table[2, 0] = 1 << 30
+    c.table[1, 1] = -(1 << 31)
+    bufs = _guarded(c)
+    c.run()
+    torch.cuda.synchronize()
+    assert int(c.err.item()) == 0
+    out, A, lse = _reference(c, [c.max_pages * 64] + kv[1:])
+    got = c.obuf.view(c.rows, c.H, c.d).double()
+    tol = 2.0 ** -8 * (A + out.abs()) + 2.0 ** -12 * A if dtype == "bf16" else 2e-5 * A
+    assert bool(((got - out).abs() <= tol).all())
+    assert (c.lse.double() - lse).abs().max().item() < (1e-4 if dtype == "bf16" else 2e-5)
+    for b in bufs:
+        assert bool((b[:GUARD] == -7.0).all()) and bool((b[GUARD + c.rows :] == -7.0).all())
+
+
 def test_more_rows_that_see_nothing_than_32_bits_count_vectors_of():
     """2^21 rows of 64 heads of 128 are 2^31 vectors of 16 bytes (34 GB): a sequence with nothing cached."""
     import torch
