@@ -17,7 +17,7 @@
 // What bounds it (32 heads over 8 KV heads of 128 where not said otherwise):
 //   long chunks: a slot's chain S (690 clocks), softmax (1900, of which the exponentials of two slots on the 16 a clock of
 //     an SM take 1024 each), P V (560) and the commits between them, beside the other slot's: a pair of blocks every 3700
-//     clocks.  4096 rows over 20096 positions: 1005 us, 1.21 PFLOP/s (0.73 of what cuBLAS reaches); 1120 us once the power
+//     clocks.  4096 rows over 20096 positions: 1010 us, 1.20 PFLOP/s (0.73 of what cuBLAS reaches); 1140 us once the power
 //     limit holds the clock down
 //   single tokens: HBM.  64 sequences over 3900..4250 positions: 168 us, 6.4 TB/s (176 under the
 //     power limit); one over 120001: 86 us, 5.7 TB/s
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---------------- K and V ----------------
             const int br = min(a.ps, kKeys), nbox = kKeys / br;
             const int box = lane / NH, half = lane % NH;
-            // Keys that one item alone reads pass through L2 without pushing out what others use: 64 tokens over 3900..4250
+            // Keys that no other item of their sequence reads pass through L2 without pushing out what others use: 64 tokens over 3900..4250
             // positions 169 us, 174 without; one over 120001 86 us, 89, and behind an L2 full of written lines 96 and 105.
             // (Sequences whose pages are the same ones lose by it: 64 tokens over the same 4000 positions 129 us, 123 without.)
             uint64_t once;
@@ -971,7 +971,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         need = true;
                     }
                     // p = 2^(s scale log2 e - m); P goes to TMEM as packed bf16 pairs over the first half of this half's
-                    // columns of S, and its sum is taken before that rounding
+                    // columns of S, and its sum is taken before that rounding.  P is rounded because the tensor cores take it in
+                    // V's type: each p is off by 2^-8 of itself at most, and a result by as much of sum p |v| / sum p (relative
+                    // L2 against 64 bits: 2.3e-3, and 1.7e-3 where only the result is rounded to bf16).  A second product with what
+                    // the rounding leaves would double P V.
                     const float off = m_use == -INFINITY ? 0.f : -m_use;
                     const uint64_t off2 = f2(off, off), sl2 = f2(a.sl2, a.sl2);
                     uint64_t s2[2] = {0, 0};

@@ -144,8 +144,9 @@ __device__ __forceinline__ void store_raw(T *p, const Raw8<T> &r) {
 // One CTA per (kCompactRows kept rows, layer).  The rows' places are looked up once; a warp then takes a head at a time: its rows
 // are one contiguous piece of a destination page (mostly of a source page too).  A lane takes 8 elements of a row's first
 // half and the matching 8 of its second (the rotary pairs), HV lanes a row, and has U rows of keys and values on the way.
-// Bound by HBM: 3.74 GB moved at 6.3 TB/s (592 us; 28 layers, 8 heads of 128, bf16), 337 MB at 5.9 TB/s (57 us), where the last
-// CTAs and the launch show.  What counts is loads in flight per SM and small CTAs to end on: 2 rows a lane in 4 CTAs of
+// Bound by HBM: 3.74 GB moved at 6.4 TB/s (582 us; 28 layers, 8 heads of 128, bf16), 337 MB at 5.9 TB/s (57 us), where the last
+// CTAs and the launch show; 7.5 GB in fp32 at 6.2 TB/s (1200 us); at head size 64 1.87 GB in bf16 at 5.7 TB/s (328 us) and 3.74 GB in
+// fp32 at 6.3 TB/s (590 us).  What counts is loads in flight per SM and small CTAs to end on: 2 rows a lane in 4 CTAs of
 // 256 threads (64 registers) against 4 rows in 2 CTAs (113 registers) take 604 against 724 us; 128 threads and 8 rows a
 // CTA 592 and 57.3, 256 threads and 16 rows 604 and 57.3, 128 and 16 590 and 59.8, 256 and 8 652 and 56.7; the
 // turns' arithmetic hides behind the loads.

@@ -371,8 +371,9 @@ typedef struct qw_chunk_attn_args {
  * new rows (none and one included) over any numbers of cached positions.  Row i of a sequence's n new rows stands at
  * position p = kv_len - n + i and sees positions max(0, p - window + 1) .. p (all up to p without a window); a row
  * that sees nothing gives zeros and an lse of -infinity.  What lies in the cache outside the positions that some row
- * of the sequence sees is never used, whatever it holds.  fp32 accumulation and softmax.  The lengths are read on the
- * device: nothing in the call depends on them, so a captured call follows new ones.  The workspace carries no results
+ * of the sequence sees is never used, whatever it holds.  Scores, maxima, sums and outputs accumulate in fp32; in bf16 the
+ * probabilities are rounded to bf16 before they multiply the values (their sum is not), and the result once; a row with NaN
+ * scores gives NaN.  The lengths are read on the device: nothing in the call depends on them, so a captured call follows new ones.  The workspace carries no results
  * between calls, but calls that overlap on the GPU need one each; a call whose wait gave up leaves counts in it that a
  * later call would take for its own, so pass err, and zero the workspace before the next call where it was set.  batch <= 1024, and in bf16 rows x heads x max_pages x
  * page_size below about 2^46 (QW_ERR_SHAPE beyond).  A row's own masked positions that others of its sequence see (those
