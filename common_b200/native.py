@@ -28,6 +28,7 @@ EXPORTS = ("qw_abi_version", "qw_build_info", "qw_get_unique_id", "qw_create", "
            "qw_stream", "qw_last_launch_count", "qw_last_error", "qw_destroy", "qw_profile_decode",
            "qw_set_device_inputs", "qw_profile_prefill", "qw_op_lm_head_argmax", "qw_op_lm_head_argmax_static", "qw_op_linear", "qw_set_sampling", "qw_decode_sample", "qw_op_sample",
            "qw_op_chunk_attn", "qw_op_chunk_attn_workspace", "qw_op_kv_copy_pages", "qw_op_kv_compact",
+           "qw_op_norm_q8", "qw_op_quant_q8", "qw_op_linear_q8", "qw_op_kv_append",
            "qw_extend", "qw_fork", "qw_truncate", "qw_compact", "qw_free_pages")
 KERNEL_NAMES = {0: "other", 1: "qkv", 2: "attn", 3: "o_proj", 4: "gate_up", 5: "down", 6: "lm_head", 7: "step"}
 
@@ -53,6 +54,29 @@ class KvPool(C.Structure):
     """qw_kv_pool: KvPool(k_ptr, v_ptr, layers, num_pages, kv_heads, page_size, head_dim, dtype)"""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + \
         [(n, C.c_int32) for n in ("layers", "num_pages", "kv_heads", "page_size", "head_dim", "dtype")]
+
+
+class NormQ8Args(C.Structure):
+    """qw_norm_q8_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "delta", "norm_w", "sum", "q", "scale")] + \
+        [(n, C.c_int64) for n in ("ld_x", "ld_delta", "ld_sum", "ld_q")] + \
+        [(n, C.c_int32) for n in ("rows", "dim", "x_dtype", "delta_dtype")] + [("eps", C.c_double)]
+
+
+class LinearQ8Args(C.Structure):
+    """qw_linear_q8_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("w", "w_scale", "x", "x_scale", "bias", "resid", "out", "err")] + \
+        [(n, C.c_int64) for n in ("ld_w", "ld_x", "ld_resid", "ld_out")] + \
+        [(n, C.c_int32) for n in ("n_out", "k", "t", "epi", "out_dtype", "reserved")]
+
+
+class KvAppendArgs(C.Structure):
+    """qw_kv_append_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_norm", "k_norm", "rope", "q_out", "k_cache", "v_cache",
+                                          "page_table", "slots", "row_start", "kv_len")] + \
+        [(n, C.c_int64) for n in ("ld_q", "ld_k", "ld_v", "ld_q_out")] + \
+        [(n, C.c_int32) for n in ("in_dtype", "dtype", "batch", "rows", "heads", "kv_heads", "head_dim", "page_size",
+                                  "num_pages", "max_pages", "qk_norm", "rope_len")] + [("eps", C.c_double)]
 
 
 class QwenError(RuntimeError):
@@ -116,6 +140,10 @@ def load() -> C.CDLL:
         "qw_op_chunk_attn_workspace": (C.c_uint64, [I32, I32, I32]),
         "qw_op_kv_copy_pages": (I32, [C.POINTER(KvPool), P, P, P, I32, P]),
         "qw_op_kv_compact": (I32, [C.POINTER(KvPool), P, P, I32, P, P, P, I32, I32, P, I32, P]),
+        "qw_op_norm_q8": (I32, [C.POINTER(NormQ8Args), P]),
+        "qw_op_quant_q8": (I32, [P, I32, I32, I32, C.c_int64, P, C.c_int64, P, P]),
+        "qw_op_linear_q8": (I32, [C.POINTER(LinearQ8Args), P]),
+        "qw_op_kv_append": (I32, [C.POINTER(KvAppendArgs), P]),
         "qw_op_lm_head_argmax_static": (I32, [P, I32, I32, I32, P, P, C.c_double, I32, P, P, P]),
     }
     for name, (res, args) in sig.items():
@@ -242,6 +270,80 @@ def op_kv_compact(pool: KvPool, src_table: int, dst_table: int, max_pages: int, 
                                            rope, rope_len, stream)
     if st:
         raise QwenError(st, op_error())
+
+
+class NormQ8:
+    """qw_op_norm_q8 over raw device pointers: the norm's weights and the types once, then one call per block."""
+
+    def __init__(self, dim: int, norm_w_ptr: int, eps: float = 1e-6, x_dtype: int = DTYPE_F32,
+                 delta_dtype: int = DTYPE_F32):
+        self._fn = load().qw_op_norm_q8
+        a = self.args = NormQ8Args()
+        a.dim, a.norm_w, a.eps, a.x_dtype, a.delta_dtype = dim, norm_w_ptr, eps, x_dtype, delta_dtype
+        self._ref = C.byref(a)
+
+    def __call__(self, x: int, q: int, scale: int, rows: int, delta: int = 0, sum_out: int = 0, ld_x: int = 0,
+                 ld_delta: int = 0, ld_sum: int = 0, ld_q: int = 0, stream: int = 0) -> None:
+        a = self.args
+        a.x, a.q, a.scale, a.rows, a.delta, a.sum = x, q, scale, rows, delta, sum_out
+        a.ld_x, a.ld_delta, a.ld_sum, a.ld_q = ld_x, ld_delta, ld_sum, ld_q
+        st = self._fn(self._ref, stream)
+        if st:
+            raise QwenError(st, op_error())
+
+
+def op_quant_q8(x_ptr: int, x_dtype: int, rows: int, dim: int, q_ptr: int, scale_ptr: int, ld_x: int = 0, ld_q: int = 0,
+                stream: int = 0) -> None:
+    """qw_op_quant_q8 over raw device pointers."""
+    st = (_lib or load()).qw_op_quant_q8(x_ptr, x_dtype, rows, dim, ld_x, q_ptr, ld_q, scale_ptr, stream)
+    if st:
+        raise QwenError(st, op_error())
+
+
+class LinearQ8:
+    """qw_op_linear_q8 over raw device pointers: a projection's codes, scales and epilogue once, then one call per step."""
+
+    def __init__(self, w: int, w_scale: int, n_out: int, k: int, ld_w: int = 0, epi: int = LINEAR_STORE, bias: int = 0,
+                 out_dtype: int = DTYPE_F32):
+        self._fn = load().qw_op_linear_q8
+        a = self.args = LinearQ8Args()
+        a.w, a.w_scale, a.n_out, a.k, a.ld_w, a.epi, a.bias, a.out_dtype = w, w_scale, n_out, k, ld_w, epi, bias, out_dtype
+        self._ref = C.byref(a)
+
+    def __call__(self, x: int, x_scale: int, t: int, out: int, resid: int = 0, ld_x: int = 0, ld_resid: int = 0,
+                 ld_out: int = 0, err: int = 0, stream: int = 0) -> None:
+        a = self.args
+        a.x, a.x_scale, a.t, a.out, a.resid, a.err = x, x_scale, t, out, resid, err
+        a.ld_x, a.ld_resid, a.ld_out = ld_x, ld_resid, ld_out
+        st = self._fn(self._ref, stream)
+        if st:
+            raise QwenError(st, op_error())
+
+
+class KvAppend:
+    """qw_op_kv_append over raw device pointers: the geometry, norms and rotation once, then one call per layer and step."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, max_pages: int,
+                 rope: int = 0, rope_len: int = 0, qk_norm: int = QKNORM_NONE, q_norm: int = 0, k_norm: int = 0,
+                 eps: float = 1e-6, in_dtype: int = DTYPE_F32, dtype: int = DTYPE_BF16):
+        self._fn = load().qw_op_kv_append
+        a = self.args = KvAppendArgs()
+        a.heads, a.kv_heads, a.head_dim = heads, kv_heads, head_dim
+        a.page_size, a.num_pages, a.max_pages = page_size, num_pages, max_pages
+        a.rope, a.rope_len, a.qk_norm, a.q_norm, a.k_norm, a.eps = rope, rope_len, qk_norm, q_norm, k_norm, eps
+        a.in_dtype, a.dtype = in_dtype, dtype
+        self._ref = C.byref(a)
+
+    def __call__(self, q: int, k: int, v: int, q_out: int, k_cache: int, v_cache: int, page_table: int, row_start: int,
+                 kv_len: int, batch: int, rows: int, slots: int = 0, ld_q: int = 0, ld_k: int = 0, ld_v: int = 0,
+                 ld_q_out: int = 0, stream: int = 0) -> None:
+        a = self.args
+        a.q, a.k, a.v, a.q_out, a.k_cache, a.v_cache = q, k, v, q_out, k_cache, v_cache
+        a.page_table, a.row_start, a.kv_len, a.batch, a.rows, a.slots = page_table, row_start, kv_len, batch, rows, slots
+        a.ld_q, a.ld_k, a.ld_v, a.ld_q_out = ld_q, ld_k, ld_v, ld_q_out
+        st = self._fn(self._ref, stream)
+        if st:
+            raise QwenError(st, op_error())
 
 
 def unique_id() -> bytes:

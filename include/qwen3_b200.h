@@ -409,6 +409,97 @@ qw_status qw_op_kv_compact(const qw_kv_pool *pool, const int32_t *src_table, con
                            int32_t max_pages, const int32_t *keep, const int32_t *keep_start, const int32_t *dst_base,
                            int32_t batch, int32_t rows, const float *rope, int32_t rope_len, void *stream);
 
+/* ---- a decoder layer in 8 bits -----------------------------------------------------------------
+ * Rows of 8-bit codes with a scale each: a row x of fp32 numbers has scale = max|x| / 127 and the codes rint(127 x / max|x|),
+ * halves to even, exactly as real arithmetic gives them; code * scale is what it stands for.  A row whose largest magnitude is
+ * below 127 * 2^-126 has scale 0 and codes 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so that every
+ * product with it is NaN.  The weights of qw_op_linear_q8 are coded by rows the same way (qw_op_quant_q8), once.
+ * One layer: qw_op_norm_q8 -> qw_op_linear_q8 (q, k, v) -> qw_op_kv_append -> qw_op_chunk_attn -> qw_op_quant_q8 ->
+ * qw_op_linear_q8 (o) -> qw_op_norm_q8 -> qw_op_linear_q8 (gate and up, SWIGLU) -> qw_op_quant_q8 -> qw_op_linear_q8 (down).
+ * The calls hold no workspace and keep nothing between them; they can be captured, and overlap on any streams.  The
+ * reference's layers are in the precision of its collections (SequentialBlock.java:413-429, NormalizationLayerFeatures.java:574-604,
+ * LayerFeatures.java:785-830); it has no coded form. */
+
+/* Arguments of qw_op_norm_q8; all pointers are device pointers.  Zero-initialise the struct. */
+typedef struct qw_norm_q8_args {
+    const void *x;       /* (rows, ld_x) in x_dtype: the residual stream */
+    const void *delta;   /* optional (rows, ld_delta) in delta_dtype: what a block adds to it */
+    const float *norm_w; /* (dim) */
+    void *sum;           /* optional (rows, ld_sum) in x_dtype: the next residual stream; may be x, or delta where delta has
+                            its type, with the same stride */
+    int8_t *q;           /* (rows, ld_q) codes */
+    float *scale;        /* (rows) */
+    int64_t ld_x, ld_delta, ld_sum, ld_q; /* row strides in elements, at least dim; 0 = dim */
+    int32_t rows, dim;
+    int32_t x_dtype, delta_dtype; /* QW_DTYPE_F32 or QW_DTYPE_BF16 */
+    double eps;
+} qw_norm_q8_args;
+
+/* Residual addition, root-mean-square norm and codes in one pass: h = x + delta (fp32), sum = h (rounded once where the
+ * stream is bf16; the norm sees h), y = h / sqrt(mean(h^2) + eps) * norm_w, then the codes and the scale of every row of y.
+ * The norm cancels in the codes: they are those of the fp32 products h * norm_w, exactly.  The sum of squares is held in
+ * 64 bits; scale is within 2^-21 of its value.  Stands in for accum + rmsnorm (SequentialBlock.java:413-429,
+ * NormalizationLayerFeatures.java:574-604), which it codes. */
+qw_status qw_op_norm_q8(const qw_norm_q8_args *args, void *stream);
+
+/* The codes (rows, ld_q) and scales (rows) of rows x (rows, ld_x) of dim numbers in x_dtype (F32 or BF16); strides in
+ * elements, 0 = dim.  For what qw_op_linear_q8 multiplies: attention results, SwiGLU products, weights. */
+qw_status qw_op_quant_q8(const void *x, int32_t x_dtype, int32_t rows, int32_t dim, int64_t ld_x, int8_t *q, int64_t ld_q,
+                         float *scale, void *stream);
+
+/* Arguments of qw_op_linear_q8; all pointers are device pointers.  Zero-initialise the struct. */
+typedef struct qw_linear_q8_args {
+    const int8_t *w;      /* (n_out, ld_w) codes, 16-byte aligned; for SWIGLU rows interleaved as for qw_op_linear */
+    const float *w_scale; /* (n_out) */
+    const int8_t *x;      /* (t, ld_x) codes, 16-byte aligned */
+    const float *x_scale; /* (t) */
+    const float *bias;    /* STORE: optional (n_out) */
+    const float *resid;   /* RESID: (t, ld_resid); out may be resid, with the same stride */
+    void *out;            /* (t, ld_out) in out_dtype; n_out / 2 columns for SWIGLU */
+    int32_t *err;         /* optional device word, set non-zero when a bounded device wait gave up */
+    int64_t ld_w, ld_x;   /* row strides in codes, multiples of 16; 0 = k.  What lies behind a row's k codes is not used */
+    int64_t ld_resid, ld_out; /* row strides in elements; 0 = the columns */
+    int32_t n_out, k, t;  /* k up to 131071: a sum of products of codes fits 32 bits */
+    int32_t epi;          /* QW_LINEAR_STORE, QW_LINEAR_RESID or QW_LINEAR_SWIGLU */
+    int32_t out_dtype;    /* STORE: F32 or BF16; RESID: F32; SWIGLU: BF16 */
+    int32_t reserved;
+} qw_linear_q8_args;
+
+/* Projection of codes on the tensor cores (tcgen05 kind::i8): s(t, f) = sum_j w(f, j) x(t, j) in 32-bit integers, exact,
+ * y(t, f) = s w_scale(f) x_scale(t), then by `epi` STORE out = y (+ bias), RESID out = resid + y, SWIGLU out = up * silu(gate).
+ * The sums being exact, results do not depend on how the work is split. */
+qw_status qw_op_linear_q8(const qw_linear_q8_args *args, void *stream);
+
+/* Arguments of qw_op_kv_append; all pointers are device pointers.  Zero-initialise the struct. */
+typedef struct qw_kv_append_args {
+    const void *q, *k, *v;     /* (rows, ld_q / ld_k / ld_v) in in_dtype: the projections of every row, side by side or apart */
+    const float *q_norm, *k_norm; /* VECTOR: (heads x head_dim), (kv_heads x head_dim); HEAD: (head_dim) each; NONE: unused */
+    const float *rope;         /* optional (rope_len, head_dim / 2, 2) = (cos, sin) of every position; NULL: no rotation */
+    void *q_out;               /* (rows, ld_q_out) in dtype; may be q where types and strides are the same; NULL: none */
+    void *k_cache, *v_cache;   /* one layer of the cache, in dtype */
+    const int32_t *page_table; /* [slot][max_pages] */
+    const int32_t *slots;      /* (batch) table row of each sequence; NULL = 0..batch-1 */
+    const int32_t *row_start;  /* (batch + 1) sequence b's new rows are row_start[b] .. row_start[b + 1] - 1 */
+    const int32_t *kv_len;     /* (batch) cached positions of each sequence, its new rows included */
+    int64_t ld_q, ld_k, ld_v, ld_q_out; /* row strides in elements, multiples of 16 bytes; 0 = the heads' columns */
+    int32_t in_dtype, dtype;   /* QW_DTYPE_F32 or QW_DTYPE_BF16 */
+    int32_t batch, rows;       /* rows: those of the buffers; rows from row_start[batch] on are left as they are */
+    int32_t heads, kv_heads, head_dim; /* head_dim a power of two in [16, 256] */
+    int32_t page_size, num_pages, max_pages;
+    int32_t qk_norm;           /* qw_qknorm */
+    int32_t rope_len;
+    double eps;                /* of the norms */
+} qw_kv_append_args;
+
+/* The new rows of a ragged batch on their way into the paged cache, in one launch: norms of q and k, rotation by their
+ * positions (split halves), queries to q_out, keys and values into their pages; row_start, kv_len, slots and tables are
+ * those that qw_op_chunk_attn then takes, read on the device.  Row i of a sequence's n new rows stands at position
+ * p = kv_len - n + i (kv_len limited to the table's positions).  A row before position 0 or, with rope, at rope_len or
+ * behind it is no row: q_out gets zeros, the cache nothing.  A position without a page takes no key and no value.  Two rows
+ * must not stand at one position of one page.  Arithmetic is in fp32, rounded once.  Stands in for QK-norm, rotation and the
+ * cache write (AttentionFeatures.java:823-891, RotationFeatures.java:124-208), one row of one sequence there. */
+qw_status qw_op_kv_append(const qw_kv_append_args *args, void *stream);
+
 /* Human-readable description of the last error on this model (never NULL).  With m == NULL:
  * the last error of an op-level entry point on this thread. */
 const char *qw_last_error(const qw_model *m);
