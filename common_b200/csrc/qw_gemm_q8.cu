@@ -15,6 +15,7 @@
 // its copies and MMAs land, frees its tensor memory and returns.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <mutex>
 #include <string>
 
@@ -28,7 +29,7 @@ namespace qw {
 namespace {
 
 constexpr int kQ8MaxK = 131071;  // |s| <= 128 * 128 * k < 2^31 for any codes
-constexpr int kQ8Threads = 192;
+constexpr int kQ8Threads = 320;  // a warp for the loads, one for the MMAs, eight for the results
 constexpr int kBM = 128, kBK = 128;  // features of a CTA, codes of a k-block
 constexpr int kABytes = kBM * kBK;
 
@@ -63,19 +64,67 @@ __device__ __forceinline__ void q8_mma(uint32_t d_tmem, uint64_t adesc, uint64_t
             "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
             : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// arrive on the mbarrier (of both CTAs of a pair) once the MMAs issued so far complete; rank: this CTA's in its cluster
+template <int CTAS>
+__device__ __forceinline__ void q8_commit(uint64_t *bar, int rank) {
+    if (CTAS == 1)
+        tc_commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+            "h"((uint16_t)(3 << (rank & ~1)))
+            : "memory");
 }
-__device__ __forceinline__ int ld_cluster(uint32_t addr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void tmem_alloc(uint32_t *base, uint32_t cols) {
+    if (CTAS == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
+    tc_fence_after();
+    if (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+// wait, bounded, for a phase that comes unless a copy or an MMA was never issued
+__device__ __forceinline__ void mbar_settle(uint64_t *bar, uint32_t parity) {
+    const uint32_t addr = smem_u32(bar);
+    const uint64_t c0 = gtime_ns();
+    while (!mbar_try(addr, parity) && gtime_ns() - c0 < kTcuWaitCycles) {
+    }
+}
+// N columns of this warp's 32 tensor-memory lanes
+template <int N>
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[N]) {
+    static_assert(N == 8 || N == 16 || N == 32, "columns");
+    if constexpr (N == 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(taddr));
+    else if constexpr (N == 16)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr));
+    else
+        tmem_ld32(taddr, r);
+    if constexpr (N < 32) asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int4 ld_cluster4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
+
+// up * gate / (1 + e^-gate): the exponential and the division are within (|gate| + 4) 2^-21 of their value, the result is rounded
+// to bf16 behind it.  A gate whose exponential leaves fp32 gives 0.
+__device__ __forceinline__ float silu_times(float g, float u) { return u * __fdividef(g, 1.0f + __expf(-g)); }
 
 // What a lane keeps for its feature f across the tokens of a tile.
 struct Q8Lane {
@@ -91,43 +140,84 @@ __device__ __forceinline__ Q8Lane q8_lane(const Q8GemmArgs &a, int f) {
     return l;
 }
 
-// Results of N consecutive tokens t0 .. t0 + nj - 1 (nj <= N) of feature f (this lane) from their sums.  The lanes of a warp hold
-// 32 consecutive features, so that a token's results are one contiguous piece of 128 (fp32), 64 or 32 bytes (bf16): whole
-// sectors where the rows are aligned to them.
-template <int EPI, int N>
-__device__ __forceinline__ void q8_emit(const Q8GemmArgs &a, const Q8Lane &l, const int (&s)[N], int f, int lane, int t0, int nj) {
-    static_assert(N <= 32 && (N == 1 || N % 2 == 0), "tokens of a piece");
-    const float xs = lane < nj ? a.x_scale[t0 + lane] : 0.f;
+// Results of N consecutive tokens t0 .. t0 + nj - 1 (nj <= N) of feature f (this lane) from their sums; xs: the tokens' scales in
+// shared memory, 16-byte aligned.  The lanes of a warp hold 32 consecutive features, so that a token's results are one
+// contiguous piece of 128 (fp32), 64 or 32 bytes (bf16): whole sectors where the rows are aligned to them.  FULL: nj = N and
+// f < M on every lane; the epilogue's instructions, on one or two warps per scheduler, are what the MMAs of short K wait for.
+template <int EPI, int N, bool FULL>
+__device__ __forceinline__ void q8_emit_some(const Q8GemmArgs &a, const Q8Lane &l, const uint32_t (&s)[N], const float *xs, int f,
+                                             int lane, long long t0, int nj) {
+    float y[N];
+    if (EPI == Q8_RESID) {  // all loads before the stores: out may be resid
+        const float *r = a.resid + t0 * a.ld_resid + f;
+#pragma unroll
+        for (int j = 0; j < N; j++, r += a.ld_resid) y[j] = FULL || (l.on && j < nj) ? *r : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(xs + j);
+        const float v[4] = {(float)(int)s[j] * l.ws * x.x, (float)(int)s[j + 1] * l.ws * x.y, (float)(int)s[j + 2] * l.ws * x.z,
+                            (float)(int)s[j + 3] * l.ws * x.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[j + i] = EPI == Q8_RESID ? y[j + i] + v[i] : EPI <= Q8_BF16 && a.bias ? v[i] + l.bias : v[i];
+    }
     if (EPI == Q8_SWIGLU) {
-        // lanes 0..15 hold gates, 16..31 the ups of the same 16 products: of two tokens the lower lane computes the first and the
-        // upper lane the second.  2^(-g log2 e) and its division are within 2^-21 (|g| + 4); the result is rounded to bf16.
-        __nv_bfloat16 *o = reinterpret_cast<__nv_bfloat16 *>(a.out);
+        // lanes 0..15 hold gates, 16..31 the ups of the same 16 products: of two tokens the lower lane computes the first and
+        // the upper lane the second
         const bool hi = lane & 16;
-        const int pair = (f >> 5) * 16 + (lane & 15);
+        __nv_bfloat16 *o = reinterpret_cast<__nv_bfloat16 *>(a.out) + (t0 + hi) * a.ld_out + (f >> 5) * 16 + (lane & 15);
 #pragma unroll
         for (int j = 0; j < N; j += 2) {
-            const float y0 = (float)s[j] * l.ws * __shfl_sync(0xffffffffu, xs, j);
-            const float y1 = N == 1 ? 0.f : (float)s[j + (N > 1)] * l.ws * __shfl_sync(0xffffffffu, xs, j + (N > 1));
-            const float other = __shfl_xor_sync(0xffffffffu, hi ? y0 : y1, 16);
-            const float g = hi ? other : y0, u = hi ? y1 : other;
-            const float h = u * __fdividef(g, 1.0f + __expf(-g));
-            if (l.on && j + hi < nj) o[(long long)(t0 + j + hi) * a.ld_out + pair] = __float2bfloat16_rn(h);
+            const float other = __shfl_xor_sync(0xffffffffu, hi ? y[j] : y[j + 1], 16);
+            y[j] = hi ? other : y[j];
+            y[j + 1] = hi ? y[j + 1] : other;
         }
-        return;
-    }
-    float r[N];
-    if (EPI == Q8_RESID) {  // all loads before the stores: out may be resid
 #pragma unroll
-        for (int j = 0; j < N; j++) r[j] = l.on && j < nj ? a.resid[(long long)(t0 + j) * a.ld_resid + f] : 0.f;
-    }
+        for (int j = 0; j < N; j += 2, o += 2 * a.ld_out) {
+            const float h = silu_times(y[j], y[j + 1]);
+            if (FULL || (l.on && j + hi < nj)) *o = __float2bfloat16_rn(h);
+        }
+    } else if (EPI == Q8_BF16) {
+        __nv_bfloat16 *o = reinterpret_cast<__nv_bfloat16 *>(a.out) + t0 * a.ld_out + f;
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-        float y = (float)s[j] * l.ws * __shfl_sync(0xffffffffu, xs, j);
-        if (EPI == Q8_RESID) y = r[j] + y;
-        else if (a.bias) y += l.bias;
-        if (l.on && j < nj) {
-            if (EPI == Q8_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[(long long)(t0 + j) * a.ld_out + f] = __float2bfloat16_rn(y);
-            else reinterpret_cast<float *>(a.out)[(long long)(t0 + j) * a.ld_out + f] = y;
+        for (int j = 0; j < N; j++, o += a.ld_out)
+            if (FULL || (l.on && j < nj)) *o = __float2bfloat16_rn(y[j]);
+    } else {
+        float *o = reinterpret_cast<float *>(a.out) + t0 * a.ld_out + f;
+#pragma unroll
+        for (int j = 0; j < N; j++, o += a.ld_out)
+            if (FULL || (l.on && j < nj)) *o = y[j];
+    }
+}
+template <int EPI, int N>
+__device__ __forceinline__ void q8_emit(const Q8GemmArgs &a, const Q8Lane &l, const uint32_t (&s)[N], const float *xs, int f, int lane,
+                                        int t0, int nj) {
+    if (nj == N && __all_sync(0xffffffffu, l.on)) q8_emit_some<EPI, N, true>(a, l, s, xs, f, lane, t0, nj);
+    else q8_emit_some<EPI, N, false>(a, l, s, xs, f, lane, t0, nj);
+}
+
+// Results of four consecutive features f .. f + 3 (this lane; 32 lanes, 128 features) of token t from their sums; add: their
+// biases or residuals.
+template <int EPI>
+__device__ __forceinline__ void q8_emit4(const Q8GemmArgs &a, const float (&ws)[4], const float (&add)[4], int4 s, float xs, int f,
+                                         int lane, long long t) {
+    float y[4] = {(float)s.x * ws[0] * xs, (float)s.y * ws[1] * xs, (float)s.z * ws[2] * xs, (float)s.w * ws[3] * xs};
+    if constexpr (EPI == Q8_SWIGLU) {
+        // of 8 lanes the first four hold 16 gates, the others their ups: each computes two of a lane's four products
+        const bool hi = lane & 4;
+        const float p = __shfl_xor_sync(0xffffffffu, hi ? y[0] : y[2], 4), q = __shfl_xor_sync(0xffffffffu, hi ? y[1] : y[3], 4);
+        const float h0 = hi ? silu_times(p, y[2]) : silu_times(y[0], p), h1 = hi ? silu_times(q, y[3]) : silu_times(y[1], q);
+        if (f >= a.M) return;
+        __nv_bfloat16 *o = reinterpret_cast<__nv_bfloat16 *>(a.out) + t * a.ld_out + (f >> 5) * 16 + (lane & 3) * 4 + (hi ? 2 : 0);
+        o[0] = __float2bfloat16_rn(h0);
+        o[1] = __float2bfloat16_rn(h1);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (f + i >= a.M) break;
+            if (EPI == Q8_RESID || a.bias) y[i] = add[i] + y[i];
+            if (EPI == Q8_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[t * a.ld_out + f + i] = __float2bfloat16_rn(y[i]);
+            else reinterpret_cast<float *>(a.out)[t * a.ld_out + f + i] = y[i];
         }
     }
 }
@@ -135,25 +225,33 @@ __device__ __forceinline__ void q8_emit(const Q8GemmArgs &a, const Q8Lane &l, co
 // ---------------------------------------------------------------------------------------------
 // few tokens: a tile's k-blocks cut over the CTAs of a cluster
 // ---------------------------------------------------------------------------------------------
-__host__ __device__ constexpr int split_stage_bytes(int bn) { return (kBM + bn) * kBK; }
-// two CTAs on an SM: one loads while the other starts or ends
-__host__ __device__ constexpr int split_stages(int bn) { return 110 * 1024 / split_stage_bytes(bn); }
-__host__ __device__ constexpr int split_smem(int bn) { return split_stages(bn) * split_stage_bytes(bn) + 1024; }
+// CTAS = 1: a CTA computes 128 features x BN tokens over its range of k-blocks.  CTAS = 2: a pair of CTAs (cta_group::2) does 256
+// features, its even CTA issuing the MMAs; each stages its own 128 rows of W and half of the tokens.  The nsplit ranges of a
+// tile are the CTAs or pairs of a cluster (up to 8 CTAs).  Their sums meet in distributed shared memory: each CTA leaves its
+// own in its ring, which is free by then, and after a cluster barrier adds up its share of the tile's tokens from all of them.
+constexpr int kClusterMax = 8;
+__host__ __device__ constexpr int split_stage_bytes(int ctas, int bn) { return (kBM + bn / ctas) * kBK; }
+// two CTAs on an SM, one of which loads while the other starts or ends; 256 tokens' sums alone take 128 KB
+__host__ __device__ constexpr int split_stages(int ctas, int bn) { return (bn > 128 ? 196 : 110) * 1024 / split_stage_bytes(ctas, bn); }
+__host__ __device__ constexpr int split_smem(int ctas, int bn) { return split_stages(ctas, bn) * split_stage_bytes(ctas, bn) + 1024; }
 
-template <int BN, int EPI>
+template <int CTAS, int BN, int EPI>
 __global__ void __launch_bounds__(kQ8Threads)
     qw_q8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Q8GemmArgs a,
                        int nsplit) {
-    constexpr int S = split_stages(BN), B_BYTES = BN * kBK;
-    constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN, IDESC = q8_idesc(kBM, BN);
+    constexpr int S = split_stages(CTAS, BN), ROWS = BN / CTAS, B_BYTES = ROWS * kBK;
+    constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN, IDESC = q8_idesc(kBM * CTAS, BN);
     static_assert(S * (kABytes + B_BYTES) >= BN * kBM * 4, "the sums of a tile lie in the ring's memory");
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], tfull_bar;
+    __shared__ __align__(16) float s_xs[BN];
     __shared__ uint32_t tmem_base_sh;
     __shared__ int abort_sh;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sA = smem, *sB = smem + S * kABytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int size = nsplit * CTAS, rank = (int)blockIdx.x % size, range = rank / CTAS, side = rank % CTAS;
+    const bool leader = side == 0;
     volatile int *abort_flag = &abort_sh;
 
     if (threadIdx.x == 0) {
@@ -167,51 +265,48 @@ __global__ void __launch_bounds__(kQ8Threads)
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmW) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmX) : "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_sh)),
-                     "r"(TMEM_COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<CTAS>(&tmem_base_sh, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
+    if (CTAS == 2) cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA arrival
     tc_fence_after();
     const uint32_t tmem = tmem_base_sh;
+
+    const int nt = (a.T + BN - 1) / BN, nkb = (a.K + kBK - 1) / kBK;
+    const int tile = (int)blockIdx.x / size;
+    const int t0 = (tile % nt) * BN, f0 = (tile / nt) * (kBM * CTAS) + side * kBM;
+    const int kb0 = (int)((long long)nkb * range / nsplit), kb1 = (int)((long long)nkb * (range + 1) / nsplit);
     griddep_wait();
     griddep_launch_dependents();
 
-    const int nt = (a.T + BN - 1) / BN, nkb = (a.K + kBK - 1) / kBK;
-    const int tile = (int)blockIdx.x / nsplit, rank = (int)blockIdx.x % nsplit;
-    const int t0 = (tile % nt) * BN, f0 = (tile / nt) * kBM;
-    const int kb0 = (int)((long long)nkb * rank / nsplit), kb1 = (int)((long long)nkb * (rank + 1) / nsplit);
-
     if (warp == 0) {
         if (lane == 0) {
+            const uint32_t full0 = CTAS == 2 ? cluster_map(smem_u32(&full_bar[0]), (uint32_t)(rank - side)) : 0u;
             int s = 0;
             uint32_t ph = 0, issued = 0, last_ph = 0;
             bool ok = true;
             for (int kb = kb0; kb < kb1; kb++) {
                 if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, a.err)) { ok = false; break; }
-                mbar_arrive_expect_tx(&full_bar[s], kABytes + B_BYTES);
-                tma_load_2d(sA + s * kABytes, &tmW, &full_bar[s], kb * kBK, f0);
-                tma_load_2d(sB + s * B_BYTES, &tmX, &full_bar[s], kb * kBK, t0);
+                if (leader) mbar_arrive_expect_tx(&full_bar[s], CTAS * (kABytes + B_BYTES));
+                if (CTAS == 2) {
+                    tma_load_2d_pair(sA + s * kABytes, &tmW, full0 + 8u * s, kb * kBK, f0);
+                    tma_load_2d_pair(sB + s * B_BYTES, &tmX, full0 + 8u * s, kb * kBK, t0 + side * ROWS);
+                } else {
+                    tma_load_2d(sA + s * kABytes, &tmW, &full_bar[s], kb * kBK, f0);
+                    tma_load_2d(sB + s * B_BYTES, &tmX, &full_bar[s], kb * kBK, t0);
+                }
                 issued |= 1u << s;
                 last_ph = (last_ph & ~(1u << s)) | (ph << s);
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
-            if (!ok) {
-                // let every issued copy land before the CTA's shared memory goes away
+            if (!ok && leader) {
+                // let every issued copy land before the shared memory goes away
                 for (int i = 0; i < S; i++)
-                    if (issued >> i & 1u) {
-                        const uint32_t addr = smem_u32(&full_bar[i]);
-                        const uint64_t c0 = gtime_ns();
-                        while (!mbar_try(addr, (last_ph >> i) & 1u) && gtime_ns() - c0 < kTcuWaitCycles) {
-                        }
-                    }
+                    if (issued >> i & 1u) mbar_settle(&full_bar[i], (last_ph >> i) & 1u);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && leader) {
             int s = 0;
             uint32_t ph = 0;
             for (int kb = kb0; kb < kb1; kb++) {
@@ -220,41 +315,49 @@ __global__ void __launch_bounds__(kQ8Threads)
                 const uint64_t ad = sw128_desc(smem_u32(sA + s * kABytes)), bd = sw128_desc(smem_u32(sB + s * B_BYTES));
 #pragma unroll
                 for (int k = 0; k < kBK / 32; k++)
-                    q8_mma<1>(tmem, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
-                tc_commit(&empty_bar[s]);
+                    q8_mma<CTAS>(tmem, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+                q8_commit<CTAS>(&empty_bar[s], rank);
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
-            tc_commit(&tfull_bar);
-            // all MMAs of this CTA complete before the TMEM is freed
-            const uint32_t addr = smem_u32(&tfull_bar);
-            const uint64_t c0 = gtime_ns();
-            while (!mbar_try(addr, 0) && gtime_ns() - c0 < kTcuWaitCycles) {
+            q8_commit<CTAS>(&tfull_bar, rank);
+        }
+        // all MMAs that use this CTA's memory complete before it is given up
+        if (lane == 0) mbar_settle(&tfull_bar, 0);
+    }
+    const bool epilogue = warp >= 2;
+    const int ncols = min(BN, a.T - t0), c0 = ncols * range / nsplit + warp - 2, c1 = ncols * (range + 1) / nsplit;
+    const int f4 = f0 + lane * 4;  // where sums are joined: a warp takes a token, a lane four features
+    float ws4[4], add4[4];
+    if (epilogue) {
+        // two warps per 32 tensor-memory lanes (= features), one for each half of the tokens
+        constexpr int HALF = BN / 2, P = HALF < 32 ? HALF : 32;
+        const int q = warp & 3, half = (warp - 2) >> 2, f = f0 + q * 32 + lane;
+        for (int j = threadIdx.x - 64; j < BN; j += kQ8Threads - 64) s_xs[j] = j < ncols ? a.x_scale[t0 + j] : 0.f;
+        Q8Lane l{};
+        if (nsplit == 1) {
+            l = q8_lane<EPI>(a, f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool on = f4 + i < a.M;
+                ws4[i] = on ? a.w_scale[f4 + i] : 0.f;
+                add4[i] = EPI <= Q8_BF16 && a.bias && on ? a.bias[f4 + i] : 0.f;
+                if (EPI == Q8_RESID && on && c0 < c1) add4[i] = a.resid[(long long)(t0 + c0) * a.ld_resid + f4 + i];
             }
         }
-    }
-    const int q = warp & 3, f = f0 + q * 32 + lane;
-    const bool epilogue = warp >= 2;
-    Q8Lane l{};
-    if (epilogue) {
-        l = q8_lane<EPI>(a, f);
+        asm volatile("bar.sync 1, %0;" ::"n"(kQ8Threads - 64) : "memory");
         mbar_wait(&tfull_bar, 0, abort_flag, a.err);
         tc_fence_after();
-        constexpr int P = BN < 32 ? 16 : 32;
-        const int ncols = min(BN, a.T - t0);
-        for (int c = 0; c < ncols; c += P) {
+        int *part = reinterpret_cast<int *>(smem) + q * 32 + lane;
+        for (int c = half * HALF; c < min(ncols, (half + 1) * HALF); c += P) {
             uint32_t r[P];
-            if constexpr (P == 16) tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
-            else tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
+            tmem_get<P>(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
             if (nsplit == 1) {
-                int v[P];
-#pragma unroll
-                for (int j = 0; j < P; j++) v[j] = (int)r[j];
-                q8_emit<EPI, P>(a, l, v, f, lane, t0 + c, min(P, ncols - c));
+                q8_emit<EPI, P>(a, l, r, s_xs + c, f, lane, t0 + c, min(P, ncols - c));
             } else {
-                // the ring is free: every MMA that read it has completed
-                int *part = reinterpret_cast<int *>(smem) + q * 32 + lane;
 #pragma unroll
-                for (int j = 0; j < P; j++) part[(c + j) * kBM] = (int)r[j];
+                for (int j = 0; j < P; j++)
+                    if (c + j < ncols) part[(c + j) * kBM] = (int)r[j];
             }
         }
     }
@@ -262,29 +365,28 @@ __global__ void __launch_bounds__(kQ8Threads)
         __syncwarp();
         cluster_sync_all();  // every CTA's sums are in its shared memory
         if (epilogue) {
-            // this CTA's share of the tile's tokens, two at a time
-            const int ncols = min(BN, a.T - t0);
-            const int c0 = ncols * rank / nsplit, c1 = ncols * (rank + 1) / nsplit;
-            const uint32_t mine = smem_u32(smem) + (uint32_t)(q * 32 + lane) * 4u;
-            for (int c = c0; c < c1; c += 2) {
-                int v[2] = {0, 0};
-                for (int p = 0; p < nsplit; p++) {
-                    const uint32_t at = cluster_map(mine, (uint32_t)p) + (uint32_t)c * (kBM * 4u);
-                    v[0] += ld_cluster(at);
-                    if (c + 1 < c1) v[1] += ld_cluster(at + kBM * 4u);
+            const uint32_t mine = smem_u32(smem) + (uint32_t)lane * 16u;
+            for (int c = c0; c < c1; c += kQ8Threads / 32 - 2) {
+                int4 v[kClusterMax / CTAS];
+#pragma unroll
+                for (int p = 0; p < kClusterMax / CTAS; p++)
+                    if (p < nsplit) v[p] = ld_cluster4(cluster_map(mine, (uint32_t)(p * CTAS + side)) + (uint32_t)c * (kBM * 4u));
+                if (EPI == Q8_RESID && c > c0) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (f4 + i < a.M) add4[i] = a.resid[(long long)(t0 + c) * a.ld_resid + f4 + i];
                 }
-                q8_emit<EPI, 2>(a, l, v, f, lane, t0 + c, min(2, c1 - c));
+#pragma unroll
+                for (int p = 1; p < kClusterMax / CTAS; p++)
+                    if (p < nsplit) { v[0].x += v[p].x; v[0].y += v[p].y; v[0].z += v[p].z; v[0].w += v[p].w; }
+                q8_emit4<EPI>(a, ws4, add4, v[0], s_xs[c], f4, lane, t0 + c);
             }
         }
-        __syncwarp();
-        cluster_sync_all();  // no CTA leaves while another reads its sums
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
-    }
+    if (size > 1) cluster_sync_all();  // no CTA leaves while another reads its sums or signals its barriers
+    if (warp == 1) tmem_free<CTAS>(tmem, TMEM_COLS);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -295,11 +397,11 @@ __global__ void __launch_bounds__(kQ8Threads)
 //   full[s]   in the even CTA: its producer's expect_tx of both CTAs' bytes; both CTAs' loads count on it;
 //   empty[s]  in each CTA, signalled by the MMA commit to both;
 //   tfull[i]  in each CTA, signalled by the commit behind the tile's last k-block;
-//   tempty[i] in the even CTA: 8 arrivals (the epilogue warps of both CTAs).
+//   tempty[i] in the even CTA: 16 arrivals (the epilogue warps of both CTAs).
 constexpr int kPairBM = 256;
 constexpr int kPairGroupT = 8;  // token tiles per group of the tile order: their X tiles stay in L2 while W passes by
 __host__ __device__ constexpr int pair_stage_bytes(int bn) { return kABytes + bn / 2 * kBK; }
-__host__ __device__ constexpr int pair_stages(int bn) { return 224 * 1024 / pair_stage_bytes(bn); }
+__host__ __device__ constexpr int pair_stages(int bn) { return 196 * 1024 / pair_stage_bytes(bn); }
 __host__ __device__ constexpr int pair_smem(int bn) { return pair_stages(bn) * pair_stage_bytes(bn) + 1024; }
 
 struct PairTile {
@@ -320,6 +422,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
     constexpr uint32_t TMEM_COLS = 2 * BN, IDESC = q8_idesc(kPairBM, BN);
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], tfull_bar[2], tempty_bar[2], done_bar;
+    __shared__ __align__(16) float s_xs[8][HALF];
     __shared__ uint32_t tmem_base_sh;
     __shared__ int abort_sh;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -336,7 +439,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&tfull_bar[i], 1);
-            mbar_init(&tempty_bar[i], 8);
+            mbar_init(&tempty_bar[i], 16);
         }
         mbar_init(&done_bar, 1);
         abort_sh = 0;
@@ -344,12 +447,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmW) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmX) : "memory");
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_sh)),
-                     "r"(TMEM_COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<2>(&tmem_base_sh, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA arrival
@@ -383,12 +481,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
             }
             if (!ok && leader) {
                 for (int i = 0; i < S; i++)
-                    if (issued >> i & 1u) {
-                        const uint32_t addr = smem_u32(&full_bar[i]);
-                        const uint64_t c0 = gtime_ns();
-                        while (!mbar_try(addr, (last_ph >> i) & 1u) && gtime_ns() - c0 < kTcuWaitCycles) {
-                        }
-                    }
+                    if (issued >> i & 1u) mbar_settle(&full_bar[i], (last_ph >> i) & 1u);
             }
         }
     } else if (warp == 1) {
@@ -410,32 +503,34 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
 #pragma unroll
                     for (int k = 0; k < kBK / 32; k++)
                         q8_mma<2>(d, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), IDESC, (kb > 0 || k > 0) ? 1u : 0u);
-                    tc_commit_pair(&empty_bar[s]);
+                    q8_commit<2>(&empty_bar[s], 0);
                     if (++s == S) { s = 0; ph ^= 1u; }
                 }
-                if (ok) tc_commit_pair(&tfull_bar[acc]);
+                if (ok) q8_commit<2>(&tfull_bar[acc], 0);
             }
-            tc_commit_pair(&done_bar);
+            q8_commit<2>(&done_bar, 0);
         }
     } else {
-        // ---------------- epilogue (warps 2..5 of both CTAs) ----------------
+        // ---------------- epilogue (warps 2..9 of both CTAs) ----------------
+        // two warps per 32 tensor-memory lanes (= features), one for each half of the tokens
         const uint32_t tempty0 = cluster_map(smem_u32(&tempty_bar[0]), 0);
-        const int q = warp & 3;
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        float *xs = s_xs[warp - 2];
         int it = 0;
         for (int tile = cid; tile < total; tile += ncl, it++) {
             const PairTile c = pair_tile<BN>(tile, nf, nt);
-            const int acc = it & 1, f = c.f0 + (int)rank * kBM + q * 32 + lane;
+            const int acc = it & 1, f = c.f0 + (int)rank * kBM + q * 32 + lane, t0 = c.t0 + half * HALF;
+            const int ncols = min(HALF, a.T - t0);
             const Q8Lane l = q8_lane<EPI>(a, f);
+#pragma unroll
+            for (int j = lane; j < HALF; j += 32) xs[j] = j < ncols ? a.x_scale[t0 + j] : 0.f;
+            __syncwarp();
             if (!mbar_wait(&tfull_bar[acc], (uint32_t)(it >> 1) & 1u, abort_flag, a.err)) break;
             tc_fence_after();
-            const int ncols = min(BN, a.T - c.t0);
             for (int cc = 0; cc < ncols; cc += 32) {
                 uint32_t r[32];
-                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + cc), r);
-                int v[32];
-#pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = (int)r[j];
-                q8_emit<EPI, 32>(a, l, v, f, lane, c.t0 + cc, min(32, ncols - cc));
+                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * HALF + cc), r);
+                q8_emit<EPI, 32>(a, l, r, xs + cc, f, lane, t0 + cc, min(32, ncols - cc));
             }
             tc_fence_before();
             __syncwarp();
@@ -445,19 +540,11 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 1 && lane == 0) {
-        // every MMA of the pair has completed (they read both CTAs' shared memory and write both TMEMs)
-        const uint32_t addr = smem_u32(&done_bar);
-        const uint64_t c0 = gtime_ns();
-        while (!mbar_try(addr, 0) && gtime_ns() - c0 < kTcuWaitCycles) {
-        }
-    }
+    // every MMA of the pair has completed (they read both CTAs' shared memory and write both TMEMs)
+    if (warp == 1 && lane == 0) mbar_settle(&done_bar, 0);
     __syncthreads();
     cluster_sync_all();  // no CTA leaves while its peer may still signal its barriers
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
-    }
+    if (warp == 1) tmem_free<2>(tmem, TMEM_COLS);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -504,87 +591,127 @@ cudaError_t codes_map(CUtensorMap *m, const int8_t *base, long long rows, long l
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// How the work is cut.  ctas: of a tile (1: 128 features, 2: 256); bn: its tokens; nsplit: ranges of its k-blocks; 0: persistent pairs.
+struct Q8Plan {
+    int ctas, bn, nsplit;
+};
 struct Q8Kernel {
     const void *fn;
     int smem;
 };
 template <int EPI>
-Q8Kernel split_kernel(int bn) {
-    switch (bn) {
-        case 16: return {(const void *)qw_q8_split_kernel<16, EPI>, split_smem(16)};
-        case 32: return {(const void *)qw_q8_split_kernel<32, EPI>, split_smem(32)};
-        case 64: return {(const void *)qw_q8_split_kernel<64, EPI>, split_smem(64)};
-        default: return {(const void *)qw_q8_split_kernel<128, EPI>, split_smem(128)};
+Q8Kernel q8_kernel(const Q8Plan &p) {
+    if (p.nsplit == 0) return {(const void *)qw_q8_pair_kernel<256, EPI>, pair_smem(256)};
+    if (p.ctas == 2) {
+        if (p.bn == 128) return {(const void *)qw_q8_split_kernel<2, 128, EPI>, split_smem(2, 128)};
+        return {(const void *)qw_q8_split_kernel<2, 256, EPI>, split_smem(2, 256)};
     }
+    if (p.bn == 16) return {(const void *)qw_q8_split_kernel<1, 16, EPI>, split_smem(1, 16)};
+    if (p.bn == 32) return {(const void *)qw_q8_split_kernel<1, 32, EPI>, split_smem(1, 32)};
+    return {(const void *)qw_q8_split_kernel<1, 64, EPI>, split_smem(1, 64)};
 }
-template <int EPI>
-Q8Kernel pair_kernel(int bn) {
-    return bn == 128 ? Q8Kernel{(const void *)qw_q8_pair_kernel<128, EPI>, pair_smem(128)}
-                     : Q8Kernel{(const void *)qw_q8_pair_kernel<256, EPI>, pair_smem(256)};
-}
-Q8Kernel q8_kernel(int epi, bool pair, int bn) {
+Q8Kernel q8_kernel(int epi, const Q8Plan &p) {
     switch (epi) {
-        case Q8_F32: return pair ? pair_kernel<Q8_F32>(bn) : split_kernel<Q8_F32>(bn);
-        case Q8_BF16: return pair ? pair_kernel<Q8_BF16>(bn) : split_kernel<Q8_BF16>(bn);
-        case Q8_RESID: return pair ? pair_kernel<Q8_RESID>(bn) : split_kernel<Q8_RESID>(bn);
-        default: return pair ? pair_kernel<Q8_SWIGLU>(bn) : split_kernel<Q8_SWIGLU>(bn);
+        case Q8_F32: return q8_kernel<Q8_F32>(p);
+        case Q8_BF16: return q8_kernel<Q8_BF16>(p);
+        case Q8_RESID: return q8_kernel<Q8_RESID>(p);
+        default: return q8_kernel<Q8_SWIGLU>(p);
     }
 }
 
-// Every kernel opted in to its shared memory, once per device.
-cudaError_t q8_prepare(int dev) {
-    static std::mutex mu;
-    static bool prepared[64] = {};
-    std::lock_guard<std::mutex> lk(mu);
-    if (dev < 64 && prepared[dev]) return cudaSuccess;
-    for (int epi = Q8_F32; epi <= Q8_SWIGLU; epi++)
-        for (int bn = 16; bn <= 256; bn *= 2)
-            for (int pair = 0; pair < 2; pair++) {
-                if (pair ? bn < 128 : bn > 128) continue;
-                const Q8Kernel k = q8_kernel(epi, pair, bn);
-                cudaError_t e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
-                if (e != cudaSuccess) return e;
-            }
-    if (dev < 64) prepared[dev] = true;
-    return cudaSuccess;
-}
+// The forms there are: pairs that stay, pairs and single CTAs over ranges of the k-blocks.
+constexpr Q8Plan kForms[] = {{2, 256, 0}, {2, 256, 1}, {2, 128, 1}, {1, 64, 1}, {1, 32, 1}, {1, 16, 1}};
 
-struct Q8Plan {
-    bool pair;
-    int bn, nsplit;
+struct Q8Device {
+    int sms = 0;
+    int clusters[2][kClusterMax + 1] = {};  // resident clusters of a size: [1] two CTAs on an SM, [0] one (256 tokens)
 };
-Q8Plan q8_plan(int M, int T, int K, int sms) {
-    const int nkb = (K + kBK - 1) / kBK;
-    const long long pairs = (long long)((M + kPairBM - 1) / kPairBM);
-    if (T > 128 && pairs * ((T + 127) / 128) >= sms / 4) {
-        if (pairs * ((T + 255) / 256) >= sms / 2) return {true, 256, 1};
-        return {true, 128, 1};
-    }
-    const int bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
-    const long long tiles = (long long)((M + kBM - 1) / kBM) * ((T + bn - 1) / bn);
-    int n = (int)(2 * sms / tiles);
-    n = n < 1 ? 1 : n > 8 ? 8 : n;
-    if (n > (nkb + 1) / 2) n = (nkb + 1) / 2;
-    return {false, bn, n};
+
+// Every kernel opted in to its shared memory, and what the device holds of them; once per device.
+cudaError_t q8_device(int dev, const Q8Device **out) {
+    static std::mutex mu;
+    static Q8Device devices[64];
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    Q8Device &d = devices[dev];
+    *out = &d;
+    if (d.sms) return cudaSuccess;
+    for (int epi = Q8_F32; epi <= Q8_SWIGLU; epi++)
+        for (const Q8Plan &p : kForms) {
+            const Q8Kernel k = q8_kernel(epi, p);
+            cudaError_t e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+            if (e != cudaSuccess) return e;
+        }
+    for (int two = 0; two < 2; two++)
+        for (int size = 1; size <= kClusterMax; size++) {
+            const Q8Kernel k = q8_kernel(Q8_F32, two ? Q8Plan{2, 128, 1} : Q8Plan{2, 256, 1});
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute at = {};
+            cfg.gridDim = dim3(size);
+            cfg.blockDim = dim3(kQ8Threads);
+            cfg.dynamicSmemBytes = k.smem;
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = size;
+            at.val.clusterDim.y = at.val.clusterDim.z = 1;
+            cfg.attrs = &at;
+            cfg.numAttrs = 1;
+            cudaError_t e = cudaOccupancyMaxActiveClusters(&d.clusters[two][size], k.fn, &cfg);
+            if (e != cudaSuccess) return e;
+            if (d.clusters[two][size] < 1) return cudaErrorInvalidConfiguration;
+        }
+    return cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
 }
 
-cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, long long ld_x, const Q8GemmArgs &a, int epi, int sms,
+// Microseconds that a form takes, from what it loads, multiplies and joins.  The constants are fitted to the times of 190 shapes
+// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 2.5 % more
+// than the fastest one on average, 21 % at most (3.9 against 3.3 us, 1152 x 896, one token).
+float q8_cost(const Q8Plan &p, const Q8Device &d, int M, int T, int nkb) {
+    const float tiles = (float)((M + p.ctas * kBM - 1) / (p.ctas * kBM)) * (float)((T + p.bn - 1) / p.bn);
+    if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(d.sms / 2)) * (0.345f * nkb + 1.2f);
+    const float ctas = tiles * p.ctas * p.nsplit, per = ctas > d.sms && p.bn <= 128 ? 2.f : 1.f;  // per SM
+    const float waves = ceilf(tiles / (float)d.clusters[p.bn <= 128][p.ctas * p.nsplit]);
+    const int kbs = (nkb + p.nsplit - 1) / p.nsplit;
+    const float kb = (kBM + p.bn / p.ctas) * (float)kBK * 1e-3f;  // kilobytes of a k-block
+    // a k-block: the ring's bytes in flight over their latency (78 GB/s a CTA), the SM's loads, its MMAs
+    const float step = fmaxf(fmaxf(kb / 78.f, per * kb / 95.f), per * p.bn * (0.236f / 128.f));
+    // and all of them: weights from HBM, operands through L2
+    const float load = fmaxf(fmaxf(waves * (kbs * step + 1.1f), (float)M * nkb * (kBK / 6.5e6f)), ctas * kbs * kb * (1.f / 8150.f));
+    return load + 0.7f / 64.f * p.bn + (p.nsplit > 1 ? 1.0f + 0.153f * p.nsplit + 0.6f / 64.f * p.bn : 0.f);
+}
+Q8Plan q8_plan(int M, int T, int K, const Q8Device &d) {
+    const int nkb = (K + kBK - 1) / kBK;
+    Q8Plan best = kForms[0];
+    float least = q8_cost(best, d, M, T, nkb);
+    for (const Q8Plan &form : kForms) {
+        if (form.nsplit == 0 || (long long)form.bn * 8 < T || (form.bn > 16 && form.bn / 2 >= T)) continue;
+        for (int n : {1, 2, 3, 4, 6, 8}) {
+            if (n > nkb || n * form.ctas > kClusterMax) break;
+            const Q8Plan p{form.ctas, form.bn, n};
+            const float c = q8_cost(p, d, M, T, nkb);
+            if (c < least) { least = c; best = p; }
+        }
+    }
+    return best;
+}
+
+cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, long long ld_x, const Q8GemmArgs &a, int epi, int dev,
                            cudaStream_t st) {
-    const Q8Plan p = q8_plan(a.M, a.T, a.K, sms);
-    const Q8Kernel k = q8_kernel(epi, p.pair, p.bn);
+    const Q8Device *d;
+    cudaError_t e = q8_device(dev, &d);
+    if (e != cudaSuccess) return e;
+    const Q8Plan p = q8_plan(a.M, a.T, a.K, *d);
+    const Q8Kernel k = q8_kernel(epi, p);
     CUtensorMap mw, mx;
-    cudaError_t e = codes_map(&mw, w, a.M, a.K, ld_w, kBM);
-    if (e == cudaSuccess) e = codes_map(&mx, x, a.T, a.K, ld_x, p.pair ? p.bn / 2 : p.bn);
+    e = codes_map(&mw, w, a.M, a.K, ld_w, kBM);
+    if (e == cudaSuccess) e = codes_map(&mx, x, a.T, a.K, ld_x, p.bn / p.ctas);
     if (e != cudaSuccess) return e;
     int nsplit = p.nsplit;
     void *args[] = {(void *)&mw, (void *)&mx, (void *)&a, (void *)&nsplit};
-    const long long tiles = (long long)((a.M + (p.pair ? kPairBM : kBM) - 1) / (p.pair ? kPairBM : kBM)) * ((a.T + p.bn - 1) / p.bn);
-    if (p.pair) {
-        const int ncl = (int)(tiles < sms / 2 ? tiles : sms / 2);
-        return launch_cluster(k.fn, 2 * ncl, 2, k.smem, st, args);
-    }
-    if (tiles * nsplit > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-    return launch_cluster(k.fn, (int)tiles * nsplit, nsplit, k.smem, st, args);
+    const long long tiles = (long long)((a.M + p.ctas * kBM - 1) / (p.ctas * kBM)) * ((a.T + p.bn - 1) / p.bn);
+    if (nsplit == 0) return launch_cluster(k.fn, 2 * (int)(tiles < d->sms / 2 ? tiles : d->sms / 2), 2, k.smem, st, args);
+    const int size = p.ctas * nsplit;
+    if (tiles * size > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+    return launch_cluster(k.fn, (int)tiles * size, size, k.smem, st, args);
 }
 
 }  // namespace
@@ -621,12 +748,9 @@ extern "C" qw_status qw_op_linear_q8(const qw_linear_q8_args *p, void *stream) {
     a.out = p->out; a.err = p->err; a.M = p->n_out; a.K = p->k; a.T = p->t;
     const int epi = p->epi == QW_LINEAR_RESID ? Q8_RESID : p->epi == QW_LINEAR_SWIGLU ? Q8_SWIGLU
                   : p->out_dtype == QW_DTYPE_BF16 ? Q8_BF16 : Q8_F32;
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return op_fail(QW_ERR_CUDA, "no current device");
-    cudaError_t e = q8_prepare(dev);
-    if (e != cudaSuccess) return op_fail(QW_ERR_CUDA, std::string("linear set-up: ") + cudaGetErrorString(e));
-    e = q8_gemm_launch(p->w, ld_w, p->x, ld_x, a, epi, sms, (cudaStream_t)stream);
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return op_fail(QW_ERR_CUDA, "no current device");
+    cudaError_t e = q8_gemm_launch(p->w, ld_w, p->x, ld_x, a, epi, dev, (cudaStream_t)stream);
     if (e != cudaSuccess) return op_fail(QW_ERR_CUDA, std::string("linear launch: ") + cudaGetErrorString(e));
     return QW_OK;
 }
