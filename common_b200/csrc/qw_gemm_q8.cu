@@ -647,7 +647,7 @@ cudaError_t q8_device(int dev, const Q8Device **out) {
             const Q8Kernel k = q8_kernel(Q8_F32, two ? Q8Plan{2, 128, 1} : Q8Plan{2, 256, 1});
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute at = {};
-            cfg.gridDim = dim3(size);
+            cfg.gridDim = dim3(size * 1024);  // more than there is room for
             cfg.blockDim = dim3(kQ8Threads);
             cfg.dynamicSmemBytes = k.smem;
             at.id = cudaLaunchAttributeClusterDimension;
