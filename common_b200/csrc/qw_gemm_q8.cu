@@ -622,54 +622,39 @@ Q8Kernel q8_kernel(int epi, const Q8Plan &p) {
 // The forms there are: pairs that stay, pairs and single CTAs over ranges of the k-blocks.
 constexpr Q8Plan kForms[] = {{2, 256, 0}, {2, 256, 1}, {2, 128, 1}, {1, 64, 1}, {1, 32, 1}, {1, 16, 1}};
 
-struct Q8Device {
-    int sms = 0;
-    int clusters[2][kClusterMax + 1] = {};  // resident clusters of a size: [1] two CTAs on an SM, [0] one (256 tokens)
-};
+// Clusters of 1..8 CTAs that a B200's 148 SMs hold at once, one CTA on an SM (256 tokens) and two (the smaller tiles): what
+// cudaOccupancyMaxActiveClusters says of kernels of the same size that hold no tensor memory.  (With it the call counts one
+// CTA on an SM; two were seen to run together.)
+constexpr int kClusters[2][kClusterMax + 1] = {{0, 148, 74, 45, 33, 26, 22, 15, 15}, {0, 296, 148, 93, 71, 56, 45, 37, 33}};
 
-// Every kernel opted in to its shared memory, and what the device holds of them; once per device.
-cudaError_t q8_device(int dev, const Q8Device **out) {
+// Every kernel opted in to its shared memory, once per device, whose SMs are counted.
+cudaError_t q8_device(int dev, int *sms) {
     static std::mutex mu;
-    static Q8Device devices[64];
+    static int count[64] = {};
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     std::lock_guard<std::mutex> lk(mu);
-    Q8Device &d = devices[dev];
-    *out = &d;
-    if (d.sms) return cudaSuccess;
-    for (int epi = Q8_F32; epi <= Q8_SWIGLU; epi++)
-        for (const Q8Plan &p : kForms) {
-            const Q8Kernel k = q8_kernel(epi, p);
-            cudaError_t e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
-            if (e != cudaSuccess) return e;
-        }
-    for (int two = 0; two < 2; two++)
-        for (int size = 1; size <= kClusterMax; size++) {
-            const Q8Kernel k = q8_kernel(Q8_F32, two ? Q8Plan{2, 128, 1} : Q8Plan{2, 256, 1});
-            cudaLaunchConfig_t cfg = {};
-            cudaLaunchAttribute at = {};
-            cfg.gridDim = dim3(size * 1024);  // more than there is room for
-            cfg.blockDim = dim3(kQ8Threads);
-            cfg.dynamicSmemBytes = k.smem;
-            at.id = cudaLaunchAttributeClusterDimension;
-            at.val.clusterDim.x = size;
-            at.val.clusterDim.y = at.val.clusterDim.z = 1;
-            cfg.attrs = &at;
-            cfg.numAttrs = 1;
-            cudaError_t e = cudaOccupancyMaxActiveClusters(&d.clusters[two][size], k.fn, &cfg);
-            if (e != cudaSuccess) return e;
-            if (d.clusters[two][size] < 1) return cudaErrorInvalidConfiguration;
-        }
-    return cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
+    if (!count[dev]) {
+        for (int epi = Q8_F32; epi <= Q8_SWIGLU; epi++)
+            for (const Q8Plan &p : kForms) {
+                const Q8Kernel k = q8_kernel(epi, p);
+                cudaError_t e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+                if (e != cudaSuccess) return e;
+            }
+        cudaError_t e = cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+    }
+    *sms = count[dev];
+    return cudaSuccess;
 }
 
 // Microseconds that a form takes, from what it loads, multiplies and joins.  The constants are fitted to the times of 190 shapes
 // (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 2.5 % more
 // than the fastest one on average, 21 % at most (3.9 against 3.3 us, 1152 x 896, one token).
-float q8_cost(const Q8Plan &p, const Q8Device &d, int M, int T, int nkb) {
+float q8_cost(const Q8Plan &p, int sms, int M, int T, int nkb) {
     const float tiles = (float)((M + p.ctas * kBM - 1) / (p.ctas * kBM)) * (float)((T + p.bn - 1) / p.bn);
-    if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(d.sms / 2)) * (0.345f * nkb + 1.2f);
-    const float ctas = tiles * p.ctas * p.nsplit, per = ctas > d.sms && p.bn <= 128 ? 2.f : 1.f;  // per SM
-    const float waves = ceilf(tiles / (float)d.clusters[p.bn <= 128][p.ctas * p.nsplit]);
+    if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(sms / 2)) * (0.345f * nkb + 1.2f);
+    const float ctas = tiles * p.ctas * p.nsplit, per = ctas > sms && p.bn <= 128 ? 2.f : 1.f;  // per SM
+    const float waves = ceilf(tiles / (float)kClusters[p.bn <= 128][p.ctas * p.nsplit]);
     const int kbs = (nkb + p.nsplit - 1) / p.nsplit;
     const float kb = (kBM + p.bn / p.ctas) * (float)kBK * 1e-3f;  // kilobytes of a k-block
     // a k-block: the ring's bytes in flight over their latency (78 GB/s a CTA), the SM's loads, its MMAs
@@ -678,16 +663,16 @@ float q8_cost(const Q8Plan &p, const Q8Device &d, int M, int T, int nkb) {
     const float load = fmaxf(fmaxf(waves * (kbs * step + 1.1f), (float)M * nkb * (kBK / 6.5e6f)), ctas * kbs * kb * (1.f / 8150.f));
     return load + 0.7f / 64.f * p.bn + (p.nsplit > 1 ? 1.0f + 0.153f * p.nsplit + 0.6f / 64.f * p.bn : 0.f);
 }
-Q8Plan q8_plan(int M, int T, int K, const Q8Device &d) {
+Q8Plan q8_plan(int M, int T, int K, int sms) {
     const int nkb = (K + kBK - 1) / kBK;
     Q8Plan best = kForms[0];
-    float least = q8_cost(best, d, M, T, nkb);
+    float least = q8_cost(best, sms, M, T, nkb);
     for (const Q8Plan &form : kForms) {
         if (form.nsplit == 0 || (long long)form.bn * 8 < T || (form.bn > 16 && form.bn / 2 >= T)) continue;
         for (int n : {1, 2, 3, 4, 6, 8}) {
             if (n > nkb || n * form.ctas > kClusterMax) break;
             const Q8Plan p{form.ctas, form.bn, n};
-            const float c = q8_cost(p, d, M, T, nkb);
+            const float c = q8_cost(p, sms, M, T, nkb);
             if (c < least) { least = c; best = p; }
         }
     }
@@ -696,10 +681,10 @@ Q8Plan q8_plan(int M, int T, int K, const Q8Device &d) {
 
 cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, long long ld_x, const Q8GemmArgs &a, int epi, int dev,
                            cudaStream_t st) {
-    const Q8Device *d;
-    cudaError_t e = q8_device(dev, &d);
+    int sms;
+    cudaError_t e = q8_device(dev, &sms);
     if (e != cudaSuccess) return e;
-    const Q8Plan p = q8_plan(a.M, a.T, a.K, *d);
+    const Q8Plan p = q8_plan(a.M, a.T, a.K, sms);
     const Q8Kernel k = q8_kernel(epi, p);
     CUtensorMap mw, mx;
     e = codes_map(&mw, w, a.M, a.K, ld_w, kBM);
@@ -708,7 +693,7 @@ cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, lon
     int nsplit = p.nsplit;
     void *args[] = {(void *)&mw, (void *)&mx, (void *)&a, (void *)&nsplit};
     const long long tiles = (long long)((a.M + p.ctas * kBM - 1) / (p.ctas * kBM)) * ((a.T + p.bn - 1) / p.bn);
-    if (nsplit == 0) return launch_cluster(k.fn, 2 * (int)(tiles < d->sms / 2 ? tiles : d->sms / 2), 2, k.smem, st, args);
+    if (nsplit == 0) return launch_cluster(k.fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), 2, k.smem, st, args);
     const int size = p.ctas * nsplit;
     if (tiles * size > 0x7FFFFFFFll) return cudaErrorInvalidValue;
     return launch_cluster(k.fn, (int)tiles * size, size, k.smem, st, args);
