@@ -16,6 +16,9 @@
 namespace qw {
 namespace {
 
+constexpr int kAppendThreads = 128;
+constexpr int kAppendFew = 1024;  // rows up to which a CTA takes one each
+constexpr int kAppendRows = 4;    // rows of a CTA beyond
 constexpr int kAppendMaxItems = 4096;  // pieces of 16 numbers of a row: heads, keys and values
 
 struct AppendArgs {
@@ -26,145 +29,386 @@ struct AppendArgs {
     const int *page_table, *slots, *row_start, *kv_len;
     long long ld_q, ld_k, ld_v, ld_q_out;
     int batch, rows, H, Hkv, d, log2_hc, log2_ps, num_pages, max_pages, mode, rope_len;
-    double eps;
+    float eps, inv_d;
 };
 
-__device__ __forceinline__ void get8(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    v[0] = bf16lo(u.x); v[1] = bf16hi(u.x); v[2] = bf16lo(u.y); v[3] = bf16hi(u.y);
-    v[4] = bf16lo(u.z); v[5] = bf16hi(u.z); v[6] = bf16lo(u.w); v[7] = bf16hi(u.w);
+// 8 numbers as they lie in memory
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ Raw8<T> get8(const T *p) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.v[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
 }
-__device__ __forceinline__ void get8(const float *p, float (&v)[8]) {
-    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// two numbers at a time
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
-__device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
-    return (uint32_t)f2bf_bits(lo) | (uint32_t)f2bf_bits(hi) << 16;
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
 }
-__device__ __forceinline__ void set8(__nv_bfloat16 *p, const float (&v)[8]) {
-    *reinterpret_cast<uint4 *>(p) =
-        make_uint4(pair_bf16(v[0], v[1]), pair_bf16(v[2], v[3]), pair_bf16(v[4], v[5]), pair_bf16(v[6], v[7]));
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
-__device__ __forceinline__ void set8(float *p, const float (&v)[8]) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 8 numbers as four pairs
+__device__ __forceinline__ void pairs(const Raw8<__nv_bfloat16> &r, uint64_t (&v)[4]) {
+    const uint4 u = r.v[0];
+    v[0] = pack2(bf16lo(u.x), bf16hi(u.x)); v[1] = pack2(bf16lo(u.y), bf16hi(u.y));
+    v[2] = pack2(bf16lo(u.z), bf16hi(u.z)); v[3] = pack2(bf16lo(u.w), bf16hi(u.w));
+}
+__device__ __forceinline__ void pairs(const Raw8<float> &r, uint64_t (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        v[2 * i] = pack2(__uint_as_float(r.v[i].x), __uint_as_float(r.v[i].y));
+        v[2 * i + 1] = pack2(__uint_as_float(r.v[i].z), __uint_as_float(r.v[i].w));
+    }
+}
+__device__ __forceinline__ uint32_t pair_bf16(uint64_t v) {
+    const float2 f = unpack2(v);
+    const __nv_bfloat162 w = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t *>(&w);
+}
+__device__ __forceinline__ void set8(__nv_bfloat16 *p, const uint64_t (&v)[4]) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(pair_bf16(v[0]), pair_bf16(v[1]), pair_bf16(v[2]), pair_bf16(v[3]));
+}
+__device__ __forceinline__ void set8(float *p, const uint64_t (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float2 a = unpack2(v[2 * i]), b = unpack2(v[2 * i + 1]);
+        reinterpret_cast<float4 *>(p)[i] = make_float4(a.x, a.y, b.x, b.y);
+    }
 }
 
-// One CTA per row.  A thread takes pieces of 8 numbers of a head's first half with the matching 8 of its second half.
-template <typename IT, typename OT>
-__global__ void __launch_bounds__(256) qw_kv_append_kernel(const AppendArgs a) {
+// the sum of n numbers' squares in consecutive lanes, n a power of two
+__device__ __forceinline__ float lanes_sum(float v, int n) {
+    for (int o = n >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ float squares(const Raw8<T> &lo, const Raw8<T> &hi) {
+    uint64_t x[4], y[4], s = 0, t = 0;
+    pairs(lo, x);
+    pairs(hi, y);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        s = fma2(x[e], x[e], s);
+        t = fma2(y[e], y[e], t);
+    }
+    const float2 a = unpack2(s), b = unpack2(t);
+    return (a.x + a.y) + (b.x + b.y);
+}
+
+// One CTA per row.  A thread takes 8 numbers of a head's first half with the matching 8 of its second (the rotary pairs), and
+// the same 8 of every further head that it serves, so that a row's angles are read once per thread; CH heads are on their way
+// at a time, the first of them while the row's sequence, position and page are looked up.
+template <typename IT, typename OT, int CH>
+__global__ void __launch_bounds__(kAppendThreads) qw_kv_append_row_kernel(const AppendArgs a) {
+    __shared__ float s_red[2][kAppendThreads / 32];
+    __shared__ int s_pos;
+    __shared__ long long s_cell;
+    const int tid = threadIdx.x, hc = 1 << a.log2_hc, d = a.d, half = d >> 1;
+    const int f = (tid & (hc - 1)) * 8, step = kAppendThreads >> a.log2_hc, first = tid >> a.log2_hc;
+    const int heads = a.H + 2 * a.Hkv;  // queries, keys, values
+    const long long r = blockIdx.x;
+    if (tid == 0) s_pos = -2;
     griddep_wait();
     griddep_launch_dependents();
-    __shared__ float s_red[2][8];
-    __shared__ int s_pos, s_slot;
-    const int r = blockIdx.x, tid = threadIdx.x;
-    if (tid == 0) s_pos = -2;
+    Raw8<IT> lo[CH], hi[CH];
+    const auto load = [&](int h0) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int h = h0 + c * step;
+            if (h >= heads) break;
+            const IT *p = h < a.H ? (const IT *)a.q + r * a.ld_q + h * d
+                                  : h < a.H + a.Hkv ? (const IT *)a.k + r * a.ld_k + (h - a.H) * d
+                                                    : (const IT *)a.v + r * a.ld_v + (h - a.H - a.Hkv) * d;
+            lo[c] = get8(p + f);
+            hi[c] = get8(p + f + half);
+        }
+    };
+    load(first);
     __syncthreads();
-    // the sequence that holds the row, its position and page
-    for (int b = tid; b < a.batch; b += 256) {
-        const int lo = min(max(a.row_start[b], 0), a.rows), hi = min(a.row_start[b + 1], a.rows);
-        if (r >= lo && r < hi) {
-            const int kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps);
-            s_pos = max(kv - (hi - r), -1);
-            s_slot = a.slots ? a.slots[b] : b;
+    for (int b = tid; b < a.batch; b += kAppendThreads) {
+        const int begin = min(max(a.row_start[b], 0), a.rows), end = min(a.row_start[b + 1], a.rows);
+        const int kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps), slot = a.slots ? a.slots[b] : b;
+        if (r >= begin && r < end) {
+            const int pos = max(kv - (end - (int)r), -1);
+            long long cell = -1;
+            if (pos >= 0 && !(a.rope && pos >= a.rope_len)) {
+                const int page = a.page_table[(long long)slot * a.max_pages + (pos >> a.log2_ps)];
+                if ((unsigned)page < (unsigned)a.num_pages)
+                    cell = ((((long long)page * a.Hkv) << a.log2_ps) + (pos & ((1 << a.log2_ps) - 1))) * d;
+            }
+            s_pos = pos;
+            s_cell = cell;
         }
     }
-    __syncthreads();
-    const int pos = s_pos;
-    if (pos == -2) return;  // behind the last sequence
-    const bool live = pos >= 0 && !(a.rope && pos >= a.rope_len);
-    const int d = a.d, half = d / 2, hc = 1 << a.log2_hc;
-    long long cell = -1;
-    if (live) {
-        const int page = a.page_table[(long long)s_slot * a.max_pages + (pos >> a.log2_ps)];
-        if ((unsigned)page < (unsigned)a.num_pages)
-            cell = (((long long)page * a.Hkv) << a.log2_ps) * d + (long long)(pos & ((1 << a.log2_ps) - 1)) * d;
-    }
-    const IT *q = (const IT *)a.q + r * a.ld_q, *k = (const IT *)a.k + r * a.ld_k, *v = (const IT *)a.v + r * a.ld_v;
-    const int nq = a.H * hc, nk = a.Hkv * hc, items = nq + 2 * nk;
     float rq = 1.f, rk = 1.f;
     if (a.mode == QW_QKNORM_VECTOR) {
         float sq = 0.f, sk = 0.f;
-        for (int i = tid; i < nq + nk; i += 256) {
-            float x[8], y[8], s = 0.f;
-            const IT *p = i < nq ? q + (i >> a.log2_hc) * d : k + ((i - nq) >> a.log2_hc) * d;
-            get8(p + (i & (hc - 1)) * 8, x);
-            get8(p + (i & (hc - 1)) * 8 + half, y);
+        for (int h0 = first; h0 < a.H + a.Hkv; h0 += CH * step) {
+            if (h0 != first) load(h0);
 #pragma unroll
-            for (int e = 0; e < 8; e++) s += x[e] * x[e] + y[e] * y[e];
-            if (i < nq) sq += s;
-            else sk += s;
+            for (int c = 0; c < CH; c++) {
+                const int h = h0 + c * step;
+                if (h >= a.H + a.Hkv) break;
+                const float s = squares(lo[c], hi[c]);
+                if (h < a.H) sq += s;
+                else sk += s;
+            }
         }
+        if (first + CH * step < a.H + a.Hkv) load(first);
         sq = warp_sum(sq);
         sk = warp_sum(sk);
         if ((tid & 31) == 0) { s_red[0][tid >> 5] = sq; s_red[1][tid >> 5] = sk; }
         __syncthreads();
         sq = sk = 0.f;
-        for (int w = 0; w < 8; w++) { sq += s_red[0][w]; sk += s_red[1][w]; }
-        rq = 1.0f / sqrtf(sq / (float)(a.H * d) + (float)a.eps);
-        rk = 1.0f / sqrtf(sk / (float)(a.Hkv * d) + (float)a.eps);
+#pragma unroll
+        for (int w = 0; w < kAppendThreads / 32; w++) { sq += s_red[0][w]; sk += s_red[1][w]; }
+        rq = rsqrtf(sq / (float)(a.H * d) + a.eps);
+        rk = rsqrtf(sk / (float)(a.Hkv * d) + a.eps);
+    } else {
+        __syncthreads();
     }
-    OT *q_out = a.q_out ? (OT *)a.q_out + r * a.ld_q_out : nullptr;
-    for (int base = 0; base < items; base += 256) {
-        const int i = base + tid;
-        const bool on = i < items, isq = i < nq, isk = !isq && i < nq + nk;
-        const int j = isq ? i : (isk ? i - nq : i - nq - nk);
-        const int h = j >> a.log2_hc, f = (j & (hc - 1)) * 8;
-        float x[8] = {}, y[8] = {};
-        if (on) {
-            const IT *p = (isq ? q : isk ? k : v) + (long long)h * d + f;
-            get8(p, x);
-            get8(p + half, y);
-        }
-        float n = isq ? rq : rk;
-        if (a.mode == QW_QKNORM_HEAD) {
-            float s = 0.f;
+    const int pos = s_pos;
+    if (pos == -2) return;  // behind the last sequence
+    const bool live = pos >= 0 && !(a.rope && pos >= a.rope_len);
+    const long long cell = live ? s_cell : -1;
+    uint64_t cs[4], sn[4];  // cosines and sines, two at a time
+    if (a.rope && live) {
+        const float4 *p = reinterpret_cast<const float4 *>(a.rope + (long long)pos * half + f);
 #pragma unroll
-            for (int e = 0; e < 8; e++) s += x[e] * x[e] + y[e] * y[e];
-            for (int o = hc >> 1; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            n = 1.0f / sqrtf(s / (float)d + (float)a.eps);
+        for (int e = 0; e < 4; e++) {
+            const float4 u = p[e];
+            cs[e] = pack2(u.x, u.z);
+            sn[e] = pack2(u.y, u.w);
         }
-        if (!on) continue;
-        if (isq || isk) {
-            if (a.mode != QW_QKNORM_NONE) {
-                const float *w = (isq ? a.qn : a.kn) + (a.mode == QW_QKNORM_VECTOR ? h * d : 0) + f;
+    } else {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    x[e] = w[e] * (x[e] * n);
-                    y[e] = w[e + half] * (y[e] * n);
+        for (int e = 0; e < 4; e++) { cs[e] = pack2(1.f, 1.f); sn[e] = 0; }
+    }
+    for (int h0 = first; h0 < first + (heads + step - 1) / step * step; h0 += CH * step) {  // the same rounds on every lane
+        if (h0 != first) load(h0);
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int h = h0 + c * step;
+            if (h - first >= heads) break;
+            const bool isq = h < a.H, isv = h >= a.H + a.Hkv;
+            float n = isq ? rq : rk;
+            if (a.mode == QW_QKNORM_HEAD)
+                n = rsqrtf(lanes_sum(h < heads ? squares(lo[c], hi[c]) : 0.f, hc) * a.inv_d + a.eps);
+            if (h >= heads) continue;
+            uint64_t x[4], y[4];
+            pairs(lo[c], x);
+            pairs(hi[c], y);
+            if (!isv) {
+                if (a.mode != QW_QKNORM_NONE) {
+                    const float *w = (isq ? a.qn : a.kn) + f;
+                    if (a.mode == QW_QKNORM_VECTOR) w += (isq ? h : h - a.H) * d;
+                    const uint64_t nn = pack2(n, n);
+                    uint64_t wx[4], wy[4];
+                    pairs(get8(w), wx);
+                    pairs(get8(w + half), wy);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[e] = mul2(wx[e], mul2(x[e], nn));
+                        y[e] = mul2(wy[e], mul2(y[e], nn));
+                    }
+                }
+                if (a.rope) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float2 u = unpack2(mul2(x[e], cs[e])), v = unpack2(y[e]), s = unpack2(sn[e]);
+                        y[e] = fma2(x[e], sn[e], mul2(y[e], cs[e]));
+                        x[e] = pack2(__fmaf_rn(-v.x, s.x, u.x), __fmaf_rn(-v.y, s.y, u.y));
+                    }
                 }
             }
-            if (a.rope && live) {
-                const float2 *cs = a.rope + (long long)pos * half + f;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float2 c = cs[e];
-                    const float u = x[e] * c.x - y[e] * c.y;
-                    y[e] = y[e] * c.x + x[e] * c.y;
-                    x[e] = u;
-                }
-            }
-        }
-        if (isq) {
-            if (q_out) {
+            if (isq) {
                 if (!live) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = y[e] = 0.f;
+                    for (int e = 0; e < 4; e++) x[e] = y[e] = 0;
                 }
-                set8(q_out + (long long)h * d + f, x);
-                set8(q_out + (long long)h * d + f + half, y);
+                if (a.q_out) {
+                    OT *to = (OT *)a.q_out + r * a.ld_q_out + h * d + f;
+                    set8(to, x);
+                    set8(to + half, y);
+                }
+            } else if (cell >= 0) {
+                const int kh = isv ? h - a.H - a.Hkv : h - a.H;
+                OT *to = (OT *)(isv ? a.v_cache : a.k_cache) + cell + ((long long)kh << a.log2_ps) * d + f;
+                set8(to, x);
+                set8(to + half, y);
             }
-        } else if (cell >= 0) {
-            OT *to = (OT *)(isk ? a.k_cache : a.v_cache) + cell + ((long long)h << a.log2_ps) * d + f;
-            set8(to, x);
-            set8(to + half, y);
         }
+    }
+}
+
+// where a row goes
+struct AppendRow {
+    long long cell;  // of its keys and values in head 0, in elements; -1: nowhere
+    int state;       // kNoRow: behind the last sequence; kNowhere: a row before position 0 or behind the angles
+};
+constexpr int kLive = 1, kNowhere = 0, kNoRow = -1;
+
+// One CTA per R rows.  A thread takes 8 numbers of a head's first half with the matching 8 of its second (the rotary pairs) of
+// every row, then the same of the next head that it serves: heads outside, rows inside, so that addresses, norm weights and the
+// choice between queries, keys and values are made once for R rows; two rows are on their way while two are turned.  The
+// rows' sequences, positions, pages and angles are looked up at once, behind the first loads.
+template <typename IT, typename OT, int R>
+__global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv_append_rows_kernel(const AppendArgs a) {
+    constexpr int STEP = 2;  // rows on their way at a time
+    extern __shared__ __align__(16) float s_angles[];  // [R][cos, sin][d / 2]
+    __shared__ AppendRow s_row[R];
+    __shared__ int s_pos[R];
+    const int tid = threadIdx.x, hc = 1 << a.log2_hc, d = a.d, half = d >> 1;
+    const int f = (tid & (hc - 1)) * 8, apart = kAppendThreads >> a.log2_hc, first = tid >> a.log2_hc;
+    const int heads = a.H + 2 * a.Hkv;  // queries, keys, values
+    const int r0 = blockIdx.x * R, nr = min(R, a.rows - r0);
+    if (tid < R) { s_row[tid].state = kNoRow; s_pos[tid] = -1; }
+    griddep_wait();
+    griddep_launch_dependents();
+
+    // head h of rows r0 + i: where it lies and how far its rows are apart
+    struct From { const IT *p; long long ld; };
+    const auto from = [&](int h) {
+        From s{(const IT *)a.q, a.ld_q};
+        if (h >= a.H) {
+            h -= a.H;
+            s = {(const IT *)a.k, a.ld_k};
+            if (h >= a.Hkv) {
+                h -= a.Hkv;
+                s = {(const IT *)a.v, a.ld_v};
+            }
+        }
+        s.p += (long long)r0 * s.ld + h * d + f;
+        return s;
+    };
+    Raw8<IT> lo[STEP], hi[STEP];
+    const auto load = [&](const From &s, int i0) {
+#pragma unroll
+        for (int i = 0; i < STEP; i++) {
+            if (i0 + i >= nr) break;
+            const IT *p = s.p + (i0 + i) * s.ld;
+            lo[i] = get8(p);
+            hi[i] = get8(p + half);
+        }
+    };
+    From src = from(first);
+    if (first < heads) load(src, 0);
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += kAppendThreads) {
+        const int begin = min(max(a.row_start[b], 0), a.rows), end = min(a.row_start[b + 1], a.rows);
+        const int kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps), slot = a.slots ? a.slots[b] : b;
+        for (int i = max(begin - r0, 0); i < min(end - r0, nr); i++) {
+            const int pos = max(kv - (end - r0 - i), -1);
+            AppendRow row{-1, kNowhere};
+            if (pos >= 0 && !(a.rope && pos >= a.rope_len)) {
+                row.state = kLive;
+                const int page = a.page_table[(long long)slot * a.max_pages + (pos >> a.log2_ps)];
+                if ((unsigned)page < (unsigned)a.num_pages)
+                    row.cell = ((((long long)page * a.Hkv) << a.log2_ps) + (pos & ((1 << a.log2_ps) - 1))) * d;
+                s_pos[i] = pos;
+            }
+            s_row[i] = row;
+        }
+    }
+    __syncthreads();
+    if (a.rope)
+        for (int i = tid; i < nr * half; i += kAppendThreads) {
+            const int row = i / half, at = i - row * half, pos = s_pos[row];
+            const float2 c = pos >= 0 ? a.rope[(long long)pos * half + at] : make_float2(0.f, 0.f);
+            s_angles[row * d + at] = c.x;
+            s_angles[row * d + half + at] = c.y;
+        }
+    __syncthreads();
+
+    const int rounds = (heads + apart - 1) / apart;  // the same on every lane
+    for (int n = 0; n < rounds; n++) {
+        const int h = first + n * apart;
+        const bool on = h < heads, isq = h < a.H, isv = h >= a.H + a.Hkv;
+        const From next = from(h + apart);
+        uint64_t wx[4], wy[4];
+        if (a.mode != QW_QKNORM_NONE && on && !isv) {
+            const float *w = (isq ? a.qn : a.kn) + f;
+            pairs(get8(w), wx);
+            pairs(get8(w + half), wy);
+        }
+        OT *to = isq ? (OT *)a.q_out + r0 * a.ld_q_out + h * d + f
+                     : (OT *)(isv ? a.v_cache : a.k_cache) + ((long long)(h - a.H - (isv ? a.Hkv : 0)) << a.log2_ps) * d + f;
+#pragma unroll
+        for (int i0 = 0; i0 < R; i0 += STEP) {
+            uint64_t x[STEP][4], y[STEP][4];
+            float m[STEP];
+#pragma unroll
+            for (int i = 0; i < STEP; i++) {
+                pairs(lo[i], x[i]);
+                pairs(hi[i], y[i]);
+                if (a.mode == QW_QKNORM_HEAD)
+                    m[i] = rsqrtf(lanes_sum(on && i0 + i < nr ? squares(lo[i], hi[i]) : 0.f, hc) * a.inv_d + a.eps);
+            }
+            if (i0 + STEP < R) load(src, i0 + STEP);
+            else if (h + apart < heads) load(next, 0);
+            if (!on) continue;
+#pragma unroll
+            for (int i = 0; i < STEP; i++) {
+                const int row = i0 + i;
+                if (row >= nr) break;
+                const AppendRow where = s_row[row];
+                if (!isv) {
+                    if (a.mode != QW_QKNORM_NONE) {
+                        const uint64_t mm = pack2(m[i], m[i]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            x[i][e] = mul2(wx[e], mul2(x[i][e], mm));
+                            y[i][e] = mul2(wy[e], mul2(y[i][e], mm));
+                        }
+                    }
+                    if (a.rope) {
+                        uint64_t cs[4], sn[4];
+                        pairs(get8(s_angles + row * d + f), cs);
+                        pairs(get8(s_angles + row * d + half + f), sn);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float2 u = unpack2(mul2(x[i][e], cs[e])), v = unpack2(y[i][e]), s = unpack2(sn[e]);
+                            y[i][e] = fma2(x[i][e], sn[e], mul2(y[i][e], cs[e]));
+                            x[i][e] = pack2(__fmaf_rn(-v.x, s.x, u.x), __fmaf_rn(-v.y, s.y, u.y));
+                        }
+                    }
+                }
+                OT *at = isq ? to + row * a.ld_q_out : to + where.cell;
+                if (isq && where.state == kNowhere) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[i][e] = y[i][e] = 0;
+                }
+                if (isq ? a.q_out && where.state != kNoRow : where.cell >= 0 && where.state == kLive) {
+                    set8(at, x[i]);
+                    set8(at + half, y[i]);
+                }
+            }
+        }
+        src = next;
     }
 }
 
 template <typename IT, typename OT>
 cudaError_t append_launch(const AppendArgs &a, cudaStream_t st) {
-    return launch_pdl(qw_kv_append_kernel<IT, OT>, dim3(a.rows), dim3(256), 0, st, a);
+    if (a.rows > kAppendFew && a.mode != QW_QKNORM_VECTOR)
+        return launch_pdl(qw_kv_append_rows_kernel<IT, OT, kAppendRows>, dim3((a.rows + kAppendRows - 1) / kAppendRows), dim3(kAppendThreads),
+                          kAppendRows * a.d * sizeof(float), st, a);
+    return launch_pdl(qw_kv_append_row_kernel<IT, OT, 3>, dim3(a.rows), dim3(kAppendThreads), 0, st, a);
 }
 
 }  // namespace
@@ -210,7 +454,8 @@ extern "C" qw_status qw_op_kv_append(const qw_kv_append_args *p, void *stream) {
     a.q_out = p->q_out; a.k_cache = p->k_cache; a.v_cache = p->v_cache;
     a.page_table = p->page_table; a.slots = p->slots; a.row_start = p->row_start; a.kv_len = p->kv_len;
     a.batch = p->batch; a.rows = p->rows; a.H = p->heads; a.Hkv = p->kv_heads; a.d = p->head_dim;
-    a.num_pages = p->num_pages; a.max_pages = p->max_pages; a.mode = p->qk_norm; a.rope_len = p->rope_len; a.eps = p->eps;
+    a.num_pages = p->num_pages; a.max_pages = p->max_pages; a.mode = p->qk_norm; a.rope_len = p->rope_len; a.eps = (float)p->eps;
+    a.inv_d = 1.0f / (float)a.d;
     while (16 << a.log2_hc < a.d) a.log2_hc++;
     while (1 << a.log2_ps < p->page_size) a.log2_ps++;
     const bool ib = p->in_dtype == QW_DTYPE_BF16, ob = p->dtype == QW_DTYPE_BF16;

@@ -72,24 +72,32 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// the codes of four numbers, one to a byte
+// The codes of four numbers, one to a byte.  COARSE: the numbers of a bf16 row.  With 8 significant bits each, |g| = a 2^p and
+// t = b 2^q, halves are common (0.2 % of a normal row's numbers: 127 g / t is 63.5 wherever g is t / 2), and nothing else comes
+// near one: 254 a 2^(p - q) / b is odd or keeps v / (254 * 255) of v = 127 |g| / t from it, where g m is off by v 2^-24.  So a
+// number that is within v 1e-6 of a half is one, and goes to the even side, without 64 bits.
+template <bool COARSE>
 __device__ __forceinline__ uint32_t q8_codes4(const float *g, float m, float t) {
     const uint64_t mm = pack2(m, m), magic = pack2(kMagic, kMagic), back = pack2(-kMagic, -kMagic), minus = pack2(-m, -m);
     const uint64_t g0 = pack2(g[0], g[1]), g1 = pack2(g[2], g[3]);
     const uint64_t r0 = fma2(g0, mm, magic), r1 = fma2(g1, mm, magic);
-    const float2 d0 = unpack2(fma2(g0, minus, add2(r0, back))), d1 = unpack2(fma2(g1, minus, add2(r1, back)));
+    const float2 d0 = unpack2(fma2(g0, minus, add2(r0, back))), d1 = unpack2(fma2(g1, minus, add2(r1, back)));  // code - value
     const float far = fmaxf(fmaxf(fabsf(d0.x), fabsf(d0.y)), fmaxf(fabsf(d1.x), fabsf(d1.y)));
     const float2 a = unpack2(r0), b = unpack2(r1);
-    uint32_t codes = __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
-                                 __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+    int c[4] = {__float_as_int(a.x), __float_as_int(a.y), __float_as_int(b.x), __float_as_int(b.y)};
     if (far > kNearHalf) {
         const float d[4] = {d0.x, d0.y, d1.x, d1.y};
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (fabsf(d[i]) > kNearHalf)
-                codes = (codes & ~(0xFFu << (8 * i))) | (uint32_t)(q8_code_near(g[i], m, t) & 0xFF) << (8 * i);
+        for (int i = 0; i < 4; i++) {
+            if (COARSE) {
+                const bool half = fabsf(d[i]) > 0.5f - 1e-6f * fabsf(g[i] * m);
+                c[i] += half && (c[i] & 1) ? (d[i] > 0.f ? -1 : 1) : 0;
+            } else if (fabsf(d[i]) > kNearHalf) {
+                c[i] = q8_code_near(g[i], m, t);
+            }
+        }
     }
-    return codes;
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
 // V consecutive numbers as they lie in memory, and as fp32
@@ -257,7 +265,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) qw_q8_rows_kernel(const Q8Rows
         widen(g[j], v);
         uint32_t c[V / 4];
 #pragma unroll
-        for (int e = 0; e < V; e += 4) c[e / 4] = coded ? q8_codes4(v + e, m, t) : 0u;
+        for (int e = 0; e < V; e += 4) c[e / 4] = coded ? q8_codes4<!NORM && sizeof(XT) == 2>(v + e, m, t) : 0u;
         if (n >= V) {
             if constexpr (V == 8) *reinterpret_cast<uint2 *>(q + j * step) = make_uint2(c[0], c[1]);
             else *reinterpret_cast<uint32_t *>(q + j * step) = c[0];
@@ -338,16 +346,21 @@ cudaError_t q8_rows_launch(const Q8RowsArgs &a, cudaStream_t st) {
                      !apart(a.q, a.ld_q, 1) && (uintptr_t)a.w % 16 == 0;
     // the norm holds its weights too: half the numbers fit its registers
     if (!vec || a.dim > (NORM ? 16384 : 32768)) return launch_pdl(qw_q8_rows_any_kernel<XT, DT, NORM>, dim3(a.rows), dim3(256), 0, st, a);
-    // few rows: as many lanes as there are pieces; many: 16 numbers a lane (32 that are coded as they are)
-    const int pieces = (a.dim + V - 1) / V, most = a.rows <= kFewRows ? 1 : (NORM ? 16 : 32) / V;
+    // Few rows: as many lanes as there are pieces (64 x 4096: 3.3 us, 4.2 with 8 pieces a lane).  Many: so many numbers a lane that
+    // the exchange between the warps is rare, and so few that several rows fit an SM: 16 beside delta and weights (8192 x 4096 in
+    // fp32: 64 us, 69 with 8 or 32), 32 alone (24576 x 4096: 73 us, 81 with 16), 64 of bf16 (8192 x 12288: 56 us, 66 with 32).
+    const int pieces = (a.dim + V - 1) / V, most = a.rows <= kFewRows ? 1 : NORM ? 16 / V : 8;
     int wpr = 1;
     while (wpr < kRowWarps && wpr * 32 * most < pieces) wpr *= 2;
     const int nc = (pieces + wpr * 32 - 1) / (wpr * 32);
     if (nc == 1) return q8_rows_regs<XT, DT, NORM, V, 1>(a, wpr, st);
     if (nc == 2) return q8_rows_regs<XT, DT, NORM, V, 2>(a, wpr, st);
-    if (nc <= 4) return q8_rows_regs<XT, DT, NORM, V, 4>(a, wpr, st);
-    if constexpr (!NORM || V == 4)
+    if (nc == 3) return q8_rows_regs<XT, DT, NORM, V, 3>(a, wpr, st);
+    if (nc == 4) return q8_rows_regs<XT, DT, NORM, V, 4>(a, wpr, st);
+    if constexpr (!NORM || V == 4) {
+        if (nc <= 6) return q8_rows_regs<XT, DT, NORM, V, 6>(a, wpr, st);
         if (nc <= 8) return q8_rows_regs<XT, DT, NORM, V, 8>(a, wpr, st);
+    }
     if constexpr (!NORM && V == 4) return q8_rows_regs<XT, DT, NORM, V, 16>(a, wpr, st);
     return cudaErrorInvalidValue;
 }
@@ -379,7 +392,8 @@ extern "C" qw_status qw_op_norm_q8(const qw_norm_q8_args *p, void *stream) {
         return op_fail(QW_ERR_ARG, "pointers must be aligned to their elements");
     a.x = p->x; a.delta = p->delta; a.w = p->norm_w; a.sum = p->sum; a.q = p->q; a.scale = p->scale;
     a.rows = p->rows; a.dim = p->dim; a.eps = p->eps;
-    const bool xb = p->x_dtype == QW_DTYPE_BF16, db = p->delta && p->delta_dtype == QW_DTYPE_BF16;
+    // without a delta its type is the stream's, so that pieces are as wide as they can be
+    const bool xb = p->x_dtype == QW_DTYPE_BF16, db = p->delta ? p->delta_dtype == QW_DTYPE_BF16 : xb;
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e = xb ? (db ? q8_rows_launch<__nv_bfloat16, __nv_bfloat16, true>(a, st)
                              : q8_rows_launch<__nv_bfloat16, float, true>(a, st))
