@@ -231,19 +231,16 @@ __device__ __forceinline__ void q8_emit4(const Q8GemmArgs &a, const float (&ws)[
 // own in its ring, which is free by then, and after a cluster barrier adds up its share of the tile's tokens from all of them.
 constexpr int kClusterMax = 8;
 __host__ __device__ constexpr int split_stage_bytes(int ctas, int bn) { return (kBM + bn / ctas) * kBK; }
-// two CTAs on an SM, one of which loads while the other starts or ends; 256 tokens' sums alone take 128 KB
-__host__ __device__ constexpr int split_stages(int ctas, int bn) { return (bn > 128 ? 196 : 110) * 1024 / split_stage_bytes(ctas, bn); }
-__host__ __device__ constexpr int split_smem(int ctas, int bn) { return split_stages(ctas, bn) * split_stage_bytes(ctas, bn) + 1024; }
+constexpr int kSplitStages = 12;  // at most
 
 template <int CTAS, int BN, int EPI>
 __global__ void __launch_bounds__(kQ8Threads)
     qw_q8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Q8GemmArgs a,
-                       int nsplit) {
-    constexpr int S = split_stages(CTAS, BN), ROWS = BN / CTAS, B_BYTES = ROWS * kBK;
+                       int nsplit, int S) {
+    constexpr int ROWS = BN / CTAS, B_BYTES = ROWS * kBK;
     constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN, IDESC = q8_idesc(kBM * CTAS, BN);
-    static_assert(S * (kABytes + B_BYTES) >= BN * kBM * 4, "the sums of a tile lie in the ring's memory");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], tfull_bar;
+    __shared__ __align__(8) uint64_t full_bar[kSplitStages], empty_bar[kSplitStages], tfull_bar;
     __shared__ __align__(16) float s_xs[BN];
     __shared__ uint32_t tmem_base_sh;
     __shared__ int abort_sh;
@@ -595,22 +592,26 @@ cudaError_t codes_map(CUtensorMap *m, const int8_t *base, long long rows, long l
 struct Q8Plan {
     int ctas, bn, nsplit;
 };
-struct Q8Kernel {
-    const void *fn;
-    int smem;
-};
-template <int EPI>
-Q8Kernel q8_kernel(const Q8Plan &p) {
-    if (p.nsplit == 0) return {(const void *)qw_q8_pair_kernel<256, EPI>, pair_smem(256)};
-    if (p.ctas == 2) {
-        if (p.bn == 128) return {(const void *)qw_q8_split_kernel<2, 128, EPI>, split_smem(2, 128)};
-        return {(const void *)qw_q8_split_kernel<2, 256, EPI>, split_smem(2, 256)};
-    }
-    if (p.bn == 16) return {(const void *)qw_q8_split_kernel<1, 16, EPI>, split_smem(1, 16)};
-    if (p.bn == 32) return {(const void *)qw_q8_split_kernel<1, 32, EPI>, split_smem(1, 32)};
-    return {(const void *)qw_q8_split_kernel<1, 64, EPI>, split_smem(1, 64)};
+// Whether a form's CTAs have an SM each: no more of them than SMs, of 64 tokens or more.  (Of fewer tokens the ring's bytes are
+// mostly weights and half the room keeps HBM busy; the other half lets the next kernel's CTAs start: 1 x 6144 x 4096 7.7 us, 8.0
+// with deep rings; 64 x 4096 x 12288 14.0, 14.9 with shallow ones.)
+bool q8_alone(const Q8Plan &p, long long ctas, int sms) { return p.bn > 128 || (p.bn >= 64 && ctas <= sms); }
+// Stages of a form's ring: as deep as its range and its share of the SM allow; the sums of a tile lie there too.
+int split_stages(const Q8Plan &p, int kbs, bool alone) {
+    const int bytes = split_stage_bytes(p.ctas, p.bn), room = (alone ? 200 : 110) * 1024 / bytes;
+    const int sums = p.nsplit > 1 ? (p.bn * kBM * 4 + bytes - 1) / bytes : 1;
+    int s = kbs < room ? kbs : room;
+    s = s < kSplitStages ? s : kSplitStages;
+    return s > sums ? s : sums;
 }
-Q8Kernel q8_kernel(int epi, const Q8Plan &p) {
+template <int EPI>
+const void *q8_kernel(const Q8Plan &p) {
+    if (p.nsplit == 0) return (const void *)qw_q8_pair_kernel<256, EPI>;
+    if (p.ctas == 2) return p.bn == 128 ? (const void *)qw_q8_split_kernel<2, 128, EPI> : (const void *)qw_q8_split_kernel<2, 256, EPI>;
+    if (p.bn == 16) return (const void *)qw_q8_split_kernel<1, 16, EPI>;
+    return p.bn == 32 ? (const void *)qw_q8_split_kernel<1, 32, EPI> : (const void *)qw_q8_split_kernel<1, 64, EPI>;
+}
+const void *q8_kernel(int epi, const Q8Plan &p) {
     switch (epi) {
         case Q8_F32: return q8_kernel<Q8_F32>(p);
         case Q8_BF16: return q8_kernel<Q8_BF16>(p);
@@ -636,8 +637,8 @@ cudaError_t q8_device(int dev, int *sms) {
     if (!count[dev]) {
         for (int epi = Q8_F32; epi <= Q8_SWIGLU; epi++)
             for (const Q8Plan &p : kForms) {
-                const Q8Kernel k = q8_kernel(epi, p);
-                cudaError_t e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+                const int most = p.nsplit == 0 ? pair_smem(256) : 200 * 1024 + 1024;
+                cudaError_t e = cudaFuncSetAttribute(q8_kernel(epi, p), cudaFuncAttributeMaxDynamicSharedMemorySize, most);
                 if (e != cudaSuccess) return e;
             }
         cudaError_t e = cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
@@ -648,20 +649,21 @@ cudaError_t q8_device(int dev, int *sms) {
 }
 
 // Microseconds that a form takes, from what it loads, multiplies and joins.  The constants are fitted to the times of 190 shapes
-// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 2.5 % more
-// than the fastest one on average, 21 % at most (3.9 against 3.3 us, 1152 x 896, one token).
+// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 2.4 % more
+// than the fastest one on average, 25 % at most (384 tokens, 4096 x 12288: 32.1 against 25.6 us).
 float q8_cost(const Q8Plan &p, int sms, int M, int T, int nkb) {
     const float tiles = (float)((M + p.ctas * kBM - 1) / (p.ctas * kBM)) * (float)((T + p.bn - 1) / p.bn);
-    if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(sms / 2)) * (0.345f * nkb + 1.2f);
+    if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(sms / 2)) * (0.34f * nkb + 1.2f);
     const float ctas = tiles * p.ctas * p.nsplit, per = ctas > sms && p.bn <= 128 ? 2.f : 1.f;  // per SM
     const float waves = ceilf(tiles / (float)kClusters[p.bn <= 128][p.ctas * p.nsplit]);
     const int kbs = (nkb + p.nsplit - 1) / p.nsplit;
     const float kb = (kBM + p.bn / p.ctas) * (float)kBK * 1e-3f;  // kilobytes of a k-block
-    // a k-block: the ring's bytes in flight over their latency (78 GB/s a CTA), the SM's loads, its MMAs
-    const float step = fmaxf(fmaxf(kb / 78.f, per * kb / 95.f), per * p.bn * (0.236f / 128.f));
+    // a k-block: the ring's bytes in flight over their latency (GB/s of a CTA), the SM's loads, its MMAs
+    const float ring = q8_alone(p, (long long)ctas, sms) ? 130.f : 75.5f;
+    const float step = fmaxf(fmaxf(kb / ring, per * kb / 95.f), per * p.bn * (0.243f / 128.f));
     // and all of them: weights from HBM, operands through L2
-    const float load = fmaxf(fmaxf(waves * (kbs * step + 1.1f), (float)M * nkb * (kBK / 6.5e6f)), ctas * kbs * kb * (1.f / 8150.f));
-    return load + 0.7f / 64.f * p.bn + (p.nsplit > 1 ? 1.0f + 0.153f * p.nsplit + 0.6f / 64.f * p.bn : 0.f);
+    const float load = fmaxf(fmaxf(waves * (kbs * step + 0.45f), (float)M * nkb * (kBK / 6.5e6f)), ctas * kbs * kb * (1.f / 7920.f));
+    return load + 0.9f / 64.f * p.bn + (p.nsplit > 1 ? 1.4f + 0.123f * p.nsplit + 0.345f / 64.f * p.bn : 0.f);
 }
 Q8Plan q8_plan(int M, int T, int K, int sms) {
     const int nkb = (K + kBK - 1) / kBK;
@@ -685,18 +687,21 @@ cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, lon
     cudaError_t e = q8_device(dev, &sms);
     if (e != cudaSuccess) return e;
     const Q8Plan p = q8_plan(a.M, a.T, a.K, sms);
-    const Q8Kernel k = q8_kernel(epi, p);
+    const void *fn = q8_kernel(epi, p);
     CUtensorMap mw, mx;
     e = codes_map(&mw, w, a.M, a.K, ld_w, kBM);
     if (e == cudaSuccess) e = codes_map(&mx, x, a.T, a.K, ld_x, p.bn / p.ctas);
     if (e != cudaSuccess) return e;
-    int nsplit = p.nsplit;
-    void *args[] = {(void *)&mw, (void *)&mx, (void *)&a, (void *)&nsplit};
     const long long tiles = (long long)((a.M + p.ctas * kBM - 1) / (p.ctas * kBM)) * ((a.T + p.bn - 1) / p.bn);
-    if (nsplit == 0) return launch_cluster(k.fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), 2, k.smem, st, args);
-    const int size = p.ctas * nsplit;
+    if (p.nsplit == 0) {
+        void *args[] = {(void *)&mw, (void *)&mx, (void *)&a};
+        return launch_cluster(fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), 2, pair_smem(256), st, args);
+    }
+    const int size = p.ctas * p.nsplit, nkb = (a.K + kBK - 1) / kBK;
     if (tiles * size > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-    return launch_cluster(k.fn, (int)tiles * size, size, k.smem, st, args);
+    int nsplit = p.nsplit, stages = split_stages(p, (nkb + nsplit - 1) / nsplit, q8_alone(p, tiles * size, sms));
+    void *args[] = {(void *)&mw, (void *)&mx, (void *)&a, (void *)&nsplit, (void *)&stages};
+    return launch_cluster(fn, (int)tiles * size, size, stages * split_stage_bytes(p.ctas, p.bn) + 1024, st, args);
 }
 
 }  // namespace
