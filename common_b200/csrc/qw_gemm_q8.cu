@@ -122,6 +122,12 @@ __device__ __forceinline__ int4 ld_cluster4(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // up * gate / (1 + e^-gate): the exponential and the division are within (|gate| + 4) 2^-21 of their value, the result is rounded
 // to bf16 behind it.  A gate whose exponential leaves fp32 gives 0.
 __device__ __forceinline__ float silu_times(float g, float u) { return u * __fdividef(g, 1.0f + __expf(-g)); }
@@ -234,7 +240,7 @@ __host__ __device__ constexpr int split_stage_bytes(int ctas, int bn) { return (
 constexpr int kSplitStages = 12;  // at most
 
 template <int CTAS, int BN, int EPI>
-__global__ void __launch_bounds__(kQ8Threads)
+__global__ void __launch_bounds__(kQ8Threads, BN > 128 ? 1 : 2)
     qw_q8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Q8GemmArgs a,
                        int nsplit, int S) {
     constexpr int ROWS = BN / CTAS, B_BYTES = ROWS * kBK;
@@ -324,7 +330,18 @@ __global__ void __launch_bounds__(kQ8Threads)
     const bool epilogue = warp >= 2;
     const int ncols = min(BN, a.T - t0), c0 = ncols * range / nsplit + warp - 2, c1 = ncols * (range + 1) / nsplit;
     const int f4 = f0 + lane * 4;  // where sums are joined: a warp takes a token, a lane four features
-    float ws4[4], add4[4];
+    constexpr int JW = kQ8Threads / 32 - 2, JC = 2;  // warps that join; tokens of a warp at a time
+    float ws4[4], add4[JC][4];
+    const auto addends = [&](int c) {  // biases, or residuals of tokens c, c + JW, ...
+#pragma unroll
+        for (int u = 0; u < JC; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool on = f4 + i < a.M;
+                if (EPI == Q8_RESID) add4[u][i] = on && c + u * JW < c1 ? a.resid[(long long)(t0 + c + u * JW) * a.ld_resid + f4 + i] : 0.f;
+                else add4[u][i] = EPI <= Q8_BF16 && a.bias && on ? a.bias[f4 + i] : 0.f;
+            }
+    };
     if (epilogue) {
         // two warps per 32 tensor-memory lanes (= features), one for each half of the tokens
         constexpr int HALF = BN / 2, P = HALF < 32 ? HALF : 32;
@@ -335,12 +352,8 @@ __global__ void __launch_bounds__(kQ8Threads)
             l = q8_lane<EPI>(a, f);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool on = f4 + i < a.M;
-                ws4[i] = on ? a.w_scale[f4 + i] : 0.f;
-                add4[i] = EPI <= Q8_BF16 && a.bias && on ? a.bias[f4 + i] : 0.f;
-                if (EPI == Q8_RESID && on && c0 < c1) add4[i] = a.resid[(long long)(t0 + c0) * a.ld_resid + f4 + i];
-            }
+            for (int i = 0; i < 4; i++) ws4[i] = f4 + i < a.M ? a.w_scale[f4 + i] : 0.f;
+            addends(c0);
         }
         asm volatile("bar.sync 1, %0;" ::"n"(kQ8Threads - 64) : "memory");
         mbar_wait(&tfull_bar, 0, abort_flag, a.err);
@@ -363,26 +376,42 @@ __global__ void __launch_bounds__(kQ8Threads)
         cluster_sync_all();  // every CTA's sums are in its shared memory
         if (epilogue) {
             const uint32_t mine = smem_u32(smem) + (uint32_t)lane * 16u;
-            for (int c = c0; c < c1; c += kQ8Threads / 32 - 2) {
-                int4 v[kClusterMax / CTAS];
+            for (int c = c0; c < c1; c += JC * JW) {
+                int4 sum[JC] = {};
 #pragma unroll
-                for (int p = 0; p < kClusterMax / CTAS; p++)
-                    if (p < nsplit) v[p] = ld_cluster4(cluster_map(mine, (uint32_t)(p * CTAS + side)) + (uint32_t)c * (kBM * 4u));
-                if (EPI == Q8_RESID && c > c0) {
+                for (int p0 = 0; p0 < kClusterMax / CTAS; p0 += 4) {
+                    int4 v[JC][4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (f4 + i < a.M) add4[i] = a.resid[(long long)(t0 + c) * a.ld_resid + f4 + i];
+                    for (int p = 0; p < 4; p++)
+#pragma unroll
+                        for (int u = 0; u < JC; u++)
+                            v[u][p] = p0 + p < nsplit && c + u * JW < c1
+                                          ? ld_cluster4(cluster_map(mine, (uint32_t)((p0 + p) * CTAS + side)) + (uint32_t)(c + u * JW) * (kBM * 4u))
+                                          : make_int4(0, 0, 0, 0);
+#pragma unroll
+                    for (int p = 0; p < 4; p++)
+#pragma unroll
+                        for (int u = 0; u < JC; u++) {
+                            sum[u].x += v[u][p].x; sum[u].y += v[u][p].y; sum[u].z += v[u][p].z; sum[u].w += v[u][p].w;
+                        }
+                    if (p0 + 4 >= nsplit) break;
                 }
+                if (EPI == Q8_RESID && c > c0) addends(c);
+                if (c + JC * JW >= c1) cluster_arrive();  // the last sums of others are read
 #pragma unroll
-                for (int p = 1; p < kClusterMax / CTAS; p++)
-                    if (p < nsplit) { v[0].x += v[p].x; v[0].y += v[p].y; v[0].z += v[p].z; v[0].w += v[p].w; }
-                q8_emit4<EPI>(a, ws4, add4, v[0], s_xs[c], f4, lane, t0 + c);
+                for (int u = 0; u < JC; u++)
+                    if (c + u * JW < c1) q8_emit4<EPI>(a, ws4, add4[u], sum[u], s_xs[c + u * JW], f4, lane, t0 + c + u * JW);
             }
+            if (c0 >= c1) cluster_arrive();
+        } else {
+            cluster_arrive();
         }
+        __syncwarp();
+        cluster_wait();  // no CTA leaves while another reads its sums
     }
     tc_fence_before();
     __syncthreads();
-    if (size > 1) cluster_sync_all();  // no CTA leaves while another reads its sums or signals its barriers
+    if (CTAS == 2 && nsplit == 1) cluster_sync_all();  // nor while its peer signals its barriers
     if (warp == 1) tmem_free<CTAS>(tmem, TMEM_COLS);
 }
 
@@ -592,10 +621,15 @@ cudaError_t codes_map(CUtensorMap *m, const int8_t *base, long long rows, long l
 struct Q8Plan {
     int ctas, bn, nsplit;
 };
-// Whether a form's CTAs have an SM each: no more of them than SMs, of 64 tokens or more.  (Of fewer tokens the ring's bytes are
+// Clusters of 1..8 CTAs that a B200's 148 SMs hold at once, one CTA on an SM (256 tokens) and two (the smaller tiles): what
+// cudaOccupancyMaxActiveClusters says of kernels of the same size that hold no tensor memory.  (With it the call counts one
+// CTA on an SM; two were seen to run together.)
+constexpr int kClusters[2][kClusterMax + 1] = {{0, 148, 74, 45, 33, 26, 22, 15, 15}, {0, 296, 148, 93, 71, 56, 45, 37, 33}};
+
+// Whether a form's CTAs have an SM each: where there is room for all of them so, and of 64 tokens or more.  (Of fewer tokens the ring's bytes are
 // mostly weights and half the room keeps HBM busy; the other half lets the next kernel's CTAs start: 1 x 6144 x 4096 7.7 us, 8.0
 // with deep rings; 64 x 4096 x 12288 14.0, 14.9 with shallow ones.)
-bool q8_alone(const Q8Plan &p, long long ctas, int sms) { return p.bn > 128 || (p.bn >= 64 && ctas <= sms); }
+bool q8_alone(const Q8Plan &p, long long tiles) { return p.bn > 128 || (p.bn >= 64 && tiles <= kClusters[0][p.ctas * p.nsplit]); }
 // Stages of a form's ring: as deep as its range and its share of the SM allow; the sums of a tile lie there too.
 int split_stages(const Q8Plan &p, int kbs, bool alone) {
     const int bytes = split_stage_bytes(p.ctas, p.bn), room = (alone ? 200 : 110) * 1024 / bytes;
@@ -623,11 +657,6 @@ const void *q8_kernel(int epi, const Q8Plan &p) {
 // The forms there are: pairs that stay, pairs and single CTAs over ranges of the k-blocks.
 constexpr Q8Plan kForms[] = {{2, 256, 0}, {2, 256, 1}, {2, 128, 1}, {1, 64, 1}, {1, 32, 1}, {1, 16, 1}};
 
-// Clusters of 1..8 CTAs that a B200's 148 SMs hold at once, one CTA on an SM (256 tokens) and two (the smaller tiles): what
-// cudaOccupancyMaxActiveClusters says of kernels of the same size that hold no tensor memory.  (With it the call counts one
-// CTA on an SM; two were seen to run together.)
-constexpr int kClusters[2][kClusterMax + 1] = {{0, 148, 74, 45, 33, 26, 22, 15, 15}, {0, 296, 148, 93, 71, 56, 45, 37, 33}};
-
 // Every kernel opted in to its shared memory, once per device, whose SMs are counted.
 cudaError_t q8_device(int dev, int *sms) {
     static std::mutex mu;
@@ -649,8 +678,8 @@ cudaError_t q8_device(int dev, int *sms) {
 }
 
 // Microseconds that a form takes, from what it loads, multiplies and joins.  The constants are fitted to the times of 190 shapes
-// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 2.4 % more
-// than the fastest one on average, 25 % at most (384 tokens, 4096 x 12288: 32.1 against 25.6 us).
+// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 2.3 % more
+// than the fastest one on average, 29 % at most (384 tokens, 4096 x 12288: 32.0 against 24.8 us).
 float q8_cost(const Q8Plan &p, int sms, int M, int T, int nkb) {
     const float tiles = (float)((M + p.ctas * kBM - 1) / (p.ctas * kBM)) * (float)((T + p.bn - 1) / p.bn);
     if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(sms / 2)) * (0.34f * nkb + 1.2f);
@@ -659,11 +688,11 @@ float q8_cost(const Q8Plan &p, int sms, int M, int T, int nkb) {
     const int kbs = (nkb + p.nsplit - 1) / p.nsplit;
     const float kb = (kBM + p.bn / p.ctas) * (float)kBK * 1e-3f;  // kilobytes of a k-block
     // a k-block: the ring's bytes in flight over their latency (GB/s of a CTA), the SM's loads, its MMAs
-    const float ring = q8_alone(p, (long long)ctas, sms) ? 130.f : 75.5f;
-    const float step = fmaxf(fmaxf(kb / ring, per * kb / 95.f), per * p.bn * (0.243f / 128.f));
+    const float ring = q8_alone(p, (long long)tiles) ? 83.5f : 63.f;
+    const float step = fmaxf(fmaxf(kb / ring, per * kb / 91.3f), per * p.bn * (0.243f / 128.f));
     // and all of them: weights from HBM, operands through L2
-    const float load = fmaxf(fmaxf(waves * (kbs * step + 0.45f), (float)M * nkb * (kBK / 6.5e6f)), ctas * kbs * kb * (1.f / 7920.f));
-    return load + 0.9f / 64.f * p.bn + (p.nsplit > 1 ? 1.4f + 0.123f * p.nsplit + 0.345f / 64.f * p.bn : 0.f);
+    const float load = fmaxf(fmaxf(waves * (kbs * step + 0.34f), (float)M * nkb * (kBK / 6.5e6f)), ctas * kbs * kb * (1.f / 7920.f));
+    return load + 0.854f / 64.f * p.bn + (p.nsplit > 1 ? 1.23f + 0.197f * p.nsplit + 0.345f / 64.f * p.bn : 0.f);
 }
 Q8Plan q8_plan(int M, int T, int K, int sms) {
     const int nkb = (K + kBK - 1) / kBK;
@@ -699,7 +728,7 @@ cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, lon
     }
     const int size = p.ctas * p.nsplit, nkb = (a.K + kBK - 1) / kBK;
     if (tiles * size > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-    int nsplit = p.nsplit, stages = split_stages(p, (nkb + nsplit - 1) / nsplit, q8_alone(p, tiles * size, sms));
+    int nsplit = p.nsplit, stages = split_stages(p, (nkb + nsplit - 1) / nsplit, q8_alone(p, tiles));
     void *args[] = {(void *)&mw, (void *)&mx, (void *)&a, (void *)&nsplit, (void *)&stages};
     return launch_cluster(fn, (int)tiles * size, size, stages * split_stage_bytes(p.ctas, p.bn) + 1024, st, args);
 }
