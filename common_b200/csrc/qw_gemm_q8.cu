@@ -7,7 +7,7 @@
 // gives the same bits, however it cuts the work:
 //   qw_q8_split_kernel  few tokens: one tile of 128 features x 16..128 tokens and one range of its k-blocks per CTA; the CTAs
 //                       of a tile form a cluster and add their sums through distributed shared memory;
-//   qw_q8_pair_kernel   many tokens: persistent CTA pairs, tiles of 256 features x 128 or 256 tokens (cta_group::2).
+//   qw_q8_pair_kernel   many tokens: persistent CTA pairs, tiles of 256 features x 256 tokens (cta_group::2).
 //
 // Both are launched with programmatic dependent launch: barriers, tensor memory and descriptors are set up behind the end of
 // the previous kernel; nothing is read or written before it has ended (codes and scales may be its results), and the next
@@ -41,6 +41,7 @@ struct Q8GemmArgs {
     int *err;
     long long ld_resid, ld_out;
     int M, K, T;
+    int group;  // pairs that stay: token tiles per group of their order
 };
 
 // Instruction descriptor of kind::i8: signed 8-bit A and B, both K-major, 32-bit integer D, M x N.
@@ -425,7 +426,13 @@ __global__ void __launch_bounds__(kQ8Threads, BN > 128 ? 1 : 2)
 //   tfull[i]  in each CTA, signalled by the commit behind the tile's last k-block;
 //   tempty[i] in the even CTA: 16 arrivals (the epilogue warps of both CTAs).
 constexpr int kPairBM = 256;
-constexpr int kPairGroupT = 8;  // token tiles per group of the tile order: their X tiles stay in L2 while W passes by
+// Token tiles per group of the tile order: their X tiles, up to 16 MB of them, stay in L2 while W passes by.  8192 x 24576 x 4096
+// takes 648 us in groups of 16, 665 of 8, 690 of 4; 8192 x 4096 x 12288 336 us in groups of 8, 349 of 5.
+int pair_group(int k) {
+    const int g = (16 << 20) / (256 * k);
+    return g < 8 ? 8 : g > 16 ? 16 : g;
+}
+
 __host__ __device__ constexpr int pair_stage_bytes(int bn) { return kABytes + bn / 2 * kBK; }
 __host__ __device__ constexpr int pair_stages(int bn) { return 196 * 1024 / pair_stage_bytes(bn); }
 __host__ __device__ constexpr int pair_smem(int bn) { return pair_stages(bn) * pair_stage_bytes(bn) + 1024; }
@@ -434,11 +441,11 @@ struct PairTile {
     int f0, t0;
 };
 template <int BN>
-__device__ __forceinline__ PairTile pair_tile(int tile, int nf, int nt) {
-    const int per_group = nf * kPairGroupT;
+__device__ __forceinline__ PairTile pair_tile(int tile, int nf, int nt, int group) {
+    const int per_group = nf * group;
     const int g = tile / per_group, r = tile % per_group;
-    const int t_in = min(kPairGroupT, nt - g * kPairGroupT);
-    return {(r / t_in) * kPairBM, (g * kPairGroupT + r % t_in) * BN};
+    const int t_in = min(group, nt - g * group);
+    return {(r / t_in) * kPairBM, (g * group + r % t_in) * BN};
 }
 
 template <int BN, int EPI>
@@ -493,7 +500,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
             uint32_t ph = 0, issued = 0, last_ph = 0;
             bool ok = true;
             for (int tile = cid; tile < total && ok; tile += ncl) {
-                const PairTile c = pair_tile<BN>(tile, nf, nt);
+                const PairTile c = pair_tile<BN>(tile, nf, nt, a.group);
                 const int wrow = c.f0 + (int)rank * kBM, trow = c.t0 + (int)rank * HALF;
                 for (int kb = 0; kb < nkb; kb++) {
                     if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, a.err)) { ok = false; break; }
@@ -544,7 +551,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         float *xs = s_xs[warp - 2];
         int it = 0;
         for (int tile = cid; tile < total; tile += ncl, it++) {
-            const PairTile c = pair_tile<BN>(tile, nf, nt);
+            const PairTile c = pair_tile<BN>(tile, nf, nt, a.group);
             const int acc = it & 1, f = c.f0 + (int)rank * kBM + q * 32 + lane, t0 = c.t0 + half * HALF;
             const int ncols = min(HALF, a.T - t0);
             const Q8Lane l = q8_lane<EPI>(a, f);
@@ -727,7 +734,6 @@ cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, lon
         return launch_cluster(fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), 2, pair_smem(256), st, args);
     }
     const int size = p.ctas * p.nsplit, nkb = (a.K + kBK - 1) / kBK;
-    if (tiles * size > 0x7FFFFFFFll) return cudaErrorInvalidValue;
     int nsplit = p.nsplit, stages = split_stages(p, (nkb + nsplit - 1) / nsplit, q8_alone(p, tiles));
     void *args[] = {(void *)&mw, (void *)&mx, (void *)&a, (void *)&nsplit, (void *)&stages};
     return launch_cluster(fn, (int)tiles * size, size, stages * split_stage_bytes(p.ctas, p.bn) + 1024, st, args);
@@ -747,6 +753,9 @@ extern "C" qw_status qw_op_linear_q8(const qw_linear_q8_args *p, void *stream) {
     if (p->bias && p->epi != QW_LINEAR_STORE) return op_fail(QW_ERR_ARG, "bias is for STORE");
     if (p->n_out < 1 || p->t < 0 || p->k < 1 || p->k > kQ8MaxK)
         return op_fail(QW_ERR_SHAPE, "n_out >= 1, t >= 0 and k in [1, " + std::to_string(kQ8MaxK) + "]");
+    // tiles are numbered in 32 bits, of the smallest form in eight ranges each
+    if (((long long)p->n_out / kBM + 1) * ((long long)p->t / 16 + 1) > 0x7FFFFFFFll / kClusterMax || p->n_out > 1 << 30 || p->t > 1 << 30)
+        return op_fail(QW_ERR_SHAPE, "n_out x t is too large for one call");
     if (p->epi == QW_LINEAR_SWIGLU && p->n_out % 32) return op_fail(QW_ERR_SHAPE, "SWIGLU needs n_out a multiple of 32");
     const int64_t cols = p->epi == QW_LINEAR_SWIGLU ? p->n_out / 2 : p->n_out;
     Q8GemmArgs a{};
@@ -764,7 +773,7 @@ extern "C" qw_status qw_op_linear_q8(const qw_linear_q8_args *p, void *stream) {
         (uintptr_t)p->out % (p->out_dtype == QW_DTYPE_BF16 ? 2 : 4))
         return op_fail(QW_ERR_ARG, "pointers must be aligned to their elements");
     a.w_scale = p->w_scale; a.x_scale = p->x_scale; a.bias = p->bias; a.resid = p->resid;
-    a.out = p->out; a.err = p->err; a.M = p->n_out; a.K = p->k; a.T = p->t;
+    a.out = p->out; a.err = p->err; a.M = p->n_out; a.K = p->k; a.T = p->t; a.group = pair_group(p->k);
     const int epi = p->epi == QW_LINEAR_RESID ? Q8_RESID : p->epi == QW_LINEAR_SWIGLU ? Q8_SWIGLU
                   : p->out_dtype == QW_DTYPE_BF16 ? Q8_BF16 : Q8_F32;
     int dev = 0;

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kAppendThreads) qw_kv_append_row_kernel(const 
     load(first);
     __syncthreads();
     for (int b = tid; b < a.batch; b += kAppendThreads) {
-        const int begin = min(max(a.row_start[b], 0), a.rows), end = min(a.row_start[b + 1], a.rows);
+        const int begin = min(max(a.row_start[b], 0), a.rows), end = min(max(a.row_start[b + 1], 0), a.rows);
         const int kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps), slot = a.slots ? a.slots[b] : b;
         if (r >= begin && r < end) {
             const int pos = max(kv - (end - (int)r), -1);
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv
     if (first < heads) load(src, 0);
     __syncthreads();
     for (int b = tid; b < a.batch; b += kAppendThreads) {
-        const int begin = min(max(a.row_start[b], 0), a.rows), end = min(a.row_start[b + 1], a.rows);
+        const int begin = min(max(a.row_start[b], 0), a.rows), end = min(max(a.row_start[b + 1], 0), a.rows);
         const int kv = min(max(a.kv_len[b], 0), a.max_pages << a.log2_ps), slot = a.slots ? a.slots[b] : b;
         for (int i = max(begin - r0, 0); i < min(end - r0, nr); i++) {
             const int pos = max(kv - (end - r0 - i), -1);

@@ -19,6 +19,7 @@ namespace {
 // the scale nor 127 / t leaves the normal range
 constexpr float kQ8Tiny = 127.0f * 1.17549435e-38f;
 
+constexpr int kQ8MaxDim = 1 << 30;
 constexpr int kFewRows = 296;
 constexpr int kRowWarps = 16;  // of a row at most
 
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) qw_q8_rows_kernel(const Q8Rows
     }
     if (first == 0) {
         const float rms = NORM ? (float)(1.0 / sqrt(ss / a.dim + a.eps)) : 1.f;
-        a.scale[r] = finite ? t * rms / 127.f : __uint_as_float(0x7FC00000u);
+        a.scale[r] = coded ? t * rms / 127.f : finite ? 0.f : __uint_as_float(0x7FC00000u);
     }
 }
 
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(256) qw_q8_rows_any_kernel(const Q8RowsArgs a)
     }
     if (tid == 0) {
         const float rms = NORM ? (float)(1.0 / sqrt(ss / a.dim + a.eps)) : 1.f;
-        a.scale[r] = finite ? t * rms / 127.f : __uint_as_float(0x7FC00000u);
+        a.scale[r] = coded ? t * rms / 127.f : finite ? 0.f : __uint_as_float(0x7FC00000u);
     }
 }
 
@@ -377,7 +378,7 @@ extern "C" qw_status qw_op_norm_q8(const qw_norm_q8_args *p, void *stream) {
     if (!p) return op_fail(QW_ERR_ARG, "null arguments");
     if (!known(p->x_dtype) || (p->delta && !known(p->delta_dtype)))
         return op_fail(QW_ERR_UNSUPPORTED, "x and delta must be fp32 or bf16");
-    if (p->rows < 0 || p->dim < 1) return op_fail(QW_ERR_SHAPE, "rows >= 0 and dim >= 1");
+    if (p->rows < 0 || p->dim < 1 || p->dim > kQ8MaxDim) return op_fail(QW_ERR_SHAPE, "rows >= 0 and dim in [1, 2^30]");
     if (!(p->eps >= 0.0)) return op_fail(QW_ERR_ARG, "eps must not be negative");
     Q8RowsArgs a{};
     a.ld_x = p->ld_x ? p->ld_x : p->dim; a.ld_delta = p->ld_delta ? p->ld_delta : p->dim;
@@ -406,7 +407,7 @@ extern "C" qw_status qw_op_norm_q8(const qw_norm_q8_args *p, void *stream) {
 extern "C" qw_status qw_op_quant_q8(const void *x, int32_t x_dtype, int32_t rows, int32_t dim, int64_t ld_x, int8_t *q,
                                     int64_t ld_q, float *scale, void *stream) {
     if (!known(x_dtype)) return op_fail(QW_ERR_UNSUPPORTED, "x must be fp32 or bf16");
-    if (rows < 0 || dim < 1) return op_fail(QW_ERR_SHAPE, "rows >= 0 and dim >= 1");
+    if (rows < 0 || dim < 1 || dim > kQ8MaxDim) return op_fail(QW_ERR_SHAPE, "rows >= 0 and dim in [1, 2^30]");
     Q8RowsArgs a{};
     a.ld_x = ld_x ? ld_x : dim; a.ld_q = ld_q ? ld_q : dim;
     if (a.ld_x < dim || a.ld_q < dim) return op_fail(QW_ERR_SHAPE, "row strides must cover dim");

@@ -273,7 +273,8 @@ def op_kv_compact(pool: KvPool, src_table: int, dst_table: int, max_pages: int, 
 
 
 class NormQ8:
-    """qw_op_norm_q8 over raw device pointers: the norm's weights and the types once, then one call per block."""
+    """qw_op_norm_q8 over raw device pointers: the norm's weights and the types once, then one call per block.  An instance
+    serves one host thread at a time (as LinearQ8 and KvAppend do): the arguments are filled in place."""
 
     def __init__(self, dim: int, norm_w_ptr: int, eps: float = 1e-6, x_dtype: int = DTYPE_F32,
                  delta_dtype: int = DTYPE_F32):

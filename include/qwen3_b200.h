@@ -413,7 +413,7 @@ qw_status qw_op_kv_compact(const qw_kv_pool *pool, const int32_t *src_table, con
  * Rows of 8-bit codes with a scale each: a row x of fp32 numbers has scale = max|x| / 127 and the codes rint(127 x / max|x|),
  * halves to even, exactly as real arithmetic gives them; code * scale is what it stands for.  A row whose largest magnitude is
  * below 127 * 2^-126 has scale 0 and codes 0; a row that holds a NaN or an infinity has scale NaN and codes 0, so that every
- * product with it is NaN.  The weights of qw_op_linear_q8 are coded by rows the same way (qw_op_quant_q8), once.
+ * product with it is NaN; so has one whose products with norm_w leave fp32.  The weights of qw_op_linear_q8 are coded by rows the same way (qw_op_quant_q8), once.
  * One layer: qw_op_norm_q8 -> qw_op_linear_q8 (q, k, v) -> qw_op_kv_append -> qw_op_chunk_attn -> qw_op_quant_q8 ->
  * qw_op_linear_q8 (o) -> qw_op_norm_q8 -> qw_op_linear_q8 (gate and up, SWIGLU) -> qw_op_quant_q8 -> qw_op_linear_q8 (down).
  * The calls hold no workspace and keep nothing between them; they can be captured, and overlap on any streams.  The
@@ -438,7 +438,7 @@ typedef struct qw_norm_q8_args {
 /* Residual addition, root-mean-square norm and codes in one pass: h = x + delta (fp32), sum = h (rounded once where the
  * stream is bf16; the norm sees h), y = h / sqrt(mean(h^2) + eps) * norm_w, then the codes and the scale of every row of y.
  * The norm cancels in the codes: they are those of the fp32 products h * norm_w, exactly.  The sum of squares is held in
- * 64 bits; scale is within 2^-21 of its value.  Stands in for accum + rmsnorm (SequentialBlock.java:413-429,
+ * 64 bits; scale is within 2^-22 of its value.  Stands in for accum + rmsnorm (SequentialBlock.java:413-429,
  * NormalizationLayerFeatures.java:574-604), which it codes. */
 qw_status qw_op_norm_q8(const qw_norm_q8_args *args, void *stream);
 

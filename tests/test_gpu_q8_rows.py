@@ -180,6 +180,19 @@ def test_norm_of_numbers_whose_squares_leave_fp32():
     check_codes(q, scale, x, 1 / torch.sqrt(x.double().square().mean(1)), 2.0 ** -22)
 
 
+@pytest.mark.parametrize("dim", [64, 4096, 40001])
+def test_norm_of_zeros_without_eps(dim):
+    import torch
+    x = torch.zeros((3, dim), device="cuda")
+    x[1] = 2.0
+    w = torch.ones(dim, device="cuda")
+    q, scale = torch.full((3, dim), 9, dtype=torch.int8, device="cuda"), torch.full((3,), 9.0, device="cuda")
+    native.NormQ8(dim, w.data_ptr(), 0.0)(x.data_ptr(), q.data_ptr(), scale.data_ptr(), 3)
+    torch.cuda.synchronize()
+    assert scale[0].item() == 0 and scale[2].item() == 0 and abs(scale[1].item() * 127 - 1) < 2.0 ** -21
+    assert bool((q[0] == 0).all()) and bool((q[1] == 127).all()) and bool((q[2] == 0).all())
+
+
 @pytest.mark.parametrize("dim", [100, 4096, 40001])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_norm_in_place(dim, kind):

@@ -34,7 +34,7 @@ def norm(**over):
     (ARG, dict(eps=float("nan"))), (ARG, dict(delta=17, delta_dtype=native.DTYPE_BF16)),
     (UNSUPPORTED, dict(x_dtype=native.DTYPE_F64)), (UNSUPPORTED, dict(delta=16, delta_dtype=native.DTYPE_F64)),
     (SHAPE, dict(rows=-1)), (SHAPE, dict(dim=0)), (SHAPE, dict(ld_x=63)), (SHAPE, dict(delta=16, ld_delta=63)),
-    (SHAPE, dict(sum_out=16, ld_sum=63)), (SHAPE, dict(ld_q=63)), (SHAPE, dict(ld_q=-64)),
+    (SHAPE, dict(sum_out=16, ld_sum=63)), (SHAPE, dict(ld_q=63)), (SHAPE, dict(ld_q=-64)), (SHAPE, dict(dim=(1 << 30) + 1)),
 ])
 def test_norm_refuses(status, over):
     refused(status, norm, **over)
@@ -75,7 +75,8 @@ def linear(**over):
     (ARG, dict(epi=native.LINEAR_SWIGLU, out_dtype=native.DTYPE_BF16, bias=16)),
     (UNSUPPORTED, dict(out_dtype=native.DTYPE_F64)), (UNSUPPORTED, dict(epi=native.LINEAR_SWIGLU)),
     (UNSUPPORTED, dict(epi=native.LINEAR_RESID, resid=16, out_dtype=native.DTYPE_BF16)),
-    (SHAPE, dict(n_out=0)), (SHAPE, dict(t=-1)), (SHAPE, dict(k=0)), (SHAPE, dict(k=131072, ld_w=131072, ld_x=131072)),
+    (SHAPE, dict(n_out=0)), (SHAPE, dict(t=-1)), (SHAPE, dict(n_out=(1 << 30) + 1)), (SHAPE, dict(t=(1 << 30) + 1)),
+    (SHAPE, dict(n_out=1 << 28, t=1 << 12)), (SHAPE, dict(k=0)), (SHAPE, dict(k=131072, ld_w=131072, ld_x=131072)),
     (SHAPE, dict(k=60)), (SHAPE, dict(ld_w=48)), (SHAPE, dict(ld_w=72)), (SHAPE, dict(ld_x=72)), (SHAPE, dict(ld_x=1 << 31)),
     (SHAPE, dict(ld_out=63)), (SHAPE, dict(epi=native.LINEAR_RESID, resid=16, ld_resid=63)),
     (SHAPE, dict(epi=native.LINEAR_SWIGLU, out_dtype=native.DTYPE_BF16, n_out=48)),
