@@ -41,6 +41,7 @@ struct Q8GemmArgs {
     int *err;
     long long ld_resid, ld_out;
     int M, K, T;
+    int aligned;  // result rows begin on 16 bytes
     int group;  // pairs that stay: token tiles per group of their order
 };
 
@@ -201,6 +202,79 @@ __device__ __forceinline__ void q8_emit(const Q8GemmArgs &a, const Q8Lane &l, co
                                         int t0, int nj) {
     if (nj == N && __all_sync(0xffffffffu, l.on)) q8_emit_some<EPI, N, true>(a, l, s, xs, f, lane, t0, nj);
     else q8_emit_some<EPI, N, false>(a, l, s, xs, f, lane, t0, nj);
+}
+
+// ---- bf16 results of 32 features x 32 tokens in whole 16-byte pieces ----
+// 16 tensor-memory lanes x 32 columns (tcgen05.ld 16x256b): register 4 i + 2 h + e of lane l is feature l / 4 + 8 h of token
+// 8 i + 2 (l % 4) + e.  So a lane has a gate and its up in the same place of two loads, two neighbouring tokens of a feature
+// make one register of bf16, and stmatrix turns 8 x 8 of them into rows of 8 features of a token.
+__device__ __forceinline__ void tmem_get_16x256(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float2 scaled2(uint32_t s0, uint32_t s1, float ws, float2 xs) {
+    return make_float2((float)(int)s0 * ws * xs.x, (float)(int)s1 * ws * xs.y);
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    const __nv_bfloat162 w = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&w);
+}
+// bytes of a token's results of a warp, and their distance in its part of shared memory: rows of 16 bytes 8 apart meet no bank
+// twice
+__host__ __device__ constexpr int row_bytes(int epi) { return epi == Q8_SWIGLU ? 32 : 64; }
+__host__ __device__ constexpr int row_apart(int epi) { return row_bytes(epi) + 16; }
+__host__ __device__ constexpr int turn_bytes(int epi) { return epi == Q8_SWIGLU || epi == Q8_BF16 ? 32 * row_apart(epi) : 0; }
+
+// 32 features from tensor-memory lane taddr on, all there, times tokens t0 .. t0 + nj - 1 (nj <= 32); ws and bias: those of
+// features lane / 4 + 0, 8, 16, 24 of them; col: the first result's column.  Rows are 16-byte aligned.
+template <int EPI>
+__device__ __forceinline__ void q8_emit_rows(const Q8GemmArgs &a, uint32_t taddr, const float (&ws)[4], const float (&bias)[4],
+                                             const float *xs, uint8_t *turn, int lane, long long t0, int nj, int col) {
+    constexpr int APART = row_apart(EPI), PIECES = row_bytes(EPI) / 16;
+    uint32_t g[16], u[16];
+    tmem_get_16x256(taddr, g);
+    tmem_get_16x256(taddr + (16u << 16), u);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    const uint32_t base = smem_u32(turn) + (uint32_t)(lane & 7) * APART;
+    uint32_t w[4][4];  // of 8 tokens: 8 features each
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 x = *reinterpret_cast<const float2 *>(xs + 8 * i + 2 * (lane & 3));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float2 y = scaled2(g[4 * i + 2 * h], g[4 * i + 2 * h + 1], ws[h], x);
+            const float2 z = scaled2(u[4 * i + 2 * h], u[4 * i + 2 * h + 1], ws[2 + h], x);
+            if (EPI == Q8_SWIGLU) {
+                w[i][h] = bf16x2(silu_times(y.x, z.x), silu_times(y.y, z.y));
+            } else {
+                w[i][h] = a.bias ? bf16x2(y.x + bias[h], y.y + bias[h]) : bf16x2(y.x, y.y);
+                w[i][2 + h] = a.bias ? bf16x2(z.x + bias[2 + h], z.y + bias[2 + h]) : bf16x2(z.x, z.y);
+            }
+        }
+    }
+    __syncwarp();  // the tokens before have left
+    if (EPI == Q8_SWIGLU) {
+        const uint32_t at = base + (uint32_t)((lane >> 3) & 1) * 16u + (uint32_t)(lane >> 4) * 8u * APART;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) stmatrix4_trans(at + (uint32_t)i * 8u * APART, w[i][0], w[i][1], w[i + 1][0], w[i + 1][1]);
+    } else {
+        const uint32_t at = base + (uint32_t)(lane >> 3) * 16u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) stmatrix4_trans(at + (uint32_t)i * 8u * APART, w[i][0], w[i][1], w[i][2], w[i][3]);
+    }
+    __syncwarp();
+    uint16_t *o = reinterpret_cast<uint16_t *>(a.out) + t0 * a.ld_out + col + (lane % PIECES) * 8;
+#pragma unroll
+    for (int k = 0; k < PIECES; k++) {
+        const int t = (lane + 32 * k) / PIECES;
+        if (t < nj) *reinterpret_cast<uint4 *>(o + t * a.ld_out) = *reinterpret_cast<const uint4 *>(turn + t * APART + (lane % PIECES) * 16);
+    }
 }
 
 // Results of four consecutive features f .. f + 3 (this lane; 32 lanes, 128 features) of token t from their sums; add: their
@@ -435,7 +509,7 @@ int pair_group(int k) {
 
 __host__ __device__ constexpr int pair_stage_bytes(int bn) { return kABytes + bn / 2 * kBK; }
 __host__ __device__ constexpr int pair_stages(int bn) { return 196 * 1024 / pair_stage_bytes(bn); }
-__host__ __device__ constexpr int pair_smem(int bn) { return pair_stages(bn) * pair_stage_bytes(bn) + 1024; }
+__host__ __device__ constexpr int pair_smem(int bn, int epi) { return pair_stages(bn) * pair_stage_bytes(bn) + 8 * turn_bytes(epi) + 1024; }
 
 struct PairTile {
     int f0, t0;
@@ -549,21 +623,39 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
         const uint32_t tempty0 = cluster_map(smem_u32(&tempty_bar[0]), 0);
         const int q = warp & 3, half = (warp - 2) >> 2;
         float *xs = s_xs[warp - 2];
+        uint8_t *turn = smem + S * (kABytes + B_BYTES) + (warp - 2) * turn_bytes(EPI);
         int it = 0;
         for (int tile = cid; tile < total; tile += ncl, it++) {
             const PairTile c = pair_tile<BN>(tile, nf, nt, a.group);
             const int acc = it & 1, f = c.f0 + (int)rank * kBM + q * 32 + lane, t0 = c.t0 + half * HALF;
             const int ncols = min(HALF, a.T - t0);
-            const Q8Lane l = q8_lane<EPI>(a, f);
+            const int fw = f - lane;  // the warp's first feature
+            const bool rows = turn_bytes(EPI) && a.aligned && fw + 32 <= a.M;
+            Q8Lane l{};
+            float ws[4] = {}, bias[4] = {};
+            if (rows) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    ws[i] = a.w_scale[fw + (lane >> 2) + 8 * i];
+                    if (EPI == Q8_BF16 && a.bias) bias[i] = a.bias[fw + (lane >> 2) + 8 * i];
+                }
+            } else {
+                l = q8_lane<EPI>(a, f);
+            }
 #pragma unroll
             for (int j = lane; j < HALF; j += 32) xs[j] = j < ncols ? a.x_scale[t0 + j] : 0.f;
             __syncwarp();
             if (!mbar_wait(&tfull_bar[acc], (uint32_t)(it >> 1) & 1u, abort_flag, a.err)) break;
             tc_fence_after();
             for (int cc = 0; cc < ncols; cc += 32) {
-                uint32_t r[32];
-                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * HALF + cc), r);
-                q8_emit<EPI, 32>(a, l, r, xs + cc, f, lane, t0 + cc, min(32, ncols - cc));
+                const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * HALF + cc);
+                if (turn_bytes(EPI) && rows) {
+                    q8_emit_rows<EPI>(a, at, ws, bias, xs + cc, turn, lane, t0 + cc, min(32, ncols - cc), EPI == Q8_SWIGLU ? fw / 2 : fw);
+                } else {
+                    uint32_t r[32];
+                    tmem_ld32(at, r);
+                    q8_emit<EPI, 32>(a, l, r, xs + cc, f, lane, t0 + cc, min(32, ncols - cc));
+                }
             }
             tc_fence_before();
             __syncwarp();
@@ -673,7 +765,7 @@ cudaError_t q8_device(int dev, int *sms) {
     if (!count[dev]) {
         for (int epi = Q8_F32; epi <= Q8_SWIGLU; epi++)
             for (const Q8Plan &p : kForms) {
-                const int most = p.nsplit == 0 ? pair_smem(256) : 200 * 1024 + 1024;
+                const int most = p.nsplit == 0 ? pair_smem(256, epi) : 200 * 1024 + 1024;
                 cudaError_t e = cudaFuncSetAttribute(q8_kernel(epi, p), cudaFuncAttributeMaxDynamicSharedMemorySize, most);
                 if (e != cudaSuccess) return e;
             }
@@ -731,7 +823,7 @@ cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, lon
     const long long tiles = (long long)((a.M + p.ctas * kBM - 1) / (p.ctas * kBM)) * ((a.T + p.bn - 1) / p.bn);
     if (p.nsplit == 0) {
         void *args[] = {(void *)&mw, (void *)&mx, (void *)&a};
-        return launch_cluster(fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), 2, pair_smem(256), st, args);
+        return launch_cluster(fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), 2, pair_smem(256, epi), st, args);
     }
     const int size = p.ctas * p.nsplit, nkb = (a.K + kBK - 1) / kBK;
     int nsplit = p.nsplit, stages = split_stages(p, (nkb + nsplit - 1) / nsplit, q8_alone(p, tiles));
@@ -774,6 +866,7 @@ extern "C" qw_status qw_op_linear_q8(const qw_linear_q8_args *p, void *stream) {
         return op_fail(QW_ERR_ARG, "pointers must be aligned to their elements");
     a.w_scale = p->w_scale; a.x_scale = p->x_scale; a.bias = p->bias; a.resid = p->resid;
     a.out = p->out; a.err = p->err; a.M = p->n_out; a.K = p->k; a.T = p->t; a.group = pair_group(p->k);
+    a.aligned = !((uintptr_t)p->out & 15) && a.ld_out % 8 == 0;
     const int epi = p->epi == QW_LINEAR_RESID ? Q8_RESID : p->epi == QW_LINEAR_SWIGLU ? Q8_SWIGLU
                   : p->out_dtype == QW_DTYPE_BF16 ? Q8_BF16 : Q8_F32;
     int dev = 0;
