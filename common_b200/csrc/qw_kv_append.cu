@@ -41,53 +41,53 @@ __device__ __forceinline__ Raw8<T> get8(const T *p) {
     for (int i = 0; i < (int)sizeof(T) / 2; i++) r.v[i] = reinterpret_cast<const uint4 *>(p)[i];
     return r;
 }
-// two numbers at a time
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-// 8 numbers as four pairs
-__device__ __forceinline__ void pairs(const Raw8<__nv_bfloat16> &r, uint64_t (&v)[4]) {
+__device__ __forceinline__ void widen8(const Raw8<__nv_bfloat16> &r, float (&v)[8]) {
     const uint4 u = r.v[0];
-    v[0] = pack2(bf16lo(u.x), bf16hi(u.x)); v[1] = pack2(bf16lo(u.y), bf16hi(u.y));
-    v[2] = pack2(bf16lo(u.z), bf16hi(u.z)); v[3] = pack2(bf16lo(u.w), bf16hi(u.w));
+    v[0] = bf16lo(u.x); v[1] = bf16hi(u.x); v[2] = bf16lo(u.y); v[3] = bf16hi(u.y);
+    v[4] = bf16lo(u.z); v[5] = bf16hi(u.z); v[6] = bf16lo(u.w); v[7] = bf16hi(u.w);
 }
-__device__ __forceinline__ void pairs(const Raw8<float> &r, uint64_t (&v)[4]) {
+__device__ __forceinline__ void widen8(const Raw8<float> &r, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        v[2 * i] = pack2(__uint_as_float(r.v[i].x), __uint_as_float(r.v[i].y));
-        v[2 * i + 1] = pack2(__uint_as_float(r.v[i].z), __uint_as_float(r.v[i].w));
+        v[4 * i] = __uint_as_float(r.v[i].x); v[4 * i + 1] = __uint_as_float(r.v[i].y);
+        v[4 * i + 2] = __uint_as_float(r.v[i].z); v[4 * i + 3] = __uint_as_float(r.v[i].w);
     }
 }
-__device__ __forceinline__ uint32_t pair_bf16(uint64_t v) {
-    const float2 f = unpack2(v);
-    const __nv_bfloat162 w = __floats2bfloat162_rn(f.x, f.y);
+__device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
+    const __nv_bfloat162 w = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&w);
 }
-__device__ __forceinline__ void set8(__nv_bfloat16 *p, const uint64_t (&v)[4]) {
-    *reinterpret_cast<uint4 *>(p) = make_uint4(pair_bf16(v[0]), pair_bf16(v[1]), pair_bf16(v[2]), pair_bf16(v[3]));
+__device__ __forceinline__ void set8(__nv_bfloat16 *p, const float (&v)[8]) {
+    *reinterpret_cast<uint4 *>(p) =
+        make_uint4(pair_bf16(v[0], v[1]), pair_bf16(v[2], v[3]), pair_bf16(v[4], v[5]), pair_bf16(v[6], v[7]));
 }
-__device__ __forceinline__ void set8(float *p, const uint64_t (&v)[4]) {
+__device__ __forceinline__ void set8(float *p, const float (&v)[8]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ float squares(const float (&x)[8], const float (&y)[8]) {
+    float s = 0.f, t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const float2 a = unpack2(v[2 * i]), b = unpack2(v[2 * i + 1]);
-        reinterpret_cast<float4 *>(p)[i] = make_float4(a.x, a.y, b.x, b.y);
+    for (int e = 0; e < 8; e++) {
+        s += x[e] * x[e];
+        t += y[e] * y[e];
+    }
+    return s + t;
+}
+// x and y times their weights and n; then turned by the angles of cosines c and sines s
+__device__ __forceinline__ void scale8(float (&x)[8], float (&y)[8], const float (&wx)[8], const float (&wy)[8], float n) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        x[e] = wx[e] * (x[e] * n);
+        y[e] = wy[e] * (y[e] * n);
+    }
+}
+__device__ __forceinline__ void turn8(float (&x)[8], float (&y)[8], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float u = x[e] * c[e] - y[e] * s[e];
+        y[e] = y[e] * c[e] + x[e] * s[e];
+        x[e] = u;
     }
 }
 
@@ -96,20 +96,6 @@ __device__ __forceinline__ float lanes_sum(float v, int n) {
     for (int o = n >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-template <typename T>
-__device__ __forceinline__ float squares(const Raw8<T> &lo, const Raw8<T> &hi) {
-    uint64_t x[4], y[4], s = 0, t = 0;
-    pairs(lo, x);
-    pairs(hi, y);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        s = fma2(x[e], x[e], s);
-        t = fma2(y[e], y[e], t);
-    }
-    const float2 a = unpack2(s), b = unpack2(t);
-    return (a.x + a.y) + (b.x + b.y);
-}
-
 // One CTA per row.  A thread takes 8 numbers of a head's first half with the matching 8 of its second (the rotary pairs), and
 // the same 8 of every further head that it serves, so that a row's angles are read once per thread; CH heads are on their way
 // at a time, the first of them while the row's sequence, position and page are looked up.
@@ -164,7 +150,10 @@ __global__ void __launch_bounds__(kAppendThreads) qw_kv_append_row_kernel(const 
             for (int c = 0; c < CH; c++) {
                 const int h = h0 + c * step;
                 if (h >= a.H + a.Hkv) break;
-                const float s = squares(lo[c], hi[c]);
+                float x[8], y[8];
+                widen8(lo[c], x);
+                widen8(hi[c], y);
+                const float s = squares(x, y);
                 if (h < a.H) sq += s;
                 else sk += s;
             }
@@ -186,18 +175,17 @@ __global__ void __launch_bounds__(kAppendThreads) qw_kv_append_row_kernel(const 
     if (pos == -2) return;  // behind the last sequence
     const bool live = pos >= 0 && !(a.rope && pos >= a.rope_len);
     const long long cell = live ? s_cell : -1;
-    uint64_t cs[4], sn[4];  // cosines and sines, two at a time
+    float cs[8], sn[8];
     if (a.rope && live) {
         const float4 *p = reinterpret_cast<const float4 *>(a.rope + (long long)pos * half + f);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float4 u = p[e];
-            cs[e] = pack2(u.x, u.z);
-            sn[e] = pack2(u.y, u.w);
+        for (int e = 0; e < 8; e += 2) {
+            const float4 u = p[e >> 1];
+            cs[e] = u.x; sn[e] = u.y; cs[e + 1] = u.z; sn[e + 1] = u.w;
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) { cs[e] = pack2(1.f, 1.f); sn[e] = 0; }
+        for (int e = 0; e < 8; e++) { cs[e] = 1.f; sn[e] = 0.f; }
     }
     for (int h0 = first; h0 < first + (heads + step - 1) / step * step; h0 += CH * step) {  // the same rounds on every lane
         if (h0 != first) load(h0);
@@ -206,40 +194,26 @@ __global__ void __launch_bounds__(kAppendThreads) qw_kv_append_row_kernel(const 
             const int h = h0 + c * step;
             if (h - first >= heads) break;
             const bool isq = h < a.H, isv = h >= a.H + a.Hkv;
-            float n = isq ? rq : rk;
-            if (a.mode == QW_QKNORM_HEAD)
-                n = rsqrtf(lanes_sum(h < heads ? squares(lo[c], hi[c]) : 0.f, hc) * a.inv_d + a.eps);
+            float x[8], y[8], n = isq ? rq : rk;
+            widen8(lo[c], x);
+            widen8(hi[c], y);
+            if (a.mode == QW_QKNORM_HEAD) n = rsqrtf(lanes_sum(h < heads ? squares(x, y) : 0.f, hc) * a.inv_d + a.eps);
             if (h >= heads) continue;
-            uint64_t x[4], y[4];
-            pairs(lo[c], x);
-            pairs(hi[c], y);
             if (!isv) {
                 if (a.mode != QW_QKNORM_NONE) {
                     const float *w = (isq ? a.qn : a.kn) + f;
                     if (a.mode == QW_QKNORM_VECTOR) w += (isq ? h : h - a.H) * d;
-                    const uint64_t nn = pack2(n, n);
-                    uint64_t wx[4], wy[4];
-                    pairs(get8(w), wx);
-                    pairs(get8(w + half), wy);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[e] = mul2(wx[e], mul2(x[e], nn));
-                        y[e] = mul2(wy[e], mul2(y[e], nn));
-                    }
+                    float wx[8], wy[8];
+                    widen8(get8(w), wx);
+                    widen8(get8(w + half), wy);
+                    scale8(x, y, wx, wy, n);
                 }
-                if (a.rope) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float2 u = unpack2(mul2(x[e], cs[e])), v = unpack2(y[e]), s = unpack2(sn[e]);
-                        y[e] = fma2(x[e], sn[e], mul2(y[e], cs[e]));
-                        x[e] = pack2(__fmaf_rn(-v.x, s.x, u.x), __fmaf_rn(-v.y, s.y, u.y));
-                    }
-                }
+                if (a.rope) turn8(x, y, cs, sn);
             }
             if (isq) {
                 if (!live) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = y[e] = 0;
+                    for (int e = 0; e < 8; e++) x[e] = y[e] = 0.f;
                 }
                 if (a.q_out) {
                     OT *to = (OT *)a.q_out + r * a.ld_q_out + h * d + f;
@@ -340,24 +314,24 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv
         const int h = first + n * apart;
         const bool on = h < heads, isq = h < a.H, isv = h >= a.H + a.Hkv;
         const From next = from(h + apart);
-        uint64_t wx[4], wy[4];
+        float wx[8], wy[8];
         if (a.mode != QW_QKNORM_NONE && on && !isv) {
             const float *w = (isq ? a.qn : a.kn) + f;
-            pairs(get8(w), wx);
-            pairs(get8(w + half), wy);
+            widen8(get8(w), wx);
+            widen8(get8(w + half), wy);
         }
         OT *to = isq ? (OT *)a.q_out + r0 * a.ld_q_out + h * d + f
                      : (OT *)(isv ? a.v_cache : a.k_cache) + ((long long)(h - a.H - (isv ? a.Hkv : 0)) << a.log2_ps) * d + f;
 #pragma unroll
         for (int i0 = 0; i0 < R; i0 += STEP) {
-            uint64_t x[STEP][4], y[STEP][4];
+            float x[STEP][8], y[STEP][8];
             float m[STEP];
 #pragma unroll
             for (int i = 0; i < STEP; i++) {
-                pairs(lo[i], x[i]);
-                pairs(hi[i], y[i]);
+                widen8(lo[i], x[i]);
+                widen8(hi[i], y[i]);
                 if (a.mode == QW_QKNORM_HEAD)
-                    m[i] = rsqrtf(lanes_sum(on && i0 + i < nr ? squares(lo[i], hi[i]) : 0.f, hc) * a.inv_d + a.eps);
+                    m[i] = rsqrtf(lanes_sum(on && i0 + i < nr ? squares(x[i], y[i]) : 0.f, hc) * a.inv_d + a.eps);
             }
             if (i0 + STEP < R) load(src, i0 + STEP);
             else if (h + apart < heads) load(next, 0);
@@ -368,30 +342,18 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv
                 if (row >= nr) break;
                 const AppendRow where = s_row[row];
                 if (!isv) {
-                    if (a.mode != QW_QKNORM_NONE) {
-                        const uint64_t mm = pack2(m[i], m[i]);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            x[i][e] = mul2(wx[e], mul2(x[i][e], mm));
-                            y[i][e] = mul2(wy[e], mul2(y[i][e], mm));
-                        }
-                    }
+                    if (a.mode != QW_QKNORM_NONE) scale8(x[i], y[i], wx, wy, m[i]);
                     if (a.rope) {
-                        uint64_t cs[4], sn[4];
-                        pairs(get8(s_angles + row * d + f), cs);
-                        pairs(get8(s_angles + row * d + half + f), sn);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float2 u = unpack2(mul2(x[i][e], cs[e])), v = unpack2(y[i][e]), s = unpack2(sn[e]);
-                            y[i][e] = fma2(x[i][e], sn[e], mul2(y[i][e], cs[e]));
-                            x[i][e] = pack2(__fmaf_rn(-v.x, s.x, u.x), __fmaf_rn(-v.y, s.y, u.y));
-                        }
+                        float cs[8], sn[8];
+                        widen8(get8(s_angles + row * d + f), cs);
+                        widen8(get8(s_angles + row * d + half + f), sn);
+                        turn8(x[i], y[i], cs, sn);
                     }
                 }
                 OT *at = isq ? to + row * a.ld_q_out : to + where.cell;
                 if (isq && where.state == kNowhere) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[i][e] = y[i][e] = 0;
+                    for (int e = 0; e < 8; e++) x[i][e] = y[i][e] = 0.f;
                 }
                 if (isq ? a.q_out && where.state != kNoRow : where.cell >= 0 && where.state == kLive) {
                     set8(at, x[i]);
