@@ -96,9 +96,12 @@ __device__ __forceinline__ float lanes_sum(float v, int n) {
     for (int o = n >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// One CTA per row.  A thread takes 8 numbers of a head's first half with the matching 8 of its second (the rotary pairs), and
-// the same 8 of every further head that it serves, so that a row's angles are read once per thread; CH heads are on their way
-// at a time, the first of them while the row's sequence, position and page are looked up.
+
+// One CTA per row, for few rows and for norms over whole vectors.  A thread takes 8 numbers of a head's first half with the
+// matching 8 of its second (the rotary pairs), and the same 8 of every further head that it serves, so that a row's angles are
+// read once per thread; CH heads are on their way at a time, the first of them while the row's sequence, position and page are
+// looked up.  64 tokens of 32 / 8 heads take 4.3 us: the launch, and lengths, page and angles one after the other.  13,800 rows with
+// norms over whole vectors take 79 us (bf16, 4.2 TB/s): every row waits for its sums, and five rows fit an SM's registers.
 template <typename IT, typename OT, int CH>
 __global__ void __launch_bounds__(kAppendThreads) qw_kv_append_row_kernel(const AppendArgs a) {
     __shared__ float s_red[2][kAppendThreads / 32];
@@ -237,10 +240,13 @@ struct AppendRow {
 };
 constexpr int kLive = 1, kNowhere = 0, kNoRow = -1;
 
-// One CTA per R rows.  A thread takes 8 numbers of a head's first half with the matching 8 of its second (the rotary pairs) of
+// One CTA per R rows, for many of them.  A thread takes 8 numbers of a head's first half with the matching 8 of its second of
 // every row, then the same of the next head that it serves: heads outside, rows inside, so that addresses, norm weights and the
 // choice between queries, keys and values are made once for R rows; two rows are on their way while two are turned.  The
-// rows' sequences, positions, pages and angles are looked up at once, behind the first loads.
+// rows' sequences, positions, pages and angles are looked up at once, behind the first loads.  13,800 rows of 32 / 8 heads of 128:
+// 64 us from bf16 with norms per head (5.2 TB/s; 80 with a CTA per row), 59 without norms, 85 from fp32 (5.9 TB/s); of 14 / 2 heads of
+// 64 27 us (49 with a CTA per row, whose threads a row of 1152 numbers does not fill).  Bound by HBM and, at 230 instructions per 32
+// pieces, by their issue (half of the slots); 8 rows a CTA take 70 us, 6 CTAs an SM (80 registers) 77.
 template <typename IT, typename OT, int R>
 __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv_append_rows_kernel(const AppendArgs a) {
     constexpr int STEP = 2;  // rows on their way at a time
@@ -367,6 +373,8 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv
 
 template <typename IT, typename OT>
 cudaError_t append_launch(const AppendArgs &a, cudaStream_t st) {
+    // A CTA per row below: 592 rows of 32 / 8 heads 7.0 us (11.5 by fours), 1024 11.6 (12.3), 2048 17.4 (15.7); of 14 / 2 heads of 64
+    // 3.8 (5.4), 6.2 (5.7), 10.7 (6.9).  Norms over whole vectors would read four rows twice: 91 us against 79.
     if (a.rows > kAppendFew && a.mode != QW_QKNORM_VECTOR)
         return launch_pdl(qw_kv_append_rows_kernel<IT, OT, kAppendRows>, dim3((a.rows + kAppendRows - 1) / kAppendRows), dim3(kAppendThreads),
                           kAppendRows * a.d * sizeof(float), st, a);
