@@ -872,6 +872,8 @@ extern "C" qw_status qw_op_linear_q8(const qw_linear_q8_args *p, void *stream) {
     if (p->t == 0) return QW_OK;
     if (!p->w || !p->w_scale || !p->x || !p->x_scale || !p->out) return op_fail(QW_ERR_ARG, "null device pointer");
     if (p->epi == QW_LINEAR_RESID && !p->resid) return op_fail(QW_ERR_ARG, "RESID needs resid");
+    if (p->epi == QW_LINEAR_RESID && p->out == (const void *)p->resid && a.ld_out != a.ld_resid)
+        return op_fail(QW_ERR_ARG, "out may be resid only with the same stride");
     if (((uintptr_t)p->w | (uintptr_t)p->x) & 15) return op_fail(QW_ERR_ARG, "w and x must be 16-byte aligned");
     if ((((uintptr_t)p->w_scale | (uintptr_t)p->x_scale | (uintptr_t)p->bias | (uintptr_t)p->resid | (uintptr_t)p->err) & 3) ||
         (uintptr_t)p->out % (p->out_dtype == QW_DTYPE_BF16 ? 2 : 4))

@@ -395,6 +395,9 @@ extern "C" qw_status qw_op_norm_q8(const qw_norm_q8_args *p, void *stream) {
     if ((uintptr_t)p->x % ex || (uintptr_t)p->sum % ex || (uintptr_t)p->delta % ed ||
         (((uintptr_t)p->norm_w | (uintptr_t)p->scale) & 3))
         return op_fail(QW_ERR_ARG, "pointers must be aligned to their elements");
+    if (p->sum && ((p->sum == p->x && a.ld_sum != a.ld_x) ||
+                   (p->sum == p->delta && (a.ld_sum != a.ld_delta || p->x_dtype != p->delta_dtype))))
+        return op_fail(QW_ERR_ARG, "sum may be x or delta only with the same type and stride");
     a.x = p->x; a.delta = p->delta; a.w = p->norm_w; a.sum = p->sum; a.q = p->q; a.scale = p->scale;
     a.rows = p->rows; a.dim = p->dim; a.eps = p->eps;
     // without a delta its type is the stream's, so that pieces are as wide as they can be

@@ -32,6 +32,8 @@ def norm(**over):
     (ARG, dict(x=0)), (ARG, dict(norm_w=0)), (ARG, dict(q=0)), (ARG, dict(scale=0)), (ARG, dict(x=18)),
     (ARG, dict(sum_out=18)), (ARG, dict(delta=17)), (ARG, dict(norm_w=18)), (ARG, dict(scale=18)), (ARG, dict(eps=-1.0)),
     (ARG, dict(eps=float("nan"))), (ARG, dict(delta=17, delta_dtype=native.DTYPE_BF16)),
+    (ARG, dict(sum_out=16, ld_sum=128)), (ARG, dict(delta=32, sum_out=32, ld_delta=72)),
+    (ARG, dict(delta=32, sum_out=32, delta_dtype=native.DTYPE_BF16)),
     (UNSUPPORTED, dict(x_dtype=native.DTYPE_F64)), (UNSUPPORTED, dict(delta=16, delta_dtype=native.DTYPE_F64)),
     (SHAPE, dict(rows=-1)), (SHAPE, dict(dim=0)), (SHAPE, dict(ld_x=63)), (SHAPE, dict(delta=16, ld_delta=63)),
     (SHAPE, dict(sum_out=16, ld_sum=63)), (SHAPE, dict(ld_q=63)), (SHAPE, dict(ld_q=-64)), (SHAPE, dict(dim=(1 << 30) + 1)),
@@ -72,6 +74,7 @@ def linear(**over):
     (ARG, dict(bias=18)), (ARG, dict(err=18)), (ARG, dict(out=17, out_dtype=native.DTYPE_BF16)),
     (ARG, dict(epi=3)), (ARG, dict(epi=-1)), (ARG, dict(epi=native.LINEAR_RESID)),
     (ARG, dict(epi=native.LINEAR_RESID, resid=18)), (ARG, dict(epi=native.LINEAR_RESID, resid=16, bias=16)),
+    (ARG, dict(epi=native.LINEAR_RESID, resid=16, ld_resid=80)),
     (ARG, dict(epi=native.LINEAR_SWIGLU, out_dtype=native.DTYPE_BF16, bias=16)),
     (UNSUPPORTED, dict(out_dtype=native.DTYPE_F64)), (UNSUPPORTED, dict(epi=native.LINEAR_SWIGLU)),
     (UNSUPPORTED, dict(epi=native.LINEAR_RESID, resid=16, out_dtype=native.DTYPE_BF16)),
