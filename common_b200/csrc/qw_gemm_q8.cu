@@ -30,6 +30,9 @@ namespace {
 
 constexpr int kQ8MaxK = 131071;  // |s| <= 128 * 128 * k < 2^31 for any codes
 constexpr int kQ8Threads = 320;  // a warp for the loads, one for the MMAs, eight for the results
+// Of 256 tokens over ranges of the k-blocks sixteen: their results leave all at once, behind the last MMA, and what bounds that is
+// the loads in flight.
+__host__ __device__ constexpr int split_threads(int bn) { return bn > 128 ? 576 : kQ8Threads; }
 constexpr int kBM = 128, kBK = 128;  // features of a CTA, codes of a k-block
 constexpr int kABytes = kBM * kBK;
 
@@ -41,7 +44,7 @@ struct Q8GemmArgs {
     int *err;
     long long ld_resid, ld_out;
     int M, K, T;
-    int aligned;  // result rows begin on 16 bytes
+    int aligned, raligned;  // rows of results and of residuals begin on 16 bytes
     int group;  // pairs that stay: token tiles per group of their order
 };
 
@@ -290,15 +293,28 @@ __device__ __forceinline__ void q8_emit4(const Q8GemmArgs &a, const float (&ws)[
         const float h0 = hi ? silu_times(p, y[2]) : silu_times(y[0], p), h1 = hi ? silu_times(q, y[3]) : silu_times(y[1], q);
         if (f >= a.M) return;
         __nv_bfloat16 *o = reinterpret_cast<__nv_bfloat16 *>(a.out) + t * a.ld_out + (f >> 5) * 16 + (lane & 3) * 4 + (hi ? 2 : 0);
-        o[0] = __float2bfloat16_rn(h0);
-        o[1] = __float2bfloat16_rn(h1);
+        if (a.aligned) {
+            *reinterpret_cast<uint32_t *>(o) = bf16x2(h0, h1);
+        } else {
+            o[0] = __float2bfloat16_rn(h0);
+            o[1] = __float2bfloat16_rn(h1);
+        }
     } else {
+        if (EPI == Q8_RESID || a.bias) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = add[i] + y[i];
+        }
+        const long long at = t * a.ld_out + f;
+        if (a.aligned && f + 4 <= a.M) {
+            if (EPI == Q8_BF16) *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + at) = make_uint2(bf16x2(y[0], y[1]), bf16x2(y[2], y[3]));
+            else *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (f + i >= a.M) break;
-            if (EPI == Q8_RESID || a.bias) y[i] = add[i] + y[i];
-            if (EPI == Q8_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[t * a.ld_out + f + i] = __float2bfloat16_rn(y[i]);
-            else reinterpret_cast<float *>(a.out)[t * a.ld_out + f + i] = y[i];
+            if (EPI == Q8_BF16) reinterpret_cast<__nv_bfloat16 *>(a.out)[at + i] = __float2bfloat16_rn(y[i]);
+            else reinterpret_cast<float *>(a.out)[at + i] = y[i];
         }
     }
 }
@@ -321,10 +337,10 @@ __host__ __device__ constexpr int split_stage_bytes(int ctas, int bn) { return (
 constexpr int kSplitStages = 12;  // at most
 
 template <int CTAS, int BN, int EPI>
-__global__ void __launch_bounds__(kQ8Threads, BN > 128 ? 1 : 2)
+__global__ void __launch_bounds__(split_threads(BN), BN > 128 ? 1 : 2)
     qw_q8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Q8GemmArgs a,
                        int nsplit, int S) {
-    constexpr int ROWS = BN / CTAS, B_BYTES = ROWS * kBK;
+    constexpr int THREADS = split_threads(BN), ROWS = BN / CTAS, B_BYTES = ROWS * kBK;
     constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN, IDESC = q8_idesc(kBM * CTAS, BN);
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kSplitStages], empty_bar[kSplitStages], tfull_bar;
@@ -411,23 +427,27 @@ __global__ void __launch_bounds__(kQ8Threads, BN > 128 ? 1 : 2)
     const bool epilogue = warp >= 2;
     const int ncols = min(BN, a.T - t0), c0 = ncols * range / nsplit + warp - 2, c1 = ncols * (range + 1) / nsplit;
     const int f4 = f0 + lane * 4;  // where sums are joined: a warp takes a token, a lane four features
-    constexpr int JW = kQ8Threads / 32 - 2, JC = 2;  // warps that join; tokens of a warp at a time
+    constexpr int JW = THREADS / 32 - 2, JC = 2;  // warps that join; tokens of a warp at a time
     float ws4[4], add4[JC][4];
     const auto addends = [&](int c) {  // biases, or residuals of tokens c, c + JW, ...
 #pragma unroll
-        for (int u = 0; u < JC; u++)
+        for (int u = 0; u < JC; u++) {
+            const float *from = EPI == Q8_RESID ? a.resid + (long long)(t0 + c + u * JW) * a.ld_resid + f4 : a.bias + f4;
+            const bool some = EPI == Q8_RESID ? c + u * JW < c1 : EPI <= Q8_BF16 && a.bias;
+            if (EPI == Q8_RESID && a.raligned && some && f4 + 4 <= a.M) {
+                const float4 v = *reinterpret_cast<const float4 *>(from);
+                add4[u][0] = v.x; add4[u][1] = v.y; add4[u][2] = v.z; add4[u][3] = v.w;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool on = f4 + i < a.M;
-                if (EPI == Q8_RESID) add4[u][i] = on && c + u * JW < c1 ? a.resid[(long long)(t0 + c + u * JW) * a.ld_resid + f4 + i] : 0.f;
-                else add4[u][i] = EPI <= Q8_BF16 && a.bias && on ? a.bias[f4 + i] : 0.f;
+                for (int i = 0; i < 4; i++) add4[u][i] = some && f4 + i < a.M ? from[i] : 0.f;
             }
+        }
     };
     if (epilogue) {
-        // two warps per 32 tensor-memory lanes (= features), one for each half of the tokens
-        constexpr int HALF = BN / 2, P = HALF < 32 ? HALF : 32;
-        const int q = warp & 3, half = (warp - 2) >> 2, f = f0 + q * 32 + lane;
-        for (int j = threadIdx.x - 64; j < BN; j += kQ8Threads - 64) s_xs[j] = j < ncols ? a.x_scale[t0 + j] : 0.f;
+        // JW / 4 warps per 32 tensor-memory lanes (= features), each for its part of the tokens
+        constexpr int PART = BN / (JW / 4), P = PART < 32 ? PART : 32;
+        const int q = warp & 3, mine0 = ((warp - 2) >> 2) * PART, f = f0 + q * 32 + lane;
+        for (int j = threadIdx.x - 64; j < BN; j += THREADS - 64) s_xs[j] = j < ncols ? a.x_scale[t0 + j] : 0.f;
         Q8Lane l{};
         if (nsplit == 1) {
             l = q8_lane<EPI>(a, f);
@@ -436,11 +456,11 @@ __global__ void __launch_bounds__(kQ8Threads, BN > 128 ? 1 : 2)
             for (int i = 0; i < 4; i++) ws4[i] = f4 + i < a.M ? a.w_scale[f4 + i] : 0.f;
             addends(c0);
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(kQ8Threads - 64) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(THREADS - 64) : "memory");
         mbar_wait(&tfull_bar, 0, abort_flag, a.err);
         tc_fence_after();
         int *part = reinterpret_cast<int *>(smem) + q * 32 + lane;
-        for (int c = half * HALF; c < min(ncols, (half + 1) * HALF); c += P) {
+        for (int c = mine0; c < min(ncols, mine0 + PART); c += P) {
             uint32_t r[P];
             tmem_get<P>(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
             if (nsplit == 1) {
@@ -687,10 +707,10 @@ __global__ void __launch_bounds__(kQ8Threads, 1)
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-cudaError_t launch_cluster(const void *fn, int grid, int cluster, int smem, cudaStream_t st, void **args) {
+cudaError_t launch_cluster(const void *fn, int grid, int threads, int cluster, int smem, cudaStream_t st, void **args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kQ8Threads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -835,12 +855,12 @@ cudaError_t q8_gemm_launch(const int8_t *w, long long ld_w, const int8_t *x, lon
     const long long tiles = (long long)((a.M + p.ctas * kBM - 1) / (p.ctas * kBM)) * ((a.T + p.bn - 1) / p.bn);
     if (p.nsplit == 0) {
         void *args[] = {(void *)&mw, (void *)&mx, (void *)&a};
-        return launch_cluster(fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), 2, pair_smem(256, epi), st, args);
+        return launch_cluster(fn, 2 * (int)(tiles < sms / 2 ? tiles : sms / 2), kQ8Threads, 2, pair_smem(256, epi), st, args);
     }
     const int size = p.ctas * p.nsplit, nkb = (a.K + kBK - 1) / kBK;
     int nsplit = p.nsplit, stages = split_stages(p, (nkb + nsplit - 1) / nsplit, q8_alone(p, tiles));
     void *args[] = {(void *)&mw, (void *)&mx, (void *)&a, (void *)&nsplit, (void *)&stages};
-    return launch_cluster(fn, (int)tiles * size, size, stages * split_stage_bytes(p.ctas, p.bn) + 1024, st, args);
+    return launch_cluster(fn, (int)tiles * size, split_threads(p.bn), size, stages * split_stage_bytes(p.ctas, p.bn) + 1024, st, args);
 }
 
 }  // namespace
@@ -880,7 +900,8 @@ extern "C" qw_status qw_op_linear_q8(const qw_linear_q8_args *p, void *stream) {
         return op_fail(QW_ERR_ARG, "pointers must be aligned to their elements");
     a.w_scale = p->w_scale; a.x_scale = p->x_scale; a.bias = p->bias; a.resid = p->resid;
     a.out = p->out; a.err = p->err; a.M = p->n_out; a.K = p->k; a.T = p->t; a.group = pair_group(p->k);
-    a.aligned = !((uintptr_t)p->out & 15) && a.ld_out % 8 == 0;
+    a.aligned = !((uintptr_t)p->out & 15) && a.ld_out % (p->out_dtype == QW_DTYPE_BF16 ? 8 : 4) == 0;
+    a.raligned = !((uintptr_t)p->resid & 15) && a.ld_resid % 4 == 0;
     const int epi = p->epi == QW_LINEAR_RESID ? Q8_RESID : p->epi == QW_LINEAR_SWIGLU ? Q8_SWIGLU
                   : p->out_dtype == QW_DTYPE_BF16 ? Q8_BF16 : Q8_F32;
     int dev = 0;
