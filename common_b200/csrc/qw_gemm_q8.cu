@@ -809,28 +809,30 @@ cudaError_t q8_device(int dev, int *sms) {
 }
 
 // Microseconds that a form takes, from what it loads, multiplies and joins.  The constants are fitted to the times of 190 shapes
-// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 2.3 % more
-// than the fastest one on average, 29 % at most (384 tokens, 4096 x 12288: 32.0 against 24.8 us).
+// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 1.5 % more
+// than the fastest one on average, 36 % at most (384 tokens, 4096 x 12288: 32.1 against 23.6 us).
 float q8_cost(const Q8Plan &p, int sms, int M, int T, int nkb) {
     const float tiles = (float)((M + p.ctas * kBM - 1) / (p.ctas * kBM)) * (float)((T + p.bn - 1) / p.bn);
-    if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(sms / 2)) * (0.34f * nkb + 1.2f);
+    if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(sms / 2)) * (0.411f * nkb + 1.2f);
     const float ctas = tiles * p.ctas * p.nsplit, per = ctas > sms && p.bn <= 128 ? 2.f : 1.f;  // per SM
     const float waves = ceilf(tiles / (float)kClusters[p.bn <= 128][p.ctas * p.nsplit]);
     const int kbs = (nkb + p.nsplit - 1) / p.nsplit;
     const float kb = (kBM + p.bn / p.ctas) * (float)kBK * 1e-3f;  // kilobytes of a k-block
     // a k-block: the ring's bytes in flight over their latency (GB/s of a CTA), the SM's loads, its MMAs
     const float ring = q8_alone(p, (long long)tiles) ? 83.5f : 63.f;
-    const float step = fmaxf(fmaxf(kb / ring, per * kb / 91.3f), per * p.bn * (0.243f / 128.f));
+    const float step = fmaxf(fmaxf(kb / ring, per * kb / 93.8f), p.bn > 128 ? 0.34f : per * p.bn * (0.277f / 128.f));
     // and all of them: weights from HBM, operands through L2
     const float load = fmaxf(fmaxf(waves * (kbs * step + 0.34f), (float)M * nkb * (kBK / 6.5e6f)), ctas * kbs * kb * (1.f / 7920.f));
-    return load + 0.854f / 64.f * p.bn + (p.nsplit > 1 ? 1.23f + 0.197f * p.nsplit + 0.345f / 64.f * p.bn : 0.f);
+    return load + 1.87f / 64.f * p.bn + (p.nsplit > 1 ? 1.45f + 0.197f * p.nsplit + 0.495f / 64.f * p.bn : 0.f);
 }
 Q8Plan q8_plan(int M, int T, int K, int sms) {
     const int nkb = (K + kBK - 1) / kBK;
-    Q8Plan best = kForms[0];
+    const long long tiles = (long long)((M + kPairBM - 1) / kPairBM) * ((T + 255) / 256);
+    // Pairs stay where there are more tiles than pairs; a tile each is done 5..19 % sooner by those that do not (more warps store).
+    Q8Plan best = tiles > sms / 2 ? Q8Plan{2, 256, 0} : Q8Plan{2, 256, 1};
     float least = q8_cost(best, sms, M, T, nkb);
     for (const Q8Plan &form : kForms) {
-        if (form.nsplit == 0 || (long long)form.bn * 8 < T || (form.bn > 16 && form.bn / 2 >= T)) continue;
+        if (form.nsplit == 0 || (form.bn < 256 && (long long)form.bn * 8 < T) || (form.bn > 16 && form.bn / 2 >= T)) continue;
         for (int n : {1, 2, 3, 4, 6, 8}) {
             if (n > nkb || n * form.ctas > kClusterMax) break;
             const Q8Plan p{form.ctas, form.bn, n};
