@@ -133,6 +133,10 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// A sum's value.  Each product is rounded, and so is what is added behind it: contracted differently here and there, the forms
+// would differ in the last bit.
+__device__ __forceinline__ float scaled(int s, float ws, float xs) { return __fmul_rn(__fmul_rn((float)s, ws), xs); }
+
 // up * gate / (1 + e^-gate): the exponential and the division are within (|gate| + 4) 2^-21 of their value, the result is rounded
 // to bf16 behind it.  A gate whose exponential leaves fp32 gives 0.
 __device__ __forceinline__ float silu_times(float g, float u) { return u * __fdividef(g, 1.0f + __expf(-g)); }
@@ -167,10 +171,11 @@ __device__ __forceinline__ void q8_emit_some(const Q8GemmArgs &a, const Q8Lane &
 #pragma unroll
     for (int j = 0; j < N; j += 4) {
         const float4 x = *reinterpret_cast<const float4 *>(xs + j);
-        const float v[4] = {(float)(int)s[j] * l.ws * x.x, (float)(int)s[j + 1] * l.ws * x.y, (float)(int)s[j + 2] * l.ws * x.z,
-                            (float)(int)s[j + 3] * l.ws * x.w};
+        const float v[4] = {scaled((int)s[j], l.ws, x.x), scaled((int)s[j + 1], l.ws, x.y), scaled((int)s[j + 2], l.ws, x.z),
+                            scaled((int)s[j + 3], l.ws, x.w)};
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[j + i] = EPI == Q8_RESID ? y[j + i] + v[i] : EPI <= Q8_BF16 && a.bias ? v[i] + l.bias : v[i];
+        for (int i = 0; i < 4; i++)
+            y[j + i] = EPI == Q8_RESID ? __fadd_rn(y[j + i], v[i]) : EPI <= Q8_BF16 && a.bias ? __fadd_rn(v[i], l.bias) : v[i];
     }
     if (EPI == Q8_SWIGLU) {
         // lanes 0..15 hold gates, 16..31 the ups of the same 16 products: of two tokens the lower lane computes the first and
@@ -222,7 +227,7 @@ __device__ __forceinline__ void stmatrix4_trans(uint32_t addr, uint32_t a, uint3
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ float2 scaled2(uint32_t s0, uint32_t s1, float ws, float2 xs) {
-    return make_float2((float)(int)s0 * ws * xs.x, (float)(int)s1 * ws * xs.y);
+    return make_float2(scaled((int)s0, ws, xs.x), scaled((int)s1, ws, xs.y));
 }
 __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
     const __nv_bfloat162 w = __floats2bfloat162_rn(lo, hi);
@@ -256,8 +261,8 @@ __device__ __forceinline__ void q8_emit_rows(const Q8GemmArgs &a, uint32_t taddr
             if (EPI == Q8_SWIGLU) {
                 w[i][h] = bf16x2(silu_times(y.x, z.x), silu_times(y.y, z.y));
             } else {
-                w[i][h] = a.bias ? bf16x2(y.x + bias[h], y.y + bias[h]) : bf16x2(y.x, y.y);
-                w[i][2 + h] = a.bias ? bf16x2(z.x + bias[2 + h], z.y + bias[2 + h]) : bf16x2(z.x, z.y);
+                w[i][h] = a.bias ? bf16x2(__fadd_rn(y.x, bias[h]), __fadd_rn(y.y, bias[h])) : bf16x2(y.x, y.y);
+                w[i][2 + h] = a.bias ? bf16x2(__fadd_rn(z.x, bias[2 + h]), __fadd_rn(z.y, bias[2 + h])) : bf16x2(z.x, z.y);
             }
         }
     }
@@ -285,7 +290,7 @@ __device__ __forceinline__ void q8_emit_rows(const Q8GemmArgs &a, uint32_t taddr
 template <int EPI>
 __device__ __forceinline__ void q8_emit4(const Q8GemmArgs &a, const float (&ws)[4], const float (&add)[4], int4 s, float xs, int f,
                                          int lane, long long t) {
-    float y[4] = {(float)s.x * ws[0] * xs, (float)s.y * ws[1] * xs, (float)s.z * ws[2] * xs, (float)s.w * ws[3] * xs};
+    float y[4] = {scaled(s.x, ws[0], xs), scaled(s.y, ws[1], xs), scaled(s.z, ws[2], xs), scaled(s.w, ws[3], xs)};
     if constexpr (EPI == Q8_SWIGLU) {
         // of 8 lanes the first four hold 16 gates, the others their ups: each computes two of a lane's four products
         const bool hi = lane & 4;
@@ -302,7 +307,7 @@ __device__ __forceinline__ void q8_emit4(const Q8GemmArgs &a, const float (&ws)[
     } else {
         if (EPI == Q8_RESID || a.bias) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = add[i] + y[i];
+            for (int i = 0; i < 4; i++) y[i] = __fadd_rn(add[i], y[i]);
         }
         const long long at = t * a.ld_out + f;
         if (a.aligned && f + 4 <= a.M) {

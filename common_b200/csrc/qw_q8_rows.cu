@@ -73,32 +73,39 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// The codes of four numbers, one to a byte.  COARSE: the numbers of a bf16 row.  With 8 significant bits each, |g| = a 2^p and
-// t = b 2^q, halves are common (0.2 % of a normal row's numbers: 127 g / t is 63.5 wherever g is t / 2), and nothing else comes
-// near one: 254 a 2^(p - q) / b is odd or keeps v / (254 * 255) of v = 127 |g| / t from it, where g m is off by v 2^-24.  So a
-// number that is within v 1e-6 of a half is one, and goes to the even side, without 64 bits.
-template <bool COARSE>
+__device__ __forceinline__ uint32_t low_bytes(uint64_t r0, uint64_t r1) {
+    const float2 a = unpack2(r0), b = unpack2(r1);
+    return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                       __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+}
+// The codes of four numbers, one to a byte.
 __device__ __forceinline__ uint32_t q8_codes4(const float *g, float m, float t) {
     const uint64_t mm = pack2(m, m), magic = pack2(kMagic, kMagic), back = pack2(-kMagic, -kMagic), minus = pack2(-m, -m);
     const uint64_t g0 = pack2(g[0], g[1]), g1 = pack2(g[2], g[3]);
     const uint64_t r0 = fma2(g0, mm, magic), r1 = fma2(g1, mm, magic);
     const float2 d0 = unpack2(fma2(g0, minus, add2(r0, back))), d1 = unpack2(fma2(g1, minus, add2(r1, back)));  // code - value
     const float far = fmaxf(fmaxf(fabsf(d0.x), fabsf(d0.y)), fmaxf(fabsf(d1.x), fabsf(d1.y)));
-    const float2 a = unpack2(r0), b = unpack2(r1);
-    int c[4] = {__float_as_int(a.x), __float_as_int(a.y), __float_as_int(b.x), __float_as_int(b.y)};
+    uint32_t codes = low_bytes(r0, r1);
     if (far > kNearHalf) {
         const float d[4] = {d0.x, d0.y, d1.x, d1.y};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (COARSE) {
-                const bool half = fabsf(d[i]) > 0.5f - 1e-6f * fabsf(g[i] * m);
-                c[i] += half && (c[i] & 1) ? (d[i] > 0.f ? -1 : 1) : 0;
-            } else if (fabsf(d[i]) > kNearHalf) {
-                c[i] = q8_code_near(g[i], m, t);
-            }
-        }
+        for (int i = 0; i < 4; i++)
+            if (fabsf(d[i]) > kNearHalf)
+                codes = (codes & ~(0xFFu << (8 * i))) | (uint32_t)(q8_code_near(g[i], m, t) & 0xFF) << (8 * i);
     }
-    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    return codes;
+}
+// The same for numbers of a bf16 row.  With 8 significant bits each, |g| = a 2^p and t = b 2^q, halves are common (0.2 % of a
+// normal row's numbers: 127 g / t is 63.5 wherever g is t / 2), and nothing else comes near one: 254 a 2^(p - q) / b is odd or
+// keeps v / (254 * 255) of v = 127 |g| / t from it.  So v is multiplied by 1 + 2^-20 and by 1 - 2^-20 (the roundings' 2^-23 are less,
+// the distance is more): the two whole numbers are the same, or one to each side of a half, and the even one is the code.
+__device__ __forceinline__ uint32_t q8_codes4_coarse(const float *g, float m) {
+    const float up = m * (1.f + 0x1p-20f), down = m * (1.f - 0x1p-20f);
+    const uint64_t uu = pack2(up, up), dd = pack2(down, down), magic = pack2(kMagic, kMagic);
+    const uint64_t g0 = pack2(g[0], g[1]), g1 = pack2(g[2], g[3]);
+    const uint32_t out = low_bytes(fma2(g0, uu, magic), fma2(g1, uu, magic)), in = low_bytes(fma2(g0, dd, magic), fma2(g1, dd, magic));
+    const uint32_t odd = (out & 0x01010101u) * 255u;
+    return (out & ~odd) | (in & odd);
 }
 
 // V consecutive numbers as they lie in memory, and as fp32
@@ -185,7 +192,7 @@ __device__ __forceinline__ unsigned top_of(const Piece<__nv_bfloat16, V> &p, uns
 // A row per `wpr` warps, held in registers: NC pieces of V numbers a lane, piece j of a lane 32 * wpr pieces behind piece j - 1.
 // One pass: the sum of squares and the largest magnitude in one exchange between the warps, codes from the registers.  Bound by
 // HBM: the norm of 8192 x 4096 in fp32 with its sum written takes 64 us (6.8 TB/s), rows of 24576 x 4096 in fp32 73 us (6.9 TB/s),
-// of 8192 x 12288 in bf16 53 us (5.7 TB/s): there the issue of some 8 instructions a number shows.  One row takes 2 us, the launch and
+// in bf16 46 us (6.5 TB/s), of 8192 x 12288 in bf16 49 us (6.2 TB/s).  One row takes 2 us, the launch and
 // one chain of a load, an exchange and a store.  CTAs that stay and have the next row on its way were slower (68, 76 and 75 us): what
 // the loads' latency costs, more small CTAs hide better than more registers.
 template <typename XT, typename DT, bool NORM, int V, int NC>
@@ -270,7 +277,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) qw_q8_rows_kernel(const Q8Rows
         widen(g[j], v);
         uint32_t c[V / 4];
 #pragma unroll
-        for (int e = 0; e < V; e += 4) c[e / 4] = coded ? q8_codes4<!NORM && sizeof(XT) == 2>(v + e, m, t) : 0u;
+        for (int e = 0; e < V; e += 4) {
+            if constexpr (!NORM && sizeof(XT) == 2) c[e / 4] = coded ? q8_codes4_coarse(v + e, m) : 0u;
+            else c[e / 4] = coded ? q8_codes4(v + e, m, t) : 0u;
+        }
         if (n >= V) {
             if constexpr (V == 8) *reinterpret_cast<uint2 *>(q + j * step) = make_uint2(c[0], c[1]);
             else *reinterpret_cast<uint32_t *>(q + j * step) = c[0];
@@ -353,7 +363,7 @@ cudaError_t q8_rows_launch(const Q8RowsArgs &a, cudaStream_t st) {
     if (!vec || a.dim > (NORM ? 16384 : 32768)) return launch_pdl(qw_q8_rows_any_kernel<XT, DT, NORM>, dim3(a.rows), dim3(256), 0, st, a);
     // Few rows: as many lanes as there are pieces (64 x 4096: 3.3 us, 4.2 with 8 pieces a lane).  Many: so many numbers a lane that
     // the exchange between the warps is rare, and so few that several rows fit an SM: 16 beside delta and weights (8192 x 4096 in
-    // fp32: 64 us, 69 with 8 or 32), 32 alone (24576 x 4096: 73 us, 81 with 16), 64 of bf16 (8192 x 12288: 56 us, 66 with 32).
+    // fp32: 64 us, 69 with 8 or 32), 32 alone (24576 x 4096: 73 us, 81 with 16), 64 of bf16 (8192 x 12288: 49 us; with an exact comparison of halves behind it, 56, and 66 with 32).
     const int pieces = (a.dim + V - 1) / V, most = a.rows <= kFewRows ? 1 : NORM ? 16 / V : 8;
     int wpr = 1;
     while (wpr < kRowWarps && wpr * 32 * most < pieces) wpr *= 2;

@@ -142,19 +142,22 @@ def test_same_bits_every_time(t, epi, bf16):
         assert torch.equal(first, c.out)
 
 
-@pytest.mark.parametrize("epi,bf16", [(STORE, False), (STORE, True), (SWIGLU, True)])
-def test_rows_do_not_depend_on_their_batch(epi, bf16):
+@pytest.mark.parametrize("epi,bf16,bias", [(STORE, False, False), (STORE, True, False), (STORE, False, True), (STORE, True, True),
+                                           (RESID, False, False), (SWIGLU, True, False)])
+@pytest.mark.parametrize("n_out,k,gap", [(1024, 2304, 0), (1024, 300, 3), (4096, 4096, 0)])
+def test_rows_do_not_depend_on_their_batch(epi, bf16, bias, n_out, k, gap):
     """A token's results are the same bits in every batch, whatever kernel and split it takes."""
     import torch
-    big = Case(1500, 1024, 2304, epi=epi, bf16=bf16, seed=6)
+    big = Case(5000, n_out, k, epi=epi, bf16=bf16, bias=bias, seed=6, gap=gap)
     big.run()
     torch.cuda.synchronize()
-    for t in (1, 16, 33, 64, 128, 257, 700):
-        c = Case(t, 1024, 2304, epi=epi, bf16=bf16)
-        c.w, c.ws, c.x, c.xs = big.w, big.ws, big.x[:t], big.xs[:t]
+    for t in (1, 16, 33, 64, 128, 257, 700, 1500):
+        c = Case(t, n_out, k, epi=epi, bf16=bf16, gap=gap)
+        c.w, c.ws, c.x, c.xs, c.bias = big.w, big.ws, big.x[:t], big.xs[:t], big.bias
+        c.resid = big.resid[:t] if epi == RESID else None
         c.run()
         torch.cuda.synchronize()
-        assert torch.equal(c.out[:t], big.out[:t])
+        assert torch.equal(c.out[:t], big.out[:t]), t
 
 
 def test_scales_that_are_none():

@@ -136,6 +136,27 @@ def test_norm(rows, dim, gap, lead, x_kind, d_kind):
     assert bool((out[rows] == 7).all()) and bool((out[:, dim:] == 7).all())
 
 
+@pytest.mark.parametrize("power", [0, 100, -100])
+def test_every_pair_of_bf16_significands(power):
+    """A row for every significand of its largest number, holding every significand at every exponent that has a code, and
+    numbers without a full significand: halves are told from what is next to them, whatever the two numbers."""
+    import torch
+    a = torch.arange(128, 256, dtype=torch.float64, device="cuda")
+    halvings = torch.tensor([2.0 ** -j for j in range(12)], dtype=torch.float64, device="cuda")
+    g = (a[:, None] * halvings).reshape(-1)
+    x = torch.stack([torch.cat([b[None], torch.where(g <= b, g, torch.zeros_like(g)), -torch.where(g <= b, g, torch.zeros_like(g))])
+                     for b in a]) * 2.0 ** power
+    rows, dim = x.shape
+    for ld in (dim, (dim + 7) // 8 * 8):  # by every number, by whole pieces
+        buf = torch.zeros((rows, ld), dtype=torch.bfloat16, device="cuda")
+        buf[:, :dim] = x
+        assert torch.equal(buf[:, :dim].double(), x)
+        q, scale = torch.zeros((rows, ld), dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+        native.op_quant_q8(buf.data_ptr(), native.DTYPE_BF16, rows, dim, q.data_ptr(), scale.data_ptr(), ld_x=ld, ld_q=ld)
+        torch.cuda.synchronize()
+        check_codes(q[:, :dim], scale, x.float(), 1.0, 2.0 ** -24)
+
+
 @pytest.mark.parametrize("dim", [40, 4096, 40001])
 def test_rows_with_nan_or_infinity_are_marked(dim):
     import torch
