@@ -332,7 +332,7 @@ __device__ __forceinline__ void q8_emit4(const Q8GemmArgs &a, const float (&ws)[
 // tile are the CTAs or pairs of a cluster (up to 8 CTAs).  Their sums meet in distributed shared memory: each CTA leaves its
 // own in its ring, which is free by then, and after a cluster barrier adds up its share of the tile's tokens from all of them.
 //
-// Bound by the weights' bytes and what stands around them.  64 tokens, 4096 x 12288, RESID: 13.8 us in a graph, of which the
+// Bound by the weights' bytes and what stands around them.  64 tokens, 4096 x 12288, RESID: 13.9 us in a graph, of which the
 // weights' 50 MB take 8.3 (6 TB/s); 1.7 to the first k-block behind the previous kernel's end, 0.3 for the sums, 1.0 for the slowest
 // CTA of a cluster, 1.3 to join and store, 1.2 to the end.  One token, 6144 x 4096: 7.5..8.1 us, 4.3 of them the weights'.  Measured and
 // rejected: asking for the weights in L2 before the previous kernel has ended (17 us against 14; the requests stand in the way of
@@ -531,7 +531,8 @@ __global__ void __launch_bounds__(split_threads(BN), BN > 128 ? 1 : 2)
 //   tfull[i]  in each CTA, signalled by the commit behind the tile's last k-block;
 //   tempty[i] in the even CTA: 16 arrivals (the epilogue warps of both CTAs).
 //
-// 8192 x 24576 x 4096 with SwiGLU: 608..622 us (2.65..2.7 POP/s, at the 1000 W limit), of which 45 are the epilogue's: without it 570.
+// 8192 x 24576 x 4096 with SwiGLU: 600..622 us (2.65..2.75 POP/s, at the 1000 W limit), of which 30..50 are the epilogue's:
+// without it 570.
 // The tensor pipe is bound by the power: SM clocks settle at 1.4 GHz, and a library's plain product of the same codes takes 508..545 us
 // with 1.3 GHz.  With four epilogue warps instead of eight the epilogue was longer than the MMAs of K = 4096 (779 us); with results
 // stored as they lie in tensor memory, 2 bytes a lane, 655.  RESID (8192 x 4096 x 12288, 336 us) gains nothing from residuals
