@@ -328,3 +328,52 @@ def test_first_calls_may_be_captured_ones():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=200)
     assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
+def test_graphs_with_copies_and_joined_streams():
+    """Captured behind copies, fills and another stream's kernels, each operator waits for all of them."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(2)
+    n, k, t = 2048, 2048, 100
+    src = torch.randn((4, t, k), device="cuda", generator=g)
+    x, x2 = torch.zeros((t, k), device="cuda"), torch.zeros((t, k), device="cuda")
+    w = torch.randn((n, k), device="cuda", generator=g)
+    cw, sw = torch.zeros((n, k), dtype=torch.int8, device="cuda"), torch.zeros(n, device="cuda")
+    cx, sx = torch.zeros((t, k), dtype=torch.int8, device="cuda"), torch.zeros(t, device="cuda")
+    w2, out, resid = torch.zeros_like(w), torch.zeros((t, n), device="cuda"), torch.zeros((t, n), device="cuda")
+    lin = native.LinearQ8(cw.data_ptr(), sw.data_ptr(), n, k, epi=native.LINEAR_RESID)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def body():
+        here = torch.cuda.current_stream()
+        st = here.cuda_stream
+        x.copy_(src[0])                                      # a copy in front
+        other.wait_stream(here)
+        with torch.cuda.stream(other):                       # weights coded on another stream meanwhile
+            w2.copy_(w).mul_(2.0)
+            native.op_quant_q8(w2.data_ptr(), native.DTYPE_F32, n, k, cw.data_ptr(), sw.data_ptr(), stream=other.cuda_stream)
+        x2.copy_(x)
+        native.op_quant_q8(x2.data_ptr(), native.DTYPE_F32, t, k, cx.data_ptr(), sx.data_ptr(), stream=st)
+        resid.zero_()
+        resid.add_(1.0)
+        here.wait_stream(other)                              # two kernels and a fill in front of the product
+        lin(cx.data_ptr(), sx.data_ptr(), t, out.data_ptr(), resid=resid.data_ptr(), stream=st)
+        out.mul_(0.5)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        body()
+    for i in range(1, 4):
+        src[0].copy_(src[i])
+        w.copy_(torch.randn((n, k), device="cuda", generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cx, Layer.coded(src[i])[0]) and torch.equal(cw, Layer.coded(2 * w)[0])
+        y = cx.double() @ cw.double().T * sw.double() * sx.double()[:, None]
+        assert bool(((2 * out.double() - 1 - y).abs() <= 2.0 ** -22 * y.abs() + 2.0 ** -24 * (1 + y).abs()).all())
+        got = out.clone()
+        with torch.cuda.stream(side):
+            body()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
