@@ -31,7 +31,7 @@ namespace {
 constexpr int kQ8MaxK = 131071;  // |s| <= 128 * 128 * k < 2^31 for any codes
 constexpr int kQ8Threads = 320;  // a warp for the loads, one for the MMAs, eight for the results
 // Of 256 tokens over ranges of the k-blocks sixteen: their results leave all at once, behind the last MMA, and what bounds that is
-// the loads in flight.
+// the loads in flight (512 x 4096 x 12288, RESID: 25.6 us, 29.5 with eight).
 __host__ __device__ constexpr int split_threads(int bn) { return bn > 128 ? 576 : kQ8Threads; }
 constexpr int kBM = 128, kBK = 128;  // features of a CTA, codes of a k-block
 constexpr int kABytes = kBM * kBK;

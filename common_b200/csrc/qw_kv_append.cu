@@ -246,7 +246,8 @@ constexpr int kLive = 1, kNowhere = 0, kNoRow = -1;
 // rows' sequences, positions, pages and angles are looked up at once, behind the first loads.  13,800 rows of 32 / 8 heads of 128:
 // 64 us from bf16 with norms per head (5.2 TB/s; 80 with a CTA per row), 59 without norms, 85 from fp32 (5.9 TB/s); of 14 / 2 heads of
 // 64 27 us (49 with a CTA per row, whose threads a row of 1152 numbers does not fill).  Bound by HBM and, at 230 instructions per 32
-// pieces, by their issue (half of the slots); 8 rows a CTA take 70 us, 6 CTAs an SM (80 registers) 77.
+// pieces, by their issue (half of the slots); 8 rows a CTA take 70 us, 6 CTAs an SM (80 registers) 77;
+// fp32 rows need the registers of 4 CTAs (5: 109 us).
 template <typename IT, typename OT, int R>
 __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv_append_rows_kernel(const AppendArgs a) {
     constexpr int STEP = 2;  // rows on their way at a time

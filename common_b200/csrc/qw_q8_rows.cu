@@ -361,7 +361,8 @@ cudaError_t q8_rows_launch(const Q8RowsArgs &a, cudaStream_t st) {
                      !apart(a.q, a.ld_q, 1) && (uintptr_t)a.w % 16 == 0;
     // the norm holds its weights too: half the numbers fit its registers
     if (!vec || a.dim > (NORM ? 16384 : 32768)) return launch_pdl(qw_q8_rows_any_kernel<XT, DT, NORM>, dim3(a.rows), dim3(256), 0, st, a);
-    // Few rows: as many lanes as there are pieces (64 x 4096: 3.3 us, 4.2 with 8 pieces a lane).  Many: so many numbers a lane that
+    // Few rows: as many lanes as there are pieces (64 x 4096: 3.3 us, 4.2 with 8 pieces a lane; at
+    // 256 rows there is nothing between them, 5.0..5.1 us).  Many: so many numbers a lane that
     // the exchange between the warps is rare, and so few that several rows fit an SM: 16 beside delta and weights (8192 x 4096 in
     // fp32: 64 us, 69 with 8 or 32), 32 alone (24576 x 4096: 73 us, 81 with 16), 64 of bf16 (8192 x 12288: 49 us; with an exact comparison of halves behind it, 56, and 66 with 32).
     const int pieces = (a.dim + V - 1) / V, most = a.rows <= kFewRows ? 1 : NORM ? 16 / V : 8;
