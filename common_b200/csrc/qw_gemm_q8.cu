@@ -5,8 +5,8 @@
 // W is the M side of the MMAs (128 features per CTA), the tokens are their N side, as in qw_gemm.cu; a k-block is 128 codes,
 // one 128-byte row of swizzled shared memory, staged by TMA (no multicast).  The sums are exact, so that every form below
 // gives the same bits, however it cuts the work:
-//   qw_q8_split_kernel  few tokens: one tile of 128 features x 16..128 tokens and one range of its k-blocks per CTA; the CTAs
-//                       of a tile form a cluster and add their sums through distributed shared memory;
+//   qw_q8_split_kernel  few tokens or tiles: one tile of 128 or 256 features x 16..256 tokens and one range of its k-blocks per
+//                       CTA or pair; the CTAs of a tile form a cluster and add their sums through distributed shared memory;
 //   qw_q8_pair_kernel   many tokens: persistent CTA pairs, tiles of 256 features x 256 tokens (cta_group::2).
 //
 // Both are launched with programmatic dependent launch: barriers, tensor memory and descriptors are set up behind the end of

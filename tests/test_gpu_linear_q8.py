@@ -195,6 +195,27 @@ def test_weights_past_32_bit_offsets():
     c.check()
 
 
+@pytest.mark.parametrize("t,n_out,k,epi,bf16,ld", [(20, 300, 600, STORE, True, 1 << 27), (20, 256, 2048, RESID, False, 1 << 27),
+                                                   (300, 19456, 256, SWIGLU, True, 1 << 23), (300, 19456, 256, STORE, True, 1 << 23)])
+def test_results_past_32_bit_offsets(t, n_out, k, epi, bf16, ld):
+    """Result (and residual) rows whose offsets pass 2^31 elements, by joined tiles and by pairs."""
+    import torch
+    c = Case(t, n_out, k, epi=epi, bf16=bf16, seed=8)
+    out = torch.zeros(((t - 1) * ld + n_out,), dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    rows = out.as_strided((t, c.cols), (ld, 1))
+    if epi == RESID:
+        rows.copy_(c.resid)
+        want, c.resid = c.resid, rows
+    c.run(out=rows)
+    torch.cuda.synchronize()
+    c.out[:t] = rows
+    if epi == RESID:
+        c.resid = want
+    c.check()
+    rows.zero_()
+    assert int(torch.count_nonzero(out)) == 0
+
+
 def test_other_streams_at_once():
     import torch
     cases = [Case(t, 4096, 1024, seed=t, epi=e, bf16=b) for t, e, b in
