@@ -340,8 +340,11 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv
                 if (a.mode == QW_QKNORM_HEAD)
                     m[i] = rsqrtf(lanes_sum(on && i0 + i < nr ? squares(x[i], y[i]) : 0.f, hc) * a.inv_d + a.eps);
             }
-            if (i0 + STEP < R) load(src, i0 + STEP);
-            else if (h + apart < heads) load(next, 0);
+            if (i0 + STEP < R) {
+                if (on) load(src, i0 + STEP);
+            } else if (h + apart < heads) {
+                load(next, 0);
+            }
             if (!on) continue;
 #pragma unroll
             for (int i = 0; i < STEP; i++) {
