@@ -18,6 +18,8 @@ static thread_local std::string g_op_error;
 
 qw_status op_fail(qw_status s, const std::string &msg) {
     g_op_error = msg;
+    // the runtime keeps a failed launch's error for whoever asks next: another call of this library, or the host's own code
+    if (s == QW_ERR_CUDA) cudaGetLastError();
     return s;
 }
 
