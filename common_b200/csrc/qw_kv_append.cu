@@ -380,7 +380,7 @@ cudaError_t append_launch(const AppendArgs &a, cudaStream_t st) {
     // A CTA per row below: 592 rows of 32 / 8 heads 7.0 us (11.5 by fours), 1024 11.6 (12.3), 2048 17.4 (15.7); of 14 / 2 heads of 64
     // 3.8 (5.4), 6.2 (5.7), 10.7 (6.9).  Norms over whole vectors would read four rows twice: 91 us against 79.
     if (a.rows > kAppendFew && a.mode != QW_QKNORM_VECTOR)
-        return launch_pdl(qw_kv_append_rows_kernel<IT, OT, kAppendRows>, dim3((a.rows + kAppendRows - 1) / kAppendRows), dim3(kAppendThreads),
+        return launch_pdl(qw_kv_append_rows_kernel<IT, OT, kAppendRows>, dim3(a.rows / kAppendRows + (a.rows % kAppendRows != 0)), dim3(kAppendThreads),
                           kAppendRows * a.d * sizeof(float), st, a);
     return launch_pdl(qw_kv_append_row_kernel<IT, OT, 3>, dim3(a.rows), dim3(kAppendThreads), 0, st, a);
 }

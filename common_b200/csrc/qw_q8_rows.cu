@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(256) qw_q8_rows_any_kernel(const Q8RowsArgs a)
 template <typename XT, typename DT, bool NORM, int V, int NC>
 cudaError_t q8_rows_regs(const Q8RowsArgs &a, int wpr, cudaStream_t st) {
     const int warps = wpr < 4 ? 4 : wpr, rows = warps / wpr;
-    return launch_pdl(qw_q8_rows_kernel<XT, DT, NORM, V, NC>, dim3((a.rows + rows - 1) / rows), dim3(32 * warps), 0, st, a, wpr);
+    return launch_pdl(qw_q8_rows_kernel<XT, DT, NORM, V, NC>, dim3(a.rows / rows + (a.rows % rows != 0)), dim3(32 * warps), 0, st, a, wpr);
 }
 
 template <typename XT, typename DT, bool NORM>
