@@ -16,7 +16,7 @@ namespace qw {
 namespace {
 
 // rows whose largest magnitude is below this are coded as zeros: 127 times the smallest normal number, so that neither
-// the scale nor 127 / t leaves the normal range
+// 127 / t nor the scale of a row without a norm leaves the normal range
 constexpr float kQ8Tiny = 127.0f * 1.17549435e-38f;
 
 constexpr int kQ8MaxDim = 1 << 30;
@@ -107,6 +107,9 @@ __device__ __forceinline__ uint32_t q8_codes4_coarse(const float *g, float m) {
     const uint32_t odd = (out & 0x01010101u) * 255u;
     return (out & ~odd) | (in & odd);
 }
+
+// t / (127 sqrt(mean)), rounded once: 1 / sqrt(mean), or t times it, may be outside fp32 where the scale is not
+__device__ __forceinline__ float norm_scale(float t, double mean) { return (float)((double)t / (127.0 * sqrt(mean))); }
 
 // V consecutive numbers as they lie in memory, and as fp32
 template <typename T, int V> struct Piece { uint32_t u[V * sizeof(T) / 4]; };
@@ -291,8 +294,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) qw_q8_rows_kernel(const Q8Rows
         }
     }
     if (first == 0) {
-        const float rms = NORM ? (float)(1.0 / sqrt(ss / a.dim + a.eps)) : 1.f;
-        a.scale[r] = coded ? t * rms / 127.f : finite ? 0.f : __uint_as_float(0x7FC00000u);
+        a.scale[r] = coded ? (NORM ? norm_scale(t, ss / a.dim + a.eps) : t / 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
     }
 }
 
@@ -339,8 +341,7 @@ __global__ void __launch_bounds__(256) qw_q8_rows_any_kernel(const Q8RowsArgs a)
         q[i] = coded ? (int8_t)q8_code(g, m, t) : 0;
     }
     if (tid == 0) {
-        const float rms = NORM ? (float)(1.0 / sqrt(ss / a.dim + a.eps)) : 1.f;
-        a.scale[r] = coded ? t * rms / 127.f : finite ? 0.f : __uint_as_float(0x7FC00000u);
+        a.scale[r] = coded ? (NORM ? norm_scale(t, ss / a.dim + a.eps) : t / 127.f) : finite ? 0.f : __uint_as_float(0x7FC00000u);
     }
 }
 

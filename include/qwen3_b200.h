@@ -438,7 +438,7 @@ typedef struct qw_norm_q8_args {
 /* Residual addition, root-mean-square norm and codes in one pass: h = x + delta (fp32), sum = h (rounded once where the
  * stream is bf16; the norm sees h), y = h / sqrt(mean(h^2) + eps) * norm_w, then the codes and the scale of every row of y.
  * The norm cancels in the codes: they are those of the fp32 products h * norm_w, exactly.  The sum of squares is held in
- * 64 bits; scale is within 2^-22 of its value.  Stands in for accum + rmsnorm (SequentialBlock.java:413-429,
+ * 64 bits, and scale is rounded once from them (infinite where it leaves fp32).  Stands in for accum + rmsnorm (SequentialBlock.java:413-429,
  * NormalizationLayerFeatures.java:574-604), which it codes. */
 qw_status qw_op_norm_q8(const qw_norm_q8_args *args, void *stream);
 
