@@ -108,8 +108,8 @@ __device__ __forceinline__ uint32_t q8_codes4_coarse(const float *g, float m) {
     return (out & ~odd) | (in & odd);
 }
 
-// t / (127 sqrt(mean)), rounded once: 1 / sqrt(mean), or t times it, may be outside fp32 where the scale is not
-__device__ __forceinline__ float norm_scale(float t, double mean) { return (float)((double)t / (127.0 * sqrt(mean))); }
+// t / (127 sqrt(mean)), rounded to fp32 once: 1 / sqrt(mean), or t times it, may be outside fp32 where the scale is not
+__device__ __forceinline__ float norm_scale(float t, double mean) { return (float)((double)t * rsqrt(mean) * (1.0 / 127.0)); }
 
 // V consecutive numbers as they lie in memory, and as fp32
 template <typename T, int V> struct Piece { uint32_t u[V * sizeof(T) / 4]; };
