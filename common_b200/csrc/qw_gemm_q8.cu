@@ -138,8 +138,14 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ float scaled(int s, float ws, float xs) { return __fmul_rn(__fmul_rn((float)s, ws), xs); }
 
 // up * gate / (1 + e^-gate): the exponential and the division are within (|gate| + 4) 2^-21 of their value, the result is rounded
-// to bf16 behind it.  A gate whose exponential leaves fp32 gives 0.
-__device__ __forceinline__ float silu_times(float g, float u) { return u * __fdividef(g, 1.0f + __expf(-g)); }
+// to bf16 behind it.  __fdividef gives 0 for divisors above 2^126: both sides are taken 2^-8 times, so that these begin at a gate
+// of -92.8, where silu(gate) is below fp32's normal numbers (-87.3 without).  An exponential below them does not count beside 1.
+__device__ __forceinline__ float silu_times(float g, float u) {
+    constexpr float LOG2E = 1.44269504f;
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmaf_rn(g, -LOG2E, -8.f)));
+    return u * __fdividef(g * 0x1p-8f, 0x1p-8f + e);
+}
 
 // What a lane keeps for its feature f across the tokens of a tile.
 struct Q8Lane {
