@@ -820,9 +820,11 @@ cudaError_t q8_device(int dev, int *sms) {
     return cudaSuccess;
 }
 
-// Microseconds that a form takes, from what it loads, multiplies and joins.  The constants are fitted to the times of 190 shapes
-// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges): the form that it picks takes 1.5 % more
-// than the fastest one on average, 36 % at most (384 tokens, 4096 x 12288: 32.1 against 23.6 us).
+// Microseconds that a form takes, from what it loads, multiplies and joins.  The constants are fitted to the times of 196 shapes
+// (1152..24576 features, 896..12288 codes, 1..4096 tokens, every form and 1..8 ranges), all STORE to bf16 without a bias: the form that
+// it picks takes 1.5 % more than the fastest one on average, 36 % at most (384 tokens, 4096 x 12288: 32.1 against 23.6 us; 23 % at
+// 1 x 1152 x 896 and 256 x 9728 x 12288).  RESID, which moves 8 bytes a result, and SWIGLU, which stores 1, are not in it:
+// 384 x 4096 x 12288 with RESID takes 42 us where 512 tokens take 26.
 float q8_cost(const Q8Plan &p, int sms, int M, int T, int nkb) {
     const float tiles = (float)((M + p.ctas * kBM - 1) / (p.ctas * kBM)) * (float)((T + p.bn - 1) / p.bn);
     if (p.nsplit == 0) return 2.5f + ceilf(tiles / (float)(sms / 2)) * (0.411f * nkb + 1.2f);

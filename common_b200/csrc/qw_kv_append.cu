@@ -100,7 +100,8 @@ __device__ __forceinline__ float lanes_sum(float v, int n) {
 // One CTA per row, for few rows and for norms over whole vectors.  A thread takes 8 numbers of a head's first half with the
 // matching 8 of its second (the rotary pairs), and the same 8 of every further head that it serves, so that a row's angles are
 // read once per thread; CH heads are on their way at a time, the first of them while the row's sequence, position and page are
-// looked up.  64 tokens of 32 / 8 heads take 4.3 us: the launch, and lengths, page and angles one after the other.  13,800 rows with
+// looked up.  64 sequences of one token, 32 / 8 heads, take 4.1 us from fp32: the launch, and lengths, page and angles one after the
+// other; 64 rows of one sequence 3.7, 1024 sequences of one token 17.5, for every CTA reads the lengths of them all.  13,800 rows with
 // norms over whole vectors take 79 us (bf16, 4.2 TB/s): every row waits for its sums, and five rows fit an SM's registers.
 template <typename IT, typename OT, int CH>
 __global__ void __launch_bounds__(kAppendThreads) qw_kv_append_row_kernel(const AppendArgs a) {
@@ -377,8 +378,8 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(IT) == 2 ? 5 : 4) qw_kv
 
 template <typename IT, typename OT>
 cudaError_t append_launch(const AppendArgs &a, cudaStream_t st) {
-    // A CTA per row below: 592 rows of 32 / 8 heads 7.0 us (11.5 by fours), 1024 11.6 (12.3), 2048 17.4 (15.7); of 14 / 2 heads of 64
-    // 3.8 (5.4), 6.2 (5.7), 10.7 (6.9).  Norms over whole vectors would read four rows twice: 91 us against 79.
+    // A CTA per row below, rows of one sequence: 592 of 32 / 8 heads from bf16 6.7 us (11.0 by fours), 1024 11.3 (11.8), 2048 17.0 (15.3);
+    // of 14 / 2 heads of 64 from fp32, without norms, 3.7 (5.4), 6.0 (5.7), 10.2 (6.8).  Norms over whole vectors would read four rows twice: 91 us against 79.
     if (a.rows > kAppendFew && a.mode != QW_QKNORM_VECTOR)
         return launch_pdl(qw_kv_append_rows_kernel<IT, OT, kAppendRows>, dim3(a.rows / kAppendRows + (a.rows % kAppendRows != 0)), dim3(kAppendThreads),
                           kAppendRows * a.d * sizeof(float), st, a);

@@ -298,7 +298,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) qw_q8_rows_kernel(const Q8Rows
     }
 }
 
-// One CTA per row of any length and alignment: two passes over the row, the second from the caches.
+// One CTA per row of any length and alignment: two passes over the row, the second from the caches, one number a load.  Bound by the
+// loads: the norm of 8192 x 4095 takes 97 us in fp32 (64 for rows of 4096), 84 in bf16 (47); codes of 8192 x 12287 in bf16 98 (49).
 template <typename XT, typename DT, bool NORM>
 __global__ void __launch_bounds__(256) qw_q8_rows_any_kernel(const Q8RowsArgs a) {
     griddep_wait();
@@ -362,8 +363,8 @@ cudaError_t q8_rows_launch(const Q8RowsArgs &a, cudaStream_t st) {
                      !apart(a.q, a.ld_q, 1) && (uintptr_t)a.w % 16 == 0;
     // the norm holds its weights too: half the numbers fit its registers
     if (!vec || a.dim > (NORM ? 16384 : 32768)) return launch_pdl(qw_q8_rows_any_kernel<XT, DT, NORM>, dim3(a.rows), dim3(256), 0, st, a);
-    // Few rows: as many lanes as there are pieces (64 x 4096: 3.3 us, 4.2 with 8 pieces a lane; at
-    // 256 rows there is nothing between them, 5.0..5.1 us).  Many: so many numbers a lane that
+    // Few rows: as many lanes as there are pieces (64 x 4096: the norm of fp32 and bf16 2.7 us, 2.9 by the rule for many; bf16 rows 1.8 and
+    // 2.3; at 256 rows 4.9 and 4.6, 2.5 both).  Many: so many numbers a lane that
     // the exchange between the warps is rare, and so few that several rows fit an SM: 16 beside delta and weights (8192 x 4096 in
     // fp32: 64 us, 69 with 8 or 32), 32 alone (24576 x 4096: 73 us, 81 with 16), 64 of bf16 (8192 x 12288: 49 us; with an exact comparison of halves behind it, 56, and 66 with 32).
     const int pieces = (a.dim + V - 1) / V, most = a.rows <= kFewRows ? 1 : NORM ? 16 / V : 8;

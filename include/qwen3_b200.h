@@ -438,8 +438,8 @@ typedef struct qw_norm_q8_args {
 /* Residual addition, root-mean-square norm and codes in one pass: h = x + delta (fp32), sum = h (rounded once where the
  * stream is bf16; the norm sees h), y = h / sqrt(mean(h^2) + eps) * norm_w, then the codes and the scale of every row of y.
  * The norm cancels in the codes: they are those of the fp32 products h * norm_w, exactly.  The sum of squares is held in
- * 64 bits, and scale is rounded once from them (infinite where it leaves fp32).  Stands in for accum + rmsnorm (SequentialBlock.java:413-429,
- * NormalizationLayerFeatures.java:574-604), which it codes. */
+ * 64 bits, and scale is rounded once from them (infinite where it leaves fp32).  Stands in for accum + rmsnorm
+ * (SequentialBlock.java:413-429, NormalizationLayerFeatures.java:574-604), which it codes. */
 qw_status qw_op_norm_q8(const qw_norm_q8_args *args, void *stream);
 
 /* The codes (rows, ld_q) and scales (rows) of rows x (rows, ld_x) of dim numbers in x_dtype (F32 or BF16); strides in
@@ -457,7 +457,7 @@ typedef struct qw_linear_q8_args {
     const float *resid;   /* RESID: (t, ld_resid); out may be resid, with the same stride */
     void *out;            /* (t, ld_out) in out_dtype; n_out / 2 columns for SWIGLU */
     int32_t *err;         /* optional device word, set non-zero when a bounded device wait gave up */
-    int64_t ld_w, ld_x;   /* row strides in codes, multiples of 16; 0 = k.  What lies behind a row's k codes is not used */
+    int64_t ld_w, ld_x;   /* row strides in codes, multiples of 16 below 2^31; 0 = k.  What lies behind a row's k codes is not used */
     int64_t ld_resid, ld_out; /* row strides in elements; 0 = the columns */
     int32_t n_out, k, t;  /* k up to 131071: a sum of products of codes fits 32 bits */
     int32_t epi;          /* QW_LINEAR_STORE, QW_LINEAR_RESID or QW_LINEAR_SWIGLU */
@@ -467,10 +467,13 @@ typedef struct qw_linear_q8_args {
 
 /* Projection of codes on the tensor cores (tcgen05 kind::i8): s(t, f) = sum_j w(f, j) x(t, j) in 32-bit integers, exact,
  * y(t, f) = s w_scale(f) x_scale(t), then by `epi` STORE out = y (+ bias), RESID out = resid + y, SWIGLU out = up * silu(gate).
- * The sums being exact, results do not depend on how the work is split. */
+ * The sums being exact, results do not depend on how the work is split.  s, its products with the scales and what is added are
+ * rounded to fp32 in turn; a gate whose silu is below fp32's normal numbers may count as none.  n_out and t up to 2^30, and
+ * (n_out / 128 + 1) (t / 16 + 1) below 2^28 (QW_ERR_SHAPE beyond). */
 qw_status qw_op_linear_q8(const qw_linear_q8_args *args, void *stream);
 
-/* Arguments of qw_op_kv_append; all pointers are device pointers.  Zero-initialise the struct. */
+/* Arguments of qw_op_kv_append; all pointers are device pointers, those to floating-point numbers 16-byte aligned.
+ * Zero-initialise the struct. */
 typedef struct qw_kv_append_args {
     const void *q, *k, *v;     /* (rows, ld_q / ld_k / ld_v) in in_dtype: the projections of every row, side by side or apart */
     const float *q_norm, *k_norm; /* VECTOR: (heads x head_dim), (kv_heads x head_dim); HEAD: (head_dim) each; NONE: unused */
@@ -496,7 +499,8 @@ typedef struct qw_kv_append_args {
  * those that qw_op_chunk_attn then takes, read on the device.  Row i of a sequence's n new rows stands at position
  * p = kv_len - n + i (kv_len limited to the table's positions).  A row before position 0 or, with rope, at rope_len or
  * behind it is no row: q_out gets zeros, the cache nothing.  A position without a page takes no key and no value.  Two rows
- * must not stand at one position of one page.  Arithmetic is in fp32, rounded once.  Stands in for QK-norm, rotation and the
+ * must not stand at one position of one page.  Arithmetic is in fp32, rounded once; the norms' squares too, so that numbers
+ * beyond about 1e16 may overflow them.  Stands in for QK-norm, rotation and the
  * cache write (AttentionFeatures.java:823-891, RotationFeatures.java:124-208), one row of one sequence there. */
 qw_status qw_op_kv_append(const qw_kv_append_args *args, void *stream);
 
