@@ -139,7 +139,8 @@ __device__ __forceinline__ float scaled(int s, float ws, float xs) { return __fm
 
 // up * gate / (1 + e^-gate): the exponential and the division are within (|gate| + 4) 2^-21 of their value, the result is rounded
 // to bf16 behind it.  __fdividef gives 0 for divisors above 2^126: both sides are taken 2^-8 times, so that these begin at a gate
-// of -92.8, where silu(gate) is below fp32's normal numbers (-87.3 without).  An exponential below them does not count beside 1.
+// of -92.8, where silu(gate) is below fp32's normal numbers (-87.3 without); what gates below 2^-118 lose by it is 2^-142 of up.  An exponential
+// below the normal numbers does not count beside 1.
 __device__ __forceinline__ float silu_times(float g, float u) {
     constexpr float LOG2E = 1.44269504f;
     float e;

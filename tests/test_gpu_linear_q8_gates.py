@@ -65,3 +65,29 @@ def test_ends_of_the_gates(t, n_out):
     ok = torch.isfinite(want)
     assert bool(((out.double() - want).abs() <= 2.0 ** -8 * 1.001 * want.abs())[ok].all())
     assert torch.equal(out[~ok & ~torch.isnan(want)].double(), want[~ok & ~torch.isnan(want)])
+
+
+@pytest.mark.parametrize("t,n_out", [(3, 64), (300, 512), (1500, 8192)])
+def test_small_gates(t, n_out):
+    """Gates down to the smallest normal number: silu is half of them.  The gate is rounded at 2^-142 (2^-16 of the smallest one), the
+    rest as above."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(n_out)
+    w = torch.zeros((n_out, 16), dtype=torch.int8, device="cuda")
+    x = torch.zeros((t, 16), dtype=torch.int8, device="cuda")
+    w[:, 0] = x[:, 0] = 1
+    is_gate = torch.arange(n_out, device="cuda") % 32 < 16
+    power = torch.randint(-126, -20, (n_out,), device="cuda", generator=g)
+    gates = torch.ldexp(1 + torch.rand(n_out, device="cuda", generator=g), power) * (1 - 2 * (power % 2))
+    ws = torch.where(is_gate, gates, 1e30 * (1 + torch.rand(n_out, device="cuda", generator=g)))
+    xs = torch.ones(t, device="cuda")
+    out = torch.empty((t, n_out // 2), dtype=torch.bfloat16, device="cuda")
+    native.LinearQ8(w.data_ptr(), ws.data_ptr(), n_out, 16, epi=native.LINEAR_SWIGLU, out_dtype=native.DTYPE_BF16)(
+        x.data_ptr(), xs.data_ptr(), t, out.data_ptr())
+    torch.cuda.synchronize()
+    gate, up = ws.double()[is_gate], ws.double()[~is_gate]
+    want = up * gate / (1 + torch.exp(-gate))
+    bound = 4 * 2.0 ** -21 * want.abs() + up.abs() * 2.0 ** -142
+    bound = bound * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs()
+    off = (out.double() - want).abs() - bound
+    assert bool((off <= 0).all()), off.max().item()
